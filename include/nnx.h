@@ -505,6 +505,127 @@ int nnx_sw_fold_finalize(const void* d_total, int num_classes, int64_t voxels, i
                          int accumulation, void* d_logits, uint16_t* d_labels,
                          unsigned int* d_invalid, void* stream);
 
+/* ---- token operators -------------------------------------------------------------
+ * Steps of a transformer block over the tokens of a volume (one token a cube of voxels),
+ * between its plain matrix products.  No reference counterpart.  Element types are
+ * NNX_TYPE_*; sums, softmax statistics and norms are held in float32 and every result is
+ * rounded once to its type.  Innermost axes are contiguous, other strides (in elements) are
+ * free; 16-byte-aligned rows run on wide loads. */
+#define NNX_TYPE_F32 0
+#define NNX_TYPE_F16 1
+#define NNX_TYPE_BF16 2
+
+/* Rotary positions of one or two tensors (batch, tokens, heads, head_dim), e.g. queries and
+ * keys, in one launch.  Pair i < rotary_dim / 2 of every head is (x[i], x[i + rotary_dim / 2]),
+ * or (x[2i], x[2i + 1]) when `interleaved`; it is turned by position[pair_axes[i]] * steps[i]
+ * turns, with steps in units of 2^-64 turns, so the product's low 64 bits are the exact
+ * fraction of a turn at any position: (a, b) -> amplitude * (a c - b s, b c + a s), s negated
+ * when `inverse`.  Elements from rotary_dim on are copied.  y may be x itself (same pointer
+ * and strides). */
+typedef struct nnx_rotary_config {
+  int type;
+  int batch, tokens;
+  int heads[2];  /* of the two tensors; heads[1] = 0: one tensor */
+  int head_dim;  /* 2..1024 */
+  int rotary_dim; /* even, 2..head_dim */
+  int axes;       /* position axes of a token, 1..8 */
+  int interleaved, inverse;
+  float amplitude;
+  int64_t x_strides[6]; /* (batch, token, head) of each tensor */
+  int64_t y_strides[6];
+  int64_t position_strides[2]; /* (batch, token) of positions (batch, tokens, axes); 0 shares */
+} nnx_rotary_config;
+int nnx_rotary(const nnx_rotary_config* config, const void* d_x1, const void* d_x2,
+               const int32_t* d_positions, const int64_t* d_steps /* rotary_dim / 2 */,
+               const int32_t* d_pair_axes /* rotary_dim / 2 */, void* d_y1, void* d_y2,
+               void* stream);
+
+/* The norm after a block, the block's gate and scale, the residual sum and the norm before the
+ * next block, in one pass over the rows (tokens):
+ *   u  = post ? norm(x; post_weight, post_bias) : x
+ *   r' = residual_scale * residual + scale[c] * act(gate) * u   -> d_residual_out
+ *   y  = norm(r'; pre_weight, pre_bias), of r' before it is rounded        -> d_y
+ * norm is LayerNorm ((v - mean) / sqrt(var + eps)) or RMS (v / sqrt(mean v^2 + eps)) over the
+ * channels, times weight plus bias (float32; NULL = 1 and 0).  NULL d_residual, d_gate or
+ * d_scale leave their factor out; NULL d_residual_out or d_y (not both) are not computed;
+ * residual_out may be residual and y may be x (same pointer and stride).  x, gate and y are of
+ * `type`, residual and residual_out of `residual_type` (`type` or NNX_TYPE_F32). */
+#define NNX_TOKEN_NORM_LAYER 0
+#define NNX_TOKEN_NORM_RMS 1
+#define NNX_GATE_NONE 0
+#define NNX_GATE_SIGMOID 1
+#define NNX_GATE_SILU 2
+typedef struct nnx_residual_norm_config {
+  int type, residual_type;
+  int64_t rows;
+  int channels; /* 1..16384 */
+  int kind;     /* NNX_TOKEN_NORM_* */
+  int post;     /* 0 or 1 */
+  int gate_activation; /* NNX_GATE_* */
+  float residual_scale, eps;
+  int64_t x_stride, residual_stride, gate_stride, residual_out_stride, y_stride; /* of rows */
+} nnx_residual_norm_config;
+int nnx_residual_norm(const nnx_residual_norm_config* config, const void* d_x,
+                      const void* d_residual, const void* d_gate, const float* d_scale,
+                      const float* d_post_weight, const float* d_post_bias,
+                      const float* d_pre_weight, const float* d_pre_bias, void* d_residual_out,
+                      void* d_y, void* stream);
+
+/* Attention over blocks of keys that a cheap score selects for each query.  Keys are cut into
+ * blocks of `block`; a block's summary is the mean of its valid keys in 8 bits; each query
+ * keeps `keep` blocks and its softmax runs over their valid keys alone.
+ *
+ * Valid keys of item b are those before d_lengths[b] (NULL: all; clamped to [0, keys]) with a
+ * nonzero d_mask[b * mask_stride + key] (NULL: all).  What invalid keys and values hold is
+ * never used, NaN included.  Query t of item b stands at position start + d_start[b] (NULL: 0)
+ * + t; with `causal` it sees the keys up to its position and the blocks up to its own.
+ * kv_heads divides heads; heads j * (heads / kv_heads) ... share key head j and its blocks. */
+typedef struct nnx_block_config {
+  int type;
+  int batch, queries, keys;
+  int heads, kv_heads;
+  int head_dim; /* a multiple of 8, 8..128 */
+  int block;    /* 16, 32, 64 or 128; at most 32768 blocks */
+  int keep;     /* 1..256 */
+  int first;    /* leading blocks kept for every query */
+  int local;    /* blocks up to the query's own kept for every query */
+  int causal;
+  int64_t start;
+  float scale; /* of the logits */
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3]; /* (batch, token, head) */
+  int64_t mask_stride;
+} nnx_block_config;
+
+/* Summaries of blocks [first_block, first_block + blocks) of every item and key head:
+ * d_codes (batch, kv_heads, nb, head_dim) int8 and d_scales (batch, kv_heads, nb) float32, nb =
+ * ceil(keys / block).  With m the largest |k| of the block (non-finite elements count as 0):
+ * s[d] = sum_j rint(k[j, d] * (32767 / m)) in whole numbers, a = max |s|, code = rint(s * (127 /
+ * a)), scale = (m / (4161409 * valid keys)) * a; m < 2^-60 or a = 0: codes and scale 0; no valid
+ * key: scale -1.  Each step is elementwise or in whole numbers, so no order of summation shows. */
+int nnx_block_summarize(const nnx_block_config* config, const void* d_k, const int32_t* d_lengths,
+                        const uint8_t* d_mask, int first_block, int blocks, int8_t* d_codes,
+                        float* d_scales, void* stream);
+
+/* Blocks kept by each query and key head: d_ids (batch, queries, kv_heads, keep) int32,
+ * ascending, -1 behind the last.  A query head's codes are rint(q * (127 / m)), m = max |q|
+ * (non-finite elements 0; m < 2^-60: codes 0, m = 1); a block's score is the largest over the
+ * heads sharing the key head of (float(codes . codes) * m) * scale.  Kept are the `first` leading
+ * blocks and the `local` ones ending at the query's own, then the highest scores, equal ones
+ * by the lower index; blocks without valid keys (scale < 0) never, nor blocks behind a causal
+ * query's own. */
+int nnx_block_select(const nnx_block_config* config, const void* d_q, const int8_t* d_codes,
+                     const float* d_scales, const int32_t* d_start, int32_t* d_ids, void* stream);
+
+/* out[q] = softmax(scale q . k) v over the valid keys of the blocks in d_ids (batch, queries,
+ * kv_heads, keep; entries outside [0, nb) are skipped, the others of a row are distinct).  A
+ * query without a valid key gets zeros.  The workspace query answers 0 for what the entry
+ * refuses. */
+size_t nnx_block_attention_workspace(const nnx_block_config* config);
+int nnx_block_attention(const nnx_block_config* config, const void* d_q, const void* d_k,
+                        const void* d_v, const int32_t* d_ids, const int32_t* d_start,
+                        const int32_t* d_lengths, const uint8_t* d_mask, void* d_out,
+                        void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* ---- kernel timing (no reference counterpart: measurement support) ----------------
  * Between nnx_profile_begin and nnx_profile_end every kernel launch of the library is
  * bracketed by HIP events on its own stream and attributed to a class (kernel name and

@@ -338,4 +338,21 @@ void sw_fold_finalize(const void* total, int k, int64_t voxels, int nfolds, int 
                       void* logits, uint16_t* labels, unsigned int* invalid, hipStream_t st);
 void fill_zero(void* ptr, size_t bytes, hipStream_t st);
 
+// Token operators (nnx_tokens.hip, nnx_blocks.hip).
+void rotary(const nnx_rotary_config& c, const void* x1, const void* x2, const int32_t* positions,
+            const int64_t* steps, const int32_t* pair_axes, void* y1, void* y2, hipStream_t st);
+void residual_norm(const nnx_residual_norm_config& c, const void* x, const void* residual,
+                   const void* gate, const float* scale, const float* post_weight,
+                   const float* post_bias, const float* pre_weight, const float* pre_bias,
+                   void* residual_out, void* y, hipStream_t st);
+void block_summarize(const nnx_block_config& c, const void* k, const int32_t* lengths,
+                     const uint8_t* mask, int first_block, int blocks, int8_t* codes,
+                     float* scales, hipStream_t st);
+void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
+                  const float* scales, const int32_t* start, int32_t* ids, hipStream_t st);
+size_t block_attention_workspace(const nnx_block_config& c);
+void block_attention(const nnx_block_config& c, const void* q, const void* k, const void* v,
+                     const int32_t* ids, const int32_t* start, const int32_t* lengths,
+                     const uint8_t* mask, void* out, void* ws, size_t ws_bytes, hipStream_t st);
+
 }  // namespace nnx

@@ -1610,4 +1610,58 @@ int nnx_avgpool3d(const float* d_x, float* d_y, int batch, const int* in_size, i
   });
 }
 
+int nnx_rotary(const nnx_rotary_config* config, const void* d_x1, const void* d_x2,
+               const int32_t* d_positions, const int64_t* d_steps, const int32_t* d_pair_axes,
+               void* d_y1, void* d_y2, void* stream) {
+  return guarded([&] {
+    require(config, "rotary: null config");
+    rotary(*config, d_x1, d_x2, d_positions, d_steps, d_pair_axes, d_y1, d_y2, as_stream(stream));
+  });
+}
+
+int nnx_residual_norm(const nnx_residual_norm_config* config, const void* d_x,
+                      const void* d_residual, const void* d_gate, const float* d_scale,
+                      const float* d_post_weight, const float* d_post_bias,
+                      const float* d_pre_weight, const float* d_pre_bias, void* d_residual_out,
+                      void* d_y, void* stream) {
+  return guarded([&] {
+    require(config, "residual norm: null config");
+    residual_norm(*config, d_x, d_residual, d_gate, d_scale, d_post_weight, d_post_bias,
+                  d_pre_weight, d_pre_bias, d_residual_out, d_y, as_stream(stream));
+  });
+}
+
+int nnx_block_summarize(const nnx_block_config* config, const void* d_k, const int32_t* d_lengths,
+                        const uint8_t* d_mask, int first_block, int blocks, int8_t* d_codes,
+                        float* d_scales, void* stream) {
+  return guarded([&] {
+    require(config, "block summaries: null config");
+    block_summarize(*config, d_k, d_lengths, d_mask, first_block, blocks, d_codes, d_scales,
+                    as_stream(stream));
+  });
+}
+
+int nnx_block_select(const nnx_block_config* config, const void* d_q, const int8_t* d_codes,
+                     const float* d_scales, const int32_t* d_start, int32_t* d_ids, void* stream) {
+  return guarded([&] {
+    require(config, "block selection: null config");
+    block_select(*config, d_q, d_codes, d_scales, d_start, d_ids, as_stream(stream));
+  });
+}
+
+size_t nnx_block_attention_workspace(const nnx_block_config* config) {
+  return config ? block_attention_workspace(*config) : 0;
+}
+
+int nnx_block_attention(const nnx_block_config* config, const void* d_q, const void* d_k,
+                        const void* d_v, const int32_t* d_ids, const int32_t* d_start,
+                        const int32_t* d_lengths, const uint8_t* d_mask, void* d_out,
+                        void* d_workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    require(config, "block attention: null config");
+    block_attention(*config, d_q, d_k, d_v, d_ids, d_start, d_lengths, d_mask, d_out,
+                    d_workspace, workspace_bytes, as_stream(stream));
+  });
+}
+
 }  // extern "C"

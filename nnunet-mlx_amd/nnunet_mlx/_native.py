@@ -40,6 +40,14 @@ NNX_NORM_ZSCORE = 2
 NNX_NORM_ZSCORE_MASKED = 3
 NNX_ACCUM_F32 = 0
 NNX_ACCUM_NNUNET_F16 = 1
+NNX_TYPE_F32 = 0
+NNX_TYPE_F16 = 1
+NNX_TYPE_BF16 = 2
+NNX_TOKEN_NORM_LAYER = 0
+NNX_TOKEN_NORM_RMS = 1
+NNX_GATE_NONE = 0
+NNX_GATE_SIGMOID = 1
+NNX_GATE_SILU = 2
 
 c_int_p = ctypes.POINTER(ctypes.c_int)
 c_i64_p = ctypes.POINTER(ctypes.c_int64)
@@ -87,6 +95,67 @@ class NnxSwConfig(ctypes.Structure):
         ("accumulation", ctypes.c_int),
         ("d_gaussian", c_void_p),
         ("tiles_per_batch", ctypes.c_int),
+    ]
+
+
+class NnxRotaryConfig(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int),
+        ("batch", ctypes.c_int),
+        ("tokens", ctypes.c_int),
+        ("heads", ctypes.c_int * 2),
+        ("head_dim", ctypes.c_int),
+        ("rotary_dim", ctypes.c_int),
+        ("axes", ctypes.c_int),
+        ("interleaved", ctypes.c_int),
+        ("inverse", ctypes.c_int),
+        ("amplitude", ctypes.c_float),
+        ("x_strides", ctypes.c_int64 * 6),
+        ("y_strides", ctypes.c_int64 * 6),
+        ("position_strides", ctypes.c_int64 * 2),
+    ]
+
+
+class NnxResidualNormConfig(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int),
+        ("residual_type", ctypes.c_int),
+        ("rows", ctypes.c_int64),
+        ("channels", ctypes.c_int),
+        ("kind", ctypes.c_int),
+        ("post", ctypes.c_int),
+        ("gate_activation", ctypes.c_int),
+        ("residual_scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("x_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64),
+        ("gate_stride", ctypes.c_int64),
+        ("residual_out_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64),
+    ]
+
+
+class NnxBlockConfig(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int),
+        ("batch", ctypes.c_int),
+        ("queries", ctypes.c_int),
+        ("keys", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("block", ctypes.c_int),
+        ("keep", ctypes.c_int),
+        ("first", ctypes.c_int),
+        ("local", ctypes.c_int),
+        ("causal", ctypes.c_int),
+        ("start", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("out_strides", ctypes.c_int64 * 3),
+        ("mask_stride", ctypes.c_int64),
     ]
 
 
@@ -280,6 +349,31 @@ _SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         ctypes.c_int,
         [c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, c_void_p, c_void_p, c_void_p,
          c_void_p],
+    ),
+    "nnx_rotary": (
+        ctypes.c_int,
+        [ctypes.POINTER(NnxRotaryConfig), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_void_p],
+    ),
+    "nnx_residual_norm": (
+        ctypes.c_int,
+        [ctypes.POINTER(NnxResidualNormConfig), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "nnx_block_summarize": (
+        ctypes.c_int,
+        [ctypes.POINTER(NnxBlockConfig), c_void_p, c_void_p, c_void_p, ctypes.c_int, ctypes.c_int,
+         c_void_p, c_void_p, c_void_p],
+    ),
+    "nnx_block_select": (
+        ctypes.c_int,
+        [ctypes.POINTER(NnxBlockConfig), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "nnx_block_attention_workspace": (ctypes.c_size_t, [ctypes.POINTER(NnxBlockConfig)]),
+    "nnx_block_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(NnxBlockConfig), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p, ctypes.c_size_t, c_void_p],
     ),
     "nnx_profile_begin": (ctypes.c_int, []),
     "nnx_profile_end": (ctypes.c_int, [c_int_p]),

@@ -1,0 +1,404 @@
+"""Token operators: the steps of a transformer block over the tokens of a volume.
+
+A volume cut into cubes is a sequence of tokens.  Between a block's plain matrix products lie
+rotary positions (``rotary_plan``, ``rotate``), attention over blocks of keys that a cheap
+score selects for each query (``summarize_blocks``, ``select_blocks``, ``block_attention``, all
+three in ``sparse_attention``) and the norms around the block with its gate and residual sum
+(``residual_norm``).  Everything runs in libnnunet_hip.so on the current stream of the tensors'
+device, forward only; float32, float16 and bfloat16 tensors with a contiguous last axis and any
+other strides.  No reference counterpart.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import math
+from typing import NamedTuple
+
+import torch
+
+from nnunet_mlx import _native
+from nnunet_mlx.errors import ContractError
+
+_TYPES = {
+    torch.float32: _native.NNX_TYPE_F32,
+    torch.float16: _native.NNX_TYPE_F16,
+    torch.bfloat16: _native.NNX_TYPE_BF16,
+}
+_KINDS = {"layer": _native.NNX_TOKEN_NORM_LAYER, "rms": _native.NNX_TOKEN_NORM_RMS}
+_GATES = {
+    "none": _native.NNX_GATE_NONE,
+    "sigmoid": _native.NNX_GATE_SIGMOID,
+    "silu": _native.NNX_GATE_SILU,
+}
+_LAYOUTS = {"half": 0, "interleaved": 1}
+BLOCK_SIZES = (16, 32, 64, 128)
+
+
+def _need(ok: bool, message: str) -> None:
+    if not ok:
+        raise ContractError(message)
+
+
+def _check(name: str, tensor: torch.Tensor, dims: int, like: torch.Tensor | None = None) -> None:
+    if tensor.dim() != dims:
+        raise ContractError(f"{name} needs {dims} axes, got shape {tuple(tensor.shape)}")
+    if not tensor.is_cuda:
+        raise ContractError("the HIP path needs device tensors")
+    if tensor.stride(-1) != 1 and tensor.shape[-1] > 1:
+        raise ContractError(f"{name} needs a contiguous last axis")
+    if like is None:
+        if tensor.dtype not in _TYPES:
+            raise ContractError(f"{name} must be float32, float16 or bfloat16, not {tensor.dtype}")
+    elif tensor.device != like.device or tensor.dtype != like.dtype:
+        raise ContractError(f"{name} is {tensor.dtype} on {tensor.device}, not {like.dtype} on {like.device}")
+
+
+def _check_side(name: str, tensor: torch.Tensor, dtype: torch.dtype, shape: tuple[int, ...],
+                device: torch.device) -> None:
+    if tensor.dtype != dtype or tuple(tensor.shape) != shape or tensor.device != device:
+        raise ContractError(f"{name} must be {dtype} {shape} on {device}, got {tensor.dtype} "
+                            f"{tuple(tensor.shape)} on {tensor.device}")
+    if not tensor.is_contiguous():
+        raise ContractError(f"{name} must be contiguous")
+
+
+def _on(device: torch.device):
+    """The device made current for a launch (nothing to do where it already is)."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _address(tensor: torch.Tensor | None) -> int | None:
+    return None if tensor is None else tensor.data_ptr()
+
+
+# ---- rotary positions -----------------------------------------------------------------
+
+
+class RotaryPlan(NamedTuple):
+    """Rotation of the pairs of a head: ``steps`` int64 in 2^-64 turns a position, ``axes`` int32
+    the position axis of each pair, ``amplitude`` the factor on the rotated elements."""
+
+    steps: torch.Tensor
+    axes: torch.Tensor
+    amplitude: float
+
+
+def rotary_plan(rotary_dim: int, *, axes: int = 1, base: float = 10000.0, scaling: str | None = None,
+                factor: float = 1.0, trained_length: int = 8192, low: float = 1.0, high: float = 32.0,
+                device: torch.device | str = "cuda") -> RotaryPlan:
+    """Frequencies base^(-i / n) for the n pairs of each position axis (the pairs are shared out
+    evenly, the first axes taking one more), stretched for contexts ``factor`` times longer:
+
+    * ``"linear"``: every frequency divided by ``factor``;
+    * ``"base"``: the base multiplied by factor^(n / (n - 1)), which divides the slowest frequency
+      by ``factor`` and keeps the fastest;
+    * ``"ramp"``: frequencies that turn fewer than ``low`` times over ``trained_length`` are divided
+      by ``factor``, those above ``high`` turns kept, a linear ramp between; the amplitude is
+      0.1 ln(factor) + 1.
+    """
+    _need(rotary_dim >= 2 and rotary_dim % 2 == 0, f"rotary_dim must be even and positive, got {rotary_dim}")
+    pairs = rotary_dim // 2
+    _need(1 <= axes <= min(8, pairs), f"axes must be 1 to min(8, {pairs}), got {axes}")
+    _need(scaling in (None, "linear", "base", "ramp"), f"unknown scaling {scaling!r}")
+    _need(math.isfinite(base) and base > 0, f"base must be positive, got {base}")
+    _need(math.isfinite(factor) and factor >= 1, f"factor must be at least 1, got {factor}")
+    _need(scaling != "ramp" or (high > low and trained_length > 0), "the ramp needs high > low and a length")
+    steps, owners = [], []
+    for axis in range(axes):
+        n = pairs // axes + (axis < pairs % axes)
+        stretched = base * factor ** (n / (n - 1)) if scaling == "base" and n > 1 else base
+        for i in range(n):
+            frequency = stretched ** (-i / n)
+            if scaling == "linear":
+                frequency /= factor
+            elif scaling == "ramp":
+                turns = trained_length * frequency / (2 * math.pi)
+                kept = min(1.0, max(0.0, (turns - low) / (high - low)))
+                frequency *= kept + (1 - kept) / factor
+            step = round(frequency / (2 * math.pi) * 2.0**64) % (1 << 64)
+            steps.append(step - (1 << 64) if step >= 1 << 63 else step)
+            owners.append(axis)
+    amplitude = 0.1 * math.log(factor) + 1.0 if scaling == "ramp" else 1.0
+    return RotaryPlan(torch.tensor(steps, dtype=torch.int64, device=device),
+                      torch.tensor(owners, dtype=torch.int32, device=device), amplitude)
+
+
+def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, plan: RotaryPlan, *,
+           layout: str = "half", inverse: bool = False,
+           out: tuple[torch.Tensor, torch.Tensor | None] | None = None,
+           ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary positions of ``q`` and ``k`` (batch, tokens, heads, head_dim) in one launch.
+
+    ``positions`` is int32 (tokens, axes) or (batch, tokens, axes).  ``layout`` pairs element i
+    with i + rotary_dim / 2 ("half") or 2i with 2i + 1 ("interleaved"); elements past the plan's
+    pairs are copied.  ``inverse`` turns back, which is also the gradient of the forward turn.
+    ``out`` may hold the results, ``(q, k)`` itself to rotate in place."""
+    _check("q", q, 4)
+    batch, tokens, heads, dim = q.shape
+    rotary_dim = 2 * plan.steps.numel()
+    _need(layout in _LAYOUTS, f"layout must be 'half' or 'interleaved', got {layout!r}")
+    if k is not None:
+        _check("k", k, 4, q)
+        _need(k.shape[:2] == q.shape[:2] and k.shape[3] == dim,
+              f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    _need(positions.dim() in (2, 3) and positions.dtype == torch.int32 and positions.device == q.device
+          and positions.shape[-2] == tokens and positions.shape[:-2] in ((), (batch,)),
+          f"positions must be int32 (tokens, axes) or (batch, tokens, axes) on {q.device}, got "
+          f"{positions.dtype} {tuple(positions.shape)} on {positions.device}")
+    axes = positions.shape[-1]
+    _need(axes == 1 or positions.stride(-1) == 1, "positions need a contiguous last axis")
+    _check_side("plan.steps", plan.steps, torch.int64, (rotary_dim // 2,), q.device)
+    _check_side("plan.axes", plan.axes, torch.int32, (rotary_dim // 2,), q.device)
+    if out is None:
+        yq = torch.empty((batch, tokens, heads, dim), dtype=q.dtype, device=q.device)
+        yk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    else:
+        yq, yk = out
+        for name, x, y in (("out[0]", q, yq), ("out[1]", k, yk)):
+            _need((x is None) == (y is None), f"{name} does not match its input")
+            if y is not None:
+                _check(name, y, 4, q)
+                _need(y.shape == x.shape, f"{name} {tuple(y.shape)} does not match its input {tuple(x.shape)}")
+    if q.numel() == 0 and (k is None or k.numel() == 0):
+        return yq, yk
+    none = (0, 0, 0)
+    config = _native.NnxRotaryConfig(
+        _TYPES[q.dtype], batch, tokens, (heads, 0 if k is None else k.shape[2]), dim, rotary_dim, axes,
+        _LAYOUTS[layout], int(inverse), plan.amplitude,
+        q.stride()[:3] + (none if k is None else k.stride()[:3]),
+        yq.stride()[:3] + (none if yk is None else yk.stride()[:3]),
+        ((0, positions.stride(0)) if positions.dim() == 2 else positions.stride()[:2]))
+    with _on(q.device):
+        _native.check(_native.load().nnx_rotary(
+            config, q.data_ptr(), _address(k), positions.data_ptr(), plan.steps.data_ptr(),
+            plan.axes.data_ptr(), yq.data_ptr(), _address(yk), _native.stream_handle(q.device)), "nnx_rotary")
+    return yq, yk
+
+
+# ---- the norms around a block ---------------------------------------------------------
+
+Affine = tuple[torch.Tensor | None, torch.Tensor | None]
+
+
+def _rows(name: str, tensor: torch.Tensor) -> int:
+    """Stride of the rows of a (..., channels) tensor whose leading axes step evenly."""
+    step = tensor.stride(-2) if tensor.dim() > 1 else tensor.shape[-1]
+    for axis in range(tensor.dim() - 2, 0, -1):
+        if tensor.shape[axis - 1] > 1 and tensor.stride(axis - 1) != tensor.stride(axis) * tensor.shape[axis]:
+            raise ContractError(f"{name}: the axes before the last must step evenly")
+    return step
+
+
+def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, *, kind: str = "layer",
+                  post: Affine | None = None, pre: Affine | None = None,
+                  gate: torch.Tensor | None = None, gate_activation: str = "none",
+                  scale: torch.Tensor | None = None, residual_scale: float = 1.0, eps: float = 1e-6,
+                  ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """The residual sum between two blocks with the norms on both its sides, in one pass:
+
+        u  = norm(x, post) if post is given, else x
+        r' = residual_scale * residual + scale * activation(gate) * u
+        y  = norm(r', pre) if pre is given
+
+    Returns ``(r', y)``, y None without ``pre``.  ``x`` (..., channels) is a block's output;
+    ``residual`` has its shape and dtype or is float32, and r' is like it (like x without one);
+    ``gate`` is like x; ``scale`` float32 (channels,).  ``post`` and ``pre`` are (weight, bias),
+    float32 (channels,) or None each.  ``kind`` is "layer" or "rms"; y is the norm of r' before
+    it is rounded to its dtype."""
+    _check("x", x, max(1, x.dim()))
+    channels = x.shape[-1]
+    rows = x.numel() // channels if channels else 0
+    _need(kind in _KINDS, f"kind must be 'layer' or 'rms', got {kind!r}")
+    _need(gate_activation in _GATES, f"unknown gate activation {gate_activation!r}")
+    _need(gate is not None or gate_activation == "none", "a gate activation needs a gate")
+    if residual is not None:
+        _check("residual", residual, x.dim(), x if residual.dtype == x.dtype else None)
+        _need(residual.shape == x.shape and residual.device == x.device
+              and residual.dtype in (x.dtype, torch.float32),
+              f"residual {residual.dtype} {tuple(residual.shape)} does not match x {x.dtype} {tuple(x.shape)}")
+    if gate is not None:
+        _check("gate", gate, x.dim(), x)
+        _need(gate.shape == x.shape, f"gate {tuple(gate.shape)} does not match x {tuple(x.shape)}")
+    vectors = (scale, *(post or (None, None)), *(pre or (None, None)))
+    for name, vector in zip(("scale", "post weight", "post bias", "pre weight", "pre bias"), vectors):
+        if vector is not None:
+            _check_side(name, vector, torch.float32, (channels,), x.device)
+    wide = x.dtype if residual is None else residual.dtype
+    total = torch.empty(x.shape, dtype=wide, device=x.device)
+    y = None if pre is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if rows == 0:
+        return total, y
+    config = _native.NnxResidualNormConfig(
+        _TYPES[x.dtype], _TYPES[wide], rows, channels, _KINDS[kind], int(post is not None),
+        _GATES[gate_activation], residual_scale, eps, _rows("x", x),
+        0 if residual is None else _rows("residual", residual), 0 if gate is None else _rows("gate", gate),
+        channels, channels)
+    with _on(x.device):
+        _native.check(_native.load().nnx_residual_norm(
+            config, x.data_ptr(), _address(residual), _address(gate), *map(_address, vectors),
+            total.data_ptr(), _address(y), _native.stream_handle(x.device)), "nnx_residual_norm")
+    return total, y
+
+
+# ---- attention over selected blocks ---------------------------------------------------
+
+
+class BlockSummary(NamedTuple):
+    """Means of the blocks' valid keys in 8 bits: ``codes`` int8 (batch, kv_heads, blocks, head_dim)
+    and ``scales`` float32 (batch, kv_heads, blocks), -1 for a block without valid keys."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _block_config(like: torch.Tensor, block: int, batch: int, queries: int, keys: int, heads: int,
+                  kv_heads: int, *, keep: int = 1, first: int = 0, local: int = 0, causal: bool = False,
+                  start: int = 0, scale: float = 1.0) -> _native.NnxBlockConfig:
+    _need(block in BLOCK_SIZES, f"block must be one of {BLOCK_SIZES}, got {block}")
+    return _native.NnxBlockConfig(_TYPES[like.dtype], batch, queries, keys, heads, kv_heads, like.shape[-1],
+                                  block, keep, first, local, int(causal), start, scale)
+
+
+def _start(start: torch.Tensor | int | None, batch: int, device: torch.device) -> tuple[int, int | None]:
+    if start is None or isinstance(start, int):
+        return start or 0, None
+    _check_side("start", start, torch.int32, (batch,), device)
+    return 0, start.data_ptr()
+
+
+def _lengths_mask(config: _native.NnxBlockConfig, lengths: torch.Tensor | None, mask: torch.Tensor | None,
+                  batch: int, keys: int, device: torch.device) -> tuple[int | None, int | None]:
+    if lengths is not None:
+        _check_side("lengths", lengths, torch.int32, (batch,), device)
+    if mask is not None:
+        _need(mask.dtype in (torch.bool, torch.uint8) and tuple(mask.shape) == (batch, keys)
+              and mask.device == device and (keys <= 1 or mask.stride(1) == 1),
+              f"key_mask must be bool or uint8 ({batch}, {keys}) on {device} with a contiguous last axis, "
+              f"got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
+        config.mask_stride = mask.stride(0)
+    return _address(lengths), _address(mask)
+
+
+def summarize_blocks(k: torch.Tensor, block: int, *, lengths: torch.Tensor | None = None,
+                     key_mask: torch.Tensor | None = None, first: int = 0, count: int | None = None,
+                     out: BlockSummary | None = None) -> BlockSummary:
+    """Summaries of the blocks of keys ``k`` (batch, keys, kv_heads, head_dim).
+
+    ``lengths`` int32 (batch,) counts the keys each item has, ``key_mask`` (batch, keys) marks the
+    ones that are seen.  ``first`` and ``count`` with ``out`` refresh those blocks of a summary
+    that is kept, as after appending keys."""
+    _check("k", k, 4)
+    batch, keys, kv_heads, dim = k.shape
+    config = _block_config(k, block, batch, 0, keys, kv_heads, kv_heads)
+    config.k_strides = k.stride()[:3]
+    blocks = -(-keys // block)
+    lengths_at, mask_at = _lengths_mask(config, lengths, key_mask, batch, keys, k.device)
+    if count is None:
+        count = blocks - first
+    if out is None:
+        _need(first == 0 and count == blocks, "summaries of some blocks need the summary to refresh (out)")
+        out = BlockSummary(torch.empty((batch, kv_heads, blocks, dim), dtype=torch.int8, device=k.device),
+                           torch.empty((batch, kv_heads, blocks), dtype=torch.float32, device=k.device))
+    else:
+        _check_side("out.codes", out.codes, torch.int8, (batch, kv_heads, blocks, dim), k.device)
+        _check_side("out.scales", out.scales, torch.float32, (batch, kv_heads, blocks), k.device)
+    if k.numel() == 0:
+        return out
+    with _on(k.device):
+        _native.check(_native.load().nnx_block_summarize(
+            config, k.data_ptr(), lengths_at, mask_at, first, count, out.codes.data_ptr(),
+            out.scales.data_ptr(), _native.stream_handle(k.device)), "nnx_block_summarize")
+    return out
+
+
+def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int, *, causal: bool = False,
+                  start: torch.Tensor | int | None = None, first: int = 0, local: int = 1) -> torch.Tensor:
+    """Blocks that each query (batch, queries, heads, head_dim) keeps for each key head: int32
+    (batch, queries, kv_heads, keep), ascending, -1 behind the last.
+
+    Kept are the ``first`` leading blocks, the ``local`` blocks ending at the query's own (its
+    position is ``start``, an int or int32 (batch,), plus its index), and the best by the largest
+    product of the summary with the query heads that share the key head; equal scores go to the
+    lower index.  The scores are formed in whole numbers, so they do not depend on how the work is
+    split.  ``causal`` leaves out the blocks behind the query's own."""
+    _check("q", q, 4)
+    batch, queries, heads, dim = q.shape
+    _need(summary.codes.dim() == 4, f"summary codes need 4 axes, got shape {tuple(summary.codes.shape)}")
+    kv_heads, blocks = summary.codes.shape[1:3]
+    _check_side("summary.codes", summary.codes, torch.int8, (batch, kv_heads, blocks, dim), q.device)
+    _check_side("summary.scales", summary.scales, torch.float32, (batch, kv_heads, blocks), q.device)
+    begin, start_at = _start(start, batch, q.device)
+    config = _block_config(q, block, batch, queries, blocks * block, heads, kv_heads, keep=keep, first=first,
+                           local=local, causal=causal, start=begin)
+    config.q_strides = q.stride()[:3]
+    ids = torch.empty((batch, queries, kv_heads, keep), dtype=torch.int32, device=q.device)
+    if q.numel() == 0:
+        return ids
+    if blocks == 0:
+        return ids.fill_(-1)
+    with _on(q.device):
+        _native.check(_native.load().nnx_block_select(
+            config, q.data_ptr(), summary.codes.data_ptr(), summary.scales.data_ptr(), start_at,
+            ids.data_ptr(), _native.stream_handle(q.device)), "nnx_block_select")
+    return ids
+
+
+def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torch.Tensor, block: int, *,
+                    scale: float | None = None, causal: bool = False,
+                    start: torch.Tensor | int | None = None, lengths: torch.Tensor | None = None,
+                    key_mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Softmax attention of q (batch, queries, heads, head_dim) over the keys k and values v
+    (batch, keys, kv_heads, head_dim) of the blocks in ``ids`` (batch, queries, kv_heads, keep).
+
+    ``scale`` defaults to head_dim^-0.5; ``causal``, ``start``, ``lengths`` and ``key_mask`` as in
+    ``select_blocks`` and ``summarize_blocks``.  A query that sees no key gets zeros."""
+    _check("q", q, 4)
+    _check("k", k, 4, q)
+    _check("v", v, 4, q)
+    batch, queries, heads, dim = q.shape
+    keys, kv_heads = k.shape[1:3]
+    _need(k.shape == (batch, keys, kv_heads, dim) and v.shape == k.shape,
+          f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match q {tuple(q.shape)}")
+    _need(ids.dim() == 4, f"ids need 4 axes, got shape {tuple(ids.shape)}")
+    keep = ids.shape[3]
+    _check_side("ids", ids, torch.int32, (batch, queries, kv_heads, keep), q.device)
+    begin, start_at = _start(start, batch, q.device)
+    config = _block_config(q, block, batch, queries, keys, heads, kv_heads, keep=keep, causal=causal,
+                           start=begin, scale=dim**-0.5 if scale is None else scale)
+    lengths_at, mask_at = _lengths_mask(config, lengths, key_mask, batch, keys, q.device)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _check("out", out, 4, q)
+        _need(out.shape == q.shape, f"out {tuple(out.shape)} does not match q {tuple(q.shape)}")
+    if q.numel() == 0:
+        return out
+    if keys == 0:
+        return out.zero_()
+    config.q_strides, config.k_strides = q.stride()[:3], k.stride()[:3]
+    config.v_strides, config.out_strides = v.stride()[:3], out.stride()[:3]
+    lib = _native.load()
+    with _on(q.device):
+        size = lib.nnx_block_attention_workspace(config)
+        work = torch.empty(max(1, size), dtype=torch.uint8, device=q.device)
+        _native.check(lib.nnx_block_attention(
+            config, q.data_ptr(), k.data_ptr(), v.data_ptr(), ids.data_ptr(), start_at, lengths_at, mask_at,
+            out.data_ptr(), work.data_ptr(), size, _native.stream_handle(q.device)), "nnx_block_attention")
+    return out
+
+
+def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block: int, keep: int, *,
+                     summary: BlockSummary | None = None, scale: float | None = None, causal: bool = False,
+                     start: torch.Tensor | int | None = None, first: int = 0, local: int = 1,
+                     lengths: torch.Tensor | None = None,
+                     key_mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``summarize_blocks`` (unless a ``summary`` is held), ``select_blocks`` and ``block_attention``;
+    returns the attention's output and the kept blocks."""
+    if summary is None:
+        summary = summarize_blocks(k, block, lengths=lengths, key_mask=key_mask)
+    ids = select_blocks(q, summary, block, keep, causal=causal, start=start, first=first, local=local)
+    return block_attention(q, k, v, ids, block, scale=scale, causal=causal, start=start, lengths=lengths,
+                           key_mask=key_mask), ids
