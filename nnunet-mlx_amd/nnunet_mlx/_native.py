@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 from typing import Any
@@ -482,6 +483,12 @@ def ptr(tensor: torch.Tensor | None) -> int | None:
 
 def stream_handle(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def packed(structure: type[ctypes.Structure], layout: struct.Struct, *values) -> ctypes.Structure:
+    """A structure from its fields' values in order, packed at once: a third of the time that setting
+    fields takes, which is most of what the smallest calls cost.  ``layout`` is the native layout."""
+    return structure.from_buffer_copy(layout.pack(*values))
 
 
 class KernelProfile:

@@ -11,8 +11,8 @@ other strides.  No reference counterpart.
 
 from __future__ import annotations
 
-import contextlib
 import math
+import struct
 from typing import NamedTuple
 
 import torch
@@ -33,6 +33,15 @@ _GATES = {
 }
 _LAYOUTS = {"half": 0, "interleaved": 1}
 BLOCK_SIZES = (16, 32, 64, 128)
+
+# native layouts of the library's configurations
+_ROTARY = struct.Struct("@10if4x14q")
+_NORM = struct.Struct("@2iq4i2f5q")
+_BLOCK = struct.Struct("@12iqf4x13q")
+
+# the current stream of a device index, as torch's own launches ask for it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _need(ok: bool, message: str) -> None:
@@ -63,11 +72,16 @@ def _check_side(name: str, tensor: torch.Tensor, dtype: torch.dtype, shape: tupl
         raise ContractError(f"{name} must be contiguous")
 
 
-def _on(device: torch.device):
-    """The device made current for a launch (nothing to do where it already is)."""
+def _launch(device: torch.device, entry: str, *arguments) -> None:
+    """Calls a library entry on the device's current stream, its last argument."""
+    function = getattr(_native.load(), entry)
     if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+        status = function(*arguments, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            status = function(*arguments, _raw_stream(device.index))
+    if status:
+        _native.check(status, entry)
 
 
 def _address(tensor: torch.Tensor | None) -> int | None:
@@ -153,8 +167,8 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
     _check_side("plan.steps", plan.steps, torch.int64, (rotary_dim // 2,), q.device)
     _check_side("plan.axes", plan.axes, torch.int32, (rotary_dim // 2,), q.device)
     if out is None:
-        yq = torch.empty((batch, tokens, heads, dim), dtype=q.dtype, device=q.device)
-        yk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        yq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        yk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
         yq, yk = out
         for name, x, y in (("out[0]", q, yq), ("out[1]", k, yk)):
@@ -165,16 +179,14 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
     if q.numel() == 0 and (k is None or k.numel() == 0):
         return yq, yk
     none = (0, 0, 0)
-    config = _native.NnxRotaryConfig(
-        _TYPES[q.dtype], batch, tokens, (heads, 0 if k is None else k.shape[2]), dim, rotary_dim, axes,
-        _LAYOUTS[layout], int(inverse), plan.amplitude,
-        q.stride()[:3] + (none if k is None else k.stride()[:3]),
-        yq.stride()[:3] + (none if yk is None else yk.stride()[:3]),
-        ((0, positions.stride(0)) if positions.dim() == 2 else positions.stride()[:2]))
-    with _on(q.device):
-        _native.check(_native.load().nnx_rotary(
-            config, q.data_ptr(), _address(k), positions.data_ptr(), plan.steps.data_ptr(),
-            plan.axes.data_ptr(), yq.data_ptr(), _address(yk), _native.stream_handle(q.device)), "nnx_rotary")
+    config = _native.packed(
+        _native.NnxRotaryConfig, _ROTARY, _TYPES[q.dtype], batch, tokens, heads, 0 if k is None else k.shape[2],
+        dim, rotary_dim, axes, _LAYOUTS[layout], int(inverse), plan.amplitude,
+        *q.stride()[:3], *(none if k is None else k.stride()[:3]),
+        *yq.stride()[:3], *(none if yk is None else yk.stride()[:3]),
+        *((0, positions.stride(0)) if positions.dim() == 2 else positions.stride()[:2]))
+    _launch(q.device, "nnx_rotary", config, q.data_ptr(), _address(k), positions.data_ptr(),
+            plan.steps.data_ptr(), plan.axes.data_ptr(), yq.data_ptr(), _address(yk))
     return yq, yk
 
 
@@ -226,20 +238,17 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, *, kind: str =
     for name, vector in zip(("scale", "post weight", "post bias", "pre weight", "pre bias"), vectors):
         if vector is not None:
             _check_side(name, vector, torch.float32, (channels,), x.device)
-    wide = x.dtype if residual is None else residual.dtype
-    total = torch.empty(x.shape, dtype=wide, device=x.device)
-    y = None if pre is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    total = torch.empty_like(x if residual is None else residual, memory_format=torch.contiguous_format)
+    y = None if pre is None else torch.empty_like(x, memory_format=torch.contiguous_format)
     if rows == 0:
         return total, y
-    config = _native.NnxResidualNormConfig(
-        _TYPES[x.dtype], _TYPES[wide], rows, channels, _KINDS[kind], int(post is not None),
-        _GATES[gate_activation], residual_scale, eps, _rows("x", x),
+    config = _native.packed(
+        _native.NnxResidualNormConfig, _NORM, _TYPES[x.dtype], _TYPES[total.dtype], rows, channels, _KINDS[kind],
+        int(post is not None), _GATES[gate_activation], residual_scale, eps, _rows("x", x),
         0 if residual is None else _rows("residual", residual), 0 if gate is None else _rows("gate", gate),
         channels, channels)
-    with _on(x.device):
-        _native.check(_native.load().nnx_residual_norm(
-            config, x.data_ptr(), _address(residual), _address(gate), *map(_address, vectors),
-            total.data_ptr(), _address(y), _native.stream_handle(x.device)), "nnx_residual_norm")
+    _launch(x.device, "nnx_residual_norm", config, x.data_ptr(), _address(residual), _address(gate),
+            *[None if v is None else v.data_ptr() for v in vectors], total.data_ptr(), _address(y))
     return total, y
 
 
@@ -254,12 +263,21 @@ class BlockSummary(NamedTuple):
     scales: torch.Tensor
 
 
+_NO_STRIDES = (0, 0, 0)
+
+
 def _block_config(like: torch.Tensor, block: int, batch: int, queries: int, keys: int, heads: int,
-                  kv_heads: int, *, keep: int = 1, first: int = 0, local: int = 0, causal: bool = False,
-                  start: int = 0, scale: float = 1.0) -> _native.NnxBlockConfig:
-    _need(block in BLOCK_SIZES, f"block must be one of {BLOCK_SIZES}, got {block}")
-    return _native.NnxBlockConfig(_TYPES[like.dtype], batch, queries, keys, heads, kv_heads, like.shape[-1],
-                                  block, keep, first, local, int(causal), start, scale)
+                  kv_heads: int, mask_stride: int, *, keep: int = 1, first: int = 0, local: int = 0,
+                  causal: bool = False, start: int = 0, scale: float = 1.0, q=_NO_STRIDES, k=_NO_STRIDES,
+                  v=_NO_STRIDES, out=_NO_STRIDES) -> _native.NnxBlockConfig:
+    if block not in BLOCK_SIZES:
+        raise ContractError(f"block must be one of {BLOCK_SIZES}, got {block}")
+    try:
+        return _native.packed(_native.NnxBlockConfig, _BLOCK, _TYPES[like.dtype], batch, queries, keys, heads,
+                              kv_heads, like.shape[-1], block, keep, first, local, bool(causal), start, scale,
+                              *q, *k, *v, *out, mask_stride)
+    except struct.error as error:
+        raise ContractError(f"a block argument is no 32-bit whole number: {error}") from error
 
 
 def _start(start: torch.Tensor | int | None, batch: int, device: torch.device) -> tuple[int, int | None]:
@@ -269,8 +287,8 @@ def _start(start: torch.Tensor | int | None, batch: int, device: torch.device) -
     return 0, start.data_ptr()
 
 
-def _lengths_mask(config: _native.NnxBlockConfig, lengths: torch.Tensor | None, mask: torch.Tensor | None,
-                  batch: int, keys: int, device: torch.device) -> tuple[int | None, int | None]:
+def _lengths_mask(lengths: torch.Tensor | None, mask: torch.Tensor | None, batch: int, keys: int,
+                  device: torch.device) -> tuple[int | None, int | None, int]:
     if lengths is not None:
         _check_side("lengths", lengths, torch.int32, (batch,), device)
     if mask is not None:
@@ -278,8 +296,7 @@ def _lengths_mask(config: _native.NnxBlockConfig, lengths: torch.Tensor | None, 
               and mask.device == device and (keys <= 1 or mask.stride(1) == 1),
               f"key_mask must be bool or uint8 ({batch}, {keys}) on {device} with a contiguous last axis, "
               f"got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
-        config.mask_stride = mask.stride(0)
-    return _address(lengths), _address(mask)
+    return _address(lengths), _address(mask), 0 if mask is None else mask.stride(0)
 
 
 def summarize_blocks(k: torch.Tensor, block: int, *, lengths: torch.Tensor | None = None,
@@ -292,10 +309,9 @@ def summarize_blocks(k: torch.Tensor, block: int, *, lengths: torch.Tensor | Non
     that is kept, as after appending keys."""
     _check("k", k, 4)
     batch, keys, kv_heads, dim = k.shape
-    config = _block_config(k, block, batch, 0, keys, kv_heads, kv_heads)
-    config.k_strides = k.stride()[:3]
+    lengths_at, mask_at, mask_stride = _lengths_mask(lengths, key_mask, batch, keys, k.device)
+    config = _block_config(k, block, batch, 0, keys, kv_heads, kv_heads, mask_stride, k=k.stride()[:3])
     blocks = -(-keys // block)
-    lengths_at, mask_at = _lengths_mask(config, lengths, key_mask, batch, keys, k.device)
     if count is None:
         count = blocks - first
     if out is None:
@@ -307,10 +323,8 @@ def summarize_blocks(k: torch.Tensor, block: int, *, lengths: torch.Tensor | Non
         _check_side("out.scales", out.scales, torch.float32, (batch, kv_heads, blocks), k.device)
     if k.numel() == 0:
         return out
-    with _on(k.device):
-        _native.check(_native.load().nnx_block_summarize(
-            config, k.data_ptr(), lengths_at, mask_at, first, count, out.codes.data_ptr(),
-            out.scales.data_ptr(), _native.stream_handle(k.device)), "nnx_block_summarize")
+    _launch(k.device, "nnx_block_summarize", config, k.data_ptr(), lengths_at, mask_at, first, count,
+            out.codes.data_ptr(), out.scales.data_ptr())
     return out
 
 
@@ -331,18 +345,16 @@ def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int,
     _check_side("summary.codes", summary.codes, torch.int8, (batch, kv_heads, blocks, dim), q.device)
     _check_side("summary.scales", summary.scales, torch.float32, (batch, kv_heads, blocks), q.device)
     begin, start_at = _start(start, batch, q.device)
-    config = _block_config(q, block, batch, queries, blocks * block, heads, kv_heads, keep=keep, first=first,
-                           local=local, causal=causal, start=begin)
-    config.q_strides = q.stride()[:3]
+    config = _block_config(q, block, batch, queries, blocks * block, heads, kv_heads, 0, keep=keep, first=first,
+                           local=local, causal=causal, start=begin, q=q.stride()[:3])
+    _need(keep >= 1, f"keep must be positive, got {keep}")
     ids = torch.empty((batch, queries, kv_heads, keep), dtype=torch.int32, device=q.device)
     if q.numel() == 0:
         return ids
     if blocks == 0:
         return ids.fill_(-1)
-    with _on(q.device):
-        _native.check(_native.load().nnx_block_select(
-            config, q.data_ptr(), summary.codes.data_ptr(), summary.scales.data_ptr(), start_at,
-            ids.data_ptr(), _native.stream_handle(q.device)), "nnx_block_select")
+    _launch(q.device, "nnx_block_select", config, q.data_ptr(), summary.codes.data_ptr(),
+            summary.scales.data_ptr(), start_at, ids.data_ptr())
     return ids
 
 
@@ -366,27 +378,23 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torc
     keep = ids.shape[3]
     _check_side("ids", ids, torch.int32, (batch, queries, kv_heads, keep), q.device)
     begin, start_at = _start(start, batch, q.device)
-    config = _block_config(q, block, batch, queries, keys, heads, kv_heads, keep=keep, causal=causal,
-                           start=begin, scale=dim**-0.5 if scale is None else scale)
-    lengths_at, mask_at = _lengths_mask(config, lengths, key_mask, batch, keys, q.device)
+    lengths_at, mask_at, mask_stride = _lengths_mask(lengths, key_mask, batch, keys, q.device)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check("out", out, 4, q)
         _need(out.shape == q.shape, f"out {tuple(out.shape)} does not match q {tuple(q.shape)}")
+    config = _block_config(q, block, batch, queries, keys, heads, kv_heads, mask_stride, keep=keep, causal=causal,
+                           start=begin, scale=dim**-0.5 if scale is None else scale, q=q.stride()[:3],
+                           k=k.stride()[:3], v=v.stride()[:3], out=out.stride()[:3])
     if q.numel() == 0:
         return out
     if keys == 0:
         return out.zero_()
-    config.q_strides, config.k_strides = q.stride()[:3], k.stride()[:3]
-    config.v_strides, config.out_strides = v.stride()[:3], out.stride()[:3]
-    lib = _native.load()
-    with _on(q.device):
-        size = lib.nnx_block_attention_workspace(config)
-        work = torch.empty(max(1, size), dtype=torch.uint8, device=q.device)
-        _native.check(lib.nnx_block_attention(
-            config, q.data_ptr(), k.data_ptr(), v.data_ptr(), ids.data_ptr(), start_at, lengths_at, mask_at,
-            out.data_ptr(), work.data_ptr(), size, _native.stream_handle(q.device)), "nnx_block_attention")
+    size = _native.load().nnx_block_attention_workspace(config)
+    work = torch.empty(max(1, size), dtype=torch.uint8, device=q.device)
+    _launch(q.device, "nnx_block_attention", config, q.data_ptr(), k.data_ptr(), v.data_ptr(), ids.data_ptr(),
+            start_at, lengths_at, mask_at, out.data_ptr(), work.data_ptr(), size)
     return out
 
 
