@@ -1,0 +1,52 @@
+// Shared by the kernels of attention over selected blocks: arguments, the chunk of work that one
+// pass of launches covers, and per-item lengths and positions.
+#pragma once
+
+#include "nnx_elements.h"
+
+namespace nnx {
+
+struct BlockArgs {
+  int batch, queries, keys, heads, kv_heads, group, dim, block, blocks, keep, first, local, causal;
+  int64_t start0;
+  float scale;
+  int64_t qs[3], ks[3], vs[3], os[3], ms;
+  const int32_t *start, *lengths;
+  const uint8_t* mask;
+};
+
+__device__ __forceinline__ int item_length(const BlockArgs& a, int b) {
+  return a.lengths ? min(max(a.lengths[b], 0), a.keys) : a.keys;
+}
+
+__device__ __forceinline__ int64_t item_start(const BlockArgs& a, int b) {
+  return a.start0 + (a.start ? a.start[b] : 0);
+}
+
+// Partial results of a chunk: key heads [unit0, unit0 + units) of all items (unit = item *
+// kv_heads + key head) and queries [t0, t0 + nt).  Row = (unit, query, head of the group); every
+// row has `keep` partials, one a kept block: `dim` values (float32, or for 16-bit types int16 in
+// 32767ths of a common factor) and (log2 of the sum of its weights, factor of the values over that
+// sum).
+struct ChunkArgs {
+  BlockArgs a;
+  const void *q, *k, *v;
+  const int32_t* ids;
+  void* part;
+  float2* meta;
+  int unit0, units, t0, nt;
+  // by block: pairs (query, slot) that keep it, list[start[u]...], in tiles of kTileRows rows
+  // (pairs * group heads), tiles[u] of them before block u = unit * blocks + block
+  const int32_t *list, *start, *tiles;
+};
+
+constexpr int kTileRows = 128;
+
+// Attention of a chunk's rows to each of their kept blocks, a partial result each.  `by_block`:
+// rows gathered by the block that they keep (list, start, tiles; `grid` workgroups share the
+// tiles), else a workgroup for each kept block of each query.
+void block_partials_f32(const ChunkArgs& c, bool by_block, int grid, hipStream_t st);
+void block_partials_f16(const ChunkArgs& c, bool by_block, int grid, hipStream_t st);
+void block_partials_bf16(const ChunkArgs& c, bool by_block, int grid, hipStream_t st);
+
+}  // namespace nnx

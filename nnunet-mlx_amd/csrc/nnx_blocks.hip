@@ -2,8 +2,9 @@
 // selection and the attention itself.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
-#include "nnx_elements.h"
+#include "nnx_blocks.h"
 
 namespace nnx {
 namespace {
@@ -11,15 +12,6 @@ namespace {
 constexpr int kMaxBlocks = 32768;
 constexpr int kMaxKeep = 256;
 constexpr float kTiny = 8.673617379884035e-19f;  // 2^-60
-
-struct BlockArgs {
-  int batch, queries, keys, heads, kv_heads, group, dim, block, blocks, keep, first, local, causal;
-  int64_t start0;
-  float scale;
-  int64_t qs[3], ks[3], vs[3], os[3], ms;
-  const int32_t *start, *lengths;
-  const uint8_t* mask;
-};
 
 void check_config(const nnx_block_config& c, const char* what, bool queries) {
   const std::string w = std::string(what) + ": ";
@@ -59,189 +51,464 @@ BlockArgs make_args(const nnx_block_config& c, const int32_t* start, const int32
   return a;
 }
 
-__device__ __forceinline__ int item_length(const BlockArgs& a, int b) {
-  return a.lengths ? min(max(a.lengths[b], 0), a.keys) : a.keys;
-}
-
-__device__ __forceinline__ int64_t item_start(const BlockArgs& a, int b) {
-  return a.start0 + (a.start ? a.start[b] : 0);
-}
-
 __device__ __forceinline__ float finite_or_zero(float v) { return fabsf(v) < INFINITY ? v : 0.f; }
 
-// A workgroup of 128 threads a block of keys, a thread a channel.
-template <class T>
-__global__ __launch_bounds__(128) void summarize_kernel(BlockArgs a, const T* k, int first,
+// ---- summaries -------------------------------------------------------------------------
+
+// A workgroup a block of keys, L = dim / 8 threads a key, each 8 channels of every RP-th key.  The
+// keys are read once for the largest magnitude and stay in registers for the whole-number sums.
+template <class T, int BK>
+__global__ __launch_bounds__(256) void summarize_kernel(BlockArgs a, const T* k, int first,
                                                         int8_t* codes, float* scales) {
-  __shared__ float top_lds[2];
-  __shared__ int most_lds[2];
-  const int j = first + blockIdx.x, g = blockIdx.y, b = blockIdx.z, d = threadIdx.x;
-  const int lo = j * a.block, hi = min(lo + a.block, item_length(a, b));
-  const T* kb = k + b * a.ks[0] + g * a.ks[2];
-  const bool has = d < a.dim;
+  constexpr int EACH = BK / 16;  // of 16 threads a key; fewer channels leave fewer keys a thread
+  __shared__ float top_lds[4];
+  __shared__ int sums[128], most_lds[4], count_lds[4];
+  const int j = first + blockIdx.x, g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int lanes = a.dim / 8, per = 256 / lanes, sub = tid / lanes, d = (tid - sub * lanes) * 8;
+  const int lo = j * BK, hi = min(lo + BK, item_length(a, b));
+  const T* kb = k + b * a.ks[0] + g * a.ks[2] + d;
+  const uint8_t* mask = a.mask ? a.mask + b * a.ms : nullptr;
+  if (tid < 128) sums[tid] = 0;
+  Vec<T, 8> v[EACH];
+  bool in[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int64_t key = lo + sub + i * per;
+    in[i] = sub < per && sub + i * per < BK && key < hi && (!mask || mask[key]);
+    if (in[i]) v[i] = load_vec<8>(kb + key * a.ks[1]);
+  }
   int count = 0;
   float top = 0.f;
-  for (int i = lo; i < hi; ++i) {
-    if (a.mask && !a.mask[b * a.ms + i]) continue;
-    ++count;
-    if (has) top = fmaxf(top, fabsf(finite_or_zero(to_float(kb[i * a.ks[1] + d]))));
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    if (!in[i]) continue;
+    count += d == 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(finite_or_zero(to_float(v[i].v[e]))));
   }
-  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if (d % 64 == 0) top_lds[d / 64] = top;
+  const auto larger = [](float x, float y) { return fmaxf(x, y); };
+  top = lanes_reduce<64>(top, larger);
+  count = (int)lanes_reduce<64>((float)count, [](float x, float y) { return x + y; });
+  if (tid % 64 == 0) top_lds[tid / 64] = top, count_lds[tid / 64] = count;
   __syncthreads();
-  top = fmaxf(top_lds[0], top_lds[1]);
-  int sum = 0;
-  if (has && top >= kTiny) {
+  top = fmaxf(fmaxf(top_lds[0], top_lds[1]), fmaxf(top_lds[2], top_lds[3]));
+  count = count_lds[0] + count_lds[1] + count_lds[2] + count_lds[3];
+  if (top >= kTiny && sub < per) {
     const float up = __fdiv_rn(32767.f, top);
-    for (int i = lo; i < hi; ++i) {
-      if (a.mask && !a.mask[b * a.ms + i]) continue;
-      sum += (int)rintf(finite_or_zero(to_float(kb[i * a.ks[1] + d])) * up);
+    int s[8] = {};
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (!in[i]) continue;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += (int)rintf(finite_or_zero(to_float(v[i].v[e])) * up);
     }
+    // whole numbers: the order of these additions does not show
+#pragma unroll
+    for (int e = 0; e < 8; ++e) atomicAdd(&sums[d + e], s[e]);
   }
-  int most = abs(sum);
-  for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
-  if (d % 64 == 0) most_lds[d / 64] = most;
   __syncthreads();
-  most = max(most_lds[0], most_lds[1]);
+  const int sum = tid < a.dim ? sums[tid] : 0;
+  // below 2^24: exact as floats
+  const float most4 = lanes_reduce<64>((float)abs(sum), larger);
+  if (tid % 64 == 0) most_lds[tid / 64] = (int)most4;
+  __syncthreads();
+  const int most = max(most_lds[0], most_lds[1]);
   const int64_t at = ((int64_t)b * a.kv_heads + g) * a.blocks + j;
-  if (has) {
+  if (tid < a.dim) {
     const float down = most ? __fdiv_rn(127.f, (float)most) : 0.f;
-    codes[at * a.dim + d] = (int8_t)(int)rintf((float)sum * down);
+    codes[at * a.dim + tid] = (int8_t)(int)rintf((float)sum * down);
   }
-  if (d == 0) {
+  if (tid == 0) {
     scales[at] = count == 0 ? -1.f
                  : most == 0 ? 0.f
                              : __fdiv_rn(top, 4161409.f * (float)count) * (float)most;
   }
 }
 
-// A workgroup a query and key head: all scores in LDS, then `keep` times the best.
-template <class T>
-__global__ __launch_bounds__(256) void select_kernel(BlockArgs a, const T* q, const int8_t* codes,
-                                                     const float* scales, int32_t* ids) {
-  extern __shared__ float score[];  // blocks
-  __shared__ int8_t qc[128];
-  __shared__ float qtop;
-  __shared__ float best_v[4];
-  __shared__ int best_i[4];
-  const int t = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
-  const int64_t at = (item_start(a, b) + t) / a.block;
-  const int64_t unit = (int64_t)b * a.kv_heads + g;
-  int32_t* row = ids + (((int64_t)b * a.queries + t) * a.kv_heads + g) * a.keep;
-  for (int j = threadIdx.x; j < a.blocks; j += 256) score[j] = -INFINITY;
-  for (int h = 0; h < a.group; ++h) {
-    const T* qr = q + b * a.qs[0] + t * a.qs[1] + (g * a.group + h) * a.qs[2];
-    __syncthreads();
-    if (threadIdx.x < 64) {
-      const int d = threadIdx.x;
-      const float v0 = d < a.dim ? finite_or_zero(to_float(qr[d])) : 0.f;
-      const float v1 = d + 64 < a.dim ? finite_or_zero(to_float(qr[d + 64])) : 0.f;
-      float top = fmaxf(fabsf(v0), fabsf(v1));
-      for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-      const float up = top < kTiny ? 0.f : __fdiv_rn(127.f, top);
-      qc[d] = (int8_t)(int)rintf(v0 * up);
-      qc[d + 64] = (int8_t)(int)rintf(v1 * up);
-      if (d == 0) qtop = top < kTiny ? 1.f : top;
+// ---- selection -------------------------------------------------------------------------
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// A wave writes the kept blocks of one row of scores (in LDS): every +inf, then the highest finite
+// ones, equal ones by the lower index; never -inf.  256 bins between the lowest and the highest
+// find the bin in which the last kept score lies; only that bin's scores are then compared.
+__device__ void select_row(const float* score, int blocks, int keep, uint32_t* bins, int32_t* out) {
+  const int lane = threadIdx.x % 64;
+  const auto larger = [](float x, float y) { return fmaxf(x, y); };
+  float lo = INFINITY, hi = -INFINITY;
+  int forced = 0, finite = 0;
+  for (int j = lane; j < blocks; j += 64) {
+    const float v = score[j];
+    const bool top = v == INFINITY, usable = fabsf(v) < INFINITY;
+    forced += __popcll(__ballot(top));
+    finite += __popcll(__ballot(usable));
+    lo = fminf(lo, usable ? v : lo);
+    hi = fmaxf(hi, usable ? v : hi);
+  }
+  // lanes past the end took part in fewer ballots; lane 0 in all
+  forced = __builtin_amdgcn_readfirstlane(forced);
+  finite = __builtin_amdgcn_readfirstlane(finite);
+  float cut = -INFINITY;  // kept: above cut, and the first `ties` that equal it
+  int ties = 0;
+  if (forced >= keep) {
+    cut = INFINITY;
+    ties = keep;
+  } else if (forced + finite > keep) {
+    lo = -lanes_reduce<64>(-lo, larger);
+    hi = lanes_reduce<64>(hi, larger);
+    const float step = 255.f / (hi - lo);
+    const auto bin_of = [&](float v) { return min(max((int)((v - lo) * step), 0), 255); };
+    *(uint4*)&bins[4 * lane] = make_uint4(0, 0, 0, 0);
+    __builtin_amdgcn_wave_barrier();
+    for (int j = lane; j < blocks; j += 64) {
+      const float v = score[j];
+      if (fabsf(v) < INFINITY) atomicAdd(&bins[bin_of(v)], 1u);
     }
-    __syncthreads();
-    for (int j = threadIdx.x; j < a.blocks; j += 256) {
-      const int8_t* cb = codes + (unit * a.blocks + j) * a.dim;
-      int dot = 0;
-      for (int d = 0; d < a.dim; ++d) dot += (int)cb[d] * (int)qc[d];
-      const float sc = scales[unit * a.blocks + j];
-      float s = ((float)dot * qtop) * sc;
-      if (j < a.first || (j <= at && j > at - a.local)) s = INFINITY;
-      if (sc < 0.f || (a.causal && j > at)) s = -INFINITY;
-      score[j] = fmaxf(score[j], s);
+    __builtin_amdgcn_wave_barrier();
+    __threadfence_block();
+    // lane l: bins 255 - 4 l down to 252 - 4 l
+    const uint4 mine = *(const uint4*)&bins[252 - 4 * lane];
+    const int own = mine.x + mine.y + mine.z + mine.w;
+    int run = own;
+    for (int o = 1; o < 64; o *= 2) {
+      const int x = __shfl_up(run, o);
+      if (lane >= o) run += x;
+    }
+    const int need = keep - forced;  // at least 1, fewer than finite
+    const int at = __ffsll(__ballot(run >= need)) - 1;
+    int before = run - own, bin = 255 - 4 * lane;
+    if (before + (int)mine.w < need) {
+      before += mine.w, --bin;
+      if (before + (int)mine.z < need) {
+        before += mine.z, --bin;
+        if (before + (int)mine.y < need) before += mine.y, --bin;
+      }
+    }
+    bin = __shfl(bin, at);
+    int rest = need - __shfl(before, at);
+    // the bin's scores from the highest on, a value at a time
+    cut = INFINITY;
+    while (true) {
+      float best = -INFINITY;
+      int same = 0;
+      for (int j = lane; j < blocks; j += 64) {
+        const float v = score[j];
+        if (fabsf(v) < INFINITY && v < cut && bin_of(v) == bin) {
+          same = v > best ? 1 : same + (v == best);
+          best = fmaxf(best, v);
+        }
+      }
+      const float all = lanes_reduce<64>(best, larger);
+      same = best == all ? same : 0;
+      for (int o = 32; o; o >>= 1) same += __shfl_xor(same, o);
+      cut = all;
+      ties = rest;
+      if (same >= rest || all == -INFINITY) break;
+      rest -= same;
     }
   }
-  __syncthreads();
-  int found = 0;
-  for (; found < a.keep; ++found) {
-    float v = -INFINITY;
-    int at_i = a.blocks;
-    for (int j = threadIdx.x; j < a.blocks; j += 256) {
-      if (score[j] > v) v = score[j], at_i = j;
-    }
-    for (int o = 32; o; o >>= 1) {
-      const float ov = __shfl_xor(v, o);
-      const int oi = __shfl_xor(at_i, o);
-      if (ov > v || (ov == v && oi < at_i)) v = ov, at_i = oi;
-    }
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) best_v[threadIdx.x / 64] = v, best_i[threadIdx.x / 64] = at_i;
-    __syncthreads();
-    for (int w = 0; w < 4; ++w) {
-      if (best_v[w] > v || (best_v[w] == v && best_i[w] < at_i)) v = best_v[w], at_i = best_i[w];
-    }
-    if (v == -INFINITY) break;
-    // ascending: the kept ones stay marked and are written in order below
-    if (threadIdx.x == 0) score[at_i] = NAN;
-    __syncthreads();
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  int done = 0, tied = 0;
+  for (int j0 = 0; j0 < blocks; j0 += 64) {
+    const int j = j0 + lane;
+    const float v = j < blocks ? score[j] : -INFINITY;
+    const uint64_t equal = __ballot(v == cut && cut != -INFINITY);
+    const bool take = v > cut || (((equal >> lane) & 1) && tied + __popcll(equal & below) < ties);
+    const uint64_t taken = __ballot(take);
+    const int to = done + __popcll(taken & below);
+    if (take && to < keep) out[to] = j;
+    tied += __popcll(equal);
+    done += __popcll(taken);
   }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int n = 0;
-    for (int j = 0; j < a.blocks && n < found; ++j) {
-      if (score[j] != score[j]) row[n++] = j;
-    }
-    for (; n < a.keep; ++n) row[n] = -1;
-  }
+  for (int i = min(done, keep) + lane; i < keep; i += 64) out[i] = -1;
 }
 
-// A wave a query row: running maximum and sum over 64 keys at a time, a lane a key.
+// `rows` <= 16 queries of one item and key head: their scores against 16 blocks at a time by 8-bit
+// products in whole numbers (a query's codes are formed in the registers that feed them), kept
+// in LDS; then a wave a query picks.  Heads that share the key head are taken HEADS at a time
+// and meet in the largest score.
 template <class T>
-__global__ __launch_bounds__(64) void attention_kernel(BlockArgs a, const T* q, const T* k,
-                                                       const T* v, const int32_t* ids, T* out) {
-  __shared__ float qv[128];
-  const int lane = threadIdx.x;
-  const int h = blockIdx.y, b = blockIdx.z, g = h / a.group;
-  const int t = blockIdx.x;
-  const T* qr = q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2];
-  for (int d = lane; d < a.dim; d += 64) qv[d] = to_float(qr[d]);
-  __syncthreads();
-  const int length = item_length(a, b);
-  const int64_t pos = item_start(a, b) + t;
-  const int32_t* row = ids + (((int64_t)b * a.queries + t) * a.kv_heads + g) * a.keep;
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int s = 0; s < a.keep; ++s) {
-    const int j = row[s];
-    if (j < 0 || j >= a.blocks) continue;
-    for (int base = j * a.block; base < min((j + 1) * a.block, length); base += 64) {
-      const int i = base + lane;
-      bool see = i < min((j + 1) * a.block, length) && (!a.causal || i <= pos);
-      if (see && a.mask) see = a.mask[b * a.ms + i] != 0;
-      float x = -INFINITY;
-      if (see) {
-        const T* kr = k + b * a.ks[0] + i * a.ks[1] + g * a.ks[2];
-        float dot = 0.f;
-        for (int d = 0; d < a.dim; ++d) dot = fmaf(qv[d], to_float(kr[d]), dot);
-        x = dot * a.scale;
+__global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, const int8_t* codes,
+                                                     const float* scales, int32_t* ids, int rows,
+                                                     int pitch) {
+  constexpr int HEADS = 4, WAVES = 8;
+  extern __shared__ __attribute__((aligned(16))) float score[];  // rows x pitch, then bins
+  uint32_t* bins = (uint32_t*)(score + rows * pitch);
+  const int t0 = blockIdx.x * rows, g = blockIdx.y, b = blockIdx.z;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, quad = lane / 16;
+  const int t = t0 + col;
+  const bool live = col < rows && t < a.queries;
+  const int64_t unit = (int64_t)b * a.kv_heads + g;
+  const int64_t own = (item_start(a, b) + t) / a.block;
+  const int8_t* cu = codes + unit * a.blocks * a.dim;
+  const float* su = scales + unit * a.blocks;
+  for (int h0 = 0; h0 < a.group; h0 += HEADS) {
+    i32x4 qc[HEADS][2];
+    float top[HEADS];
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      Vec<T, 8> v[4];
+      float m = 0.f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int d = (s / 2) * 64 + quad * 16 + (s % 2) * 8;
+        v[s] = Vec<T, 8>{};
+        if (live && h0 + h < a.group && d < a.dim)
+          v[s] = load_vec<8>(q + b * a.qs[0] + t * a.qs[1] + (g * a.group + h0 + h) * a.qs[2] + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(finite_or_zero(to_float(v[s].v[e]))));
       }
-      float top = x;
-      for (int w = 32; w; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
-      const float mn = fmaxf(m, top);
-      if (mn == -INFINITY) continue;
-      const float p = see ? expf(x - mn) : 0.f;
-      float sum = p;
-      for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w);
-      const float old = expf(m - mn);
-      l = l * old + sum;
-      o0 *= old, o1 *= old;
-      m = mn;
-      for (int w = 0; w < 64; ++w) {
-        const float pw = __shfl(p, w);
-        if (pw == 0.f) continue;  // unseen values are never read
-        const T* vr = v + b * a.vs[0] + (int64_t)(base + w) * a.vs[1] + g * a.vs[2];
-        if (lane < a.dim) o0 = fmaf(pw, to_float(vr[lane]), o0);
-        if (lane + 64 < a.dim) o1 = fmaf(pw, to_float(vr[lane + 64]), o1);
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      const float up = m < kTiny ? 0.f : __fdiv_rn(127.f, m);
+      top[h] = m < kTiny ? 1.f : m;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint32_t word = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            word |= ((uint32_t)(int)rintf(finite_or_zero(to_float(v[s].v[4 * w + e])) * up) & 255u) << (8 * e);
+          qc[h][s / 2][(s % 2) * 2 + w] = (int)word;
+        }
+    }
+    for (int j0 = wave * 16; j0 < a.blocks; j0 += WAVES * 16) {
+      i32x4 kc[2] = {};
+      const int8_t* row = cu + (int64_t)min(j0 + col, a.blocks - 1) * a.dim;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int d = (s / 2) * 64 + quad * 16 + (s % 2) * 8;
+        if (d < a.dim) {
+          int w[2];
+          __builtin_memcpy(w, row + d, 8);
+          kc[s / 2][(s % 2) * 2] = w[0];
+          kc[s / 2][(s % 2) * 2 + 1] = w[1];
+        }
+      }
+      float scale[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) scale[r] = su[min(j0 + quad * 4 + r, a.blocks - 1)];
+      float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int h = 0; h < HEADS; ++h) {
+        if (h0 + h >= a.group) break;
+        i32x4 dot = {0, 0, 0, 0};
+        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[0], qc[h][0], dot, 0, 0, 0);
+        if (a.dim > 64) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[1], qc[h][1], dot, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) best[r] = fmaxf(best[r], ((float)dot[r] * top[h]) * scale[r]);
+      }
+      if (col < rows) {
+        float4* to = (float4*)&score[col * pitch + j0 + quad * 4];
+        if (h0) {
+          const float4 z = *to;
+          best[0] = fmaxf(best[0], z.x), best[1] = fmaxf(best[1], z.y);
+          best[2] = fmaxf(best[2], z.z), best[3] = fmaxf(best[3], z.w);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = j0 + quad * 4 + r;
+          if (j < a.first || (j <= own && j > own - a.local)) best[r] = INFINITY;
+          if (scale[r] < 0.f || (a.causal && j > own)) best[r] = -INFINITY;
+        }
+        *to = make_float4(best[0], best[1], best[2], best[3]);
       }
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  T* orow = out + b * a.os[0] + t * a.os[1] + h * a.os[2];
-  if (lane < a.dim) orow[lane] = from_float<T>(o0 * inv);
-  if (lane + 64 < a.dim) orow[lane + 64] = from_float<T>(o1 * inv);
+  __syncthreads();
+  for (int r = wave; r < rows && t0 + r < a.queries; r += WAVES)
+    select_row(score + r * pitch, a.blocks, a.keep, bins + wave * 256,
+               ids + (((int64_t)b * a.queries + t0 + r) * a.kv_heads + g) * a.keep);
+}
+
+// ---- the attention ---------------------------------------------------------------------
+//
+// Rows that keep the same block need the same keys and values, and rows near each other mostly
+// keep different ones.  So the pairs (query, kept block) are gathered by block: dense tiles of
+// rows against a block that stays in LDS, one partial softmax a pair, and a last pass that joins
+// each row's partials.  Few pairs skip the gathering: a workgroup each.
+
+// Pairs of a chunk in groups of `per` queries of one unit (grid: groups, units).  Counts by block
+// in LDS; each group takes its range of every block's list by one addition to the block's total.
+// The order of groups in a list is left to chance and shows in no result: a row's partial does not
+// depend on its neighbours in a tile.
+__global__ __launch_bounds__(256) void count_pairs_kernel(ChunkArgs c, int per, int32_t* total,
+                                                          int32_t* base, int32_t* rank) {
+  extern __shared__ int32_t hist[];
+  const BlockArgs& a = c.a;
+  const int unit = blockIdx.y, t_lo = blockIdx.x * per, t_hi = min(t_lo + per, c.nt);
+  const int b = (c.unit0 + unit) / a.kv_heads, g = c.unit0 + unit - b * a.kv_heads;
+  for (int j = threadIdx.x; j < a.blocks; j += 256) hist[j] = 0;
+  __syncthreads();
+  const int32_t* ids = c.ids + (((int64_t)b * a.queries + c.t0) * a.kv_heads + g) * a.keep;
+  for (int e = t_lo * a.keep + threadIdx.x; e < t_hi * a.keep; e += 256) {
+    const int t = e / a.keep, s = e - t * a.keep;
+    const int j = ids[(int64_t)t * a.kv_heads * a.keep + s];
+    if (j >= 0 && j < a.blocks) rank[(int64_t)unit * c.nt * a.keep + e] = atomicAdd(&hist[j], 1);
+  }
+  __syncthreads();
+  int32_t* mine = base + ((int64_t)unit * gridDim.x + blockIdx.x) * a.blocks;
+  for (int j = threadIdx.x; j < a.blocks; j += 256)
+    if (hist[j]) mine[j] = atomicAdd(&total[unit * a.blocks + j], hist[j]);
+}
+
+// Where each block's list starts, and its tiles: running sums over n totals, by one workgroup.
+__global__ __launch_bounds__(1024) void scan_pairs_kernel(const int32_t* total, int n, int group,
+                                                          int32_t* start, int32_t* tiles) {
+  __shared__ int2 part[16];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  int2 before = make_int2(0, 0);
+  for (int at = 0; at < n; at += 4096) {
+    int2 mine[4], sum = make_int2(0, 0);
+    const int i0 = at + threadIdx.x * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pairs = i0 + i < n ? total[i0 + i] : 0;
+      mine[i] = sum;
+      sum.x += pairs;
+      sum.y += (int)(((int64_t)pairs * group + kTileRows - 1) / kTileRows);
+    }
+    int2 run = sum;
+    for (int o = 1; o < 64; o *= 2) {
+      const int x = __shfl_up(run.x, o), y = __shfl_up(run.y, o);
+      if (lane >= o) run.x += x, run.y += y;
+    }
+    __syncthreads();
+    if (lane == 63) part[wave] = run;
+    __syncthreads();
+    int2 offset = before;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) offset.x += part[w].x, offset.y += part[w].y;
+      before.x += part[w].x, before.y += part[w].y;
+    }
+    offset.x += run.x - sum.x, offset.y += run.y - sum.y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i0 + i < n) start[i0 + i] = offset.x + mine[i].x, tiles[i0 + i] = offset.y + mine[i].y;
+  }
+  if (threadIdx.x == 0) start[n] = before.x, tiles[n] = before.y;
+}
+
+__global__ __launch_bounds__(256) void place_pairs_kernel(ChunkArgs c, int per, int groups,
+                                                          const int32_t* base, const int32_t* rank,
+                                                          int32_t* list) {
+  const BlockArgs& a = c.a;
+  const int unit = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= c.nt * a.keep) return;
+  const int b = (c.unit0 + unit) / a.kv_heads, g = c.unit0 + unit - b * a.kv_heads;
+  const int t = e / a.keep, s = e - t * a.keep;
+  const int j = c.ids[(((int64_t)b * a.queries + c.t0 + t) * a.kv_heads + g) * a.keep + s];
+  if (j < 0 || j >= a.blocks) return;
+  const int from = base[((int64_t)unit * groups + t / per) * a.blocks + j];
+  list[c.start[unit * a.blocks + j] + from + rank[(int64_t)unit * c.nt * a.keep + e]] = e;
+}
+
+// out = sum_s w_s O_s / sum_s w_s with w_s = 2^(log2 sum_s - largest), O_s a partial under its
+// factor.  dim / 8 lanes a row, `share` groups of lanes a row where rows are few.
+template <class T>
+__global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out, int share) {
+  using P = typename std::conditional<sizeof(T) == 2, int16_t, float>::type;
+  constexpr float kUnit = sizeof(T) == 2 ? 1.f / 32767.f : 1.f;
+  __shared__ float sums[256][9];
+  const BlockArgs& a = c.a;
+  const int lanes = a.dim / 8, sub = threadIdx.x / lanes, u = threadIdx.x - sub * lanes;
+  const int each = 256 / (lanes * share);  // rows of a workgroup
+  const int own = sub / share, part0 = sub - own * share;
+  const int64_t row = (int64_t)blockIdx.x * each + own, rows = (int64_t)c.units * c.nt * a.group;
+  const bool live = own < each && row < rows;
+  float o[8] = {}, l = 0.f;
+  int64_t ut = 0;
+  int unit = 0, t = 0, h = 0, b = 0, g = 0;
+  if (live) {
+    ut = row / a.group;
+    h = (int)(row - ut * a.group);
+    unit = (int)(ut / c.nt);
+    t = (int)(ut - (int64_t)unit * c.nt);
+    b = (c.unit0 + unit) / a.kv_heads;
+    g = c.unit0 + unit - b * a.kv_heads;
+    const int32_t* ids = c.ids + (((int64_t)b * a.queries + c.t0 + t) * a.kv_heads + g) * a.keep;
+    const float2* meta = c.meta + row * a.keep;
+    const P* part = (const P*)c.part + row * a.keep * a.dim + 8 * u;
+    float top = -INFINITY;
+    for (int s = 0; s < a.keep; ++s)
+      if ((unsigned)ids[s] < (unsigned)a.blocks) top = fmaxf(top, meta[s].x);
+    if (top == -INFINITY) top = 0.f;
+#pragma unroll 4
+    for (int s = part0; s < a.keep; s += share) {
+      if ((unsigned)ids[s] >= (unsigned)a.blocks) continue;
+      const float2 m = meta[s];
+      const Vec<P, 8> x = load_vec<8>(part + (int64_t)s * a.dim);
+      const float w = __builtin_amdgcn_exp2f(m.x - top), f = w * m.y * kUnit;
+      l += w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = fmaf(f, (float)x.v[i], o[i]);
+    }
+  }
+  if (share > 1) {
+    for (int i = 0; i < 8; ++i) sums[threadIdx.x][i] = o[i];
+    sums[threadIdx.x][8] = l;
+    __syncthreads();
+    if (!live || part0) return;
+    for (int p = 1; p < share; ++p) {
+      for (int i = 0; i < 8; ++i) o[i] += sums[threadIdx.x + p * lanes][i];
+      l += sums[threadIdx.x + p * lanes][8];
+    }
+  }
+  if (!live) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  Vec<T, 8> r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = from_float<T>(o[i] * inv);
+  store_vec(out + b * a.os[0] + (c.t0 + t) * a.os[1] + (int64_t)(g * a.group + h) * a.os[2] + 8 * u, r);
+}
+
+// One pass's work and where it lies in the workspace.  Chunks hold whole units where those fit the
+// budget, else parts of one unit's queries.
+constexpr size_t kPartialBudget = (size_t)1 << 30;
+constexpr int64_t kDirectPairs = 8192;
+
+struct AttentionPlan {
+  bool by_block;
+  int units, nt;     // of a chunk
+  int per, groups;   // queries of a counting group, groups of a unit
+  int64_t pairs;     // of a chunk
+  size_t total, base, start, tiles, rank, list, meta, part, bytes;
+};
+
+AttentionPlan make_plan(const nnx_block_config& c) {
+  AttentionPlan p;
+  const int64_t group = c.heads / c.kv_heads, blocks = ceil_div(c.keys, c.block);
+  const size_t row = (size_t)c.keep * (8 + (size_t)c.head_dim * type_bytes(c.type));
+  const int64_t all_units = (int64_t)c.batch * c.kv_heads;
+  const int64_t query = group * row;  // bytes of a query's partials in one unit
+  p.nt = (int)std::max<int64_t>(1, std::min<int64_t>(c.queries, kPartialBudget / query));
+  p.units = p.nt < c.queries
+                ? 1
+                : (int)std::max<int64_t>(1, std::min<int64_t>(all_units, kPartialBudget / (query * p.nt)));
+  // counts and tiles are 32-bit, and a chunk's units a grid axis
+  p.units = (int)std::min<int64_t>(p.units, std::max<int64_t>(1, std::min<int64_t>(65535, (1 << 30) / blocks)));
+  p.pairs = (int64_t)p.units * p.nt * c.keep;
+  p.by_block = all_units * c.queries * c.keep > kDirectPairs;
+  p.per = (int)std::min<int64_t>(p.nt, ceil_div(std::max<int64_t>(4096, 2 * blocks), c.keep));
+  p.groups = (int)ceil_div(p.nt, p.per);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  const size_t lists = p.by_block ? (size_t)p.units * blocks : 0;
+  p.total = take(lists * 4);
+  p.base = take(lists * p.groups * 4);
+  p.start = take((lists + 1) * 4);
+  p.tiles = take((lists + 1) * 4);
+  p.rank = take(p.by_block ? p.pairs * 4 : 0);
+  p.list = take(p.by_block ? p.pairs * 4 : 0);
+  p.meta = take((size_t)p.pairs * group * 8);
+  p.part = take((size_t)p.pairs * group * c.head_dim * type_bytes(c.type));
+  p.bytes = at;
+  return p;
 }
 
 }  // namespace
@@ -259,8 +526,15 @@ void block_summarize(const nnx_block_config& c, const void* k, const int32_t* le
   ProfScope prof("block_summarize", 3.0 * n, n * type_bytes(c.type), st);
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    summarize_kernel<T><<<dim3(blocks, c.kv_heads, c.batch), 128, 0, st>>>(a, (const T*)k, first_block,
-                                                                           codes, scales);
+    const dim3 grid(blocks, c.kv_heads, c.batch);
+    auto go = [&](auto bk) {
+      summarize_kernel<T, decltype(bk)::value><<<grid, 256, 0, st>>>(a, (const T*)k, first_block, codes, scales);
+    };
+    using std::integral_constant;
+    if (c.block == 16) return go(integral_constant<int, 16>{});
+    if (c.block == 32) return go(integral_constant<int, 32>{});
+    if (c.block == 64) return go(integral_constant<int, 64>{});
+    go(integral_constant<int, 128>{});
   });
   launch_check("block_summarize");
 }
@@ -270,13 +544,16 @@ void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
   check_config(c, "block selection", true);
   require(q && codes && scales && ids, "block selection: null pointer");
   const BlockArgs a = make_args(c, start, nullptr, nullptr);
-  const double rows = (double)c.batch * c.queries * c.heads;
-  ProfScope prof("block_select", 2.0 * rows * a.blocks * c.head_dim,
-                 rows * c.head_dim * type_bytes(c.type), st);
+  const double products = (double)c.batch * c.queries * c.heads * c.head_dim;
+  ProfScope prof("block_select", 2.0 * products * a.blocks, products * type_bytes(c.type), st);
+  // As many queries a workgroup as the products take, while their scores fit the LDS.
+  const int pitch = (int)ceil_div(a.blocks, 16) * 16 + 4;
+  int rows = 16;
+  while (rows > 1 && (size_t)rows * pitch * 4 + 8192 > 147456) rows /= 2;
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    select_kernel<T><<<dim3(c.queries, c.kv_heads, c.batch), 256, a.blocks * sizeof(float), st>>>(
-        a, (const T*)q, codes, scales, ids);
+    select_kernel<T><<<dim3((unsigned)ceil_div(c.queries, rows), c.kv_heads, c.batch), 512,
+                       rows * pitch * sizeof(float) + 8192, st>>>(a, (const T*)q, codes, scales, ids, rows, pitch);
   });
   launch_check("block_select");
 }
@@ -287,7 +564,7 @@ size_t block_attention_workspace(const nnx_block_config& c) {
   } catch (const Error&) {
     return 0;
   }
-  return 16;
+  return make_plan(c).bytes;
 }
 
 void block_attention(const nnx_block_config& c, const void* q, const void* k, const void* v,
@@ -295,16 +572,65 @@ void block_attention(const nnx_block_config& c, const void* q, const void* k, co
                      const uint8_t* mask, void* out, void* ws, size_t ws_bytes, hipStream_t st) {
   check_config(c, "block attention", true);
   require(q && k && v && ids && out && ws, "block attention: null pointer");
-  require(ws_bytes >= block_attention_workspace(c), "block attention: workspace too small");
-  const BlockArgs a = make_args(c, start, lengths, mask);
-  const double pairs = (double)c.batch * c.queries * c.heads * c.keep * c.block;
-  ProfScope prof("block_attention", 4.0 * pairs * c.head_dim, 0.0, st);
-  with_type(c.type, [&](auto t) {
-    using T = decltype(t);
-    attention_kernel<T><<<dim3(c.queries, c.heads, c.batch), 64, 0, st>>>(
-        a, (const T*)q, (const T*)k, (const T*)v, ids, (T*)out);
-  });
-  launch_check("block_attention");
+  const AttentionPlan p = make_plan(c);
+  require(ws_bytes >= p.bytes && reinterpret_cast<uintptr_t>(ws) % 16 == 0,
+          "block attention: the workspace is too small or not 16-byte aligned");
+  ChunkArgs k0;
+  k0.a = make_args(c, start, lengths, mask);
+  const BlockArgs& a = k0.a;
+  char* w = (char*)ws;
+  auto at = [&](size_t offset) { return (int32_t*)(w + offset); };
+  k0.q = q, k0.k = k, k0.v = v, k0.ids = ids;
+  k0.part = w + p.part;
+  k0.meta = (float2*)(w + p.meta);
+  k0.list = at(p.list), k0.start = at(p.start), k0.tiles = at(p.tiles);
+  const int all_units = c.batch * c.kv_heads;
+  const double flops = 4.0 * c.heads / c.kv_heads * c.keep * c.block * c.head_dim;
+  for (int u = 0; u < all_units; u += p.units) {
+    for (int t = 0; t < c.queries; t += p.nt) {
+      ChunkArgs m = k0;
+      m.unit0 = u, m.units = std::min(p.units, all_units - u);
+      m.t0 = t, m.nt = std::min(p.nt, c.queries - t);
+      const int64_t pairs = (int64_t)m.units * m.nt * c.keep;
+      int grid = (int)pairs;
+      if (p.by_block) {
+        const int lists = m.units * a.blocks, groups = (int)ceil_div(m.nt, p.per);
+        ProfScope prof("block_lists", 0.0, 16.0 * pairs, st);
+        fill_zero(w + p.total, (size_t)lists * 4, st);
+        count_pairs_kernel<<<dim3(groups, m.units), 256, a.blocks * 4, st>>>(
+            m, p.per, at(p.total), at(p.base), at(p.rank));
+        launch_check("count_pairs");
+        scan_pairs_kernel<<<1, 1024, 0, st>>>(at(p.total), lists, a.group, at(p.start), at(p.tiles));
+        launch_check("scan_pairs");
+        place_pairs_kernel<<<dim3((unsigned)ceil_div((int64_t)m.nt * c.keep, 256), m.units), 256, 0, st>>>(
+            m, p.per, groups, at(p.base), at(p.rank), at(p.list));
+        launch_check("place_pairs");
+        grid = (int)std::min<int64_t>(ceil_div(pairs * a.group, kTileRows) + lists, 4 * compute_units());
+      }
+      {
+        ProfScope prof("block_partials", flops * m.units * m.nt, 0.0, st);
+        if (c.type == NNX_TYPE_F32) {
+          block_partials_f32(m, p.by_block, grid, st);
+        } else if (c.type == NNX_TYPE_F16) {
+          block_partials_f16(m, p.by_block, grid, st);
+        } else {
+          block_partials_bf16(m, p.by_block, grid, st);
+        }
+      }
+      const int64_t rows = (int64_t)m.units * m.nt * a.group;
+      const int lanes = a.dim / 8;
+      // groups of lanes a row: more while rows are too few for the CUs
+      int share = 1;
+      while (share * 2 * lanes <= 256 && share * 2 <= c.keep && rows * lanes * share < 65536) share *= 2;
+      ProfScope prof("block_join", 2.0 * rows * c.keep * c.head_dim,
+                     (double)rows * c.keep * (8 + c.head_dim * type_bytes(c.type)), st);
+      with_type(c.type, [&](auto z) {
+        using T = decltype(z);
+        join_partials_kernel<T><<<(unsigned)ceil_div(rows, 256 / (lanes * share)), 256, 0, st>>>(m, (T*)out, share);
+      });
+      launch_check("block_join");
+    }
+  }
 }
 
 }  // namespace nnx

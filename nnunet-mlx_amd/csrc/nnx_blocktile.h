@@ -1,0 +1,379 @@
+// Attention of query rows to one block of keys, the partial results of attention over selected
+// blocks; included by one source a type.
+#pragma once
+
+#include <type_traits>
+
+#include "nnx_blocks.h"
+
+namespace nnx {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// One of the two lane halves' values in both: {lower half's, upper half's}.
+__device__ __forceinline__ float2 both_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <class T>
+using Frag = T __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x16 mfma(Frag<f16> a, Frag<f16> b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(Frag<bf16> a, Frag<bf16> b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(float a, float b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+
+// Tile geometry.  Rows of keys and values lie in LDS in 16-byte chunks, chunk c of row r at place
+// c ^ turn(r), so that 16 lanes that read the same chunk of 16 rows meet all banks.
+template <class T, int DP, int BK>
+struct Tile {
+  static constexpr int CH = 16 / sizeof(T);        // elements of a chunk
+  static constexpr int CHUNKS = DP / CH;           // chunks of a row
+  static constexpr int ROWS = BK < 32 ? 32 : BK;   // rows of keys that the products read
+  static constexpr int KT = ROWS / 32;             // 32-key tiles
+  static constexpr int REGS = BK < 32 ? 8 : 16;    // scores of a 32-key tile that a lane uses
+  static constexpr int ROW_BYTES = DP * sizeof(T);
+  static constexpr int PER = ROW_BYTES >= 256 ? 1 : 256 / ROW_BYTES;  // rows in 256 bytes
+  static constexpr int TURNS = CHUNKS & -CHUNKS;   // a power of two that divides CHUNKS
+  static constexpr size_t LDS = (size_t)2 * ROWS * ROW_BYTES + ROWS * sizeof(float);
+  static __device__ __forceinline__ int at(int row, int chunk) {
+    const int turn = (row / PER) & (TURNS - 1);
+    return row * DP + (chunk ^ turn) * CH;
+  }
+};
+
+// The block's keys and values into LDS, zeros for those that are not valid, and what their scores
+// start from: 0, or -inf for keys that are not valid.  Whether any value is not finite (16-bit types).
+template <class T, int DP, int BK>
+__device__ __forceinline__ bool stage_block(const ChunkArgs& c, int b, int g, int j, T* lk, T* lv,
+                                            float* bias) {
+  using G = Tile<T, DP, BK>;
+  const int length = item_length(c.a, b), first = j * BK;
+  const T* k = (const T*)c.k + b * c.a.ks[0] + g * c.a.ks[2];
+  const T* v = (const T*)c.v + b * c.a.vs[0] + g * c.a.vs[2];
+  const uint8_t* mask = c.a.mask ? c.a.mask + b * c.a.ms : nullptr;
+  constexpr int N = BK * G::CHUNKS, EACH = (N + 255) / 256;
+  Vec<T, G::CH> kr[EACH], vr[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int n = threadIdx.x + i * 256, row = n / G::CHUNKS, d = (n % G::CHUNKS) * G::CH;
+    const int64_t key = first + row;
+    kr[i] = vr[i] = Vec<T, G::CH>{};
+    if (n < N && d < c.a.dim && key < length && (!mask || mask[key])) {
+      kr[i] = load_vec<G::CH>(k + key * c.a.ks[1] + d);
+      vr[i] = load_vec<G::CH>(v + key * c.a.vs[1] + d);
+    }
+  }
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int n = threadIdx.x + i * 256;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int e = 0; e < G::CH; ++e) odd |= !(fabsf(to_float(vr[i].v[e])) < INFINITY);
+    }
+    if (n < N) {
+      const int at = G::at(n / G::CHUNKS, n % G::CHUNKS);
+      *(Vec<T, G::CH>*)__builtin_assume_aligned(lk + at, 16) = kr[i];
+      *(Vec<T, G::CH>*)__builtin_assume_aligned(lv + at, 16) = vr[i];
+    }
+  }
+  if (threadIdx.x < BK) {
+    const int key = first + threadIdx.x;
+    bias[threadIdx.x] = key < length && (!mask || mask[key]) ? 0.f : -INFINITY;
+  }
+  return __syncthreads_or(odd);
+}
+
+// 32 query rows, a lane pair (l, l + 32) each: S^T = K Q^T leaves a row's scores in its two
+// lanes' registers, so the softmax needs one exchange between halves, and its weights are
+// already the second operand of O^T = V^T P^T (the order of keys is that of the registers; values
+// are read transposed to match).
+template <class T, int DP, int BK>
+__device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, const T* lv,
+                                            const float* bias, bool live, const T* q, int64_t last,
+                                            int first_key, float c2, bool negate, bool odd,
+                                            int64_t partial) {
+  using G = Tile<T, DP, BK>;
+  const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;
+  f32x16 acc[G::KT];
+#pragma unroll
+  for (int kt = 0; kt < G::KT; ++kt)
+#pragma unroll
+    for (int r = 0; r < G::REGS; r += 4) {
+      const float4 z = *(const float4*)&bias[kt * 32 + 2 * r + 4 * half];
+      acc[kt][r] = z.x, acc[kt][r + 1] = z.y, acc[kt][r + 2] = z.z, acc[kt][r + 3] = z.w;
+    }
+  if constexpr (G::REGS < 16) {
+#pragma unroll
+    for (int r = G::REGS; r < 16; ++r) acc[0][r] = 0.f;  // rows past the block, never used
+  }
+  if constexpr (sizeof(T) == 2) {
+    Frag<T> qf[DP / 16];
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      const int d = 16 * s + 8 * half;
+      qf[s] = Frag<T>{};
+      if (live && d < c.a.dim) __builtin_memcpy(&qf[s], q + d, 16);
+      if (negate) qf[s] = -qf[s];
+    }
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+      for (int kt = 0; kt < G::KT; ++kt)
+        acc[kt] = mfma(*(const Frag<T>*)(lk + G::at(kt * 32 + col, 2 * s + half)), qf[s], acc[kt]);
+  } else {
+#pragma unroll
+    for (int s = 0; s < DP / 8; ++s) {
+      const int d = 8 * s + 4 * half;
+      Vec<float, 4> qf{};
+      if (live && d < c.a.dim) qf = load_vec<4>((const float*)q + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf.v[i] = negate ? -qf.v[i] : qf.v[i];
+#pragma unroll
+      for (int kt = 0; kt < G::KT; ++kt) {
+        const float4 kf = *(const float4*)(lk + G::at(kt * 32 + col, 2 * s + half));
+        acc[kt] = mfma(kf.x, qf.v[0], acc[kt]);
+        acc[kt] = mfma(kf.y, qf.v[1], acc[kt]);
+        acc[kt] = mfma(kf.z, qf.v[2], acc[kt]);
+        acc[kt] = mfma(kf.w, qf.v[3], acc[kt]);
+      }
+    }
+  }
+  if (c.a.causal && __any(live && last < first_key + BK - 1)) {
+#pragma unroll
+    for (int kt = 0; kt < G::KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < G::REGS; ++r) {
+        const int key = first_key + kt * 32 + 8 * (r / 4) + 4 * half + r % 4;
+        if (key > last) acc[kt][r] = -INFINITY;
+      }
+  }
+  float m = -INFINITY;
+#pragma unroll
+  for (int kt = 0; kt < G::KT; ++kt)
+#pragma unroll
+    for (int r = 0; r < G::REGS; ++r) m = fmaxf(m, acc[kt][r]);
+  const float2 mh = both_halves(m);
+  m = fmaxf(mh.x, mh.y);
+  const float top = m == -INFINITY ? 0.f : m * c2;  // nothing seen: all weights 2^-inf
+  float l = 0.f;
+#pragma unroll
+  for (int kt = 0; kt < G::KT; ++kt)
+#pragma unroll
+    for (int r = 0; r < G::REGS; ++r) {
+      acc[kt][r] = __builtin_amdgcn_exp2f(fmaf(acc[kt][r], c2, -top));
+      l += acc[kt][r];
+    }
+  const float2 lh = both_halves(l);
+  l = lh.x + lh.y;
+  f32x16 o[DP / 32];
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < BK / 16; ++i) {
+      Frag<T> p;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) p[r] = from_float<T>(acc[i / 2][8 * (i % 2) + r]);
+      const int row = 16 * i + 4 * half + lane % 16 / 4;
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) {
+        const int d = dt * 32 + lane / 16 % 2 * 16 + lane % 4 * 4;
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+        union {
+          s16x4 h[2];
+          Frag<T> f;
+        } vt;
+        vt.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lv + G::at(row, d / 8) + d % 8));
+        vt.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lv + G::at(row + 8, d / 8) + d % 8));
+        o[dt] = mfma(vt.f, p, o[dt]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int kt = 0; kt < G::KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < G::REGS; ++r) {
+        const int row = kt * 32 + 8 * (r / 4) + 4 * half + r % 4;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) {
+          const int d = dt * 32 + col;
+          o[dt] = mfma(lv[G::at(row, d / 4) + d % 4], acc[kt][r], o[dt]);
+        }
+      }
+  }
+  // Registers 4i .. 4i + 3 of o[dt] are channels 32 dt + 8 i + 4 half + 0..3 of the lane's row.
+  const float sum = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // 0: nothing seen; NaN stays
+  float2 meta = make_float2(l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l), sum);
+  if constexpr (sizeof(T) == 2) {
+    // In whole 2^-15ths of the row's largest magnitude: an error of 2^-16 of it, a tenth of what
+    // float16 would leave.  An infinite magnitude makes the row NaN; NaN alone hides from the
+    // maximum and is looked for where the block's values hold any.
+    float big = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(o[dt][r]));
+    if (odd) {
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) big = o[dt][r] == o[dt][r] ? big : INFINITY;
+    }
+    const float2 bh = both_halves(big);
+    big = fmaxf(fmaxf(bh.x, bh.y), 7.52e-37f);  // 2^-120, where the reciprocal is finite
+    const float down = 1.f / big;
+    meta.y *= big;
+    if (live && half == 0) c.meta[partial] = meta;
+    int16_t* part = (int16_t*)c.part + partial * c.a.dim;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const auto pair = __builtin_amdgcn_cvt_pknorm_i16(o[dt][8 * i + 2 * r] * down,
+                                                            o[dt][8 * i + 2 * r + 1] * down);
+          __builtin_memcpy(&w[r], &pair, 4);
+        }
+        // channels 8 apart, 4 a half, become 8 neighbours a half
+        const auto r0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+        const auto r1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+        const Vec<uint32_t, 4> out{{r0[0], r1[0], r0[1], r1[1]}};
+        const int d = 32 * dt + 16 * i + 8 * half;
+        if (live && d < c.a.dim) store_vec((uint32_t*)(part + d), out);
+      }
+  } else {
+    if (live && half == 0) c.meta[partial] = meta;
+    float* part = (float*)c.part + partial * c.a.dim;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * dt + 8 * i + 4 * half;
+        const Vec<float, 4> out{{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]}};
+        if (live && d < c.a.dim) store_vec(part + d, out);
+      }
+  }
+}
+
+// The last u in [0, n) with tiles[u] <= tile, by all lanes at once.
+__device__ __forceinline__ int find_tile(const int32_t* tiles, int n, int tile) {
+  const int lane = threadIdx.x % 64;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 63) / 64, at = lane * step;
+    const int below = __popcll(__ballot(at < n && tiles[lo + min(at, n - 1)] <= tile));
+    const int to = (below - 1) * step;
+    lo += to;
+    n = min(step, n - to);
+  }
+  return lo;
+}
+
+template <class T, int DP, int BK, bool BY_BLOCK>
+__global__ __launch_bounds__(256) void block_partials_kernel(ChunkArgs c) {
+  using G = Tile<T, DP, BK>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* lk = (T*)lds;
+  T* lv = lk + G::ROWS * DP;
+  float* bias = (float*)(lv + G::ROWS * DP);
+  const BlockArgs& a = c.a;
+  const int wave = threadIdx.x / 64, col = threadIdx.x % 32;
+  // scores' sign in the queries, so that the largest weight belongs to the largest product; a
+  // factor of 0 stays above it, which keeps -inf times it -inf
+  const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-35f);
+  const bool negate = a.scale < 0.f;
+  if constexpr (BY_BLOCK) {
+    const int all = c.units * a.blocks;
+    const int total = c.tiles[all];
+    const int t_lo = (int)((int64_t)blockIdx.x * total / gridDim.x);
+    const int t_hi = (int)((int64_t)(blockIdx.x + 1) * total / gridDim.x);
+    int held = -1, unit = 0, b = 0, g = 0, j = 0, first_tile = 0, next_tile = 0, rows = 0, list0 = 0;
+    int64_t start = 0;
+    bool odd = false;
+    for (int tile = t_lo; tile < t_hi; ++tile) {
+      if (held < 0 || tile >= next_tile) {
+        held = held < 0 ? find_tile(c.tiles, all, tile)
+                        : held + 1 + find_tile(c.tiles + held + 1, all - held - 1, tile);
+        unit = held / a.blocks;
+        j = held - unit * a.blocks;
+        b = (c.unit0 + unit) / a.kv_heads;
+        g = c.unit0 + unit - b * a.kv_heads;
+        first_tile = c.tiles[held];
+        next_tile = c.tiles[held + 1];
+        list0 = c.start[held];
+        rows = (c.start[held + 1] - list0) * a.group;
+        start = item_start(a, b) + c.t0;
+        __syncthreads();  // the block before has been read
+        odd = stage_block<T, DP, BK>(c, b, g, j, lk, lv, bias);
+      }
+      const int row = (tile - first_tile) * kTileRows + wave * 32 + col;
+      if (__all(row >= rows)) continue;
+      const bool live = row < rows;
+      const int pair = live ? row / a.group : 0, h = live ? row - pair * a.group : 0;
+      const int entry = c.list[list0 + pair];
+      const int t = entry / a.keep, slot = entry - t * a.keep;
+      const T* q = (const T*)c.q + b * a.qs[0] + (c.t0 + t) * a.qs[1] + (g * a.group + h) * a.qs[2];
+      const int64_t partial = (((int64_t)unit * c.nt + t) * a.group + h) * a.keep + slot;
+      attend_rows<T, DP, BK>(c, lk, lv, bias, live, q, start + t, j * BK, c2, negate, odd, partial);
+    }
+  } else {
+    const int item = blockIdx.x, slot = item % a.keep, ut = item / a.keep;
+    const int unit = ut / c.nt, t = ut - unit * c.nt;
+    const int b = (c.unit0 + unit) / a.kv_heads, g = c.unit0 + unit - b * a.kv_heads;
+    const int j = c.ids[(((int64_t)b * a.queries + c.t0 + t) * a.kv_heads + g) * a.keep + slot];
+    if (j < 0 || j >= a.blocks) return;
+    const bool odd = stage_block<T, DP, BK>(c, b, g, j, lk, lv, bias);
+    for (int h0 = wave * 32; h0 < a.group; h0 += 128) {
+      const bool live = h0 + col < a.group;
+      const int h = live ? h0 + col : 0;
+      const T* q = (const T*)c.q + b * a.qs[0] + (c.t0 + t) * a.qs[1] + (g * a.group + h) * a.qs[2];
+      const int64_t partial = (((int64_t)unit * c.nt + t) * a.group + h) * a.keep + slot;
+      attend_rows<T, DP, BK>(c, lk, lv, bias, live, q, item_start(a, b) + c.t0 + t, j * BK, c2, negate,
+                             odd, partial);
+    }
+  }
+}
+
+template <class T, int DP, int BK>
+void launch_partials(const ChunkArgs& c, bool by_block, int grid, hipStream_t st) {
+  constexpr size_t bytes = Tile<T, DP, BK>::LDS;
+  if (by_block) {
+    block_partials_kernel<T, DP, BK, true><<<grid, 256, bytes, st>>>(c);
+  } else {
+    block_partials_kernel<T, DP, BK, false><<<grid, 256, bytes, st>>>(c);
+  }
+  launch_check("block_partials");
+}
+
+template <class T>
+void block_partials(const ChunkArgs& c, bool by_block, int grid, hipStream_t st) {
+  using std::integral_constant;
+  auto keys = [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    if (c.a.block == 16) return launch_partials<T, DP, 16>(c, by_block, grid, st);
+    if (c.a.block == 32) return launch_partials<T, DP, 32>(c, by_block, grid, st);
+    if (c.a.block == 64) return launch_partials<T, DP, 64>(c, by_block, grid, st);
+    launch_partials<T, DP, 128>(c, by_block, grid, st);
+  };
+  if (c.a.dim <= 32) return keys(integral_constant<int, 32>{});
+  if (c.a.dim <= 64) return keys(integral_constant<int, 64>{});
+  if (c.a.dim <= 96) return keys(integral_constant<int, 96>{});
+  keys(integral_constant<int, 128>{});
+}
+
+}  // namespace
+}  // namespace nnx

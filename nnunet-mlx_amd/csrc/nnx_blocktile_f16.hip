@@ -1,0 +1,9 @@
+#include "nnx_blocktile.h"
+
+namespace nnx {
+
+void block_partials_f16(const ChunkArgs& c, bool by_block, int grid, hipStream_t st) {
+  block_partials<f16>(c, by_block, grid, st);
+}
+
+}  // namespace nnx
