@@ -129,150 +129,159 @@ __global__ __launch_bounds__(256) void summarize_kernel(BlockArgs a, const T* k,
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// A wave writes the kept blocks of one row of scores (in LDS): every +inf, then the highest finite
-// ones, equal ones by the lower index; never -inf.  256 bins between the lowest and the highest
-// find the bin in which the last kept score lies; only that bin's scores are then compared.
-__device__ void select_row(const float* score, int blocks, int keep, uint32_t* bins, int32_t* out) {
-  const int lane = threadIdx.x % 64;
-  const auto larger = [](float x, float y) { return fmaxf(x, y); };
-  float lo = INFINITY, hi = -INFINITY;
-  int forced = 0, finite = 0;
-  for (int j = lane; j < blocks; j += 64) {
-    const float v = score[j];
-    const bool top = v == INFINITY, usable = fabsf(v) < INFINITY;
-    forced += __popcll(__ballot(top));
-    finite += __popcll(__ballot(usable));
-    lo = fminf(lo, usable ? v : lo);
-    hi = fmaxf(hi, usable ? v : hi);
+// The kept blocks of one row of scores (in LDS), written by a wave: the `keep` highest, equal ones by
+// the lower index, never -inf.  A cut is searched by halving until exactly `keep` scores lie above
+// it: of the values at first, which ends in some 9 steps for scores with gaps, then of their order
+// as whole numbers, which ends in 32 at a value whose equals are taken from the lowest index on.
+// N > 0: the row stays in N registers a lane; N = 0: it is read from LDS for every step.
+template <int N>
+__device__ __forceinline__ void select_row(const float* score, int blocks, int keep, int32_t* out) {
+  const int lane = threadIdx.x % 64, n = N ? N : (blocks + 63) / 64;
+  float held[N ? N : 1];
+  const auto value = [&](int i) { return i * 64 + lane < blocks ? score[i * 64 + lane] : -INFINITY; };
+  if constexpr (N > 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) held[i] = value(i);
   }
-  // lanes past the end took part in fewer ballots; lane 0 in all
-  forced = __builtin_amdgcn_readfirstlane(forced);
-  finite = __builtin_amdgcn_readfirstlane(finite);
-  float cut = -INFINITY;  // kept: above cut, and the first `ties` that equal it
+  const auto each = [&](auto&& body) {
+    if constexpr (N > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) body(i, held[i]);
+    } else {
+      for (int i = 0; i < n; ++i) body(i, value(i));
+    }
+  };
+  const auto above = [&](float x) {
+    int count = 0;
+    each([&](int, float v) { count += __popcll(__ballot(v > x)); });
+    return count;
+  };
+  const auto larger = [](float x, float y) { return fmaxf(x, y); };
+  float cut = -INFINITY;  // kept: scores above it, and the first `ties` that equal it
   int ties = 0;
-  if (forced >= keep) {
-    cut = INFINITY;
-    ties = keep;
-  } else if (forced + finite > keep) {
-    lo = -lanes_reduce<64>(-lo, larger);
-    hi = lanes_reduce<64>(hi, larger);
-    const float step = 255.f / (hi - lo);
-    const auto bin_of = [&](float v) { return min(max((int)((v - lo) * step), 0), 255); };
-    *(uint4*)&bins[4 * lane] = make_uint4(0, 0, 0, 0);
-    __builtin_amdgcn_wave_barrier();
-    for (int j = lane; j < blocks; j += 64) {
-      const float v = score[j];
-      if (fabsf(v) < INFINITY) atomicAdd(&bins[bin_of(v)], 1u);
-    }
-    __builtin_amdgcn_wave_barrier();
-    __threadfence_block();
-    // lane l: bins 255 - 4 l down to 252 - 4 l
-    const uint4 mine = *(const uint4*)&bins[252 - 4 * lane];
-    const int own = mine.x + mine.y + mine.z + mine.w;
-    int run = own;
-    for (int o = 1; o < 64; o *= 2) {
-      const int x = __shfl_up(run, o);
-      if (lane >= o) run += x;
-    }
-    const int need = keep - forced;  // at least 1, fewer than finite
-    const int at = __ffsll(__ballot(run >= need)) - 1;
-    int before = run - own, bin = 255 - 4 * lane;
-    if (before + (int)mine.w < need) {
-      before += mine.w, --bin;
-      if (before + (int)mine.z < need) {
-        before += mine.z, --bin;
-        if (before + (int)mine.y < need) before += mine.y, --bin;
+  if (above(-INFINITY) > keep) {
+    float low = INFINITY, high = -INFINITY;  // above(low) >= keep > above(high)
+    each([&](int, float v) {
+      low = fminf(low, v > -INFINITY ? v : low);
+      high = fmaxf(high, v);
+    });
+    low = -lanes_reduce<64>(-low, larger);
+    high = lanes_reduce<64>(high, larger);
+    bool found = false;
+    if (high == INFINITY) {  // blocks kept whatever their score
+      const int forced = above(3.4028235e38f);
+      if (forced >= keep) {
+        cut = INFINITY;
+        ties = keep;
+        found = true;
+      } else {
+        high = -INFINITY;
+        each([&](int, float v) { high = fmaxf(high, v < INFINITY ? v : high); });
+        high = lanes_reduce<64>(high, larger);
       }
     }
-    bin = __shfl(bin, at);
-    int rest = need - __shfl(before, at);
-    // the bin's scores from the highest on, a value at a time
-    cut = INFINITY;
-    while (true) {
-      float best = -INFINITY;
-      int same = 0;
-      for (int j = lane; j < blocks; j += 64) {
-        const float v = score[j];
-        if (fabsf(v) < INFINITY && v < cut && bin_of(v) == bin) {
-          same = v > best ? 1 : same + (v == best);
-          best = fmaxf(best, v);
-        }
+    if (!found && above(low) < keep) {  // the lowest score is the last one kept
+      cut = low;
+      ties = keep - above(low);
+      found = true;
+    }
+    for (int step = 0; step < 14 && !found; ++step) {
+      const float mid = 0.5f * low + 0.5f * high;
+      const int count = above(mid);
+      if (count == keep) {
+        cut = mid;
+        found = true;
       }
-      const float all = lanes_reduce<64>(best, larger);
-      same = best == all ? same : 0;
-      for (int o = 32; o; o >>= 1) same += __shfl_xor(same, o);
-      cut = all;
-      ties = rest;
-      if (same >= rest || all == -INFINITY) break;
-      rest -= same;
+      (count < keep ? high : low) = mid;
+    }
+    if (!found) {
+      const auto order = [](float v) {
+        const int32_t b = __float_as_int(v + 0.f);
+        return b ^ (b >> 31 & 0x7fffffff);
+      };
+      const auto back = [](int32_t o) { return __int_as_float(o ^ (o >> 31 & 0x7fffffff)); };
+      int32_t lo = order(low), hi = order(high);
+      while ((int64_t)hi - lo > 1) {
+        const int32_t mid = (int32_t)(((int64_t)lo + hi) >> 1);
+        (above(back(mid)) < keep ? hi : lo) = mid;
+      }
+      cut = back(hi);
+      ties = keep - above(cut);
     }
   }
   const uint64_t below = ((uint64_t)1 << lane) - 1;
   int done = 0, tied = 0;
-  for (int j0 = 0; j0 < blocks; j0 += 64) {
-    const int j = j0 + lane;
-    const float v = j < blocks ? score[j] : -INFINITY;
-    const uint64_t equal = __ballot(v == cut && cut != -INFINITY);
-    const bool take = v > cut || (((equal >> lane) & 1) && tied + __popcll(equal & below) < ties);
+  each([&](int i, float v) {
+    bool take = v > cut;
+    if (ties) {
+      const uint64_t equal = __ballot(v == cut);
+      take |= ((equal >> lane) & 1) && tied + __popcll(equal & below) < ties;
+      tied += __popcll(equal);
+    }
     const uint64_t taken = __ballot(take);
     const int to = done + __popcll(taken & below);
-    if (take && to < keep) out[to] = j;
-    tied += __popcll(equal);
+    if (take && to < keep) out[to] = i * 64 + lane;
     done += __popcll(taken);
-  }
+  });
   for (int i = min(done, keep) + lane; i < keep; i += 64) out[i] = -1;
 }
 
 // `rows` <= 16 queries of one item and key head: their scores against 16 blocks at a time by 8-bit
-// products in whole numbers (a query's codes are formed in the registers that feed them), kept
-// in LDS; then a wave a query picks.  Heads that share the key head are taken HEADS at a time
-// and meet in the largest score.
-template <class T>
+// products in whole numbers, kept in LDS; then a wave a query picks.  Heads that share the key
+// head are taken HEADS at a time (their codes in LDS) and meet in the largest score.
+template <class T, int N>
 __global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, const int8_t* codes,
                                                      const float* scales, int32_t* ids, int rows,
                                                      int pitch) {
   constexpr int HEADS = 4, WAVES = 8;
-  extern __shared__ __attribute__((aligned(16))) float score[];  // rows x pitch, then bins
-  uint32_t* bins = (uint32_t*)(score + rows * pitch);
+  extern __shared__ __attribute__((aligned(16))) float score[];  // rows x pitch
+  __shared__ i32x4 qcode[HEADS][2][64];
+  __shared__ float qtop[HEADS][16];
   const int t0 = blockIdx.x * rows, g = blockIdx.y, b = blockIdx.z;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, quad = lane / 16;
-  const int t = t0 + col;
-  const bool live = col < rows && t < a.queries;
   const int64_t unit = (int64_t)b * a.kv_heads + g;
-  const int64_t own = (item_start(a, b) + t) / a.block;
+  const int64_t own = (item_start(a, b) + t0 + col) / a.block;
   const int8_t* cu = codes + unit * a.blocks * a.dim;
   const float* su = scales + unit * a.blocks;
   for (int h0 = 0; h0 < a.group; h0 += HEADS) {
-    i32x4 qc[HEADS][2];
-    float top[HEADS];
-#pragma unroll
-    for (int h = 0; h < HEADS; ++h) {
-      Vec<T, 8> v[4];
+    const int heads = min(HEADS, a.group - h0);
+    if (h0) __syncthreads();
+    if (wave < heads) {  // a wave a head, in the lanes' places of the products' second operand
+      const bool live = col < rows && t0 + col < a.queries;
+      const T* row = q + b * a.qs[0] + (int64_t)(t0 + col) * a.qs[1] +
+                     (int64_t)(g * a.group + h0 + wave) * a.qs[2];
+      float v[32];
       float m = 0.f;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const int d = (s / 2) * 64 + quad * 16 + (s % 2) * 8;
-        v[s] = Vec<T, 8>{};
-        if (live && h0 + h < a.group && d < a.dim)
-          v[s] = load_vec<8>(q + b * a.qs[0] + t * a.qs[1] + (g * a.group + h0 + h) * a.qs[2] + d);
+        Vec<T, 8> x{};
+        if (live && d < a.dim) x = load_vec<8>(row + d);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(finite_or_zero(to_float(v[s].v[e]))));
+        for (int e = 0; e < 8; ++e) {
+          v[8 * s + e] = finite_or_zero(to_float(x.v[e]));
+          m = fmaxf(m, fabsf(v[8 * s + e]));
+        }
       }
       m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
       const float up = m < kTiny ? 0.f : __fdiv_rn(127.f, m);
-      top[h] = m < kTiny ? 1.f : m;
+      if (quad == 0) qtop[wave][col] = m < kTiny ? 1.f : m;
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+      for (int s = 0; s < 2; ++s) {
+        i32x4 word;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint32_t word = 0;
+        for (int w = 0; w < 4; ++w) {
+          uint32_t bytes = 0;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            word |= ((uint32_t)(int)rintf(finite_or_zero(to_float(v[s].v[4 * w + e])) * up) & 255u) << (8 * e);
-          qc[h][s / 2][(s % 2) * 2 + w] = (int)word;
+            bytes |= ((uint32_t)(int)rintf(v[16 * s + 4 * w + e] * up) & 255u) << (8 * e);
+          word[w] = (int)bytes;
         }
+        qcode[wave][s][lane] = word;
+      }
     }
+    __syncthreads();
     for (int j0 = wave * 16; j0 < a.blocks; j0 += WAVES * 16) {
       i32x4 kc[2] = {};
       const int8_t* row = cu + (int64_t)min(j0 + col, a.blocks - 1) * a.dim;
@@ -290,14 +299,13 @@ __global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, co
 #pragma unroll
       for (int r = 0; r < 4; ++r) scale[r] = su[min(j0 + quad * 4 + r, a.blocks - 1)];
       float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int h = 0; h < HEADS; ++h) {
-        if (h0 + h >= a.group) break;
+      for (int h = 0; h < heads; ++h) {
         i32x4 dot = {0, 0, 0, 0};
-        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[0], qc[h][0], dot, 0, 0, 0);
-        if (a.dim > 64) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[1], qc[h][1], dot, 0, 0, 0);
+        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[0], qcode[h][0][lane], dot, 0, 0, 0);
+        if (a.dim > 64) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[1], qcode[h][1][lane], dot, 0, 0, 0);
+        const float top = qtop[h][col];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) best[r] = fmaxf(best[r], ((float)dot[r] * top[h]) * scale[r]);
+        for (int r = 0; r < 4; ++r) best[r] = fmaxf(best[r], ((float)dot[r] * top) * scale[r]);
       }
       if (col < rows) {
         float4* to = (float4*)&score[col * pitch + j0 + quad * 4];
@@ -318,8 +326,8 @@ __global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, co
   }
   __syncthreads();
   for (int r = wave; r < rows && t0 + r < a.queries; r += WAVES)
-    select_row(score + r * pitch, a.blocks, a.keep, bins + wave * 256,
-               ids + (((int64_t)b * a.queries + t0 + r) * a.kv_heads + g) * a.keep);
+    select_row<N>(score + r * pitch, a.blocks, a.keep,
+                  ids + (((int64_t)b * a.queries + t0 + r) * a.kv_heads + g) * a.keep);
 }
 
 // ---- the attention ---------------------------------------------------------------------
@@ -405,42 +413,55 @@ __global__ __launch_bounds__(256) void place_pairs_kernel(ChunkArgs c, int per, 
 }
 
 // out = sum_s w_s O_s / sum_s w_s with w_s = 2^(log2 sum_s - largest), O_s a partial under its
-// factor.  dim / 8 lanes a row, `share` groups of lanes a row where rows are few.
+// factor.  A workgroup forms the weights of its rows together, then dim / 8 lanes a row add up
+// (`share` groups of them a row, each every share-th partial, where rows are few or have many).
+constexpr int kJoinWeights = 4096;
+
 template <class T>
-__global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out, int share) {
+__global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out, int share, int each) {
   using P = typename std::conditional<sizeof(T) == 2, int16_t, float>::type;
   constexpr float kUnit = sizeof(T) == 2 ? 1.f / 32767.f : 1.f;
   __shared__ float sums[256][9];
+  __shared__ float2 weight[kJoinWeights];  // of the sum, of the values; by row and slot
   const BlockArgs& a = c.a;
-  const int lanes = a.dim / 8, sub = threadIdx.x / lanes, u = threadIdx.x - sub * lanes;
-  const int each = 256 / (lanes * share);  // rows of a workgroup
-  const int own = sub / share, part0 = sub - own * share;
-  const int64_t row = (int64_t)blockIdx.x * each + own, rows = (int64_t)c.units * c.nt * a.group;
-  const bool live = own < each && row < rows;
-  float o[8] = {}, l = 0.f;
-  int64_t ut = 0;
-  int unit = 0, t = 0, h = 0, b = 0, g = 0;
-  if (live) {
-    ut = row / a.group;
+  const int64_t row0 = (int64_t)blockIdx.x * each, rows = (int64_t)c.units * c.nt * a.group;
+  const int here = (int)min((int64_t)each, rows - row0);
+  const auto place = [&](int64_t row, int& b, int& t, int& g, int& h) {
+    const int64_t ut = row / a.group;
+    const int unit = (int)(ut / c.nt);
     h = (int)(row - ut * a.group);
-    unit = (int)(ut / c.nt);
-    t = (int)(ut - (int64_t)unit * c.nt);
+    t = c.t0 + (int)(ut - (int64_t)unit * c.nt);
     b = (c.unit0 + unit) / a.kv_heads;
     g = c.unit0 + unit - b * a.kv_heads;
-    const int32_t* ids = c.ids + (((int64_t)b * a.queries + c.t0 + t) * a.kv_heads + g) * a.keep;
-    const float2* meta = c.meta + row * a.keep;
-    const P* part = (const P*)c.part + row * a.keep * a.dim + 8 * u;
+  };
+  for (int i = threadIdx.x; i < here * a.keep; i += 256) {
+    const int r = i / a.keep, s = i - r * a.keep;
+    int b, t, g, h;
+    place(row0 + r, b, t, g, h);
+    const int j = c.ids[(((int64_t)b * a.queries + t) * a.kv_heads + g) * a.keep + s];
+    weight[i] = (unsigned)j < (unsigned)a.blocks ? c.meta[(row0 + r) * a.keep + s]
+                                                 : make_float2(-INFINITY, 0.f);
+  }
+  __syncthreads();
+  const int lanes = a.dim / 8, sub = threadIdx.x / lanes, u = threadIdx.x - sub * lanes;
+  const int own = sub / share, part0 = sub - own * share;
+  const bool live = own < here;
+  float o[8] = {}, l = 0.f;
+  if (live) {
+    const float2* w = weight + own * a.keep;
     float top = -INFINITY;
-    for (int s = 0; s < a.keep; ++s)
-      if ((unsigned)ids[s] < (unsigned)a.blocks) top = fmaxf(top, meta[s].x);
+#pragma unroll 8
+    for (int s = 0; s < a.keep; ++s) top = fmaxf(top, w[s].x);
     if (top == -INFINITY) top = 0.f;
-#pragma unroll 4
+    const P* part = (const P*)c.part + (row0 + own) * a.keep * a.dim + 8 * u;
+#pragma unroll 8
     for (int s = part0; s < a.keep; s += share) {
-      if ((unsigned)ids[s] >= (unsigned)a.blocks) continue;
-      const float2 m = meta[s];
-      const Vec<P, 8> x = load_vec<8>(part + (int64_t)s * a.dim);
-      const float w = __builtin_amdgcn_exp2f(m.x - top), f = w * m.y * kUnit;
-      l += w;
+      const float2 m = w[s];
+      // a partial of an entry that is no block was never written
+      Vec<P, 8> x{};
+      if (m.x > -INFINITY || m.x != m.x) x = load_vec<8>(part + (int64_t)s * a.dim);
+      const float ws = __builtin_amdgcn_exp2f(m.x - top), f = ws * m.y * kUnit;
+      l += ws;
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = fmaf(f, (float)x.v[i], o[i]);
     }
@@ -456,11 +477,13 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
     }
   }
   if (!live) return;
+  int b, t, g, h;
+  place(row0 + own, b, t, g, h);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   Vec<T, 8> r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) r.v[i] = from_float<T>(o[i] * inv);
-  store_vec(out + b * a.os[0] + (c.t0 + t) * a.os[1] + (int64_t)(g * a.group + h) * a.os[2] + 8 * u, r);
+  store_vec(out + b * a.os[0] + t * a.os[1] + (int64_t)(g * a.group + h) * a.os[2] + 8 * u, r);
 }
 
 // One pass's work and where it lies in the workspace.  Chunks hold whole units where those fit the
@@ -546,14 +569,27 @@ void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
   const BlockArgs a = make_args(c, start, nullptr, nullptr);
   const double products = (double)c.batch * c.queries * c.heads * c.head_dim;
   ProfScope prof("block_select", 2.0 * products * a.blocks, products * type_bytes(c.type), st);
-  // As many queries a workgroup as the products take, while their scores fit the LDS.
+  // As many queries a workgroup as the products take, while their scores fit the LDS; rows of up to
+  // 2048 blocks are picked from registers.
   const int pitch = (int)ceil_div(a.blocks, 16) * 16 + 4;
   int rows = 16;
-  while (rows > 1 && (size_t)rows * pitch * 4 + 8192 > 147456) rows /= 2;
+  while (rows > 1 && (size_t)rows * pitch * 4 > 139264) rows /= 2;
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    select_kernel<T><<<dim3((unsigned)ceil_div(c.queries, rows), c.kv_heads, c.batch), 512,
-                       rows * pitch * sizeof(float) + 8192, st>>>(a, (const T*)q, codes, scales, ids, rows, pitch);
+    const dim3 grid((unsigned)ceil_div(c.queries, rows), c.kv_heads, c.batch);
+    auto go = [&](auto n) {
+      select_kernel<T, decltype(n)::value><<<grid, 512, rows * pitch * sizeof(float), st>>>(
+          a, (const T*)q, codes, scales, ids, rows, pitch);
+    };
+    using std::integral_constant;
+    const int64_t n = ceil_div(a.blocks, 64);
+    if (n <= 1) return go(integral_constant<int, 1>{});
+    if (n <= 2) return go(integral_constant<int, 2>{});
+    if (n <= 4) return go(integral_constant<int, 4>{});
+    if (n <= 8) return go(integral_constant<int, 8>{});
+    if (n <= 16) return go(integral_constant<int, 16>{});
+    if (n <= 32) return go(integral_constant<int, 32>{});
+    go(integral_constant<int, 0>{});
   });
   launch_check("block_select");
 }
@@ -619,14 +655,18 @@ void block_attention(const nnx_block_config& c, const void* q, const void* k, co
       }
       const int64_t rows = (int64_t)m.units * m.nt * a.group;
       const int lanes = a.dim / 8;
-      // groups of lanes a row: more while rows are too few for the CUs
+      // groups of lanes a row: more while rows are too few for the CUs or their weights for the LDS
       int share = 1;
-      while (share * 2 * lanes <= 256 && share * 2 <= c.keep && rows * lanes * share < 65536) share *= 2;
+      const auto each = [&] { return 256 / (lanes * share); };
+      while (lanes * share * 2 <= 256 &&
+             (each() * c.keep > kJoinWeights || (share * 2 <= c.keep && rows * lanes * share < 65536)))
+        share *= 2;
+      const int here = std::min(each(), kJoinWeights / c.keep);
       ProfScope prof("block_join", 2.0 * rows * c.keep * c.head_dim,
                      (double)rows * c.keep * (8 + c.head_dim * type_bytes(c.type)), st);
       with_type(c.type, [&](auto z) {
         using T = decltype(z);
-        join_partials_kernel<T><<<(unsigned)ceil_div(rows, 256 / (lanes * share)), 256, 0, st>>>(m, (T*)out, share);
+        join_partials_kernel<T><<<(unsigned)ceil_div(rows, here), 256, 0, st>>>(m, (T*)out, share, here);
       });
       launch_check("block_join");
     }

@@ -96,11 +96,29 @@ __device__ __forceinline__ bool stage_block(const ChunkArgs& c, int b, int g, in
 // lanes' registers, so the softmax needs one exchange between halves, and its weights are
 // already the second operand of O^T = V^T P^T (the order of keys is that of the registers; values
 // are read transposed to match).
+template <class T, int DP>
+struct QueryRow {
+  static constexpr int CH = 16 / sizeof(T), N = DP / (2 * CH);
+  Vec<T, CH> v[N];  // a half's chunks: 2 s + half
+};
+
+template <class T, int DP>
+__device__ __forceinline__ void load_query(QueryRow<T, DP>& row, const T* q, bool live, int dim) {
+  using Q = QueryRow<T, DP>;
+  const int half = threadIdx.x % 64 / 32;
+#pragma unroll
+  for (int s = 0; s < Q::N; ++s) {
+    const int d = (2 * s + half) * Q::CH;
+    row.v[s] = Vec<T, Q::CH>{};
+    if (live && d < dim) row.v[s] = load_vec<Q::CH>(q + d);
+  }
+}
+
 template <class T, int DP, int BK>
 __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, const T* lv,
-                                            const float* bias, bool live, const T* q, int64_t last,
-                                            int first_key, float c2, bool negate, bool odd,
-                                            int64_t partial) {
+                                            const float* bias, bool live, const QueryRow<T, DP>& q,
+                                            int64_t last, int first_key, float c2, bool negate,
+                                            bool odd, int64_t partial) {
   using G = Tile<T, DP, BK>;
   const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;
   f32x16 acc[G::KT];
@@ -119,9 +137,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
     Frag<T> qf[DP / 16];
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
-      const int d = 16 * s + 8 * half;
-      qf[s] = Frag<T>{};
-      if (live && d < c.a.dim) __builtin_memcpy(&qf[s], q + d, 16);
+      __builtin_memcpy(&qf[s], &q.v[s], 16);
       if (negate) qf[s] = -qf[s];
     }
 #pragma unroll
@@ -132,9 +148,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
   } else {
 #pragma unroll
     for (int s = 0; s < DP / 8; ++s) {
-      const int d = 8 * s + 4 * half;
-      Vec<float, 4> qf{};
-      if (live && d < c.a.dim) qf = load_vec<4>((const float*)q + d);
+      Vec<float, 4> qf = q.v[s];
 #pragma unroll
       for (int i = 0; i < 4; ++i) qf.v[i] = negate ? -qf.v[i] : qf.v[i];
 #pragma unroll
@@ -326,7 +340,9 @@ __global__ __launch_bounds__(256) void block_partials_kernel(ChunkArgs c) {
       const int pair = live ? row / a.group : 0, h = live ? row - pair * a.group : 0;
       const int entry = c.list[list0 + pair];
       const int t = entry / a.keep, slot = entry - t * a.keep;
-      const T* q = (const T*)c.q + b * a.qs[0] + (c.t0 + t) * a.qs[1] + (g * a.group + h) * a.qs[2];
+      QueryRow<T, DP> q;
+      load_query<T, DP>(q, (const T*)c.q + b * a.qs[0] + (c.t0 + t) * a.qs[1] + (g * a.group + h) * a.qs[2],
+                        live, a.dim);
       const int64_t partial = (((int64_t)unit * c.nt + t) * a.group + h) * a.keep + slot;
       attend_rows<T, DP, BK>(c, lk, lv, bias, live, q, start + t, j * BK, c2, negate, odd, partial);
     }
@@ -340,7 +356,9 @@ __global__ __launch_bounds__(256) void block_partials_kernel(ChunkArgs c) {
     for (int h0 = wave * 32; h0 < a.group; h0 += 128) {
       const bool live = h0 + col < a.group;
       const int h = live ? h0 + col : 0;
-      const T* q = (const T*)c.q + b * a.qs[0] + (c.t0 + t) * a.qs[1] + (g * a.group + h) * a.qs[2];
+      QueryRow<T, DP> q;
+      load_query<T, DP>(q, (const T*)c.q + b * a.qs[0] + (c.t0 + t) * a.qs[1] + (g * a.group + h) * a.qs[2],
+                        live, a.dim);
       const int64_t partial = (((int64_t)unit * c.nt + t) * a.group + h) * a.keep + slot;
       attend_rows<T, DP, BK>(c, lk, lv, bias, live, q, item_start(a, b) + c.t0 + t, j * BK, c2, negate,
                              odd, partial);
