@@ -6,6 +6,20 @@
 
 namespace nnx {
 
+// n / d for 0 <= n < 2^31 by one product: m = ceil(2^(31 + l) / d) with 2^l >= d errs by less than
+// d / 2^(31 + l) a unit, less than 1 / d over n.
+struct FastDiv {
+  uint32_t m;
+  int l;
+  explicit FastDiv(uint32_t d = 1) : l(0) {
+    while ((1ull << l) < d) ++l;
+    m = (uint32_t)(((1ull << (31 + l)) + d - 1) / d);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return (int)(__umulhi((uint32_t)n << 1, m) >> l);
+  }
+};
+
 struct BlockArgs {
   int batch, queries, keys, heads, kv_heads, group, dim, block, blocks, keep, first, local, causal;
   int64_t start0;
@@ -35,6 +49,7 @@ struct ChunkArgs {
   void* part;
   float2* meta;
   int unit0, units, t0, nt;
+  FastDiv by_keep, by_group, by_nt;
   // by block: pairs (query, slot) that keep it, list[start[u]...], in tiles of kTileRows rows
   // (pairs * group heads), tiles[u] of them before block u = unit * blocks + block
   const int32_t *list, *start, *tiles;

@@ -238,9 +238,15 @@ __global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, co
   __shared__ i32x4 qcode[HEADS][2][64];
   __shared__ float qtop[HEADS][16];
   const int t0 = blockIdx.x * rows, g = blockIdx.y, b = blockIdx.z;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, quad = lane / 16;
+  const int lane = threadIdx.x % 64, col = lane % 16, quad = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int64_t unit = (int64_t)b * a.kv_heads + g;
-  const int64_t own = (item_start(a, b) + t0 + col) / a.block;
+  // the block of a query's own position: -1 before the first key, at most 2^24 (past the last block)
+  const auto own_block = [&](int r) {
+    const int64_t at = item_start(a, b) + t0 + r;
+    return at < 0 ? -1 : (int)min(at / a.block, (int64_t)1 << 24);
+  };
+  const int own = a.causal ? own_block(col) : 1 << 24;
   const int8_t* cu = codes + unit * a.blocks * a.dim;
   const float* su = scales + unit * a.blocks;
   for (int h0 = 0; h0 < a.group; h0 += HEADS) {
@@ -298,14 +304,17 @@ __global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, co
       float scale[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) scale[r] = su[min(j0 + quad * 4 + r, a.blocks - 1)];
-      float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float best[4];
       for (int h = 0; h < heads; ++h) {
         i32x4 dot = {0, 0, 0, 0};
         dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[0], qcode[h][0][lane], dot, 0, 0, 0);
         if (a.dim > 64) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[1], qcode[h][1][lane], dot, 0, 0, 0);
         const float top = qtop[h][col];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) best[r] = fmaxf(best[r], ((float)dot[r] * top) * scale[r]);
+        for (int r = 0; r < 4; ++r) {
+          const float x = ((float)dot[r] * top) * scale[r];
+          best[r] = h ? fmaxf(best[r], x) : x;
+        }
       }
       if (col < rows) {
         float4* to = (float4*)&score[col * pitch + j0 + quad * 4];
@@ -315,19 +324,30 @@ __global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, co
           best[2] = fmaxf(best[2], z.z), best[3] = fmaxf(best[3], z.w);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int j = j0 + quad * 4 + r;
-          if (j < a.first || (j <= own && j > own - a.local)) best[r] = INFINITY;
-          if (scale[r] < 0.f || (a.causal && j > own)) best[r] = -INFINITY;
+        for (int r = 0; r < 4; ++r)
+          if (scale[r] < 0.f) best[r] = -INFINITY;  // no valid key
+        if (a.causal) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (j0 + quad * 4 + r > own) best[r] = -INFINITY;
         }
         *to = make_float4(best[0], best[1], best[2], best[3]);
       }
     }
   }
   __syncthreads();
-  for (int r = wave; r < rows && t0 + r < a.queries; r += WAVES)
-    select_row<N>(score + r * pitch, a.blocks, a.keep,
+  for (int r = wave; r < rows && t0 + r < a.queries; r += WAVES) {
+    float* row = score + r * pitch;
+    const int at = own_block(r);
+    // blocks kept whatever their score, where they can be
+    const auto keep_block = [&](int j) {
+      if (j < a.blocks && row[j] > -INFINITY) row[j] = INFINITY;
+    };
+    for (int j = lane; j < min(a.first, a.blocks); j += 64) keep_block(j);
+    for (int i = max(at - a.blocks + 1, 0) + lane; i < min(a.local, at + 1); i += 64) keep_block(at - i);
+    select_row<N>(row, a.blocks, a.keep,
                   ids + (((int64_t)b * a.queries + t0 + r) * a.kv_heads + g) * a.keep);
+  }
 }
 
 // ---- the attention ---------------------------------------------------------------------
@@ -351,7 +371,7 @@ __global__ __launch_bounds__(256) void count_pairs_kernel(ChunkArgs c, int per, 
   __syncthreads();
   const int32_t* ids = c.ids + (((int64_t)b * a.queries + c.t0) * a.kv_heads + g) * a.keep;
   for (int e = t_lo * a.keep + threadIdx.x; e < t_hi * a.keep; e += 256) {
-    const int t = e / a.keep, s = e - t * a.keep;
+    const int t = c.by_keep(e), s = e - t * a.keep;
     const int j = ids[(int64_t)t * a.kv_heads * a.keep + s];
     if (j >= 0 && j < a.blocks) rank[(int64_t)unit * c.nt * a.keep + e] = atomicAdd(&hist[j], 1);
   }
@@ -405,7 +425,7 @@ __global__ __launch_bounds__(256) void place_pairs_kernel(ChunkArgs c, int per, 
   const int unit = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x;
   if (e >= c.nt * a.keep) return;
   const int b = (c.unit0 + unit) / a.kv_heads, g = c.unit0 + unit - b * a.kv_heads;
-  const int t = e / a.keep, s = e - t * a.keep;
+  const int t = c.by_keep(e), s = e - t * a.keep;
   const int j = c.ids[(((int64_t)b * a.queries + c.t0 + t) * a.kv_heads + g) * a.keep + s];
   if (j < 0 || j >= a.blocks) return;
   const int from = base[((int64_t)unit * groups + t / per) * a.blocks + j];
@@ -421,21 +441,21 @@ template <class T>
 __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out, int share, int each) {
   using P = typename std::conditional<sizeof(T) == 2, int16_t, float>::type;
   constexpr float kUnit = sizeof(T) == 2 ? 1.f / 32767.f : 1.f;
-  __shared__ float sums[256][9];
-  __shared__ float2 weight[kJoinWeights];  // of the sum, of the values; by row and slot
+  // by row and slot the weight of the sum and the factor of the values; then the shares' sums
+  extern __shared__ float2 weight[];
+  float(*sums)[9] = (float(*)[9])(weight + each * c.a.keep);
   const BlockArgs& a = c.a;
   const int64_t row0 = (int64_t)blockIdx.x * each, rows = (int64_t)c.units * c.nt * a.group;
   const int here = (int)min((int64_t)each, rows - row0);
   const auto place = [&](int64_t row, int& b, int& t, int& g, int& h) {
-    const int64_t ut = row / a.group;
-    const int unit = (int)(ut / c.nt);
-    h = (int)(row - ut * a.group);
-    t = c.t0 + (int)(ut - (int64_t)unit * c.nt);
+    const int ut = c.by_group((int)row), unit = c.by_nt(ut);
+    h = (int)row - ut * a.group;
+    t = c.t0 + ut - unit * c.nt;
     b = (c.unit0 + unit) / a.kv_heads;
     g = c.unit0 + unit - b * a.kv_heads;
   };
   for (int i = threadIdx.x; i < here * a.keep; i += 256) {
-    const int r = i / a.keep, s = i - r * a.keep;
+    const int r = c.by_keep(i), s = i - r * a.keep;
     int b, t, g, h;
     place(row0 + r, b, t, g, h);
     const int j = c.ids[(((int64_t)b * a.queries + t) * a.kv_heads + g) * a.keep + s];
@@ -627,6 +647,7 @@ void block_attention(const nnx_block_config& c, const void* q, const void* k, co
       ChunkArgs m = k0;
       m.unit0 = u, m.units = std::min(p.units, all_units - u);
       m.t0 = t, m.nt = std::min(p.nt, c.queries - t);
+      m.by_keep = FastDiv(c.keep), m.by_group = FastDiv(a.group), m.by_nt = FastDiv(m.nt);
       const int64_t pairs = (int64_t)m.units * m.nt * c.keep;
       int grid = (int)pairs;
       if (p.by_block) {
@@ -666,7 +687,8 @@ void block_attention(const nnx_block_config& c, const void* q, const void* k, co
                      (double)rows * c.keep * (8 + c.head_dim * type_bytes(c.type)), st);
       with_type(c.type, [&](auto z) {
         using T = decltype(z);
-        join_partials_kernel<T><<<(unsigned)ceil_div(rows, here), 256, 0, st>>>(m, (T*)out, share, here);
+        const size_t bytes = (size_t)here * c.keep * 8 + (share > 1 ? 256 * 9 * 4 : 0);
+        join_partials_kernel<T><<<(unsigned)ceil_div(rows, here), 256, bytes, st>>>(m, (T*)out, share, here);
       });
       launch_check("block_join");
     }

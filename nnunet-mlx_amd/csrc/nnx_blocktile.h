@@ -53,7 +53,7 @@ struct Tile {
 // start from: 0, or -inf for keys that are not valid.  Whether any value is not finite (16-bit types).
 template <class T, int DP, int BK>
 __device__ __forceinline__ bool stage_block(const ChunkArgs& c, int b, int g, int j, T* lk, T* lv,
-                                            float* bias) {
+                                            float* bias, bool negate) {
   using G = Tile<T, DP, BK>;
   const int length = item_length(c.a, b), first = j * BK;
   const T* k = (const T*)c.k + b * c.a.ks[0] + g * c.a.ks[2];
@@ -78,6 +78,10 @@ __device__ __forceinline__ bool stage_block(const ChunkArgs& c, int b, int g, in
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int e = 0; e < G::CH; ++e) odd |= !(fabsf(to_float(vr[i].v[e])) < INFINITY);
+    }
+    if (negate) {
+#pragma unroll
+      for (int e = 0; e < G::CH; ++e) kr[i].v[e] = -kr[i].v[e];
     }
     if (n < N) {
       const int at = G::at(n / G::CHUNKS, n % G::CHUNKS);
@@ -117,8 +121,7 @@ __device__ __forceinline__ void load_query(QueryRow<T, DP>& row, const T* q, boo
 template <class T, int DP, int BK>
 __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, const T* lv,
                                             const float* bias, bool live, const QueryRow<T, DP>& q,
-                                            int64_t last, int first_key, float c2, bool negate,
-                                            bool odd, int64_t partial) {
+                                            int last, float c2, bool odd, int64_t partial) {
   using G = Tile<T, DP, BK>;
   const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;
   f32x16 acc[G::KT];
@@ -136,10 +139,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
   if constexpr (sizeof(T) == 2) {
     Frag<T> qf[DP / 16];
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      __builtin_memcpy(&qf[s], &q.v[s], 16);
-      if (negate) qf[s] = -qf[s];
-    }
+    for (int s = 0; s < DP / 16; ++s) __builtin_memcpy(&qf[s], &q.v[s], 16);
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
@@ -148,9 +148,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
   } else {
 #pragma unroll
     for (int s = 0; s < DP / 8; ++s) {
-      Vec<float, 4> qf = q.v[s];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) qf.v[i] = negate ? -qf.v[i] : qf.v[i];
+      const Vec<float, 4> qf = q.v[s];
 #pragma unroll
       for (int kt = 0; kt < G::KT; ++kt) {
         const float4 kf = *(const float4*)(lk + G::at(kt * 32 + col, 2 * s + half));
@@ -161,14 +159,13 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
       }
     }
   }
-  if (c.a.causal && __any(live && last < first_key + BK - 1)) {
+  if (__any(last < BK - 1)) {  // the query's own block, or one behind it
+    const int seen = last - 4 * half;
 #pragma unroll
     for (int kt = 0; kt < G::KT; ++kt)
 #pragma unroll
-      for (int r = 0; r < G::REGS; ++r) {
-        const int key = first_key + kt * 32 + 8 * (r / 4) + 4 * half + r % 4;
-        if (key > last) acc[kt][r] = -INFINITY;
-      }
+      for (int r = 0; r < G::REGS; ++r)
+        if (kt * 32 + 8 * (r / 4) + r % 4 > seen) acc[kt][r] = -INFINITY;
   }
   float m = -INFINITY;
 #pragma unroll
@@ -228,7 +225,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
       }
   }
   // Registers 4i .. 4i + 3 of o[dt] are channels 32 dt + 8 i + 4 half + 0..3 of the lane's row.
-  const float sum = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // 0: nothing seen; NaN stays
+  const float sum = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);  // 0: nothing seen; NaN stays
   float2 meta = make_float2(l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l), sum);
   if constexpr (sizeof(T) == 2) {
     // In whole 2^-15ths of the row's largest magnitude: an error of 2^-16 of it, a tenth of what
@@ -238,7 +235,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(o[dt][r]));
+      for (int r = 0; r < 16; r += 2) big = fmaxf(fmaxf(big, fabsf(o[dt][r])), fabsf(o[dt][r + 1]));
     if (odd) {
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
@@ -247,7 +244,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
     }
     const float2 bh = both_halves(big);
     big = fmaxf(fmaxf(bh.x, bh.y), 7.52e-37f);  // 2^-120, where the reciprocal is finite
-    const float down = 1.f / big;
+    const float down = __builtin_amdgcn_rcpf(big);
     meta.y *= big;
     if (live && half == 0) c.meta[partial] = meta;
     int16_t* part = (int16_t*)c.part + partial * c.a.dim;
@@ -297,71 +294,103 @@ __device__ __forceinline__ int find_tile(const int32_t* tiles, int n, int tile) 
   return lo;
 }
 
+// How many of a block's keys a query at `at` sees, less one: below 0 none, BK - 1 all.
+__device__ __forceinline__ int last_seen(const BlockArgs& a, int64_t at, int first_key) {
+  return a.causal ? (int)min(max(at - first_key, (int64_t)-1), (int64_t)1 << 20) : 1 << 20;
+}
+
+// Registers for two waves a SIMD where that leaves nothing in memory (accumulators then stay
+// where vector instructions reach them).
+template <class T, int DP, int BK>
+constexpr int kWaves = sizeof(T) == 2 || DP * BK <= 64 * 64 ? 2 : 1;
+
 template <class T, int DP, int BK, bool BY_BLOCK>
-__global__ __launch_bounds__(256) void block_partials_kernel(ChunkArgs c) {
+__global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kernel(ChunkArgs c) {
   using G = Tile<T, DP, BK>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* lk = (T*)lds;
   T* lv = lk + G::ROWS * DP;
   float* bias = (float*)(lv + G::ROWS * DP);
   const BlockArgs& a = c.a;
-  const int wave = threadIdx.x / 64, col = threadIdx.x % 32;
-  // scores' sign in the queries, so that the largest weight belongs to the largest product; a
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = threadIdx.x % 32;
+  // the scale's sign goes to the keys, so that the largest weight belongs to the largest product; a
   // factor of 0 stays above it, which keeps -inf times it -inf
   const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-35f);
   const bool negate = a.scale < 0.f;
   if constexpr (BY_BLOCK) {
     const int all = c.units * a.blocks;
     const int total = c.tiles[all];
-    const int t_lo = (int)((int64_t)blockIdx.x * total / gridDim.x);
     const int t_hi = (int)((int64_t)(blockIdx.x + 1) * total / gridDim.x);
-    int held = -1, unit = 0, b = 0, g = 0, j = 0, first_tile = 0, next_tile = 0, rows = 0, list0 = 0;
-    int64_t start = 0;
-    bool odd = false;
-    for (int tile = t_lo; tile < t_hi; ++tile) {
-      if (held < 0 || tile >= next_tile) {
-        held = held < 0 ? find_tile(c.tiles, all, tile)
-                        : held + 1 + find_tile(c.tiles + held + 1, all - held - 1, tile);
-        unit = held / a.blocks;
-        j = held - unit * a.blocks;
-        b = (c.unit0 + unit) / a.kv_heads;
-        g = c.unit0 + unit - b * a.kv_heads;
-        first_tile = c.tiles[held];
-        next_tile = c.tiles[held + 1];
-        list0 = c.start[held];
-        rows = (c.start[held + 1] - list0) * a.group;
-        start = item_start(a, b) + c.t0;
-        __syncthreads();  // the block before has been read
-        odd = stage_block<T, DP, BK>(c, b, g, j, lk, lv, bias);
+    int tile = (int)((int64_t)blockIdx.x * total / gridDim.x), held = -1;
+    while (tile < t_hi) {
+      held = held < 0 ? find_tile(c.tiles, all, tile)
+                      : held + 1 + find_tile(c.tiles + held + 1, all - held - 1, tile);
+      held = __builtin_amdgcn_readfirstlane(held);
+      const int unit = held / a.blocks, j = held - unit * a.blocks;
+      const int b = (c.unit0 + unit) / a.kv_heads, g = c.unit0 + unit - b * a.kv_heads;
+      const int first_tile = c.tiles[held], to = min(c.tiles[held + 1], t_hi);
+      const int32_t* list = c.list + c.start[held];
+      const int rows = (c.start[held + 1] - c.start[held]) * a.group;
+      const int64_t start = item_start(a, b) + c.t0;
+      const T* queries = (const T*)c.q + b * a.qs[0] + c.t0 * a.qs[1] + (int64_t)g * a.group * a.qs[2];
+      const int64_t partials = (int64_t)unit * c.nt * a.group;
+      // a row of the tile: its list entry a tile ahead, its query a tile ahead of its products
+      struct Row {
+        int entry, h;
+        bool live;
+      };
+      const auto locate = [&](int at) {
+        const int row = (at - first_tile) * kTileRows + wave * 32 + col;
+        Row r;
+        r.live = at < to && row < rows;
+        const int pair = r.live ? c.by_group(row) : 0;
+        r.h = r.live ? row - pair * a.group : 0;
+        r.entry = list[pair];
+        return r;
+      };
+      const auto fetch = [&](const Row& r, QueryRow<T, DP>& q) {
+        load_query<T, DP>(q, queries + c.by_keep(r.entry) * a.qs[1] + r.h * a.qs[2], r.live, a.dim);
+      };
+      constexpr bool AHEAD = sizeof(QueryRow<T, DP>) <= 128;
+      Row row = locate(tile), next = locate(tile + 1);
+      __syncthreads();  // the block before has been read
+      const bool odd = stage_block<T, DP, BK>(c, b, g, j, lk, lv, bias, negate);
+      QueryRow<T, DP> q, q_next;
+      if constexpr (AHEAD) fetch(row, q);
+      for (; tile < to; ++tile) {
+        if constexpr (AHEAD) {
+          fetch(next, q_next);
+        } else {
+          fetch(row, q);
+        }
+        const Row after = locate(tile + 2);
+        if (__any(row.live)) {
+          const int t = c.by_keep(row.entry), slot = row.entry - t * a.keep;
+          const int64_t partial = (partials + (int64_t)t * a.group + row.h) * a.keep + slot;
+          attend_rows<T, DP, BK>(c, lk, lv, bias, row.live, q, last_seen(a, start + t, j * BK), c2, odd,
+                                 partial);
+        }
+        row = next;
+        next = after;
+        if constexpr (AHEAD) q = q_next;
       }
-      const int row = (tile - first_tile) * kTileRows + wave * 32 + col;
-      if (__all(row >= rows)) continue;
-      const bool live = row < rows;
-      const int pair = live ? row / a.group : 0, h = live ? row - pair * a.group : 0;
-      const int entry = c.list[list0 + pair];
-      const int t = entry / a.keep, slot = entry - t * a.keep;
-      QueryRow<T, DP> q;
-      load_query<T, DP>(q, (const T*)c.q + b * a.qs[0] + (c.t0 + t) * a.qs[1] + (g * a.group + h) * a.qs[2],
-                        live, a.dim);
-      const int64_t partial = (((int64_t)unit * c.nt + t) * a.group + h) * a.keep + slot;
-      attend_rows<T, DP, BK>(c, lk, lv, bias, live, q, start + t, j * BK, c2, negate, odd, partial);
     }
   } else {
-    const int item = blockIdx.x, slot = item % a.keep, ut = item / a.keep;
+    const int item = blockIdx.x, ut = c.by_keep(item), slot = item - ut * a.keep;
     const int unit = ut / c.nt, t = ut - unit * c.nt;
     const int b = (c.unit0 + unit) / a.kv_heads, g = c.unit0 + unit - b * a.kv_heads;
     const int j = c.ids[(((int64_t)b * a.queries + c.t0 + t) * a.kv_heads + g) * a.keep + slot];
     if (j < 0 || j >= a.blocks) return;
-    const bool odd = stage_block<T, DP, BK>(c, b, g, j, lk, lv, bias);
+    const bool odd = stage_block<T, DP, BK>(c, b, g, j, lk, lv, bias, negate);
+    const int last = last_seen(a, item_start(a, b) + c.t0 + t, j * BK);
     for (int h0 = wave * 32; h0 < a.group; h0 += 128) {
       const bool live = h0 + col < a.group;
       const int h = live ? h0 + col : 0;
       QueryRow<T, DP> q;
-      load_query<T, DP>(q, (const T*)c.q + b * a.qs[0] + (c.t0 + t) * a.qs[1] + (g * a.group + h) * a.qs[2],
+      load_query<T, DP>(q, (const T*)c.q + b * a.qs[0] + (c.t0 + t) * a.qs[1] + (int64_t)(g * a.group + h) * a.qs[2],
                         live, a.dim);
       const int64_t partial = (((int64_t)unit * c.nt + t) * a.group + h) * a.keep + slot;
-      attend_rows<T, DP, BK>(c, lk, lv, bias, live, q, item_start(a, b) + c.t0 + t, j * BK, c2, negate,
-                             odd, partial);
+      attend_rows<T, DP, BK>(c, lk, lv, bias, live, q, last, c2, odd, partial);
     }
   }
 }
