@@ -37,27 +37,36 @@ __device__ __forceinline__ int64_t item_start(const BlockArgs& a, int b) {
   return a.start0 + (a.start ? a.start[b] : 0);
 }
 
-// Partial results of a chunk: key heads [unit0, unit0 + units) of all items (unit = item *
-// kv_heads + key head) and queries [t0, t0 + nt).  Row = (unit, query, head of the group); every
-// row has `keep` partials, one a kept block: `dim` values (float32, or for 16-bit types int16 in
-// 32767ths of a common factor) and (log2 of the sum of its weights, factor of the values over that
-// sum).
+// The queries of each key head of each item are cut into `splits` spans of `nt`; span v = (item *
+// kv_heads + key head) * splits + split.  A launch covers spans [span0, span0 + spans).  Row =
+// (span, query of the span, head of the group), counted from span0; every row has `keep`
+// partials, one a kept block: `dim` values (float32, or for 16-bit types int16 in 32767ths of a
+// common factor) and (log2 of the sum of its weights, factor of the values over that sum).
 struct ChunkArgs {
   BlockArgs a;
   const void *q, *k, *v;
   const int32_t* ids;
   void* part;
   float2* meta;
-  int unit0, units, t0, nt;
+  int span0, spans, splits, nt;
   FastDiv by_keep, by_group, by_nt;
-  // by block: pairs (query, slot) that keep it, list[start[u]...], in tiles of kTileRows rows
-  // (pairs * group heads), tiles[u] of them before block u = unit * blocks + block
+  // by block: pairs (query, slot) of a span that keep it, list[start[u]...], in tiles of kTileRows
+  // rows (pairs * group heads), tiles[u] of them before block u = (span - span0) * blocks + block
   const int32_t *list, *start, *tiles;
 };
 
+struct Span {
+  int b, g, t0, queries;
+};
+
+__device__ __forceinline__ Span span_of(const ChunkArgs& c, int v) {
+  const int unit = v / c.splits, b = unit / c.a.kv_heads, t0 = (v - unit * c.splits) * c.nt;
+  return {b, unit - b * c.a.kv_heads, t0, min(c.nt, c.a.queries - t0)};
+}
+
 constexpr int kTileRows = 128;
 
-// Attention of a chunk's rows to each of their kept blocks, a partial result each.  `by_block`:
+// Attention of a launch's rows to each of their kept blocks, a partial result each.  `by_block`:
 // rows gathered by the block that they keep (list, start, tiles; `grid` workgroups share the
 // tiles), else a workgroup for each kept block of each query.
 void block_partials_f32(const ChunkArgs& c, bool by_block, int grid, hipStream_t st);

@@ -357,28 +357,34 @@ __global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, co
 // rows against a block that stays in LDS, one partial softmax a pair, and a last pass that joins
 // each row's partials.  Few pairs skip the gathering: a workgroup each.
 
-// Pairs of a chunk in groups of `per` queries of one unit (grid: groups, units).  Counts by block
-// in LDS; each group takes its range of every block's list by one addition to the block's total.
-// The order of groups in a list is left to chance and shows in no result: a row's partial does not
-// depend on its neighbours in a tile.
-__global__ __launch_bounds__(256) void count_pairs_kernel(ChunkArgs c, int per, int32_t* total,
-                                                          int32_t* base, int32_t* rank) {
-  extern __shared__ int32_t hist[];
+// Calls body(entry, block) for the pairs of `per` queries of a span (grid: groups, spans).
+template <class F>
+__device__ __forceinline__ void each_pair(const ChunkArgs& c, int per, F&& body) {
   const BlockArgs& a = c.a;
-  const int unit = blockIdx.y, t_lo = blockIdx.x * per, t_hi = min(t_lo + per, c.nt);
-  const int b = (c.unit0 + unit) / a.kv_heads, g = c.unit0 + unit - b * a.kv_heads;
-  for (int j = threadIdx.x; j < a.blocks; j += 256) hist[j] = 0;
-  __syncthreads();
-  const int32_t* ids = c.ids + (((int64_t)b * a.queries + c.t0) * a.kv_heads + g) * a.keep;
+  const Span s = span_of(c, c.span0 + blockIdx.y);
+  const int t_lo = blockIdx.x * per, t_hi = min(t_lo + per, s.queries);
+  const int32_t* ids = c.ids + (((int64_t)s.b * a.queries + s.t0) * a.kv_heads + s.g) * a.keep;
   for (int e = t_lo * a.keep + threadIdx.x; e < t_hi * a.keep; e += 256) {
-    const int t = c.by_keep(e), s = e - t * a.keep;
-    const int j = ids[(int64_t)t * a.kv_heads * a.keep + s];
-    if (j >= 0 && j < a.blocks) rank[(int64_t)unit * c.nt * a.keep + e] = atomicAdd(&hist[j], 1);
+    const int t = c.by_keep(e);
+    const int j = ids[(int64_t)t * a.kv_heads * a.keep + e - t * a.keep];
+    if ((unsigned)j < (unsigned)a.blocks) body(e, j);
   }
+}
+
+// Counts by block in LDS; each group takes its range of every block's list by one addition to the
+// block's total.  The order of groups and pairs in a list is left to chance and shows in no
+// result: a row's partial does not depend on its neighbours in a tile.
+__global__ __launch_bounds__(256) void count_pairs_kernel(ChunkArgs c, int per, int32_t* total,
+                                                          int32_t* base) {
+  extern __shared__ int32_t hist[];
+  const int blocks = c.a.blocks;
+  for (int j = threadIdx.x; j < blocks; j += 256) hist[j] = 0;
   __syncthreads();
-  int32_t* mine = base + ((int64_t)unit * gridDim.x + blockIdx.x) * a.blocks;
-  for (int j = threadIdx.x; j < a.blocks; j += 256)
-    if (hist[j]) mine[j] = atomicAdd(&total[unit * a.blocks + j], hist[j]);
+  each_pair(c, per, [&](int, int j) { atomicAdd(&hist[j], 1); });
+  __syncthreads();
+  int32_t* mine = base + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * blocks;
+  for (int j = threadIdx.x; j < blocks; j += 256)
+    if (hist[j]) mine[j] = atomicAdd(&total[blockIdx.y * blocks + j], hist[j]);
 }
 
 // Where each block's list starts, and its tiles: running sums over n totals, by one workgroup.
@@ -418,18 +424,15 @@ __global__ __launch_bounds__(1024) void scan_pairs_kernel(const int32_t* total, 
   if (threadIdx.x == 0) start[n] = before.x, tiles[n] = before.y;
 }
 
-__global__ __launch_bounds__(256) void place_pairs_kernel(ChunkArgs c, int per, int groups,
-                                                          const int32_t* base, const int32_t* rank,
+__global__ __launch_bounds__(256) void place_pairs_kernel(ChunkArgs c, int per, const int32_t* base,
                                                           int32_t* list) {
-  const BlockArgs& a = c.a;
-  const int unit = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x;
-  if (e >= c.nt * a.keep) return;
-  const int b = (c.unit0 + unit) / a.kv_heads, g = c.unit0 + unit - b * a.kv_heads;
-  const int t = c.by_keep(e), s = e - t * a.keep;
-  const int j = c.ids[(((int64_t)b * a.queries + c.t0 + t) * a.kv_heads + g) * a.keep + s];
-  if (j < 0 || j >= a.blocks) return;
-  const int from = base[((int64_t)unit * groups + t / per) * a.blocks + j];
-  list[c.start[unit * a.blocks + j] + from + rank[(int64_t)unit * c.nt * a.keep + e]] = e;
+  extern __shared__ int32_t next[];
+  const int blocks = c.a.blocks;
+  const int32_t* mine = base + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * blocks;
+  // base holds nothing for blocks without pairs here, and their place is not asked for
+  for (int j = threadIdx.x; j < blocks; j += 256) next[j] = c.start[blockIdx.y * blocks + j] + mine[j];
+  __syncthreads();
+  each_pair(c, per, [&](int e, int j) { list[atomicAdd(&next[j], 1)] = e; });
 }
 
 // out = sum_s w_s O_s / sum_s w_s with w_s = 2^(log2 sum_s - largest), O_s a partial under its
@@ -445,21 +448,23 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
   extern __shared__ float2 weight[];
   float(*sums)[9] = (float(*)[9])(weight + each * c.a.keep);
   const BlockArgs& a = c.a;
-  const int64_t row0 = (int64_t)blockIdx.x * each, rows = (int64_t)c.units * c.nt * a.group;
+  const int64_t row0 = (int64_t)blockIdx.x * each, rows = (int64_t)c.spans * c.nt * a.group;
   const int here = (int)min((int64_t)each, rows - row0);
-  const auto place = [&](int64_t row, int& b, int& t, int& g, int& h) {
-    const int ut = c.by_group((int)row), unit = c.by_nt(ut);
-    h = (int)row - ut * a.group;
-    t = c.t0 + ut - unit * c.nt;
-    b = (c.unit0 + unit) / a.kv_heads;
-    g = c.unit0 + unit - b * a.kv_heads;
+  const auto place = [&](int64_t row, Span& s, int& t, int& h) {
+    const int vt = c.by_group((int)row), span = c.by_nt(vt);
+    h = (int)row - vt * a.group;
+    t = vt - span * c.nt;
+    s = span_of(c, c.span0 + span);
   };
   for (int i = threadIdx.x; i < here * a.keep; i += 256) {
-    const int r = c.by_keep(i), s = i - r * a.keep;
-    int b, t, g, h;
-    place(row0 + r, b, t, g, h);
-    const int j = c.ids[(((int64_t)b * a.queries + t) * a.kv_heads + g) * a.keep + s];
-    weight[i] = (unsigned)j < (unsigned)a.blocks ? c.meta[(row0 + r) * a.keep + s]
+    const int r = c.by_keep(i), slot = i - r * a.keep;
+    Span s;
+    int t, h;
+    place(row0 + r, s, t, h);
+    int j = -1;
+    if (t < s.queries)
+      j = c.ids[(((int64_t)s.b * a.queries + s.t0 + t) * a.kv_heads + s.g) * a.keep + slot];
+    weight[i] = (unsigned)j < (unsigned)a.blocks ? c.meta[(row0 + r) * a.keep + slot]
                                                  : make_float2(-INFINITY, 0.f);
   }
   __syncthreads();
@@ -497,42 +502,51 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
     }
   }
   if (!live) return;
-  int b, t, g, h;
-  place(row0 + own, b, t, g, h);
+  Span s;
+  int t, h;
+  place(row0 + own, s, t, h);
+  if (t >= s.queries) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   Vec<T, 8> r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) r.v[i] = from_float<T>(o[i] * inv);
-  store_vec(out + b * a.os[0] + t * a.os[1] + (int64_t)(g * a.group + h) * a.os[2] + 8 * u, r);
+  store_vec(out + s.b * a.os[0] + (s.t0 + t) * a.os[1] + (int64_t)(s.g * a.group + h) * a.os[2] + 8 * u, r);
 }
 
-// One pass's work and where it lies in the workspace.  Chunks hold whole units where those fit the
-// budget, else parts of one unit's queries.
-constexpr size_t kPartialBudget = (size_t)1 << 30;
+// Where the work is cut and where it lies in the workspace.  Spans and the launches that cover
+// some of them are sized for their partials to stay in the 256 MiB last-level cache until they are
+// joined (a launch over everything took 1.35 times as long at 5 x 32768 queries of 32 blocks);
+// the lists of many launches are formed at once.
+constexpr size_t kPartialBudget = (size_t)160 << 20;
+constexpr int64_t kListPairs = (int64_t)1 << 27;
 constexpr int64_t kDirectPairs = 8192;
 
 struct AttentionPlan {
   bool by_block;
-  int units, nt;     // of a chunk
-  int per, groups;   // queries of a counting group, groups of a unit
-  int64_t pairs;     // of a chunk
-  size_t total, base, start, tiles, rank, list, meta, part, bytes;
+  int splits, nt, spans;      // spans in all
+  int at_once, listed;        // spans of a launch, spans whose lists are formed together
+  int per, groups;            // queries of a counting group, groups of a span
+  size_t total, base, start, tiles, list, meta, part, bytes;
 };
 
 AttentionPlan make_plan(const nnx_block_config& c) {
   AttentionPlan p;
   const int64_t group = c.heads / c.kv_heads, blocks = ceil_div(c.keys, c.block);
-  const size_t row = (size_t)c.keep * (8 + (size_t)c.head_dim * type_bytes(c.type));
-  const int64_t all_units = (int64_t)c.batch * c.kv_heads;
-  const int64_t query = group * row;  // bytes of a query's partials in one unit
-  p.nt = (int)std::max<int64_t>(1, std::min<int64_t>(c.queries, kPartialBudget / query));
-  p.units = p.nt < c.queries
-                ? 1
-                : (int)std::max<int64_t>(1, std::min<int64_t>(all_units, kPartialBudget / (query * p.nt)));
-  // counts and tiles are 32-bit, and a chunk's units a grid axis
-  p.units = (int)std::min<int64_t>(p.units, std::max<int64_t>(1, std::min<int64_t>(65535, (1 << 30) / blocks)));
-  p.pairs = (int64_t)p.units * p.nt * c.keep;
-  p.by_block = all_units * c.queries * c.keep > kDirectPairs;
+  // bytes of the partials of a query and key head: at most 256 * 130 * 4 a head
+  const int64_t query = group * c.keep * (8 + (int64_t)c.head_dim * type_bytes(c.type));
+  const int64_t fit = std::max<int64_t>(1, kPartialBudget / query);
+  p.nt = (int)ceil_div(c.queries, ceil_div(c.queries, fit));
+  p.splits = (int)ceil_div(c.queries, p.nt);
+  const int64_t spans = (int64_t)c.batch * c.kv_heads * p.splits;
+  require(spans < (int64_t)1 << 31, "block attention: too many queries and key heads");
+  p.spans = (int)spans;
+  p.by_block = (double)c.batch * c.kv_heads * c.queries * c.keep > kDirectPairs;
+  p.at_once = (int)std::max<int64_t>(1, std::min(spans, fit / p.nt));
+  // counts and tiles are 32-bit, and spans a grid axis
+  const int64_t most = std::min<int64_t>({spans, 65535, ((int64_t)1 << 30) / blocks, kListPairs / ((int64_t)p.nt * c.keep)});
+  p.at_once = (int)std::min<int64_t>(p.at_once, std::max<int64_t>(1, std::min<int64_t>(65535, ((int64_t)1 << 30) / blocks)));
+  p.at_once = (int)ceil_div(spans, ceil_div(spans, p.at_once));  // launches of one size
+  p.listed = p.by_block ? (int)std::max<int64_t>(p.at_once, most) : p.at_once;
   p.per = (int)std::min<int64_t>(p.nt, ceil_div(std::max<int64_t>(4096, 2 * blocks), c.keep));
   p.groups = (int)ceil_div(p.nt, p.per);
   size_t at = 0;
@@ -541,15 +555,15 @@ AttentionPlan make_plan(const nnx_block_config& c) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  const size_t lists = p.by_block ? (size_t)p.units * blocks : 0;
+  const size_t lists = p.by_block ? (size_t)p.listed * blocks : 0;
+  const size_t rows = (size_t)p.at_once * p.nt * group * c.keep;
   p.total = take(lists * 4);
   p.base = take(lists * p.groups * 4);
   p.start = take((lists + 1) * 4);
   p.tiles = take((lists + 1) * 4);
-  p.rank = take(p.by_block ? p.pairs * 4 : 0);
-  p.list = take(p.by_block ? p.pairs * 4 : 0);
-  p.meta = take((size_t)p.pairs * group * 8);
-  p.part = take((size_t)p.pairs * group * c.head_dim * type_bytes(c.type));
+  p.list = take(p.by_block ? (size_t)p.listed * p.nt * c.keep * 4 : 0);
+  p.meta = take(rows * 8);
+  p.part = take(rows * c.head_dim * type_bytes(c.type));
   p.bytes = at;
   return p;
 }
@@ -617,10 +631,10 @@ void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
 size_t block_attention_workspace(const nnx_block_config& c) {
   try {
     check_config(c, "block attention", true);
+    return make_plan(c).bytes;
   } catch (const Error&) {
     return 0;
   }
-  return make_plan(c).bytes;
 }
 
 void block_attention(const nnx_block_config& c, const void* q, const void* k, const void* v,
@@ -639,33 +653,39 @@ void block_attention(const nnx_block_config& c, const void* q, const void* k, co
   k0.q = q, k0.k = k, k0.v = v, k0.ids = ids;
   k0.part = w + p.part;
   k0.meta = (float2*)(w + p.meta);
-  k0.list = at(p.list), k0.start = at(p.start), k0.tiles = at(p.tiles);
-  const int all_units = c.batch * c.kv_heads;
-  const double flops = 4.0 * c.heads / c.kv_heads * c.keep * c.block * c.head_dim;
-  for (int u = 0; u < all_units; u += p.units) {
-    for (int t = 0; t < c.queries; t += p.nt) {
+  k0.list = at(p.list);
+  k0.splits = p.splits, k0.nt = p.nt;
+  k0.by_keep = FastDiv(c.keep), k0.by_group = FastDiv(a.group), k0.by_nt = FastDiv(p.nt);
+  const double flops = 4.0 * a.group * c.keep * c.block * c.head_dim * p.nt;
+  for (int l0 = 0; l0 < p.spans; l0 += p.listed) {
+    const int listed = std::min(p.listed, p.spans - l0);
+    if (p.by_block) {
+      const int lists = listed * a.blocks;
       ChunkArgs m = k0;
-      m.unit0 = u, m.units = std::min(p.units, all_units - u);
-      m.t0 = t, m.nt = std::min(p.nt, c.queries - t);
-      m.by_keep = FastDiv(c.keep), m.by_group = FastDiv(a.group), m.by_nt = FastDiv(m.nt);
-      const int64_t pairs = (int64_t)m.units * m.nt * c.keep;
+      m.span0 = l0, m.spans = listed;
+      m.start = at(p.start);
+      ProfScope prof("block_lists", 0.0, 12.0 * listed * p.nt * c.keep, st);
+      fill_zero(w + p.total, (size_t)lists * 4, st);
+      count_pairs_kernel<<<dim3(p.groups, listed), 256, a.blocks * 4, st>>>(m, p.per, at(p.total), at(p.base));
+      launch_check("count_pairs");
+      scan_pairs_kernel<<<1, 1024, 0, st>>>(at(p.total), lists, a.group, at(p.start), at(p.tiles));
+      launch_check("scan_pairs");
+      place_pairs_kernel<<<dim3(p.groups, listed), 256, a.blocks * 4, st>>>(m, p.per, at(p.base), at(p.list));
+      launch_check("place_pairs");
+    }
+    for (int s0 = 0; s0 < listed; s0 += p.at_once) {
+      ChunkArgs m = k0;
+      m.span0 = l0 + s0, m.spans = std::min(p.at_once, listed - s0);
+      m.start = at(p.start) + (size_t)s0 * a.blocks;
+      m.tiles = at(p.tiles) + (size_t)s0 * a.blocks;
+      const int64_t pairs = (int64_t)m.spans * p.nt * c.keep;
       int grid = (int)pairs;
       if (p.by_block) {
-        const int lists = m.units * a.blocks, groups = (int)ceil_div(m.nt, p.per);
-        ProfScope prof("block_lists", 0.0, 16.0 * pairs, st);
-        fill_zero(w + p.total, (size_t)lists * 4, st);
-        count_pairs_kernel<<<dim3(groups, m.units), 256, a.blocks * 4, st>>>(
-            m, p.per, at(p.total), at(p.base), at(p.rank));
-        launch_check("count_pairs");
-        scan_pairs_kernel<<<1, 1024, 0, st>>>(at(p.total), lists, a.group, at(p.start), at(p.tiles));
-        launch_check("scan_pairs");
-        place_pairs_kernel<<<dim3((unsigned)ceil_div((int64_t)m.nt * c.keep, 256), m.units), 256, 0, st>>>(
-            m, p.per, groups, at(p.base), at(p.rank), at(p.list));
-        launch_check("place_pairs");
-        grid = (int)std::min<int64_t>(ceil_div(pairs * a.group, kTileRows) + lists, 4 * compute_units());
+        grid = (int)std::min<int64_t>(ceil_div(pairs * a.group, kTileRows) + (int64_t)m.spans * a.blocks,
+                                      3 * compute_units());
       }
       {
-        ProfScope prof("block_partials", flops * m.units * m.nt, 0.0, st);
+        ProfScope prof("block_partials", flops * m.spans, 0.0, st);
         if (c.type == NNX_TYPE_F32) {
           block_partials_f32(m, p.by_block, grid, st);
         } else if (c.type == NNX_TYPE_F16) {
@@ -674,7 +694,7 @@ void block_attention(const nnx_block_config& c, const void* q, const void* k, co
           block_partials_bf16(m, p.by_block, grid, st);
         }
       }
-      const int64_t rows = (int64_t)m.units * m.nt * a.group;
+      const int64_t rows = (int64_t)m.spans * p.nt * a.group;
       const int lanes = a.dim / 8;
       // groups of lanes a row: more while rows are too few for the CUs or their weights for the LDS
       int share = 1;

@@ -42,7 +42,9 @@ struct Tile {
   static constexpr int ROW_BYTES = DP * sizeof(T);
   static constexpr int PER = ROW_BYTES >= 256 ? 1 : 256 / ROW_BYTES;  // rows in 256 bytes
   static constexpr int TURNS = CHUNKS & -CHUNKS;   // a power of two that divides CHUNKS
-  static constexpr size_t LDS = (size_t)2 * ROWS * ROW_BYTES + ROWS * sizeof(float);
+  // keys, values, where scores start from, and for each wave 32 rows of 128 bytes on their way out
+  static constexpr int OUT = 32 * 128;
+  static constexpr size_t LDS = (size_t)2 * ROWS * ROW_BYTES + ROWS * sizeof(float) + 4 * OUT;
   static __device__ __forceinline__ int at(int row, int chunk) {
     const int turn = (row / PER) & (TURNS - 1);
     return row * DP + (chunk ^ turn) * CH;
@@ -96,6 +98,41 @@ __device__ __forceinline__ bool stage_block(const ChunkArgs& c, int b, int g, in
   return __syncthreads_or(odd);
 }
 
+// Stores into the partials go through buffer instructions: 32-bit offsets, and one past the buffer's
+// end stores nothing, so that a tile's dead rows need no branch (a branch around a store leaves its
+// count of outstanding accesses open, and the next tile's queries would be waited for with it).
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t kNowhere = 0xffffff00u;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(void* p, size_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, (int)(uint32_t)bytes, 0x00027000);
+}
+
+// Chunks of 16 bytes, one row's in two lanes (8 of them make 128 bytes of a row), leave as whole
+// rows: through LDS, 8 lanes a row.
+struct RowWriter {
+  char* lds;  // of the wave
+  __amdgpu_buffer_rsrc_t part;
+  uint32_t row;  // offset of the lane's row, kNowhere for none
+  uint32_t bytes;  // of a row
+  __device__ __forceinline__ void put(int chunk, u32x4 v) const {
+    const int col = threadIdx.x % 32;
+    *(u32x4*)__builtin_assume_aligned(lds + col * 128 + ((chunk ^ (col & 7)) * 16), 16) = v;
+  }
+  __device__ __forceinline__ void flush(int pass) const {
+    const int lane = threadIdx.x % 64, chunk = lane % 8;
+    const uint32_t at = pass * 128 + chunk * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + lane / 8;
+      const u32x4 v = *(const u32x4*)__builtin_assume_aligned(lds + r * 128 + ((chunk ^ (r & 7)) * 16), 16);
+      const uint32_t to = __shfl(row, r);
+      __builtin_amdgcn_raw_buffer_store_b128(v, part, at < bytes && to != kNowhere ? to + at : kNowhere, 0, 0);
+    }
+  }
+};
+
 // 32 query rows, a lane pair (l, l + 32) each: S^T = K Q^T leaves a row's scores in its two
 // lanes' registers, so the softmax needs one exchange between halves, and its weights are
 // already the second operand of O^T = V^T P^T (the order of keys is that of the registers; values
@@ -103,25 +140,25 @@ __device__ __forceinline__ bool stage_block(const ChunkArgs& c, int b, int g, in
 template <class T, int DP>
 struct QueryRow {
   static constexpr int CH = 16 / sizeof(T), N = DP / (2 * CH);
-  Vec<T, CH> v[N];  // a half's chunks: 2 s + half
+  u32x4 v[N];  // a half's chunks: 2 s + half
 };
 
+// Chunks past the row's end are filled from inside it; the keys are 0 there.
 template <class T, int DP>
-__device__ __forceinline__ void load_query(QueryRow<T, DP>& row, const T* q, bool live, int dim) {
+__device__ __forceinline__ void load_query(QueryRow<T, DP>& row, const T* q, int dim) {
   using Q = QueryRow<T, DP>;
   const int half = threadIdx.x % 64 / 32;
 #pragma unroll
-  for (int s = 0; s < Q::N; ++s) {
-    const int d = (2 * s + half) * Q::CH;
-    row.v[s] = Vec<T, Q::CH>{};
-    if (live && d < dim) row.v[s] = load_vec<Q::CH>(q + d);
-  }
+  for (int s = 0; s < Q::N; ++s)
+    __builtin_memcpy(&row.v[s], q + min((2 * s + half) * Q::CH, dim - Q::CH), 16);
 }
 
-template <class T, int DP, int BK>
+template <class T, int DP, int BK, class F>
 __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, const T* lv,
-                                            const float* bias, bool live, const QueryRow<T, DP>& q,
-                                            int last, float c2, bool odd, int64_t partial) {
+                                            const float* bias, char* out_lds,
+                                            __amdgpu_buffer_rsrc_t part, __amdgpu_buffer_rsrc_t metas,
+                                            const QueryRow<T, DP>& q, int last, float c2, bool odd,
+                                            uint32_t partial, F&& before_stores) {
   using G = Tile<T, DP, BK>;
   const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;
   f32x16 acc[G::KT];
@@ -148,7 +185,8 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
   } else {
 #pragma unroll
     for (int s = 0; s < DP / 8; ++s) {
-      const Vec<float, 4> qf = q.v[s];
+      Vec<float, 4> qf;
+      __builtin_memcpy(&qf, &q.v[s], 16);
 #pragma unroll
       for (int kt = 0; kt < G::KT; ++kt) {
         const float4 kf = *(const float4*)(lk + G::at(kt * 32 + col, 2 * s + half));
@@ -226,6 +264,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
   }
   // Registers 4i .. 4i + 3 of o[dt] are channels 32 dt + 8 i + 4 half + 0..3 of the lane's row.
   const float sum = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);  // 0: nothing seen; NaN stays
+  before_stores();
   float2 meta = make_float2(l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l), sum);
   if constexpr (sizeof(T) == 2) {
     // In whole 2^-15ths of the row's largest magnitude: an error of 2^-16 of it, a tenth of what
@@ -246,10 +285,10 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
     big = fmaxf(fmaxf(bh.x, bh.y), 7.52e-37f);  // 2^-120, where the reciprocal is finite
     const float down = __builtin_amdgcn_rcpf(big);
     meta.y *= big;
-    if (live && half == 0) c.meta[partial] = meta;
-    int16_t* part = (int16_t*)c.part + partial * c.a.dim;
+    const uint32_t bytes = c.a.dim * 2;
+    const RowWriter writer{out_lds, part, partial == kNowhere ? kNowhere : partial * bytes, bytes};
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
+    for (int dt = 0; dt < DP / 32; ++dt) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t w[4];
@@ -262,22 +301,27 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
         // channels 8 apart, 4 a half, become 8 neighbours a half
         const auto r0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
         const auto r1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-        const Vec<uint32_t, 4> out{{r0[0], r1[0], r0[1], r1[1]}};
-        const int d = 32 * dt + 16 * i + 8 * half;
-        if (live && d < c.a.dim) store_vec((uint32_t*)(part + d), out);
+        writer.put(4 * (dt % 2) + 2 * i + half, u32x4{r0[0], r1[0], r0[1], r1[1]});
       }
+      if (dt % 2 || dt + 1 == DP / 32) writer.flush(dt / 2);
+    }
   } else {
-    if (live && half == 0) c.meta[partial] = meta;
-    float* part = (float*)c.part + partial * c.a.dim;
+    const uint32_t bytes = c.a.dim * 4;
+    const RowWriter writer{out_lds, part, partial == kNowhere ? kNowhere : partial * bytes, bytes};
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
+    for (int dt = 0; dt < DP / 32; ++dt) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int d = 32 * dt + 8 * i + 4 * half;
-        const Vec<float, 4> out{{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]}};
-        if (live && d < c.a.dim) store_vec(part + d, out);
+        u32x4 w;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = __float_as_uint(o[dt][4 * i + r]);
+        writer.put(2 * i + half, w);
       }
+      writer.flush(dt);
+    }
   }
+  const u32x2 words{__float_as_uint(meta.x), __float_as_uint(meta.y)};
+  __builtin_amdgcn_raw_buffer_store_b64(words, metas, half || partial == kNowhere ? kNowhere : partial * 8, 0, 0);
 }
 
 // The last u in [0, n) with tiles[u] <= tile, by all lanes at once.
@@ -302,7 +346,7 @@ __device__ __forceinline__ int last_seen(const BlockArgs& a, int64_t at, int fir
 // Registers for two waves a SIMD where that leaves nothing in memory (accumulators then stay
 // where vector instructions reach them).
 template <class T, int DP, int BK>
-constexpr int kWaves = sizeof(T) == 2 || DP * BK <= 64 * 64 ? 2 : 1;
+constexpr int kWaves = DP * BK * sizeof(T) <= (sizeof(T) == 2 ? 128 * 96 * 2 : 64 * 64 * 4) ? 2 : 1;
 
 template <class T, int DP, int BK, bool BY_BLOCK>
 __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kernel(ChunkArgs c) {
@@ -311,29 +355,33 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
   T* lk = (T*)lds;
   T* lv = lk + G::ROWS * DP;
   float* bias = (float*)(lv + G::ROWS * DP);
+  char* out_lds = (char*)(bias + G::ROWS) + threadIdx.x / 64 * G::OUT;
   const BlockArgs& a = c.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = threadIdx.x % 32;
   // the scale's sign goes to the keys, so that the largest weight belongs to the largest product; a
   // factor of 0 stays above it, which keeps -inf times it -inf
   const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-35f);
   const bool negate = a.scale < 0.f;
+  const size_t partials_all = (size_t)c.spans * c.nt * a.group * a.keep;
+  const auto part = buffer_of(c.part, partials_all * a.dim * (sizeof(T) == 2 ? 2 : 4));
+  const auto metas = buffer_of(c.meta, partials_all * 8);
   if constexpr (BY_BLOCK) {
-    const int all = c.units * a.blocks;
-    const int total = c.tiles[all];
-    const int t_hi = (int)((int64_t)(blockIdx.x + 1) * total / gridDim.x);
-    int tile = (int)((int64_t)blockIdx.x * total / gridDim.x), held = -1;
+    const int all = c.spans * a.blocks, tile0 = c.tiles[0];
+    const int64_t total = c.tiles[all] - tile0;
+    const int t_hi = tile0 + (int)((blockIdx.x + 1) * total / gridDim.x);
+    int tile = tile0 + (int)(blockIdx.x * total / gridDim.x), held = -1;
     while (tile < t_hi) {
       held = held < 0 ? find_tile(c.tiles, all, tile)
                       : held + 1 + find_tile(c.tiles + held + 1, all - held - 1, tile);
       held = __builtin_amdgcn_readfirstlane(held);
-      const int unit = held / a.blocks, j = held - unit * a.blocks;
-      const int b = (c.unit0 + unit) / a.kv_heads, g = c.unit0 + unit - b * a.kv_heads;
+      const int span = held / a.blocks, j = held - span * a.blocks;
+      const Span s = span_of(c, c.span0 + span);
       const int first_tile = c.tiles[held], to = min(c.tiles[held + 1], t_hi);
       const int32_t* list = c.list + c.start[held];
       const int rows = (c.start[held + 1] - c.start[held]) * a.group;
-      const int64_t start = item_start(a, b) + c.t0;
-      const T* queries = (const T*)c.q + b * a.qs[0] + c.t0 * a.qs[1] + (int64_t)g * a.group * a.qs[2];
-      const int64_t partials = (int64_t)unit * c.nt * a.group;
+      const int64_t start = item_start(a, s.b) + s.t0;
+      const T* queries = (const T*)c.q + s.b * a.qs[0] + s.t0 * a.qs[1] + (int64_t)s.g * a.group * a.qs[2];
+      const uint32_t partials = (uint32_t)span * c.nt * a.group;
       // a row of the tile: its list entry a tile ahead, its query a tile ahead of its products
       struct Row {
         int entry, h;
@@ -349,48 +397,75 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
         return r;
       };
       const auto fetch = [&](const Row& r, QueryRow<T, DP>& q) {
-        load_query<T, DP>(q, queries + c.by_keep(r.entry) * a.qs[1] + r.h * a.qs[2], r.live, a.dim);
+        load_query<T, DP>(q, queries + c.by_keep(r.entry) * a.qs[1] + r.h * a.qs[2], a.dim);
       };
-      constexpr bool AHEAD = sizeof(QueryRow<T, DP>) <= 128;
+      bool odd;
+      const auto attend = [&](const Row& r, const QueryRow<T, DP>& q, auto&& before_stores) {
+        const int t = c.by_keep(r.entry), slot = r.entry - t * a.keep;
+        const uint32_t partial = (partials + t * a.group + r.h) * a.keep + slot;
+        attend_rows<T, DP, BK>(c, lk, lv, bias, out_lds, part, metas, q, last_seen(a, start + t, j * BK), c2,
+                               odd, r.live ? partial : kNowhere, before_stores);
+      };
+      // What was asked for during a tile is waited for before the tile's stores: accesses end in
+      // order, and a wait behind the stores would be one for them too.
+      const auto settle = [](QueryRow<T, DP>& q, Row& r) {
+#pragma unroll
+        for (u32x4& v : q.v) asm volatile("" : "+v"(v));
+        asm volatile("" : "+v"(r.entry));
+      };
       Row row = locate(tile), next = locate(tile + 1);
       __syncthreads();  // the block before has been read
-      const bool odd = stage_block<T, DP, BK>(c, b, g, j, lk, lv, bias, negate);
-      QueryRow<T, DP> q, q_next;
-      if constexpr (AHEAD) fetch(row, q);
-      for (; tile < to; ++tile) {
-        if constexpr (AHEAD) {
-          fetch(next, q_next);
-        } else {
-          fetch(row, q);
+      odd = stage_block<T, DP, BK>(c, s.b, s.g, j, lk, lv, bias, negate);
+      QueryRow<T, DP> q0;
+      fetch(row, q0);
+      settle(q0, next);
+      if constexpr (sizeof(q0) <= 128) {
+        // Two tiles a turn, so that the queries on their way stay in the registers they arrive in.
+        QueryRow<T, DP> q1;
+        while (true) {
+          Row after = locate(tile + 2);
+          fetch(next, q1);
+          attend(row, q0, [&] { settle(q1, after); });
+          if (++tile >= to) break;
+          row = locate(tile + 2);
+          fetch(after, q0);
+          attend(next, q1, [&] { settle(q0, row); });
+          if (++tile >= to) break;
+          next = row;
+          row = after;
         }
-        const Row after = locate(tile + 2);
-        if (__any(row.live)) {
-          const int t = c.by_keep(row.entry), slot = row.entry - t * a.keep;
-          const int64_t partial = (partials + (int64_t)t * a.group + row.h) * a.keep + slot;
-          attend_rows<T, DP, BK>(c, lk, lv, bias, row.live, q, last_seen(a, start + t, j * BK), c2, odd,
-                                 partial);
+      } else {
+        while (true) {
+          Row after = locate(tile + 2);
+          attend(row, q0, [&] {
+            fetch(next, q0);
+            settle(q0, after);
+          });
+          if (++tile >= to) break;
+          row = next;
+          next = after;
         }
-        row = next;
-        next = after;
-        if constexpr (AHEAD) q = q_next;
       }
     }
   } else {
-    const int item = blockIdx.x, ut = c.by_keep(item), slot = item - ut * a.keep;
-    const int unit = ut / c.nt, t = ut - unit * c.nt;
-    const int b = (c.unit0 + unit) / a.kv_heads, g = c.unit0 + unit - b * a.kv_heads;
-    const int j = c.ids[(((int64_t)b * a.queries + c.t0 + t) * a.kv_heads + g) * a.keep + slot];
+    const int item = blockIdx.x, vt = c.by_keep(item), slot = item - vt * a.keep;
+    const int span = c.by_nt(vt), t = vt - span * c.nt;
+    const Span s = span_of(c, c.span0 + span);
+    if (t >= s.queries) return;
+    const int j = c.ids[(((int64_t)s.b * a.queries + s.t0 + t) * a.kv_heads + s.g) * a.keep + slot];
     if (j < 0 || j >= a.blocks) return;
-    const bool odd = stage_block<T, DP, BK>(c, b, g, j, lk, lv, bias, negate);
-    const int last = last_seen(a, item_start(a, b) + c.t0 + t, j * BK);
+    const bool odd = stage_block<T, DP, BK>(c, s.b, s.g, j, lk, lv, bias, negate);
+    const int last = last_seen(a, item_start(a, s.b) + s.t0 + t, j * BK);
     for (int h0 = wave * 32; h0 < a.group; h0 += 128) {
       const bool live = h0 + col < a.group;
       const int h = live ? h0 + col : 0;
       QueryRow<T, DP> q;
-      load_query<T, DP>(q, (const T*)c.q + b * a.qs[0] + (c.t0 + t) * a.qs[1] + (int64_t)(g * a.group + h) * a.qs[2],
-                        live, a.dim);
-      const int64_t partial = (((int64_t)unit * c.nt + t) * a.group + h) * a.keep + slot;
-      attend_rows<T, DP, BK>(c, lk, lv, bias, live, q, last, c2, odd, partial);
+      load_query<T, DP>(q, (const T*)c.q + s.b * a.qs[0] + (s.t0 + t) * a.qs[1] +
+                               (int64_t)(s.g * a.group + h) * a.qs[2],
+                        a.dim);
+      const uint32_t partial = (vt * a.group + h) * a.keep + slot;
+      attend_rows<T, DP, BK>(c, lk, lv, bias, out_lds, part, metas, q, last, c2, odd,
+                             live ? partial : kNowhere, [] {});
     }
   }
 }
