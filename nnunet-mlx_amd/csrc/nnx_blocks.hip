@@ -129,118 +129,157 @@ __global__ __launch_bounds__(256) void summarize_kernel(BlockArgs a, const T* k,
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// The kept blocks of one row of scores (in LDS), written by a wave: the `keep` highest, equal ones by
-// the lower index, never -inf.  A cut is searched by halving until exactly `keep` scores lie above
-// it: of the values at first, which ends in some 9 steps for scores with gaps, then of their order
-// as whole numbers, which ends in 32 at a value whose equals are taken from the lowest index on.
-// N > 0: the row stays in N registers a lane; N = 0: it is read from LDS for every step.
+// The kept blocks of one row of scores, written by a wave: those of `forced` and the highest scores,
+// equal ones by the lower index.  A score that is no candidate is NaN, which no comparison takes.
+// A cut is searched by halving until exactly as many scores as are wanted lie above it: of the
+// values at first, which ends in some 9 steps for scores with gaps, then of their order as whole
+// numbers, which ends in 32 at a value whose equals are taken from the lowest index on.
+struct Cut {
+  float above;  // kept: scores above it, and the first `ties` that equal it
+  int ties;
+};
+
+template <class Above, class Range>
+__device__ __forceinline__ Cut find_cut(int want, Above&& above, Range&& range) {
+  if (want <= 0) return {INFINITY, 0};
+  if (above(-INFINITY) <= want) return {-INFINITY, 0};
+  float low, high;  // above(low) >= want > above(high), but for the lowest score
+  range(low, high);
+  const int over = above(low);
+  if (over < want) return {low, want - over};
+  for (int step = 0; step < 14; ++step) {
+    const float mid = 0.5f * low + 0.5f * high;
+    const int count = above(mid);
+    if (count == want) return {mid, 0};
+    (count < want ? high : low) = mid;
+  }
+  const auto order = [](float v) {
+    const int32_t b = __float_as_int(v + 0.f);
+    return b ^ (b >> 31 & 0x7fffffff);
+  };
+  const auto back = [](int32_t o) { return __int_as_float(o ^ (o >> 31 & 0x7fffffff)); };
+  int32_t lo = order(low), hi = order(high);
+  while ((int64_t)hi - lo > 1) {
+    const int32_t mid = (int32_t)(((int64_t)lo + hi) >> 1);
+    (above(back(mid)) < want ? hi : lo) = mid;
+  }
+  return {back(hi), want - above(back(hi))};
+}
+
+__device__ __forceinline__ int lanes_before(uint64_t lanes, int from) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32),
+                                        __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, (uint32_t)from));
+}
+
+// N > 0: the row (in LDS, filled up to 64 N with NaN) is held in N registers a lane; N = 0: it is read
+// again for every step.
 template <int N>
-__device__ __forceinline__ void select_row(const float* score, int blocks, int keep, int32_t* out) {
-  const int lane = threadIdx.x % 64, n = N ? N : (blocks + 63) / 64;
-  float held[N ? N : 1];
-  const auto value = [&](int i) { return i * 64 + lane < blocks ? score[i * 64 + lane] : -INFINITY; };
-  if constexpr (N > 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) held[i] = value(i);
-  }
-  const auto each = [&](auto&& body) {
-    if constexpr (N > 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) body(i, held[i]);
-    } else {
-      for (int i = 0; i < n; ++i) body(i, value(i));
+__device__ __forceinline__ void select_row(float* score, int blocks, int keep, int first, int local,
+                                           int own, int32_t* out) {
+  const int lane = threadIdx.x % 64;
+  uint32_t marks = 0;  // N > 0: chunks of 64 in which this lane's block is forced; N = 0: +inf marks it
+  int forced = 0;
+  const auto force = [&](int begin, int end) {  // blocks begin .. end - 1 as far as they are candidates
+    for (int j0 = begin / 64 * 64; j0 < end; j0 += 64) {
+      const int j = j0 + lane;
+      const bool take = j >= begin && j < end && score[j] > -INFINITY && score[j] < INFINITY;
+      if (take) {
+        score[j] = N ? NAN : INFINITY;
+        marks |= 1u << (j / 64 % 32);
+      }
+      forced += __popcll(__ballot(take));
     }
   };
-  const auto above = [&](float x) {
-    int count = 0;
-    each([&](int, float v) { count += __popcll(__ballot(v > x)); });
-    return count;
-  };
-  const auto larger = [](float x, float y) { return fmaxf(x, y); };
-  float cut = -INFINITY;  // kept: scores above it, and the first `ties` that equal it
-  int ties = 0;
-  if (above(-INFINITY) > keep) {
-    float low = INFINITY, high = -INFINITY;  // above(low) >= keep > above(high)
-    each([&](int, float v) {
-      low = fminf(low, v > -INFINITY ? v : low);
-      high = fmaxf(high, v);
-    });
-    low = -lanes_reduce<64>(-low, larger);
-    high = lanes_reduce<64>(high, larger);
-    bool found = false;
-    if (high == INFINITY) {  // blocks kept whatever their score
-      const int forced = above(3.4028235e38f);
-      if (forced >= keep) {
-        cut = INFINITY;
-        ties = keep;
-        found = true;
-      } else {
-        high = -INFINITY;
-        each([&](int, float v) { high = fmaxf(high, v < INFINITY ? v : high); });
-        high = lanes_reduce<64>(high, larger);
-      }
-    }
-    if (!found && above(low) < keep) {  // the lowest score is the last one kept
-      cut = low;
-      ties = keep - above(low);
-      found = true;
-    }
-    for (int step = 0; step < 14 && !found; ++step) {
-      const float mid = 0.5f * low + 0.5f * high;
-      const int count = above(mid);
-      if (count == keep) {
-        cut = mid;
-        found = true;
-      }
-      (count < keep ? high : low) = mid;
-    }
-    if (!found) {
-      const auto order = [](float v) {
-        const int32_t b = __float_as_int(v + 0.f);
-        return b ^ (b >> 31 & 0x7fffffff);
-      };
-      const auto back = [](int32_t o) { return __int_as_float(o ^ (o >> 31 & 0x7fffffff)); };
-      int32_t lo = order(low), hi = order(high);
-      while ((int64_t)hi - lo > 1) {
-        const int32_t mid = (int32_t)(((int64_t)lo + hi) >> 1);
-        (above(back(mid)) < keep ? hi : lo) = mid;
-      }
-      cut = back(hi);
-      ties = keep - above(cut);
-    }
-  }
-  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  force(0, min(first, blocks));
+  force(max(own + 1 - local, 0), min(own + 1, blocks));
   int done = 0, tied = 0;
-  each([&](int i, float v) {
-    bool take = v > cut;
+  const auto emit = [&](int i, uint64_t equal, bool take, int ties) {
     if (ties) {
-      const uint64_t equal = __ballot(v == cut);
-      take |= ((equal >> lane) & 1) && tied + __popcll(equal & below) < ties;
+      take |= ((equal >> lane) & 1) && lanes_before(equal, tied) < ties;
       tied += __popcll(equal);
     }
     const uint64_t taken = __ballot(take);
-    const int to = done + __popcll(taken & below);
-    if (take && to < keep) out[to] = i * 64 + lane;
+    const int to = lanes_before(taken, done);
+    if (take && to < keep) out[(uint32_t)to] = i * 64 + lane;
     done += __popcll(taken);
-  });
+  };
+  const auto larger = [](float x, float y) { return fmaxf(x, y); };
+  if constexpr (N > 0) {
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = score[i * 64 + lane];
+    uint32_t chunks = 0;  // in which any lane's block is forced
+    for (uint64_t lanes = __ballot(marks != 0); lanes; lanes &= lanes - 1)
+      chunks |= __builtin_amdgcn_readlane(marks, __builtin_ctzll(lanes));
+    const Cut cut = find_cut(
+        keep - forced,
+        [&](float x) {
+          int count = 0;
+#pragma unroll
+          for (int i = 0; i < N; ++i) count += __popcll(__ballot(v[i] > x));
+          return count;
+        },
+        [&](float& low, float& high) {
+          low = INFINITY, high = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < N; ++i) low = v[i] < low ? v[i] : low, high = v[i] > high ? v[i] : high;
+          low = -lanes_reduce<64>(-low, larger);
+          high = lanes_reduce<64>(high, larger);
+        });
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      bool take = v[i] > cut.above;
+      if (chunks >> i & 1) take |= marks >> i & 1;
+      emit(i, cut.ties ? __ballot(v[i] == cut.above) : 0, take, cut.ties);
+    }
+  } else {
+    const int n = (blocks + 63) / 64;
+    const auto value = [&](int i) { return i * 64 + lane < blocks ? score[i * 64 + lane] : NAN; };
+    const Cut cut = find_cut(
+        keep - forced,
+        [&](float x) {
+          int count = 0;
+          for (int i = 0; i < n; ++i) {
+            const float v = value(i);
+            count += __popcll(__ballot(v > x && v < INFINITY));
+          }
+          return count;
+        },
+        [&](float& low, float& high) {
+          low = INFINITY, high = -INFINITY;
+          for (int i = 0; i < n; ++i) {
+            const float v = value(i);
+            low = v < low ? v : low, high = v > high && v < INFINITY ? v : high;
+          }
+          low = -lanes_reduce<64>(-low, larger);
+          high = lanes_reduce<64>(high, larger);
+        });
+    for (int i = 0; i < n; ++i) {
+      const float v = value(i);
+      emit(i, __ballot(cut.ties && v == cut.above), v > cut.above || v == INFINITY, cut.ties);
+    }
+  }
   for (int i = min(done, keep) + lane; i < keep; i += 64) out[i] = -1;
 }
 
 // `rows` <= 16 queries of one item and key head: their scores against 16 blocks at a time by 8-bit
 // products in whole numbers, kept in LDS; then a wave a query picks.  Heads that share the key
-// head are taken HEADS at a time (their codes in LDS) and meet in the largest score.
+// head are taken kScoreHeads at a time (their codes in LDS) and meet in the largest score.  A
+// wave's next blocks are on their way while it scores the ones before.
+constexpr int kScoreHeads = 8;
+
 template <class T, int N>
-__global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, const int8_t* codes,
-                                                     const float* scales, int32_t* ids, int rows,
-                                                     int pitch) {
-  constexpr int HEADS = 4, WAVES = 8;
+__global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, const int8_t* codes,
+                                                      const float* scales, int32_t* ids, int rows,
+                                                      int pitch) {
   extern __shared__ __attribute__((aligned(16))) float score[];  // rows x pitch
-  __shared__ i32x4 qcode[HEADS][2][64];
-  __shared__ float qtop[HEADS][16];
+  i32x4* qcode = (i32x4*)(score + rows * pitch);                 // by head, 64 channels, lane
+  __shared__ float qtop[kScoreHeads][16];
   const int t0 = blockIdx.x * rows, g = blockIdx.y, b = blockIdx.z;
   const int lane = threadIdx.x % 64, col = lane % 16, quad = lane / 16;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
   const int64_t unit = (int64_t)b * a.kv_heads + g;
+  const bool wide = a.dim > 64;
   // the block of a query's own position: -1 before the first key, at most 2^24 (past the last block)
   const auto own_block = [&](int r) {
     const int64_t at = item_start(a, b) + t0 + r;
@@ -249,71 +288,70 @@ __global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, co
   const int own = a.causal ? own_block(col) : 1 << 24;
   const int8_t* cu = codes + unit * a.blocks * a.dim;
   const float* su = scales + unit * a.blocks;
-  for (int h0 = 0; h0 < a.group; h0 += HEADS) {
-    const int heads = min(HEADS, a.group - h0);
+  struct Blocks {
+    i32x4 k[2];
+    float scale[4];
+  };
+  // Past the last block and past the head's end anything in range: the first is not kept, and the
+  // queries' codes are 0 in the second.
+  const auto load = [&](Blocks& x, int j0) {
+    const int8_t* row = cu + (int64_t)min(j0 + col, a.blocks - 1) * a.dim;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s && !wide) break;
+      int w[4];
+      __builtin_memcpy(w, row + min(s * 64 + quad * 16, a.dim - 8), 8);
+      __builtin_memcpy(w + 2, row + min(s * 64 + quad * 16 + 8, a.dim - 8), 8);
+      x.k[s] = i32x4{w[0], w[1], w[2], w[3]};
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x.scale[r] = su[min(j0 + quad * 4 + r, a.blocks - 1)];
+  };
+  if (N) {
+    const int full = (a.blocks + 15) / 16 * 16, rest = N * 64 - full;
+    for (int i = threadIdx.x; i < rows * rest; i += blockDim.x)
+      score[i / rest * pitch + full + i % rest] = NAN;
+  }
+  for (int h0 = 0; h0 < a.group; h0 += kScoreHeads) {
+    const int heads = min(kScoreHeads, a.group - h0);
+    Blocks x0, x1;
+    load(x0, wave * 16);
     if (h0) __syncthreads();
-    if (wave < heads) {  // a wave a head, in the lanes' places of the products' second operand
-      const bool live = col < rows && t0 + col < a.queries;
-      const T* row = q + b * a.qs[0] + (int64_t)(t0 + col) * a.qs[1] +
-                     (int64_t)(g * a.group + h0 + wave) * a.qs[2];
-      float v[32];
-      float m = 0.f;
+    // 16 lanes a query and head, 8 channels each, into the places of the products' second operand
+    for (int i = threadIdx.x / 16; i < heads * 16; i += blockDim.x / 16) {
+      const int h = i / 16, t = i % 16, d = lane % 16 * 8;
+      Vec<T, 8> x{};
+      if (t < rows && t0 + t < a.queries && d < a.dim)
+        x = load_vec<8>(q + b * a.qs[0] + (int64_t)(t0 + t) * a.qs[1] + (int64_t)(g * a.group + h0 + h) * a.qs[2] + d);
+      float v[8], m = 0.f;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int d = (s / 2) * 64 + quad * 16 + (s % 2) * 8;
-        Vec<T, 8> x{};
-        if (live && d < a.dim) x = load_vec<8>(row + d);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[8 * s + e] = finite_or_zero(to_float(x.v[e]));
-          m = fmaxf(m, fabsf(v[8 * s + e]));
-        }
+      for (int e = 0; e < 8; ++e) {
+        v[e] = finite_or_zero(to_float(x.v[e]));
+        m = fmaxf(m, fabsf(v[e]));
       }
-      m = fmaxf(m, __shfl_xor(m, 16));
-      m = fmaxf(m, __shfl_xor(m, 32));
+      m = lanes_reduce<16>(m, [](float p, float r) { return fmaxf(p, r); });
       const float up = m < kTiny ? 0.f : __fdiv_rn(127.f, m);
-      if (quad == 0) qtop[wave][col] = m < kTiny ? 1.f : m;
+      uint32_t w[2] = {0, 0};
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        i32x4 word;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t bytes = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            bytes |= ((uint32_t)(int)rintf(v[16 * s + 4 * w + e] * up) & 255u) << (8 * e);
-          word[w] = (int)bytes;
-        }
-        qcode[wave][s][lane] = word;
+      for (int e = 0; e < 8; ++e) w[e / 4] |= ((uint32_t)(int)rintf(v[e] * up) & 255u) << (8 * (e % 4));
+      if (d < 64 || wide) {
+        uint32_t* to = (uint32_t*)&qcode[(h * 2 + d / 64) * 64 + d % 64 / 16 * 16 + t] + d % 16 / 4;
+        to[0] = w[0], to[1] = w[1];
       }
+      if (lane % 16 == 0) qtop[h][t] = m < kTiny ? 1.f : m;
     }
     __syncthreads();
-    for (int j0 = wave * 16; j0 < a.blocks; j0 += WAVES * 16) {
-      i32x4 kc[2] = {};
-      const int8_t* row = cu + (int64_t)min(j0 + col, a.blocks - 1) * a.dim;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int d = (s / 2) * 64 + quad * 16 + (s % 2) * 8;
-        if (d < a.dim) {
-          int w[2];
-          __builtin_memcpy(w, row + d, 8);
-          kc[s / 2][(s % 2) * 2] = w[0];
-          kc[s / 2][(s % 2) * 2 + 1] = w[1];
-        }
-      }
-      float scale[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) scale[r] = su[min(j0 + quad * 4 + r, a.blocks - 1)];
+    const auto compute = [&](const Blocks& x, int j0) {
       float best[4];
       for (int h = 0; h < heads; ++h) {
         i32x4 dot = {0, 0, 0, 0};
-        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[0], qcode[h][0][lane], dot, 0, 0, 0);
-        if (a.dim > 64) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[1], qcode[h][1][lane], dot, 0, 0, 0);
+        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[0], qcode[h * 128 + lane], dot, 0, 0, 0);
+        if (wide) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[1], qcode[h * 128 + 64 + lane], dot, 0, 0, 0);
         const float top = qtop[h][col];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float x = ((float)dot[r] * top) * scale[r];
-          best[r] = h ? fmaxf(best[r], x) : x;
+          const float y = ((float)dot[r] * top) * x.scale[r];
+          best[r] = h ? fmaxf(best[r], y) : y;
         }
       }
       if (col < rows) {
@@ -325,29 +363,31 @@ __global__ __launch_bounds__(512) void select_kernel(BlockArgs a, const T* q, co
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (scale[r] < 0.f) best[r] = -INFINITY;  // no valid key
-        if (a.causal) {
+          if (x.scale[r] < 0.f) best[r] = NAN;  // no valid key
+        if (a.causal || j0 + 16 > a.blocks) {
+          const int end = min(own, a.blocks - 1);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (j0 + quad * 4 + r > own) best[r] = -INFINITY;
+            if (j0 + quad * 4 + r > end) best[r] = NAN;
         }
         *to = make_float4(best[0], best[1], best[2], best[3]);
       }
+    };
+    int j0 = wave * 16;
+    while (j0 < a.blocks) {
+      load(x1, j0 + waves * 16);
+      compute(x0, j0);
+      j0 += waves * 16;
+      if (j0 >= a.blocks) break;
+      load(x0, j0 + waves * 16);
+      compute(x1, j0);
+      j0 += waves * 16;
     }
   }
   __syncthreads();
-  for (int r = wave; r < rows && t0 + r < a.queries; r += WAVES) {
-    float* row = score + r * pitch;
-    const int at = own_block(r);
-    // blocks kept whatever their score, where they can be
-    const auto keep_block = [&](int j) {
-      if (j < a.blocks && row[j] > -INFINITY) row[j] = INFINITY;
-    };
-    for (int j = lane; j < min(a.first, a.blocks); j += 64) keep_block(j);
-    for (int i = max(at - a.blocks + 1, 0) + lane; i < min(a.local, at + 1); i += 64) keep_block(at - i);
-    select_row<N>(row, a.blocks, a.keep,
+  for (int r = wave; r < rows && t0 + r < a.queries; r += waves)
+    select_row<N>(score + r * pitch, a.blocks, a.keep, a.first, a.local, own_block(r),
                   ids + (((int64_t)b * a.queries + t0 + r) * a.kv_heads + g) * a.keep);
-  }
 }
 
 // ---- the attention ---------------------------------------------------------------------
@@ -604,25 +644,29 @@ void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
   const double products = (double)c.batch * c.queries * c.heads * c.head_dim;
   ProfScope prof("block_select", 2.0 * products * a.blocks, products * type_bytes(c.type), st);
   // As many queries a workgroup as the products take, while their scores fit the LDS; rows of up to
-  // 2048 blocks are picked from registers.
-  const int pitch = (int)ceil_div(a.blocks, 16) * 16 + 4;
+  // 2048 blocks are picked from registers.  Few workgroups take twice the waves.
+  int n = 1;
+  while (n < 32 && n * 64 < a.blocks) n *= 2;
+  if (n * 64 < a.blocks) n = 0;
+  const int pitch = (n ? n * 64 : (int)ceil_div(a.blocks, 16) * 16) + 4;
+  const size_t heads = (size_t)std::min(a.group, kScoreHeads) * 2048;
   int rows = 16;
-  while (rows > 1 && (size_t)rows * pitch * 4 > 139264) rows /= 2;
+  while (rows > 1 && (size_t)rows * pitch * 4 + heads > 160 * 1024 - 1024) rows /= 2;
+  const dim3 grid((unsigned)ceil_div(c.queries, rows), c.kv_heads, c.batch);
+  const int threads = (double)grid.x * grid.y * grid.z < 2 * compute_units() ? 1024 : 512;
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    const dim3 grid((unsigned)ceil_div(c.queries, rows), c.kv_heads, c.batch);
-    auto go = [&](auto n) {
-      select_kernel<T, decltype(n)::value><<<grid, 512, rows * pitch * sizeof(float), st>>>(
+    auto go = [&](auto k) {
+      select_kernel<T, decltype(k)::value><<<grid, threads, rows * pitch * sizeof(float) + heads, st>>>(
           a, (const T*)q, codes, scales, ids, rows, pitch);
     };
     using std::integral_constant;
-    const int64_t n = ceil_div(a.blocks, 64);
-    if (n <= 1) return go(integral_constant<int, 1>{});
-    if (n <= 2) return go(integral_constant<int, 2>{});
-    if (n <= 4) return go(integral_constant<int, 4>{});
-    if (n <= 8) return go(integral_constant<int, 8>{});
-    if (n <= 16) return go(integral_constant<int, 16>{});
-    if (n <= 32) return go(integral_constant<int, 32>{});
+    if (n == 1) return go(integral_constant<int, 1>{});
+    if (n == 2) return go(integral_constant<int, 2>{});
+    if (n == 4) return go(integral_constant<int, 4>{});
+    if (n == 8) return go(integral_constant<int, 8>{});
+    if (n == 16) return go(integral_constant<int, 16>{});
+    if (n == 32) return go(integral_constant<int, 32>{});
     go(integral_constant<int, 0>{});
   });
   launch_check("block_select");
