@@ -66,6 +66,11 @@ __device__ __forceinline__ Span span_of(const ChunkArgs& c, int v) {
 
 constexpr int kTileRows = 128;
 
+// Buffer accesses take 32-bit offsets, and past the buffer's end load 0 and store nothing.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, size_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)(uint32_t)bytes, 0x00027000);
+}
+
 // Attention of a launch's rows to each of their kept blocks, a partial result each.  `by_block`:
 // rows gathered by the block that they keep (list, start, tiles; `grid` workgroups share the
 // tiles), else a workgroup for each kept block of each query.

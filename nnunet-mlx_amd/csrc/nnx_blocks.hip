@@ -141,7 +141,7 @@ struct Cut {
 
 template <class Above, class Range>
 __device__ __forceinline__ Cut find_cut(int want, Above&& above, Range&& range) {
-  if (want <= 0) return {INFINITY, 0};
+  if (want <= 0) return {3.4028235e38f, 0};  // but +inf, which forced blocks have in the end
   if (above(-INFINITY) <= want) return {-INFINITY, 0};
   float low, high;  // above(low) >= want > above(high), but for the lowest score
   range(low, high);
@@ -177,7 +177,9 @@ template <int N>
 __device__ __forceinline__ void select_row(float* score, int blocks, int keep, int first, int local,
                                            int own, int32_t* out) {
   const int lane = threadIdx.x % 64;
-  uint32_t marks = 0;  // N > 0: chunks of 64 in which this lane's block is forced; N = 0: +inf marks it
+  // N > 0: chunks of 64 in which this lane's block is forced, NaN while the others are compared;
+  // N = 0: forced blocks are +inf all the time
+  uint32_t marks = 0;
   int forced = 0;
   const auto force = [&](int begin, int end) {  // blocks begin .. end - 1 as far as they are candidates
     for (int j0 = begin / 64 * 64; j0 < end; j0 += 64) {
@@ -190,8 +192,8 @@ __device__ __forceinline__ void select_row(float* score, int blocks, int keep, i
       forced += __popcll(__ballot(take));
     }
   };
-  force(0, min(first, blocks));
-  force(max(own + 1 - local, 0), min(own + 1, blocks));
+  if (first) force(0, min(first, blocks));
+  if (local) force(max(own + 1 - local, 0), min(own + 1, blocks));
   int done = 0, tied = 0;
   const auto emit = [&](int i, uint64_t equal, bool take, int ties) {
     if (ties) {
@@ -208,9 +210,6 @@ __device__ __forceinline__ void select_row(float* score, int blocks, int keep, i
     float v[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = score[i * 64 + lane];
-    uint32_t chunks = 0;  // in which any lane's block is forced
-    for (uint64_t lanes = __ballot(marks != 0); lanes; lanes &= lanes - 1)
-      chunks |= __builtin_amdgcn_readlane(marks, __builtin_ctzll(lanes));
     const Cut cut = find_cut(
         keep - forced,
         [&](float x) {
@@ -226,11 +225,23 @@ __device__ __forceinline__ void select_row(float* score, int blocks, int keep, i
           low = -lanes_reduce<64>(-low, larger);
           high = lanes_reduce<64>(high, larger);
         });
+    if (forced) {
+      for (uint32_t m = marks; m; m &= m - 1) score[__builtin_ctz(m) * 64 + lane] = INFINITY;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      bool take = v[i] > cut.above;
-      if (chunks >> i & 1) take |= marks >> i & 1;
-      emit(i, cut.ties ? __ballot(v[i] == cut.above) : 0, take, cut.ties);
+      for (int i = 0; i < N; ++i) v[i] = score[i * 64 + lane];
+    }
+    if (cut.ties || forced > keep) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        emit(i, __ballot(v[i] == cut.above), v[i] > cut.above || v[i] == INFINITY, cut.ties);
+    } else {  // no more than `keep` lie above the cut
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool take = v[i] > cut.above;
+        const uint64_t taken = __ballot(take);
+        if (take) out[(uint32_t)lanes_before(taken, done)] = i * 64 + lane;
+        done += __popcll(taken);
+      }
     }
   } else {
     const int n = (blocks + 63) / 64;
@@ -280,32 +291,33 @@ __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, c
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
   const int64_t unit = (int64_t)b * a.kv_heads + g;
   const bool wide = a.dim > 64;
+  const int shift = __builtin_ctz(a.block);
   // the block of a query's own position: -1 before the first key, at most 2^24 (past the last block)
   const auto own_block = [&](int r) {
-    const int64_t at = item_start(a, b) + t0 + r;
-    return at < 0 ? -1 : (int)min(at / a.block, (int64_t)1 << 24);
+    const int64_t at = (item_start(a, b) + t0 + r) >> shift;
+    return (int)min(max(at, (int64_t)-1), (int64_t)1 << 24);
   };
   const int own = a.causal ? own_block(col) : 1 << 24;
-  const int8_t* cu = codes + unit * a.blocks * a.dim;
-  const float* su = scales + unit * a.blocks;
+  const uint32_t unit_bytes = (uint32_t)a.blocks * a.dim;
+  const auto cu = buffer_of(codes + unit * unit_bytes, unit_bytes);
+  const auto su = buffer_of(scales + unit * a.blocks, a.blocks * 4);
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
   struct Blocks {
-    i32x4 k[2];
-    float scale[4];
+    i32x2 k[4];
+    int scale[4];
   };
-  // Past the last block and past the head's end anything in range: the first is not kept, and the
-  // queries' codes are 0 in the second.
+  // Past the last block all is 0 and not kept; past the head's end lie the next block's codes, and the
+  // queries' codes are 0.
+  const uint32_t code_at = (uint32_t)(col * a.dim + quad * 16), scale_at = (uint32_t)(quad * 16);
   const auto load = [&](Blocks& x, int j0) {
-    const int8_t* row = cu + (int64_t)min(j0 + col, a.blocks - 1) * a.dim;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (s && !wide) break;
-      int w[4];
-      __builtin_memcpy(w, row + min(s * 64 + quad * 16, a.dim - 8), 8);
-      __builtin_memcpy(w + 2, row + min(s * 64 + quad * 16 + 8, a.dim - 8), 8);
-      x.k[s] = i32x4{w[0], w[1], w[2], w[3]};
+    for (int s = 0; s < 4; ++s) {
+      if (s > 1 && !wide) break;
+      x.k[s] = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(
+                                             cu, code_at + s / 2 * 64 + s % 2 * 8, j0 * a.dim, 0));
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x.scale[r] = su[min(j0 + quad * 4 + r, a.blocks - 1)];
+    for (int r = 0; r < 4; ++r) x.scale[r] = (int)__builtin_amdgcn_raw_buffer_load_b32(su, scale_at + 4 * r, j0 * 4, 0);
   };
   if (N) {
     const int full = (a.blocks + 15) / 16 * 16, rest = N * 64 - full;
@@ -342,16 +354,20 @@ __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, c
     }
     __syncthreads();
     const auto compute = [&](const Blocks& x, int j0) {
-      float best[4];
+      const i32x4 k0{x.k[0][0], x.k[0][1], x.k[1][0], x.k[1][1]};
+      const i32x4 k1{x.k[2][0], x.k[2][1], x.k[3][0], x.k[3][1]};
+      float best[4], scale[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) scale[r] = __int_as_float(x.scale[r]);
       for (int h = 0; h < heads; ++h) {
         i32x4 dot = {0, 0, 0, 0};
-        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[0], qcode[h * 128 + lane], dot, 0, 0, 0);
-        if (wide) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.k[1], qcode[h * 128 + 64 + lane], dot, 0, 0, 0);
+        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(k0, qcode[h * 128 + lane], dot, 0, 0, 0);
+        if (wide) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(k1, qcode[h * 128 + 64 + lane], dot, 0, 0, 0);
         const float top = qtop[h][col];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float y = ((float)dot[r] * top) * x.scale[r];
-          best[r] = h ? fmaxf(best[r], y) : y;
+          const float y = ((float)dot[r] * top) * scale[r];
+          best[r] = h && !(y > best[r]) ? best[r] : y;
         }
       }
       if (col < rows) {
@@ -361,9 +377,11 @@ __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, c
           best[0] = fmaxf(best[0], z.x), best[1] = fmaxf(best[1], z.y);
           best[2] = fmaxf(best[2], z.z), best[3] = fmaxf(best[3], z.w);
         }
+        if (__any(fminf(fminf(scale[0], scale[1]), fminf(scale[2], scale[3])) < 0.f)) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (x.scale[r] < 0.f) best[r] = NAN;  // no valid key
+          for (int r = 0; r < 4; ++r)
+            if (scale[r] < 0.f) best[r] = NAN;  // no valid key
+        }
         if (a.causal || j0 + 16 > a.blocks) {
           const int end = min(own, a.blocks - 1);
 #pragma unroll

@@ -105,10 +105,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kNowhere = 0xffffff00u;
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(void* p, size_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(p, 0, (int)(uint32_t)bytes, 0x00027000);
-}
-
 // Chunks of 16 bytes, one row's in two lanes (8 of them make 128 bytes of a row), leave as whole
 // rows: through LDS, 8 lanes a row.
 struct RowWriter {
