@@ -422,10 +422,17 @@ __device__ __forceinline__ void each_pair(const ChunkArgs& c, int per, F&& body)
   const Span s = span_of(c, c.span0 + blockIdx.y);
   const int t_lo = blockIdx.x * per, t_hi = min(t_lo + per, s.queries);
   const int32_t* ids = c.ids + (((int64_t)s.b * a.queries + s.t0) * a.kv_heads + s.g) * a.keep;
-  for (int e = t_lo * a.keep + threadIdx.x; e < t_hi * a.keep; e += 256) {
-    const int t = c.by_keep(e);
-    const int j = ids[(int64_t)t * a.kv_heads * a.keep + e - t * a.keep];
-    if ((unsigned)j < (unsigned)a.blocks) body(e, j);
+  const int end = t_hi * a.keep;
+  for (int e0 = t_lo * a.keep + threadIdx.x; e0 < end; e0 += 4 * 256) {
+    int j[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = min(e0 + i * 256, end - 1), t = c.by_keep(e);
+      j[i] = ids[(int64_t)t * a.kv_heads * a.keep + e - t * a.keep];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (e0 + i * 256 < end && (unsigned)j[i] < (unsigned)a.blocks) body(e0 + i * 256, j[i]);
   }
 }
 
@@ -525,10 +532,19 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
     weight[i] = (unsigned)j < (unsigned)a.blocks ? c.meta[(row0 + r) * a.keep + slot]
                                                  : make_float2(-INFINITY, 0.f);
   }
-  __syncthreads();
   const int lanes = a.dim / 8, sub = threadIdx.x / lanes, u = threadIdx.x - sub * lanes;
   const int own = sub / share, part0 = sub - own * share;
   const bool live = own < here;
+  // Partials of entries that are no block were never written: whatever is there is left out below.
+  constexpr int AHEAD = 8;
+  const P* part = (const P*)c.part + (row0 + (live ? own : 0)) * a.keep * a.dim + 8 * u;
+  Vec<P, 8> x[AHEAD];
+  const auto fetch = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) x[i] = load_vec<8>(part + (int64_t)min(s0 + i * share, a.keep - 1) * a.dim);
+  };
+  fetch(part0);
+  __syncthreads();
   float o[8] = {}, l = 0.f;
   if (live) {
     const float2* w = weight + own * a.keep;
@@ -536,17 +552,22 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
 #pragma unroll 8
     for (int s = 0; s < a.keep; ++s) top = fmaxf(top, w[s].x);
     if (top == -INFINITY) top = 0.f;
-    const P* part = (const P*)c.part + (row0 + own) * a.keep * a.dim + 8 * u;
-#pragma unroll 8
-    for (int s = part0; s < a.keep; s += share) {
-      const float2 m = w[s];
-      // a partial of an entry that is no block was never written
-      Vec<P, 8> x{};
-      if (m.x > -INFINITY || m.x != m.x) x = load_vec<8>(part + (int64_t)s * a.dim);
-      const float ws = __builtin_amdgcn_exp2f(m.x - top), f = ws * m.y * kUnit;
-      l += ws;
+    for (int s0 = part0; s0 < a.keep; s0 += AHEAD * share) {
+      if (s0 != part0) fetch(s0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = fmaf(f, (float)x.v[i], o[i]);
+      for (int i = 0; i < AHEAD; ++i) {
+        const int s = s0 + i * share;
+        const float2 m = s < a.keep ? w[s] : make_float2(-INFINITY, 0.f);
+        const float ws = __builtin_amdgcn_exp2f(m.x - top), f = ws * m.y * kUnit;
+        const bool written = !(m.x == -INFINITY);
+        l += ws;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = (float)x[i].v[e];
+          if (sizeof(T) == 4) v = written ? v : 0.f;  // whole numbers times 0 are 0 anyway
+          o[e] = fmaf(f, v, o[e]);
+        }
+      }
     }
   }
   if (share > 1) {

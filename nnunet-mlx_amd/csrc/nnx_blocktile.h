@@ -149,12 +149,12 @@ __device__ __forceinline__ void load_query(QueryRow<T, DP>& row, const T* q, int
     __builtin_memcpy(&row.v[s], q + min((2 * s + half) * Q::CH, dim - Q::CH), 16);
 }
 
-template <class T, int DP, int BK, class F>
+template <class T, int DP, int BK, class F, class G0>
 __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, const T* lv,
                                             const float* bias, char* out_lds,
                                             __amdgpu_buffer_rsrc_t part, __amdgpu_buffer_rsrc_t metas,
-                                            const QueryRow<T, DP>& q, int last, float c2, bool odd,
-                                            uint32_t partial, F&& before_stores) {
+                                            QueryRow<T, DP>& q, int last, float c2, bool odd,
+                                            uint32_t partial, F&& after_scores, G0&& before_stores) {
   using G = Tile<T, DP, BK>;
   const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;
   f32x16 acc[G::KT];
@@ -193,6 +193,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
       }
     }
   }
+  after_scores();
   if (__any(last < BK - 1)) {  // the query's own block, or one behind it
     const int seen = last - 4 * half;
 #pragma unroll
@@ -342,7 +343,7 @@ __device__ __forceinline__ int last_seen(const BlockArgs& a, int64_t at, int fir
 // Registers for two waves a SIMD where that leaves nothing in memory (accumulators then stay
 // where vector instructions reach them).
 template <class T, int DP, int BK>
-constexpr int kWaves = DP * BK * sizeof(T) <= (sizeof(T) == 2 ? 128 * 96 * 2 : 64 * 64 * 4) ? 2 : 1;
+constexpr int kWaves = (sizeof(T) == 2 ? DP * BK < 128 * 128 : DP + BK <= 128) ? 2 : 1;
 
 template <class T, int DP, int BK, bool BY_BLOCK>
 __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kernel(ChunkArgs c) {
@@ -396,51 +397,28 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
         load_query<T, DP>(q, queries + c.by_keep(r.entry) * a.qs[1] + r.h * a.qs[2], a.dim);
       };
       bool odd;
-      const auto attend = [&](const Row& r, const QueryRow<T, DP>& q, auto&& before_stores) {
-        const int t = c.by_keep(r.entry), slot = r.entry - t * a.keep;
-        const uint32_t partial = (partials + t * a.group + r.h) * a.keep + slot;
-        attend_rows<T, DP, BK>(c, lk, lv, bias, out_lds, part, metas, q, last_seen(a, start + t, j * BK), c2,
-                               odd, r.live ? partial : kNowhere, before_stores);
-      };
-      // What was asked for during a tile is waited for before the tile's stores: accesses end in
-      // order, and a wait behind the stores would be one for them too.
-      const auto settle = [](QueryRow<T, DP>& q, Row& r) {
-#pragma unroll
-        for (u32x4& v : q.v) asm volatile("" : "+v"(v));
-        asm volatile("" : "+v"(r.entry));
-      };
       Row row = locate(tile), next = locate(tile + 1);
       __syncthreads();  // the block before has been read
       odd = stage_block<T, DP, BK>(c, s.b, s.g, j, lk, lv, bias, negate);
-      QueryRow<T, DP> q0;
-      fetch(row, q0);
-      settle(q0, next);
-      if constexpr (sizeof(q0) <= 128) {
-        // Two tiles a turn, so that the queries on their way stay in the registers they arrive in.
-        QueryRow<T, DP> q1;
-        while (true) {
-          Row after = locate(tile + 2);
-          fetch(next, q1);
-          attend(row, q0, [&] { settle(q1, after); });
-          if (++tile >= to) break;
-          row = locate(tile + 2);
-          fetch(after, q0);
-          attend(next, q1, [&] { settle(q0, row); });
-          if (++tile >= to) break;
-          next = row;
-          row = after;
-        }
-      } else {
-        while (true) {
-          Row after = locate(tile + 2);
-          attend(row, q0, [&] {
-            fetch(next, q0);
-            settle(q0, after);
-          });
-          if (++tile >= to) break;
-          row = next;
-          next = after;
-        }
+      QueryRow<T, DP> q;
+      fetch(row, q);
+      for (; tile < to; ++tile) {
+        Row after = locate(tile + 2);
+        const int t = c.by_keep(row.entry), slot = row.entry - t * a.keep;
+        const uint32_t partial = (partials + t * a.group + row.h) * a.keep + slot;
+        // The next tile's queries take the registers of this one's after its scores, and are waited for
+        // before its stores: accesses end in order, and a wait behind the stores would be one for
+        // them too.
+        attend_rows<T, DP, BK>(
+            c, lk, lv, bias, out_lds, part, metas, q, last_seen(a, start + t, j * BK), c2, odd,
+            row.live ? partial : kNowhere, [&] { fetch(next, q); },
+            [&] {
+#pragma unroll
+              for (u32x4& v : q.v) asm volatile("" : "+v"(v));
+              asm volatile("" : "+v"(after.entry));
+            });
+        row = next;
+        next = after;
       }
     }
   } else {
@@ -461,7 +439,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
                         a.dim);
       const uint32_t partial = (vt * a.group + h) * a.keep + slot;
       attend_rows<T, DP, BK>(c, lk, lv, bias, out_lds, part, metas, q, last, c2, odd,
-                             live ? partial : kNowhere, [] {});
+                             live ? partial : kNowhere, [] {}, [] {});
     }
   }
 }
