@@ -72,6 +72,27 @@ def _check_side(name: str, tensor: torch.Tensor, dtype: torch.dtype, shape: tupl
         raise ContractError(f"{name} must be contiguous")
 
 
+def _address(tensor: torch.Tensor | None) -> int | None:
+    return None if tensor is None else tensor.data_ptr()
+
+
+# What calls have been checked and how the library is told of them, by the shapes, strides, types and
+# devices of their tensors and their other arguments (never by what the tensors hold or where):
+# checking again would be half of what the smallest calls cost.
+_checked: dict = {}
+
+
+def _signature(*tensors: torch.Tensor | None) -> tuple:
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors])
+
+
+def _remember(key: tuple, value):
+    if len(_checked) >= 1024:
+        _checked.clear()
+    _checked[key] = value
+    return value
+
+
 def _launch(device: torch.device, entry: str, *arguments) -> None:
     """Calls a library entry on the device's current stream, its last argument."""
     function = getattr(_native.load(), entry)
@@ -150,6 +171,28 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
     with i + rotary_dim / 2 ("half") or 2i with 2i + 1 ("interleaved"); elements past the plan's
     pairs are copied.  ``inverse`` turns back, which is also the gradient of the forward turn.
     ``out`` may hold the results, ``(q, k)`` itself to rotate in place."""
+    key = ("rotate", _signature(q, k, positions, plan.steps, plan.axes, *(out or (None,))), plan.amplitude,
+           layout, inverse)
+    config = _checked.get(key)
+    if config is None:
+        config = _remember(key, _rotary_config(q, k, positions, plan, layout, inverse, out))
+    if out is None:
+        yq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        yk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+    else:
+        yq, yk = out
+    if config:
+        _launch(q.device, "nnx_rotary", config, q.data_ptr(), _address(k), positions.data_ptr(),
+                plan.steps.data_ptr(), plan.axes.data_ptr(), yq.data_ptr(), _address(yk))
+    return yq, yk
+
+
+def _contiguous_strides(shape: torch.Size) -> tuple[int, int, int]:
+    return (shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3])
+
+
+def _rotary_config(q, k, positions, plan, layout, inverse, out):
+    """The checked configuration of a rotation, False where there is nothing to do."""
     _check("q", q, 4)
     batch, tokens, heads, dim = q.shape
     rotary_dim = 2 * plan.steps.numel()
@@ -166,28 +209,23 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
     _need(axes == 1 or positions.stride(-1) == 1, "positions need a contiguous last axis")
     _check_side("plan.steps", plan.steps, torch.int64, (rotary_dim // 2,), q.device)
     _check_side("plan.axes", plan.axes, torch.int32, (rotary_dim // 2,), q.device)
+    none = (0, 0, 0)
     if out is None:
-        yq = torch.empty_like(q, memory_format=torch.contiguous_format)
-        yk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+        strides = _contiguous_strides(q.shape), none if k is None else _contiguous_strides(k.shape)
     else:
-        yq, yk = out
-        for name, x, y in (("out[0]", q, yq), ("out[1]", k, yk)):
+        for name, x, y in (("out[0]", q, out[0]), ("out[1]", k, out[1])):
             _need((x is None) == (y is None), f"{name} does not match its input")
             if y is not None:
                 _check(name, y, 4, q)
                 _need(y.shape == x.shape, f"{name} {tuple(y.shape)} does not match its input {tuple(x.shape)}")
+        strides = [none if y is None else y.stride()[:3] for y in out]
     if q.numel() == 0 and (k is None or k.numel() == 0):
-        return yq, yk
-    none = (0, 0, 0)
-    config = _native.packed(
+        return False
+    return _native.packed(
         _native.NnxRotaryConfig, _ROTARY, _TYPES[q.dtype], batch, tokens, heads, 0 if k is None else k.shape[2],
         dim, rotary_dim, axes, _LAYOUTS[layout], int(inverse), plan.amplitude,
-        *q.stride()[:3], *(none if k is None else k.stride()[:3]),
-        *yq.stride()[:3], *(none if yk is None else yk.stride()[:3]),
+        *q.stride()[:3], *(none if k is None else k.stride()[:3]), *strides[0], *strides[1],
         *((0, positions.stride(0)) if positions.dim() == 2 else positions.stride()[:2]))
-    _launch(q.device, "nnx_rotary", config, q.data_ptr(), _address(k), positions.data_ptr(),
-            plan.steps.data_ptr(), plan.axes.data_ptr(), yq.data_ptr(), _address(yk))
-    return yq, yk
 
 
 # ---- the norms around a block ---------------------------------------------------------
@@ -220,6 +258,23 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, *, kind: str =
     ``gate`` is like x; ``scale`` float32 (channels,).  ``post`` and ``pre`` are (weight, bias),
     float32 (channels,) or None each.  ``kind`` is "layer" or "rms"; y is the norm of r' before
     it is rounded to its dtype."""
+    vectors = (scale, *(post or (None, None)), *(pre or (None, None)))
+    key = ("norm", _signature(x, residual, gate, *vectors), kind, post is None, pre is None, gate_activation,
+           residual_scale, eps)
+    config = _checked.get(key)
+    if config is None:
+        config = _remember(key, _norm_config(x, residual, gate, vectors, kind, post is not None,
+                                             gate_activation, residual_scale, eps))
+    total = torch.empty_like(x if residual is None else residual, memory_format=torch.contiguous_format)
+    y = None if pre is None else torch.empty_like(x, memory_format=torch.contiguous_format)
+    if config:
+        _launch(x.device, "nnx_residual_norm", config, x.data_ptr(), _address(residual), _address(gate),
+                *[None if v is None else v.data_ptr() for v in vectors], total.data_ptr(), _address(y))
+    return total, y
+
+
+def _norm_config(x, residual, gate, vectors, kind, post, gate_activation, residual_scale, eps):
+    """The checked configuration of a residual norm, False where there is nothing to do."""
     _check("x", x, max(1, x.dim()))
     channels = x.shape[-1]
     rows = x.numel() // channels if channels else 0
@@ -234,22 +289,17 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, *, kind: str =
     if gate is not None:
         _check("gate", gate, x.dim(), x)
         _need(gate.shape == x.shape, f"gate {tuple(gate.shape)} does not match x {tuple(x.shape)}")
-    vectors = (scale, *(post or (None, None)), *(pre or (None, None)))
     for name, vector in zip(("scale", "post weight", "post bias", "pre weight", "pre bias"), vectors):
         if vector is not None:
             _check_side(name, vector, torch.float32, (channels,), x.device)
-    total = torch.empty_like(x if residual is None else residual, memory_format=torch.contiguous_format)
-    y = None if pre is None else torch.empty_like(x, memory_format=torch.contiguous_format)
     if rows == 0:
-        return total, y
-    config = _native.packed(
-        _native.NnxResidualNormConfig, _NORM, _TYPES[x.dtype], _TYPES[total.dtype], rows, channels, _KINDS[kind],
-        int(post is not None), _GATES[gate_activation], residual_scale, eps, _rows("x", x),
+        return False
+    wide = _TYPES[x.dtype if residual is None else residual.dtype]
+    return _native.packed(
+        _native.NnxResidualNormConfig, _NORM, _TYPES[x.dtype], wide, rows, channels, _KINDS[kind], int(post),
+        _GATES[gate_activation], residual_scale, eps, _rows("x", x),
         0 if residual is None else _rows("residual", residual), 0 if gate is None else _rows("gate", gate),
         channels, channels)
-    _launch(x.device, "nnx_residual_norm", config, x.data_ptr(), _address(residual), _address(gate),
-            *[None if v is None else v.data_ptr() for v in vectors], total.data_ptr(), _address(y))
-    return total, y
 
 
 # ---- attention over selected blocks ---------------------------------------------------
@@ -267,9 +317,9 @@ _NO_STRIDES = (0, 0, 0)
 
 
 def _block_config(like: torch.Tensor, block: int, batch: int, queries: int, keys: int, heads: int,
-                  kv_heads: int, mask_stride: int, *, keep: int = 1, first: int = 0, local: int = 0,
-                  causal: bool = False, start: int = 0, scale: float = 1.0, q=_NO_STRIDES, k=_NO_STRIDES,
-                  v=_NO_STRIDES, out=_NO_STRIDES) -> _native.NnxBlockConfig:
+                  kv_heads: int, *, keep: int = 1, first: int = 0, local: int = 0, causal: bool = False,
+                  start: int = 0, scale: float = 1.0, q=_NO_STRIDES, k=_NO_STRIDES, v=_NO_STRIDES,
+                  out=_NO_STRIDES, mask_stride: int = 0) -> _native.NnxBlockConfig:
     if block not in BLOCK_SIZES:
         raise ContractError(f"block must be one of {BLOCK_SIZES}, got {block}")
     try:
@@ -280,23 +330,23 @@ def _block_config(like: torch.Tensor, block: int, batch: int, queries: int, keys
         raise ContractError(f"a block argument is no 32-bit whole number: {error}") from error
 
 
-def _start(start: torch.Tensor | int | None, batch: int, device: torch.device) -> tuple[int, int | None]:
-    if start is None or isinstance(start, int):
-        return start or 0, None
-    _check_side("start", start, torch.int32, (batch,), device)
-    return 0, start.data_ptr()
+def _check_start(start: torch.Tensor | int | None, batch: int, device: torch.device) -> None:
+    if isinstance(start, torch.Tensor):
+        _check_side("start", start, torch.int32, (batch,), device)
 
 
-def _lengths_mask(lengths: torch.Tensor | None, mask: torch.Tensor | None, batch: int, keys: int,
-                  device: torch.device) -> tuple[int | None, int | None, int]:
+def _check_lengths_mask(lengths: torch.Tensor | None, mask: torch.Tensor | None, batch: int, keys: int,
+                        device: torch.device) -> int:
+    """Checks both and returns the mask's stride."""
     if lengths is not None:
         _check_side("lengths", lengths, torch.int32, (batch,), device)
-    if mask is not None:
-        _need(mask.dtype in (torch.bool, torch.uint8) and tuple(mask.shape) == (batch, keys)
-              and mask.device == device and (keys <= 1 or mask.stride(1) == 1),
-              f"key_mask must be bool or uint8 ({batch}, {keys}) on {device} with a contiguous last axis, "
-              f"got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
-    return _address(lengths), _address(mask), 0 if mask is None else mask.stride(0)
+    if mask is None:
+        return 0
+    _need(mask.dtype in (torch.bool, torch.uint8) and tuple(mask.shape) == (batch, keys)
+          and mask.device == device and (keys <= 1 or mask.stride(1) == 1),
+          f"key_mask must be bool or uint8 ({batch}, {keys}) on {device} with a contiguous last axis, "
+          f"got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
+    return mask.stride(0)
 
 
 def summarize_blocks(k: torch.Tensor, block: int, *, lengths: torch.Tensor | None = None,
@@ -307,25 +357,38 @@ def summarize_blocks(k: torch.Tensor, block: int, *, lengths: torch.Tensor | Non
     ``lengths`` int32 (batch,) counts the keys each item has, ``key_mask`` (batch, keys) marks the
     ones that are seen.  ``first`` and ``count`` with ``out`` refresh those blocks of a summary
     that is kept, as after appending keys."""
+    codes, scales = out or (None, None)
+    key = ("summarize", _signature(k, lengths, key_mask, codes, scales), block, first, count)
+    known = _checked.get(key)
+    if known is None:
+        known = _remember(key, _summary_config(k, block, lengths, key_mask, first, count, out))
+    config, blocks, count = known
+    if out is None:
+        batch, _, kv_heads, dim = k.shape
+        out = BlockSummary(torch.empty((batch, kv_heads, blocks, dim), dtype=torch.int8, device=k.device),
+                           torch.empty((batch, kv_heads, blocks), dtype=torch.float32, device=k.device))
+    if config:
+        _launch(k.device, "nnx_block_summarize", config, k.data_ptr(), _address(lengths), _address(key_mask),
+                first, count, out.codes.data_ptr(), out.scales.data_ptr())
+    return out
+
+
+def _summary_config(k, block, lengths, key_mask, first, count, out):
+    """The checked configuration (False where there is nothing to do), blocks in all and asked for."""
     _check("k", k, 4)
     batch, keys, kv_heads, dim = k.shape
-    lengths_at, mask_at, mask_stride = _lengths_mask(lengths, key_mask, batch, keys, k.device)
-    config = _block_config(k, block, batch, 0, keys, kv_heads, kv_heads, mask_stride, k=k.stride()[:3])
+    mask_stride = _check_lengths_mask(lengths, key_mask, batch, keys, k.device)
+    config = _block_config(k, block, batch, 0, keys, kv_heads, kv_heads, k=k.stride()[:3],
+                           mask_stride=mask_stride)
     blocks = -(-keys // block)
     if count is None:
         count = blocks - first
     if out is None:
         _need(first == 0 and count == blocks, "summaries of some blocks need the summary to refresh (out)")
-        out = BlockSummary(torch.empty((batch, kv_heads, blocks, dim), dtype=torch.int8, device=k.device),
-                           torch.empty((batch, kv_heads, blocks), dtype=torch.float32, device=k.device))
     else:
         _check_side("out.codes", out.codes, torch.int8, (batch, kv_heads, blocks, dim), k.device)
         _check_side("out.scales", out.scales, torch.float32, (batch, kv_heads, blocks), k.device)
-    if k.numel() == 0:
-        return out
-    _launch(k.device, "nnx_block_summarize", config, k.data_ptr(), lengths_at, mask_at, first, count,
-            out.codes.data_ptr(), out.scales.data_ptr())
-    return out
+    return config if k.numel() else False, blocks, count
 
 
 def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int, *, causal: bool = False,
@@ -338,24 +401,35 @@ def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int,
     product of the summary with the query heads that share the key head; equal scores go to the
     lower index.  The scores are formed in whole numbers, so they do not depend on how the work is
     split.  ``causal`` leaves out the blocks behind the query's own."""
+    placed = isinstance(start, torch.Tensor)
+    key = ("select", _signature(q, *summary, start if placed else None), block, keep, causal,
+           None if placed else start, first, local)
+    config = _checked.get(key)
+    if config is None:
+        config = _remember(key, _selection_config(q, summary, block, keep, causal, start, first, local))
+    ids = torch.empty((q.shape[0], q.shape[1], summary.codes.shape[1], keep), dtype=torch.int32, device=q.device)
+    if config:
+        _launch(q.device, "nnx_block_select", config, q.data_ptr(), summary.codes.data_ptr(),
+                summary.scales.data_ptr(), start.data_ptr() if placed else None, ids.data_ptr())
+    elif ids.numel():
+        ids.fill_(-1)
+    return ids
+
+
+def _selection_config(q, summary, block, keep, causal, start, first, local):
+    """The checked configuration of a selection, False where there is nothing to select from."""
     _check("q", q, 4)
     batch, queries, heads, dim = q.shape
     _need(summary.codes.dim() == 4, f"summary codes need 4 axes, got shape {tuple(summary.codes.shape)}")
     kv_heads, blocks = summary.codes.shape[1:3]
     _check_side("summary.codes", summary.codes, torch.int8, (batch, kv_heads, blocks, dim), q.device)
     _check_side("summary.scales", summary.scales, torch.float32, (batch, kv_heads, blocks), q.device)
-    begin, start_at = _start(start, batch, q.device)
-    config = _block_config(q, block, batch, queries, blocks * block, heads, kv_heads, 0, keep=keep, first=first,
-                           local=local, causal=causal, start=begin, q=q.stride()[:3])
+    _check_start(start, batch, q.device)
     _need(keep >= 1, f"keep must be positive, got {keep}")
-    ids = torch.empty((batch, queries, kv_heads, keep), dtype=torch.int32, device=q.device)
-    if q.numel() == 0:
-        return ids
-    if blocks == 0:
-        return ids.fill_(-1)
-    _launch(q.device, "nnx_block_select", config, q.data_ptr(), summary.codes.data_ptr(),
-            summary.scales.data_ptr(), start_at, ids.data_ptr())
-    return ids
+    config = _block_config(q, block, batch, queries, blocks * block, heads, kv_heads, keep=keep, first=first,
+                           local=local, causal=causal, start=start if isinstance(start, int) else 0,
+                           q=q.stride()[:3])
+    return config if q.numel() and blocks else False
 
 
 def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torch.Tensor, block: int, *,
@@ -367,6 +441,27 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torc
 
     ``scale`` defaults to head_dim^-0.5; ``causal``, ``start``, ``lengths`` and ``key_mask`` as in
     ``select_blocks`` and ``summarize_blocks``.  A query that sees no key gets zeros."""
+    placed = isinstance(start, torch.Tensor)
+    key = ("attention", _signature(q, k, v, ids, start if placed else None, lengths, key_mask, out), block, scale,
+           causal, None if placed else start)
+    known = _checked.get(key)
+    if known is None:
+        known = _remember(key, _attention_config(q, k, v, ids, block, scale, causal, start, lengths, key_mask, out))
+    config, size = known
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if config:
+        work = torch.empty(size, dtype=torch.uint8, device=q.device)
+        _launch(q.device, "nnx_block_attention", config, q.data_ptr(), k.data_ptr(), v.data_ptr(), ids.data_ptr(),
+                start.data_ptr() if placed else None, _address(lengths), _address(key_mask), out.data_ptr(),
+                work.data_ptr(), size)
+    elif out.numel():
+        out.zero_()
+    return out
+
+
+def _attention_config(q, k, v, ids, block, scale, causal, start, lengths, key_mask, out):
+    """The checked configuration (False where there is nothing to attend to) and workspace bytes."""
     _check("q", q, 4)
     _check("k", k, 4, q)
     _check("v", v, 4, q)
@@ -377,25 +472,20 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torc
     _need(ids.dim() == 4, f"ids need 4 axes, got shape {tuple(ids.shape)}")
     keep = ids.shape[3]
     _check_side("ids", ids, torch.int32, (batch, queries, kv_heads, keep), q.device)
-    begin, start_at = _start(start, batch, q.device)
-    lengths_at, mask_at, mask_stride = _lengths_mask(lengths, key_mask, batch, keys, q.device)
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    else:
+    _check_start(start, batch, q.device)
+    mask_stride = _check_lengths_mask(lengths, key_mask, batch, keys, q.device)
+    if out is not None:
         _check("out", out, 4, q)
         _need(out.shape == q.shape, f"out {tuple(out.shape)} does not match q {tuple(q.shape)}")
-    config = _block_config(q, block, batch, queries, keys, heads, kv_heads, mask_stride, keep=keep, causal=causal,
-                           start=begin, scale=dim**-0.5 if scale is None else scale, q=q.stride()[:3],
-                           k=k.stride()[:3], v=v.stride()[:3], out=out.stride()[:3])
-    if q.numel() == 0:
-        return out
-    if keys == 0:
-        return out.zero_()
-    size = _native.load().nnx_block_attention_workspace(config)
-    work = torch.empty(max(1, size), dtype=torch.uint8, device=q.device)
-    _launch(q.device, "nnx_block_attention", config, q.data_ptr(), k.data_ptr(), v.data_ptr(), ids.data_ptr(),
-            start_at, lengths_at, mask_at, out.data_ptr(), work.data_ptr(), size)
-    return out
+    config = _block_config(
+        q, block, batch, queries, keys, heads, kv_heads, keep=keep, causal=causal,
+        start=start if isinstance(start, int) else 0, scale=dim**-0.5 if scale is None else scale,
+        q=q.stride()[:3], k=k.stride()[:3], v=v.stride()[:3],
+        out=_contiguous_strides(q.shape) if out is None else out.stride()[:3], mask_stride=mask_stride)
+    if q.numel() == 0 or keys == 0:
+        return False, 0
+    # 0 for what the library refuses, with the reason, when it is called
+    return config, max(1, _native.load().nnx_block_attention_workspace(config))
 
 
 def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block: int, keep: int, *,
