@@ -72,8 +72,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, size_
 }
 
 // Attention of a launch's rows to each of their kept blocks, a partial result each.  `by_block`:
-// rows gathered by the block that they keep (list, start, tiles; `grid` workgroups share the
-// tiles), else a workgroup for each kept block of each query.
+// rows gathered by the block that they keep (list, start, tiles; at most `grid` tiles), else a
+// workgroup for each of `grid` kept blocks of queries.
 void block_partials_f32(const ChunkArgs& c, bool by_block, int grid, hipStream_t st);
 void block_partials_f16(const ChunkArgs& c, bool by_block, int grid, hipStream_t st);
 void block_partials_bf16(const ChunkArgs& c, bool by_block, int grid, hipStream_t st);

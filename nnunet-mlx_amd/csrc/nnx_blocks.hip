@@ -764,8 +764,7 @@ void block_attention(const nnx_block_config& c, const void* q, const void* k, co
       const int64_t pairs = (int64_t)m.spans * p.nt * c.keep;
       int grid = (int)pairs;
       if (p.by_block) {
-        grid = (int)std::min<int64_t>(ceil_div(pairs * a.group, kTileRows) + (int64_t)m.spans * a.blocks,
-                                      3 * compute_units());
+        grid = (int)std::min<int64_t>(ceil_div(pairs * a.group, kTileRows) + (int64_t)m.spans * a.blocks, 1 << 30);
       }
       {
         ProfScope prof("block_partials", flops * m.spans, 0.0, st);

@@ -2,6 +2,7 @@
 // blocks; included by one source a type.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "nnx_blocks.h"
@@ -448,6 +449,14 @@ template <class T, int DP, int BK>
 void launch_partials(const ChunkArgs& c, bool by_block, int grid, hipStream_t st) {
   constexpr size_t bytes = Tile<T, DP, BK>::LDS;
   if (by_block) {
+    // as many workgroups as run at once: they share the tiles evenly
+    static const int per_cu = [] {
+      int n = 0;
+      hip_check(hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, block_partials_kernel<T, DP, BK, true>, 256, bytes),
+                "block attention: occupancy");
+      return std::max(1, n);
+    }();
+    grid = (int)std::min<int64_t>(grid, (int64_t)per_cu * compute_units());
     block_partials_kernel<T, DP, BK, true><<<grid, 256, bytes, st>>>(c);
   } else {
     block_partials_kernel<T, DP, BK, false><<<grid, 256, bytes, st>>>(c);
