@@ -43,19 +43,24 @@ struct Tile {
   static constexpr int ROW_BYTES = DP * sizeof(T);
   static constexpr int PER = ROW_BYTES >= 256 ? 1 : 256 / ROW_BYTES;  // rows in 256 bytes
   static constexpr int TURNS = CHUNKS & -CHUNKS;   // a power of two that divides CHUNKS
-  // keys, values, where scores start from, and for each wave 32 rows of 128 bytes on their way out
+  // keys, values, what is added to their scores, and for each wave 32 rows of 128 bytes on their way out
   static constexpr int OUT = 32 * 128;
-  static constexpr size_t LDS = (size_t)2 * ROWS * ROW_BYTES + ROWS * sizeof(float) + 4 * OUT;
+  static constexpr size_t LDS = (size_t)2 * ROWS * ROW_BYTES + ROWS * sizeof(float) + 16 + 4 * OUT;
   static __device__ __forceinline__ int at(int row, int chunk) {
     const int turn = (row / PER) & (TURNS - 1);
     return row * DP + (chunk ^ turn) * CH;
   }
 };
 
-// The block's keys and values into LDS, zeros for those that are not valid, and what their scores
-// start from: 0, or -inf for keys that are not valid.  Whether any value is not finite (16-bit types).
+struct Staged {
+  bool full;  // every key is valid
+  bool odd;   // some value is not finite (looked for in 16-bit types)
+};
+
+// The block's keys and values into LDS, zeros for those that are not valid, and what is added to
+// their scores: 0, or -inf for keys that are not valid.
 template <class T, int DP, int BK>
-__device__ __forceinline__ bool stage_block(const ChunkArgs& c, int b, int g, int j, T* lk, T* lv,
+__device__ __forceinline__ Staged stage_block(const ChunkArgs& c, int b, int g, int j, T* lk, T* lv,
                                             float* bias, bool negate) {
   using G = Tile<T, DP, BK>;
   const int length = item_length(c.a, b), first = j * BK;
@@ -92,11 +97,18 @@ __device__ __forceinline__ bool stage_block(const ChunkArgs& c, int b, int g, in
       *(Vec<T, G::CH>*)__builtin_assume_aligned(lv + at, 16) = vr[i];
     }
   }
+  bool missing = false;
   if (threadIdx.x < BK) {
     const int key = first + threadIdx.x;
-    bias[threadIdx.x] = key < length && (!mask || mask[key]) ? 0.f : -INFINITY;
+    missing = !(key < length && (!mask || mask[key]));
+    bias[threadIdx.x] = missing ? -INFINITY : 0.f;
   }
-  return __syncthreads_or(odd);
+  int* seen = (int*)(bias + G::ROWS);  // of each wave
+  const int mine = (__any(odd) ? 1 : 0) | (__any(missing) ? 2 : 0);
+  if (threadIdx.x % 64 == 0) seen[threadIdx.x / 64] = mine;
+  __syncthreads();
+  const int any = __builtin_amdgcn_readfirstlane(seen[0] | seen[1] | seen[2] | seen[3]);
+  return {!(any & 2), (any & 1) != 0};
 }
 
 // Stores into the partials go through buffer instructions: 32-bit offsets, and one past the buffer's
@@ -154,22 +166,11 @@ template <class T, int DP, int BK, class F, class G0>
 __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, const T* lv,
                                             const float* bias, char* out_lds,
                                             __amdgpu_buffer_rsrc_t part, __amdgpu_buffer_rsrc_t metas,
-                                            QueryRow<T, DP>& q, int last, float c2, bool odd,
+                                            QueryRow<T, DP>& q, int last, float c2, Staged block,
                                             uint32_t partial, F&& after_scores, G0&& before_stores) {
   using G = Tile<T, DP, BK>;
   const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;
-  f32x16 acc[G::KT];
-#pragma unroll
-  for (int kt = 0; kt < G::KT; ++kt)
-#pragma unroll
-    for (int r = 0; r < G::REGS; r += 4) {
-      const float4 z = *(const float4*)&bias[kt * 32 + 2 * r + 4 * half];
-      acc[kt][r] = z.x, acc[kt][r + 1] = z.y, acc[kt][r + 2] = z.z, acc[kt][r + 3] = z.w;
-    }
-  if constexpr (G::REGS < 16) {
-#pragma unroll
-    for (int r = G::REGS; r < 16; ++r) acc[0][r] = 0.f;  // rows past the block, never used
-  }
+  f32x16 acc[G::KT] = {};
   if constexpr (sizeof(T) == 2) {
     Frag<T> qf[DP / 16];
 #pragma unroll
@@ -195,6 +196,15 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
     }
   }
   after_scores();
+  if (!block.full) {
+#pragma unroll
+    for (int kt = 0; kt < G::KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < G::REGS; r += 4) {
+        const float4 z = *(const float4*)&bias[kt * 32 + 2 * r + 4 * half];
+        acc[kt][r] += z.x, acc[kt][r + 1] += z.y, acc[kt][r + 2] += z.z, acc[kt][r + 3] += z.w;
+      }
+  }
   if (__any(last < BK - 1)) {  // the query's own block, or one behind it
     const int seen = last - 4 * half;
 #pragma unroll
@@ -273,7 +283,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) big = fmaxf(fmaxf(big, fabsf(o[dt][r])), fabsf(o[dt][r + 1]));
-    if (odd) {
+    if (block.odd) {
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -353,7 +363,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
   T* lk = (T*)lds;
   T* lv = lk + G::ROWS * DP;
   float* bias = (float*)(lv + G::ROWS * DP);
-  char* out_lds = (char*)(bias + G::ROWS) + threadIdx.x / 64 * G::OUT;
+  char* out_lds = (char*)(bias + G::ROWS) + 16 + threadIdx.x / 64 * G::OUT;
   const BlockArgs& a = c.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = threadIdx.x % 32;
   // the scale's sign goes to the keys, so that the largest weight belongs to the largest product; a
@@ -397,10 +407,9 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
       const auto fetch = [&](const Row& r, QueryRow<T, DP>& q) {
         load_query<T, DP>(q, queries + c.by_keep(r.entry) * a.qs[1] + r.h * a.qs[2], a.dim);
       };
-      bool odd;
       Row row = locate(tile), next = locate(tile + 1);
       __syncthreads();  // the block before has been read
-      odd = stage_block<T, DP, BK>(c, s.b, s.g, j, lk, lv, bias, negate);
+      const Staged block = stage_block<T, DP, BK>(c, s.b, s.g, j, lk, lv, bias, negate);
       QueryRow<T, DP> q;
       fetch(row, q);
       for (; tile < to; ++tile) {
@@ -411,7 +420,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
         // before its stores: accesses end in order, and a wait behind the stores would be one for
         // them too.
         attend_rows<T, DP, BK>(
-            c, lk, lv, bias, out_lds, part, metas, q, last_seen(a, start + t, j * BK), c2, odd,
+            c, lk, lv, bias, out_lds, part, metas, q, last_seen(a, start + t, j * BK), c2, block,
             row.live ? partial : kNowhere, [&] { fetch(next, q); },
             [&] {
 #pragma unroll
@@ -429,7 +438,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
     if (t >= s.queries) return;
     const int j = c.ids[(((int64_t)s.b * a.queries + s.t0 + t) * a.kv_heads + s.g) * a.keep + slot];
     if (j < 0 || j >= a.blocks) return;
-    const bool odd = stage_block<T, DP, BK>(c, s.b, s.g, j, lk, lv, bias, negate);
+    const Staged block = stage_block<T, DP, BK>(c, s.b, s.g, j, lk, lv, bias, negate);
     const int last = last_seen(a, item_start(a, s.b) + s.t0 + t, j * BK);
     for (int h0 = wave * 32; h0 < a.group; h0 += 128) {
       const bool live = h0 + col < a.group;
@@ -439,7 +448,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
                                (int64_t)(s.g * a.group + h) * a.qs[2],
                         a.dim);
       const uint32_t partial = (vt * a.group + h) * a.keep + slot;
-      attend_rows<T, DP, BK>(c, lk, lv, bias, out_lds, part, metas, q, last, c2, odd,
+      attend_rows<T, DP, BK>(c, lk, lv, bias, out_lds, part, metas, q, last, c2, block,
                              live ? partial : kNowhere, [] {}, [] {});
     }
   }
