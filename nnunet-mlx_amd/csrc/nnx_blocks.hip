@@ -141,18 +141,12 @@ struct Cut {
   int ties;
 };
 
-template <class Above, class Range>
-__device__ __forceinline__ Cut find_cut(int want, Above&& above, Range&& range) {
-  if (want <= 0) return {3.4028235e38f, 0};  // but +inf, which forced blocks have in the end
-  if (above(-INFINITY) <= want) return {-INFINITY, 0};
-  float low, high;
-  range(low, high);
-  low = fmaxf(low, -3.4028235e38f), high = fminf(high, 3.4028235e38f);  // products can overflow
-  const int over = above(low);  // above(low) >= want > above(high), but for the lowest score
-  if (over < want) return {low, want - over};
+// Needs above(low) >= want > above(high).
+template <class Above>
+__device__ __forceinline__ Cut refine_cut(float low, float high, int want, Above&& above) {
   for (int step = 0; step < 14; ++step) {
     const float mid = 0.5f * low + 0.5f * high;
-    const int count = above(mid);
+    const int count = (int)above(mid);
     if (count == want) return {mid, 0};
     (count < want ? high : low) = mid;
   }
@@ -164,9 +158,23 @@ __device__ __forceinline__ Cut find_cut(int want, Above&& above, Range&& range) 
   int32_t lo = order(low), hi = order(high);
   while ((int64_t)hi - lo > 1) {
     const int32_t mid = (int32_t)(((int64_t)lo + hi) >> 1);
-    (above(back(mid)) < want ? hi : lo) = mid;
+    ((int)above(back(mid)) < want ? hi : lo) = mid;
   }
-  return {back(hi), want - above(back(hi))};
+  return {back(hi), want - (int)above(back(hi))};
+}
+
+constexpr float kMostFloat = 3.4028235e38f;  // products can overflow
+
+template <class Above, class Range>
+__device__ __forceinline__ Cut find_cut(int want, Above&& above, Range&& range) {
+  if (want <= 0) return {kMostFloat, 0};  // but +inf, which forced blocks have in the end
+  if (above(-INFINITY) <= want) return {-INFINITY, 0};
+  float low, high;
+  range(low, high);
+  low = fmaxf(low, -kMostFloat), high = fminf(high, kMostFloat);
+  const int over = above(low);
+  if (over < want) return {low, want - over};
+  return refine_cut(low, high, want, above);
 }
 
 __device__ __forceinline__ int lanes_before(uint64_t lanes, int from) {
@@ -198,14 +206,14 @@ __device__ __forceinline__ void select_row(float* score, int blocks, int keep, i
   if (first) force(0, min(first, blocks));
   if (local) force(max(own + 1 - local, 0), min(own + 1, blocks));
   int done = 0, tied = 0;
-  const auto emit = [&](int i, uint64_t equal, bool take, int ties) {
+  const auto emit = [&](int block, uint64_t equal, bool take, int ties) {
     if (ties) {
       take |= ((equal >> lane) & 1) && lanes_before(equal, tied) < ties;
       tied += __popcll(equal);
     }
     const uint64_t taken = __ballot(take);
     const int to = lanes_before(taken, done);
-    if (take && to < keep) out[(uint32_t)to] = i * 64 + lane;
+    if (take && to < keep) out[(uint32_t)to] = block;
     done += __popcll(taken);
   };
   const auto larger = [](float x, float y) { return fmaxf(x, y); };
@@ -213,30 +221,79 @@ __device__ __forceinline__ void select_row(float* score, int blocks, int keep, i
     float v[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = score[i * 64 + lane];
-    const Cut cut = find_cut(
-        keep - forced,
-        [&](float x) {
-          int count = 0;
+    const auto above = [&](float x) {
+      int count = 0;
 #pragma unroll
-          for (int i = 0; i < N; ++i) count += __popcll(__ballot(v[i] > x));
-          return count;
-        },
-        [&](float& low, float& high) {
-          low = INFINITY, high = -INFINITY;
+      for (int i = 0; i < N; ++i) count += __popcll(__ballot(v[i] > x));
+      return count;
+    };
+    const auto range = [&](float& low, float& high) {
+      low = INFINITY, high = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < N; ++i) low = v[i] < low ? v[i] : low, high = v[i] > high ? v[i] : high;
-          low = -lanes_reduce<64>(-low, larger);
-          high = lanes_reduce<64>(high, larger);
-        });
-    if (forced) {
+      for (int i = 0; i < N; ++i) low = v[i] < low ? v[i] : low, high = v[i] > high ? v[i] : high;
+      low = -lanes_reduce<64>(-low, larger);
+      high = lanes_reduce<64>(high, larger);
+    };
+    const auto restore = [&] {  // forced blocks above all others
       for (uint32_t m = marks; m; m &= m - 1) score[__builtin_ctz(m) * 64 + lane] = INFINITY;
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = score[i * 64 + lane];
+    };
+    if constexpr (N >= 4) {
+      // Once no more than 128 scores are left above the lower end, they and their blocks are packed
+      // into two registers (by way of the row's own place), where the rest of the search and the
+      // writing cost a fraction.
+      const int want = keep - forced;
+      int over = above(-INFINITY);
+      if (keep <= 128 && want > 0 && over > want) {
+        float low, high;
+        range(low, high);
+        high = fminf(high, kMostFloat);
+        low = fmaxf(low - fabsf(low) * 1e-6f - 1e-30f, -kMostFloat);  // below all
+        for (int step = 0; step < 14 && over + forced > 128; ++step) {
+          const float mid = 0.5f * low + 0.5f * high;
+          const int count = above(mid);
+          if (count < want) {
+            high = mid;
+          } else {
+            low = mid, over = count;
+          }
+        }
+        if (over + forced <= 128) {
+          if (forced) restore();
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const bool take = v[i] > low;
+            const uint64_t taken = __ballot(take);
+            const int to = lanes_before(taken, n);
+            if (take && to < 128) score[to] = v[i], score[128 + to] = __int_as_float(i * 64 + lane);
+            n += __popcll(taken);
+          }
+          float w[2];
+          int32_t at[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const bool in = i * 64 + lane < n;
+            w[i] = in ? score[i * 64 + lane] : NAN;
+            at[i] = in ? __float_as_int(score[128 + i * 64 + lane]) : 0;
+          }
+          const Cut cut = refine_cut(low, high, keep, [&](float x) {
+            return __popcll(__ballot(w[0] > x)) + __popcll(__ballot(w[1] > x));
+          });
+#pragma unroll
+          for (int i = 0; i < 2; ++i) emit(at[i], cut.ties ? __ballot(w[i] == cut.above) : 0, w[i] > cut.above, cut.ties);
+          for (int i = min(done, keep) + lane; i < keep; i += 64) out[i] = -1;
+          return;
+        }
+      }
     }
+    const Cut cut = find_cut(keep - forced, above, range);
+    if (forced) restore();
     if (cut.ties || forced > keep) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        emit(i, __ballot(v[i] == cut.above), v[i] > cut.above || v[i] == INFINITY, cut.ties);
+        emit(i * 64 + lane, __ballot(v[i] == cut.above), v[i] > cut.above || v[i] == INFINITY, cut.ties);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -271,7 +328,7 @@ __device__ __forceinline__ void select_row(float* score, int blocks, int keep, i
         });
     for (int i = 0; i < n; ++i) {
       const float v = value(i);
-      emit(i, __ballot(cut.ties && v == cut.above), v > cut.above || v == INFINITY, cut.ties);
+      emit(i * 64 + lane, __ballot(cut.ties && v == cut.above), v > cut.above || v == INFINITY, cut.ties);
     }
   }
   for (int i = min(done, keep) + lane; i < keep; i += 64) out[i] = -1;
