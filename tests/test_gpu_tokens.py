@@ -379,6 +379,29 @@ def test_selection_over_many_blocks(device, keys, block, keep):
     assert np.array_equal(got.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("levels", [2, 7, 127])
+@pytest.mark.parametrize("blocks,keep,first,local", [
+    (3, 2, 0, 1), (64, 64, 1, 1), (65, 17, 0, 0), (200, 128, 0, 3), (256, 1, 0, 0), (257, 129, 2, 1),
+    (512, 32, 0, 1), (700, 256, 5, 70), (1500, 100, 90, 90), (2048, 128, 0, 1), (2100, 40, 1, 2), (130, 20, 30, 0)])
+def test_selection_with_equal_scores(device, blocks, keep, first, local, levels):
+    """Scores of few values, so that cuts fall between equals, among empty blocks, more forced blocks than
+    are kept, and queries before the first key and behind the last."""
+    gen = _gen(blocks + keep + levels)
+    codes = torch.randint(0, levels, (1, 2, blocks, 40), generator=gen, dtype=torch.int8)
+    codes[..., 3:] = 0
+    scales = torch.randint(0, 3, (1, 2, blocks), generator=gen).float() * 0.5
+    scales[torch.rand(1, 2, blocks, generator=gen) < 0.1] = -1
+    q = torch.randint(-1, 2, (1, 21, 6, 40), generator=gen).float()
+    q[0, 5] = 0
+    for causal, begin in ((False, -3), (True, -3), (True, blocks * 16 - 9), (False, blocks * 16 + 50)):
+        start = torch.tensor([begin], dtype=torch.int32)
+        got = tokens.select_blocks(q.cuda(), tokens.BlockSummary(codes.cuda(), scales.cuda()), 16, keep,
+                                   start=start.cuda(), first=first, local=local, causal=causal)
+        want = ot.select(q.numpy(), codes.numpy(), scales.numpy(), 16, keep, start=start.numpy(), first=first,
+                         local=local, causal=causal)
+        assert np.array_equal(got.cpu().numpy(), want)
+
+
 def test_attention_skips_entries_that_are_no_blocks(device):
     case = (1, 70, 100, 2, 2, 64, 32, 4, 0, 0, False, False, False)
     q, k, v = _attention_inputs(case, torch.float16)
@@ -392,6 +415,26 @@ def test_attention_skips_entries_that_are_no_blocks(device):
         assert (np.abs(_f64(got) - want) <= (4 * 2.0**-11 + 5e-4) * size[..., None]).all()
     none = torch.full((1, 70, 2, 4), -1, dtype=torch.int32, device="cuda")
     assert not tokens.block_attention(q, k, v, none, 32).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", [3, 400])
+def test_attention_of_values_that_are_not_finite(device, dtype, queries):
+    """NaN among the values that a query weighs makes its row NaN; rows that do not keep the block are
+    untouched.  A negative scale turns the order of the weights, a scale of 0 makes them equal."""
+    case = (1, queries, 200, 2, 1, 64, 32, 2, 0, 0, False, False, False)
+    q, k, v = _attention_inputs(case, dtype)
+    ids = torch.tensor([[1, 4], [2, 5]], dtype=torch.int32).repeat(queries // 2 + 1, 1)[:queries]
+    ids = ids.reshape(1, queries, 1, 2).contiguous().cuda()
+    plain = {scale: tokens.block_attention(q, k, v, ids, 32, scale=scale) for scale in (0.125, -0.125, 0.0)}
+    see = ot.seen(ids.cpu().numpy(), 200, 32, np.ones((1, 200), bool))
+    for scale, got in plain.items():
+        want, size = ot.attention(_f64(q), _f64(k), _f64(v), see, scale)
+        assert (np.abs(_f64(got) - want) <= (4 * U[dtype] + 5e-4) * size[..., None]).all()
+    v[0, 40, 0, 3] = float("nan")
+    got = tokens.block_attention(q, k, v, ids, 32)
+    assert torch.isnan(got[0, 0::2, :, 3]).all()
+    assert torch.equal(got[0, 1::2], plain[0.125][0, 1::2])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
