@@ -579,7 +579,8 @@ int nnx_residual_norm(const nnx_residual_norm_config* config, const void* d_x,
  * nonzero d_mask[b * mask_stride + key] (NULL: all).  What invalid keys and values hold is
  * never used, NaN included.  Query t of item b stands at position start + d_start[b] (NULL: 0)
  * + t; with `causal` it sees the keys up to its position and the blocks up to its own.
- * kv_heads divides heads; heads j * (heads / kv_heads) ... share key head j and its blocks. */
+ * kv_heads divides heads; heads j * (heads / kv_heads) ... (at most 1024) share key head j and its
+ * blocks. */
 typedef struct nnx_block_config {
   int type;
   int batch, queries, keys;
@@ -618,8 +619,8 @@ int nnx_block_select(const nnx_block_config* config, const void* d_q, const int8
 
 /* out[q] = softmax(scale q . k) v over the valid keys of the blocks in d_ids (batch, queries,
  * kv_heads, keep; entries outside [0, nb) are skipped, the others of a row are distinct).  A
- * query without a valid key gets zeros.  The workspace query answers 0 for what the entry
- * refuses. */
+ * query without a valid key gets zeros.  In 16-bit types a value that is not finite, weighed by a
+ * query, makes its row NaN.  The workspace query answers 0 for what the entry refuses. */
 size_t nnx_block_attention_workspace(const nnx_block_config* config);
 int nnx_block_attention(const nnx_block_config* config, const void* d_q, const void* d_k,
                         const void* d_v, const int32_t* d_ids, const int32_t* d_start,

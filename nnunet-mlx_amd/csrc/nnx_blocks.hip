@@ -26,6 +26,7 @@ void check_config(const nnx_block_config& c, const char* what, bool queries) {
   if (queries) {
     require(c.queries >= 1, w + "no queries");
     require(c.heads >= 1 && c.heads % c.kv_heads == 0, w + "heads must be a multiple of the key heads");
+    require(c.heads / c.kv_heads <= 1024, w + "at most 1024 heads may share a key head");
     require(c.keep >= 1 && c.keep <= kMaxKeep, w + "keep must be 1..256");
     require((double)c.batch * c.queries * c.kv_heads * c.keep < 2147483648.0 &&
                 (double)c.batch * c.queries * c.heads < 2147483648.0,
@@ -660,7 +661,10 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
 // the lists of many launches are formed at once.
 constexpr size_t kPartialBudget = (size_t)160 << 20;
 constexpr int64_t kListPairs = (int64_t)1 << 27;
-constexpr int64_t kDirectPairs = 8192;
+// Pairs go one by one while they and the keys and values that they read come to no more than this: 5120
+// pairs of 16 KiB took 28 us one by one and 16 + 16 us by block (lists, partials), 8192 of 32 KiB 71
+// and 19 + 21, 1280 of 16 KiB 13 and 16 + 15.
+constexpr double kDirectPairs = 8192, kDirectBytes = 80e6;
 
 struct AttentionPlan {
   bool by_block;
@@ -681,7 +685,8 @@ AttentionPlan make_plan(const nnx_block_config& c) {
   const int64_t spans = (int64_t)c.batch * c.kv_heads * p.splits;
   require(spans < (int64_t)1 << 31, "block attention: too many queries and key heads");
   p.spans = (int)spans;
-  p.by_block = (double)c.batch * c.kv_heads * c.queries * c.keep > kDirectPairs;
+  const double pairs = (double)c.batch * c.kv_heads * c.queries * c.keep;
+  p.by_block = pairs > kDirectPairs || pairs * c.block * c.head_dim * 2 * type_bytes(c.type) > kDirectBytes;
   p.at_once = (int)std::max<int64_t>(1, std::min(spans, fit / p.nt));
   // counts and tiles are 32-bit, and spans a grid axis
   const int64_t most = std::min<int64_t>({spans, 65535, ((int64_t)1 << 30) / blocks, kListPairs / ((int64_t)p.nt * c.keep)});

@@ -45,12 +45,13 @@ __device__ __forceinline__ void sincos_turns(int32_t turns, float& s, float& c) 
   c = (quarter + 1) & 2 ? -b : b;
 }
 
-// A wave turns heads of one token, each lane W neighbouring elements of a head, so that its
-// accesses are whole rows of memory whatever the rotated part; lanes / head = dim / W.  A lane
-// forms its elements' sines once and keeps them for all its heads.  When the pairs lie half the
-// rotated part apart, the partners come from the lane that holds them.  HB heads' loads are in
-// flight at a time.  (Threads that loaded both elements of their pairs, half a row apart, moved
-// 2 x 65536 x 20 heads of 128 in 543 us.)
+// Bound by memory: 2 x 65536 tokens of 20 heads of 128 float16, 96 of them rotated, move 1.34 GB in 258 us,
+// 5.2 TB/s (a large copy reaches 4.8).  A wave turns heads of one token, each lane W neighbouring
+// elements of a head, so that its accesses are whole rows of memory whatever the rotated part;
+// lanes / head = dim / W.  A lane forms its elements' sines once and keeps them for all its heads.
+// When the pairs lie half the rotated part apart, the partners come from the lane that holds them.
+// HB heads' loads are in flight at a time.  (Threads that load both elements of their pairs, half a
+// row apart, as below, took 543 us.)
 template <class T, int W, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_wave_kernel(RotaryArgs a, int lanes, int steps_per,
                                                           int groups, int64_t waves) {
@@ -133,10 +134,11 @@ template <class T, int W>
 void rotary_wave_launch(const RotaryArgs& a, hipStream_t st) {
   const int lanes = a.dim / W, at_once = 64 / lanes;
   const int steps = (int)ceil_div(a.heads[0] + a.heads[1], at_once);
-  // Heads a wave: as many as leave each SIMD 8 waves, so that few sines are formed twice.
+  // Heads a wave: as many as leave each SIMD 2 waves, so that few sines are formed twice (all 20 heads of
+  // 128: 4096 tokens 13.6 us against 24.8 with 4 heads a wave, 65536 tokens 140 against 336).
   const int64_t rows = (int64_t)a.batch * a.tokens;
   int per = 1;
-  while (per < steps && rows * ceil_div(steps, 2 * per) >= 8192) per *= 2;
+  while (per < steps && rows * ceil_div(steps, 2 * per) >= 2048) per *= 2;
   per = std::min(per, steps);
   const int groups = (int)ceil_div(steps, per);
   const int64_t waves = rows * groups;
@@ -148,9 +150,10 @@ void rotary_wave_launch(const RotaryArgs& a, hipStream_t st) {
   }
 }
 
-// A thread holds the sines of W neighbouring elements' pairs of one token (of W / 2 pairs when
-// they are interleaved) and turns them in `per` heads, HB heads' loads in flight at a time; the
-// elements past the pairs are copied by further threads.
+// Heads that a wave does not hold (dim / W above 64: wide heads, or pairs that W must divide and are
+// odd).  A thread holds the sines of W neighbouring elements' pairs of one token (of W / 2 pairs
+// when they are interleaved) and turns them in `per` heads, HB heads' loads in flight at a time;
+// the elements past the pairs are copied by further threads.
 template <class T, int W, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int units, int rotated, int per,
                                                      int groups, int64_t threads) {
@@ -348,8 +351,10 @@ __device__ __forceinline__ float open_gate(float g, int act) {
   return act == NNX_GATE_SIGMOID ? s : g * s;
 }
 
-// G threads a row, each K runs of W channels; the row stays in registers from its one read to its
-// one write, and both norms take their moments there (mean first, then squares about it).  A run
+// Bound by memory: 262144 rows of 320, bf16 with a float32 residual and both norms, move 1.0 GB in 193 us,
+// 5.2 TB/s (a large copy reaches 4.8).  G threads a row, each K runs of W channels; the row stays in
+// registers from its one read to its one write, and both norms take their moments there (mean first,
+// then squares about it).  A run
 // that passes the row's end is moved back to end with it: its first `skip` channels are another
 // thread's, written twice with the same values and left out of the sums; runs wholly past the
 // end skip all W and write nothing.  Needs channels >= W.
@@ -501,8 +506,12 @@ __global__ __launch_bounds__(256) void residual_norm_narrow_kernel(NormArgs a, i
     if (c < a.channels) ((T*)a.y)[row * a.ys + c] = from_float<T>(u[c]);
 }
 
-// The fewest lanes that hold a row in at most 24 channels a thread (16 lanes: four rows a wave and
-// sums that stay inside 16 lanes), the fewest runs a thread that do.
+// The fewest lanes that hold a row in at most 24 channels a thread, the fewest runs a thread that do:
+// 16 lanes put four rows in a wave and keep its sums within 16 lanes (262144 rows of 320: 161 us
+// against 215 with a wave a row, of 64: 47 against 162), but leave few rows too few waves to hide
+// their loads (4096 of 320: 10.4 us against 7.7; even at 8192).
+constexpr int64_t kManyRows = 8192;
+
 template <class T, class R>
 void residual_norm_launch(const NormArgs& a, int rms, hipStream_t st) {
   constexpr int W = 16 / sizeof(T), S = 8 / W;
@@ -526,7 +535,7 @@ void residual_norm_launch(const NormArgs& a, int rms, hipStream_t st) {
     if (need <= 2) return go(g, two);
     go(g, three);
   };
-  if (a.channels <= 16 * 24) return lanes(integral_constant<int, 16>{});
+  if (a.channels <= 128 || (a.channels <= 16 * 24 && a.rows >= kManyRows)) return lanes(integral_constant<int, 16>{});
   if (a.channels <= 64 * 24) return lanes(integral_constant<int, 64>{});
   if (a.channels <= 256 * 24) return lanes(integral_constant<int, 256>{});
   go(integral_constant<int, 1024>{}, two);

@@ -305,6 +305,49 @@ def test_attention_strides(device, dtype):
     assert torch.equal(again, tokens.block_attention(q, shared.contiguous(), shared.contiguous(), ids, 32))
 
 
+def _some_rows_alone(q, k, v, ids, block, rows, dtype):
+    """A few of many queries, computed among all and alone."""
+    many = tokens.block_attention(q, k, v, ids, block)
+    for t in rows:
+        alone = tokens.block_attention(q[:, t:t + 1], k, v, ids[:, t:t + 1].contiguous(), block)
+        off = (many[:, t:t + 1].double() - alone.double()).abs().max()
+        assert float(off) <= (4 * U[dtype] + 5e-4) * float(v.abs().max()), t
+    return many
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_queries_cut_into_spans(device, dtype):
+    """Partials of more than the workspace holds at once: 40000 queries of three heads to a key head
+    that keep 50 blocks."""
+    case = (1, 40000, 4000, 6, 2, 64, 16, 50, 0, 0, False, False, False)
+    q, k, v = _attention_inputs(case, dtype)
+    ids = torch.rand(1, 40000, 2, 250, generator=_gen(50)).topk(50).indices.sort(-1).values.to(torch.int32).cuda()
+    many = _some_rows_alone(q, k, v, ids, 16, (0, 1, 9999, 13333, 13334, 26667, 39999), dtype)
+    assert torch.equal(many, tokens.block_attention(q, k, v, ids, 16))
+
+
+def test_as_many_blocks_as_there_may_be(device):
+    case = (1, 700, 32768 * 16, 2, 1, 32, 16, 40, 0, 0, False, False, False)
+    q, k, v = _attention_inputs(case, torch.float16)
+    ids = torch.randint(0, 32768 // 40, (1, 700, 1, 40), generator=_gen(51), dtype=torch.int32)
+    ids = (ids + torch.arange(40, dtype=torch.int32) * (32768 // 40)).cuda()
+    ids[0, :, 0, 39] = 32767
+    _some_rows_alone(q, k, v, ids, 16, (0, 350, 699), torch.float16)
+
+
+def test_many_heads_to_a_key_head(device):
+    case = (1, 9, 300, 200, 2, 40, 32, 3, 0, 0, False, False, False)
+    q, k, v = _attention_inputs(case, torch.float16)
+    summary = tokens.summarize_blocks(k, 32)
+    ids = tokens.select_blocks(q, summary, 32, 3, local=0)
+    codes, scales = (a.cpu().numpy() for a in summary)
+    assert np.array_equal(ids.cpu().numpy(), ot.select(_np32(q), codes, scales, 32, 3, local=0))
+    want, size = ot.attention(_f64(q), _f64(k), _f64(v), ot.seen(ids.cpu().numpy(), 300, 32, np.ones((1, 300), bool)),
+                              40**-0.5)
+    got = tokens.block_attention(q, k, v, ids, 32)
+    assert (np.abs(_f64(got) - want) <= (4 * 2.0**-11 + 5e-4) * size[..., None]).all()
+
+
 def test_rows_are_the_same_however_many_queries_come_along(device):
     """Selection is independent of what else is computed; so is a float32 result's order of
     magnitude: one query alone and among many agree within the derived float32 error."""

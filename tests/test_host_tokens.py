@@ -58,7 +58,7 @@ def test_residual_norm(change, text):
     (dict(type=9), "type"), (dict(batch=0), "items"), (dict(batch=65536), "items"), (dict(keys=0), "items"),
     (dict(kv_heads=0), "key heads"), (dict(head_dim=60), "head_dim"), (dict(head_dim=136), "head_dim"),
     (dict(block=48), "block"), (dict(keys=32768 * 16 + 1), "32768"), (dict(queries=0), "queries"),
-    (dict(heads=5), "multiple"), (dict(keep=0), "keep"), (dict(keep=257), "keep"),
+    (dict(heads=5), "multiple"), (dict(heads=2 * 1025), "share"), (dict(keep=0), "keep"), (dict(keep=257), "keep"),
     (dict(queries=1 << 30, keep=2), "2^31"), (dict(scale=float("inf")), "scale"), (dict(start=-1), "start"),
     (dict(first=-1), "first"), ({}, "null pointer")])
 def test_blocks(change, text):
