@@ -610,12 +610,15 @@ int nnx_block_summarize(const nnx_block_config* config, const void* d_k, const i
 /* Blocks kept by each query and key head: d_ids (batch, queries, kv_heads, keep) int32,
  * ascending, -1 behind the last.  A query head's codes are rint(q * (127 / m)), m = max |q|
  * (non-finite elements 0; m < 2^-60: codes 0, m = 1); a block's score is the largest over the
- * heads sharing the key head of (float(codes . codes) * m) * scale.  Kept are the `first` leading
- * blocks and the `local` ones ending at the query's own, then the highest scores, equal ones
- * by the lower index; blocks without valid keys (scale < 0) never, nor blocks behind a causal
- * query's own. */
+ * heads sharing the key head of (float(codes . codes) * m) * scale, at most the largest finite
+ * value in magnitude.  Kept are the `first` leading blocks and the `local` ones ending at the
+ * query's own, then the highest scores, equal ones by the lower index; blocks without valid keys
+ * (scale < 0) never, nor blocks behind a causal query's own.  A workspace of 0 bytes may be null;
+ * the workspace query answers 0 for what the entry refuses, too. */
+size_t nnx_block_select_workspace(const nnx_block_config* config);
 int nnx_block_select(const nnx_block_config* config, const void* d_q, const int8_t* d_codes,
-                     const float* d_scales, const int32_t* d_start, int32_t* d_ids, void* stream);
+                     const float* d_scales, const int32_t* d_start, int32_t* d_ids,
+                     void* d_workspace, size_t workspace_bytes, void* stream);
 
 /* out[q] = softmax(scale q . k) v over the valid keys of the blocks in d_ids (batch, queries,
  * kv_heads, keep; entries outside [0, nb) are skipped, the others of a row are distinct).  A

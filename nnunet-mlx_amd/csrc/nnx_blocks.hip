@@ -164,7 +164,7 @@ __device__ __forceinline__ Cut refine_cut(float low, float high, int want, Above
   return {back(hi), want - (int)above(back(hi))};
 }
 
-constexpr float kMostFloat = 3.4028235e38f;  // products can overflow
+constexpr float kMostFloat = 3.4028235e38f;
 
 template <class Above, class Range>
 __device__ __forceinline__ Cut find_cut(int want, Above&& above, Range&& range) {
@@ -172,7 +172,6 @@ __device__ __forceinline__ Cut find_cut(int want, Above&& above, Range&& range) 
   if (above(-INFINITY) <= want) return {-INFINITY, 0};
   float low, high;
   range(low, high);
-  low = fmaxf(low, -kMostFloat), high = fminf(high, kMostFloat);
   const int over = above(low);
   if (over < want) return {low, want - over};
   return refine_cut(low, high, want, above);
@@ -183,29 +182,53 @@ __device__ __forceinline__ int lanes_before(uint64_t lanes, int from) {
                                         __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, (uint32_t)from));
 }
 
-// N > 0: the row (in LDS, filled up to 64 N with NaN) is held in N registers a lane; N = 0: it is read
-// again for every step.
+// The row lies in LDS, `chunks` times 64 filled up with NaN; N > 0: N = chunks, held in N registers a
+// lane; N = 0: read again for every step.  `spare`: 256 places, for N > 0 the row's own.
 template <int N>
-__device__ __forceinline__ void select_row(float* score, int blocks, int keep, int first, int local,
-                                           int own, int32_t* out) {
+__device__ __forceinline__ void select_row(float* score, float* spare, int chunks, int blocks, int keep,
+                                           int first, int local, int own, int32_t* out) {
   const int lane = threadIdx.x % 64;
-  // N > 0: chunks of 64 in which this lane's block is forced, NaN while the others are compared;
-  // N = 0: forced blocks are +inf all the time
-  uint32_t marks = 0;
+  constexpr uint32_t kForced = 0x7fc00001u;  // a forced block: a NaN of its own while the others are compared
   int forced = 0;
   const auto force = [&](int begin, int end) {  // blocks begin .. end - 1 as far as they are candidates
     for (int j0 = begin / 64 * 64; j0 < end; j0 += 64) {
       const int j = j0 + lane;
       const bool take = j >= begin && j < end && score[j] > -INFINITY && score[j] < INFINITY;
-      if (take) {
-        score[j] = N ? NAN : INFINITY;
-        marks |= 1u << (j / 64 % 32);
-      }
+      if (take) score[j] = __uint_as_float(kForced);
       forced += __popcll(__ballot(take));
     }
   };
   if (first) force(0, min(first, blocks));
   if (local) force(max(own + 1 - local, 0), min(own + 1, blocks));
+  float v[N ? N : 1];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = score[i * 64 + lane];
+  const auto each = [&](auto&& body) {
+    if constexpr (N > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) body(i, v[i]);
+    } else {
+      for (int i = 0; i < chunks; ++i) body(i, score[i * 64 + lane]);
+    }
+  };
+  const auto above = [&](float x) {
+    int count = 0;
+    each([&](int, float y) { count += __popcll(__ballot(y > x)); });
+    return count;
+  };
+  const auto larger = [](float x, float y) { return fmaxf(x, y); };
+  const auto range = [&](float& low, float& high) {
+    low = INFINITY, high = -INFINITY;
+    each([&](int, float y) { low = y < low ? y : low, high = y > high ? y : high; });
+    low = -lanes_reduce<64>(-low, larger);
+    high = lanes_reduce<64>(high, larger);
+  };
+  const auto restore = [&] {  // forced blocks above all others
+    const auto shown = [](float y) { return __float_as_uint(y) == kForced ? INFINITY : y; };
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = shown(v[i]);
+    for (int i = 0; !N && i < chunks; ++i) score[i * 64 + lane] = shown(score[i * 64 + lane]);
+  };
   int done = 0, tied = 0;
   const auto emit = [&](int block, uint64_t equal, bool take, int ties) {
     if (ties) {
@@ -217,122 +240,61 @@ __device__ __forceinline__ void select_row(float* score, int blocks, int keep, i
     if (take && to < keep) out[(uint32_t)to] = block;
     done += __popcll(taken);
   };
-  const auto larger = [](float x, float y) { return fmaxf(x, y); };
-  if constexpr (N > 0) {
-    float v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = score[i * 64 + lane];
-    const auto above = [&](float x) {
-      int count = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) count += __popcll(__ballot(v[i] > x));
-      return count;
-    };
-    const auto range = [&](float& low, float& high) {
-      low = INFINITY, high = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < N; ++i) low = v[i] < low ? v[i] : low, high = v[i] > high ? v[i] : high;
-      low = -lanes_reduce<64>(-low, larger);
-      high = lanes_reduce<64>(high, larger);
-    };
-    const auto restore = [&] {  // forced blocks above all others
-      for (uint32_t m = marks; m; m &= m - 1) score[__builtin_ctz(m) * 64 + lane] = INFINITY;
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = score[i * 64 + lane];
-    };
-    if constexpr (N >= 4) {
-      // Once no more than 128 scores are left above the lower end, they and their blocks are packed
-      // into two registers (by way of the row's own place), where the rest of the search and the
-      // writing cost a fraction.
-      const int want = keep - forced;
-      int over = above(-INFINITY);
-      if (keep <= 128 && want > 0 && over > want) {
-        float low, high;
-        range(low, high);
-        high = fminf(high, kMostFloat);
-        low = fmaxf(low - fabsf(low) * 1e-6f - 1e-30f, -kMostFloat);  // below all
-        for (int step = 0; step < 14 && over + forced > 128; ++step) {
-          const float mid = 0.5f * low + 0.5f * high;
-          const int count = above(mid);
-          if (count < want) {
-            high = mid;
-          } else {
-            low = mid, over = count;
-          }
-        }
-        if (over + forced <= 128) {
-          if (forced) restore();
-          int n = 0;
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const bool take = v[i] > low;
-            const uint64_t taken = __ballot(take);
-            const int to = lanes_before(taken, n);
-            if (take && to < 128) score[to] = v[i], score[128 + to] = __int_as_float(i * 64 + lane);
-            n += __popcll(taken);
-          }
-          float w[2];
-          int32_t at[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const bool in = i * 64 + lane < n;
-            w[i] = in ? score[i * 64 + lane] : NAN;
-            at[i] = in ? __float_as_int(score[128 + i * 64 + lane]) : 0;
-          }
-          const Cut cut = refine_cut(low, high, keep, [&](float x) {
-            return __popcll(__ballot(w[0] > x)) + __popcll(__ballot(w[1] > x));
-          });
-#pragma unroll
-          for (int i = 0; i < 2; ++i) emit(at[i], cut.ties ? __ballot(w[i] == cut.above) : 0, w[i] > cut.above, cut.ties);
-          for (int i = min(done, keep) + lane; i < keep; i += 64) out[i] = -1;
-          return;
+  const auto finish = [&] {
+    for (int i = min(done, keep) + lane; i < keep; i += 64) out[i] = -1;
+  };
+  if constexpr (N == 0 || N >= 4) {
+    // Once no more than 128 scores are left above the lower end, they and their blocks are packed into two
+    // registers (by way of `spare`), where the rest of the search and the writing cost a fraction.  (A first
+    // guess from two or four samples a lane saved steps and no time: 153 us against 153.)
+    const int want = keep - forced, room = 128 - forced;
+    int over = above(-INFINITY);
+    if (keep <= 128 && want > 0 && over > want) {
+      float low, high;
+      range(low, high);
+      low -= fabsf(low) * 1e-6f + 1e-30f;  // below all, -inf at worst
+      for (int step = 0; step < 14 && over > room; ++step) {
+        const float mid = 0.5f * low + 0.5f * high;
+        const int count = above(mid);
+        if (count < want) {
+          high = mid;
+        } else {
+          low = mid, over = count;
         }
       }
-    }
-    const Cut cut = find_cut(keep - forced, above, range);
-    if (forced) restore();
-    if (cut.ties || forced > keep) {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        emit(i * 64 + lane, __ballot(v[i] == cut.above), v[i] > cut.above || v[i] == INFINITY, cut.ties);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const bool take = v[i] > cut.above;
-        const uint64_t taken = __ballot(take);
-        const int to = lanes_before(taken, done);
-        if (take && to < keep) out[(uint32_t)to] = i * 64 + lane;
-        done += __popcll(taken);
-      }
-    }
-  } else {
-    const int n = (blocks + 63) / 64;
-    const auto value = [&](int i) { return i * 64 + lane < blocks ? score[i * 64 + lane] : NAN; };
-    const Cut cut = find_cut(
-        keep - forced,
-        [&](float x) {
-          int count = 0;
-          for (int i = 0; i < n; ++i) {
-            const float v = value(i);
-            count += __popcll(__ballot(v > x && v < INFINITY));
-          }
-          return count;
-        },
-        [&](float& low, float& high) {
-          low = INFINITY, high = -INFINITY;
-          for (int i = 0; i < n; ++i) {
-            const float v = value(i);
-            low = v < low ? v : low, high = v > high && v < INFINITY ? v : high;
-          }
-          low = -lanes_reduce<64>(-low, larger);
-          high = lanes_reduce<64>(high, larger);
+      if (over <= room) {
+        if (forced) restore();
+        int n = 0;
+        each([&](int i, float y) {
+          const bool take = y > low;
+          const uint64_t taken = __ballot(take);
+          const int to = lanes_before(taken, n);
+          if (take && to < 128) spare[to] = y, spare[128 + to] = __int_as_float(i * 64 + lane);
+          n += __popcll(taken);
         });
-    for (int i = 0; i < n; ++i) {
-      const float v = value(i);
-      emit(i * 64 + lane, __ballot(cut.ties && v == cut.above), v > cut.above || v == INFINITY, cut.ties);
+        float w[2];
+        int32_t at[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const bool in = i * 64 + lane < n;
+          w[i] = in ? spare[i * 64 + lane] : NAN;
+          at[i] = in ? __float_as_int(spare[128 + i * 64 + lane]) : 0;
+        }
+        const Cut cut = refine_cut(low, high, keep, [&](float x) {
+          return __popcll(__ballot(w[0] > x)) + __popcll(__ballot(w[1] > x));
+        });
+#pragma unroll
+        for (int i = 0; i < 2; ++i) emit(at[i], cut.ties ? __ballot(w[i] == cut.above) : 0, w[i] > cut.above, cut.ties);
+        return finish();
+      }
     }
   }
-  for (int i = min(done, keep) + lane; i < keep; i += 64) out[i] = -1;
+  const Cut cut = find_cut(keep - forced, above, range);
+  if (forced) restore();
+  each([&](int i, float y) {
+    emit(i * 64 + lane, cut.ties ? __ballot(y == cut.above) : 0, y > cut.above || y == INFINITY, cut.ties);
+  });
+  finish();
 }
 
 // `rows` <= 16 queries of one item and key head: their scores against 16 blocks at a time by 8-bit
@@ -340,27 +302,42 @@ __device__ __forceinline__ void select_row(float* score, int blocks, int keep, i
 // head are taken kScoreHeads at a time (their codes in LDS) and meet in the largest score.  A
 // wave's next AHEAD times 16 blocks are on their way while it scores the ones before.
 constexpr int kScoreHeads = 8;
+// Rows of up to 2048 blocks (32 registers a lane) are scored and picked from by one workgroup, a tile
+// of 16 queries each, unless there are few tiles and each has much to score (blocks times heads, twice
+// for more than 64 channels).  One kernel against parts, 4 tiles: 8192 15 us and 17, 16384 20 to 29 and
+// 17 to 21, 32768 32 and 23; 32768 at 32 tiles 32 and 32, at 128 34 and 57.
+constexpr int kWholeBlocks = 2048, kFewTiles = 16, kMuchWork = 16384;
+constexpr int64_t kScoreBudget = (int64_t)128 << 20;
+
+struct Parts {
+  int count, blocks;  // of a row; of a part
+  int rows, pitch;    // queries of a launch, places of one
+  float* scores;      // by item, key head and query
+};
+
+// The block of a query's own position: -1 before the first key, at most 2^24 (past the last block).
+__device__ __forceinline__ int own_block(const BlockArgs& a, int b, int t) {
+  const int64_t at = (item_start(a, b) + t) >> __builtin_ctz(a.block);
+  return (int)min(max(at, (int64_t)-1), (int64_t)1 << 24);
+}
+constexpr int kPart = -1;  // the scores of a part of the blocks only, to global memory
 
 template <class T, int N>
 __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, const int8_t* codes,
                                                       const float* scales, int32_t* ids, int rows,
-                                                      int pitch) {
+                                                      int pitch, int from, Parts parts) {
   extern __shared__ __attribute__((aligned(16))) float score[];  // rows x pitch
   i32x4* qcode = (i32x4*)(score + rows * pitch);                 // by head, 64 channels, lane
   __shared__ float qtop[kScoreHeads][16];
-  const int t0 = blockIdx.x * rows, g = blockIdx.y, b = blockIdx.z;
+  const int t0 = from + (N == kPart ? blockIdx.x / parts.count : blockIdx.x) * rows, g = blockIdx.y, b = blockIdx.z;
+  const int begin = N == kPart ? blockIdx.x % parts.count * parts.blocks : 0;
+  const int stop = N == kPart ? min(begin + parts.blocks, a.blocks) : a.blocks;
   const int lane = threadIdx.x % 64, col = lane % 16, quad = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
   const int64_t unit = (int64_t)b * a.kv_heads + g;
-  constexpr int AHEAD = 2;
+  constexpr int AHEAD = N == kPart ? 1 : 2;
   const bool wide = a.dim > 64;
-  const int shift = __builtin_ctz(a.block);
-  // the block of a query's own position: -1 before the first key, at most 2^24 (past the last block)
-  const auto own_block = [&](int r) {
-    const int64_t at = (item_start(a, b) + t0 + r) >> shift;
-    return (int)min(max(at, (int64_t)-1), (int64_t)1 << 24);
-  };
-  const int own = a.causal ? own_block(col) : 1 << 24;
+  const int own = a.causal ? own_block(a, b, t0 + col) : 1 << 24;
   const uint32_t unit_bytes = (uint32_t)a.blocks * a.dim;
   const auto cu = buffer_of(codes + unit * unit_bytes, unit_bytes);
   const auto su = buffer_of(scales + unit * a.blocks, a.blocks * 4);
@@ -382,7 +359,7 @@ __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, c
 #pragma unroll
     for (int r = 0; r < 4; ++r) x.scale[r] = (int)__builtin_amdgcn_raw_buffer_load_b32(su, scale_at + 4 * r, j0 * 4, 0);
   };
-  if (N) {
+  if (N > 0) {
     const int full = (a.blocks + 15) / 16 * 16, rest = N * 64 - full;
     for (int i = threadIdx.x; i < rows * rest; i += blockDim.x)
       score[i / rest * pitch + full + i % rest] = NAN;
@@ -391,7 +368,7 @@ __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, c
     const int heads = min(kScoreHeads, a.group - h0);
     Blocks x[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) load(x[i], (wave + i * waves) * 16);
+    for (int i = 0; i < AHEAD; ++i) load(x[i], begin + (wave + i * waves) * 16);
     if (h0) __syncthreads();
     // 16 lanes a query and head, 8 channels each, into the places of the products' second operand
     for (int i = threadIdx.x / 16; i < heads * 16; i += blockDim.x / 16) {
@@ -423,7 +400,6 @@ __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, c
       float best[4], scale[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) scale[r] = __int_as_float(x.scale[r]);
-#pragma unroll 4
       for (int h = 0; h < heads; ++h) {
         i32x4 dot = {0, 0, 0, 0};
         dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(k0, qcode[h * 128 + lane], dot, 0, 0, 0);
@@ -435,8 +411,11 @@ __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, c
           best[r] = h && !(y > best[r]) ? best[r] : y;
         }
       }
+      // products can overflow; infinities mean something else to what follows
+#pragma unroll
+      for (int r = 0; r < 4; ++r) best[r] = __builtin_amdgcn_fmed3f(best[r], -kMostFloat, kMostFloat);
       if (col < rows) {
-        float4* to = (float4*)&score[col * pitch + j0 + quad * 4];
+        float4* to = (float4*)&score[col * pitch + j0 - begin + quad * 4];
         if (h0) {
           const float4 z = *to;
           best[0] = fmaxf(best[0], z.x), best[1] = fmaxf(best[1], z.y);
@@ -456,19 +435,80 @@ __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, c
         *to = make_float4(best[0], best[1], best[2], best[3]);
       }
     };
-    for (int j0 = wave * 16; j0 < a.blocks; j0 += AHEAD * waves * 16) {
+    for (int j0 = begin + wave * 16; j0 < stop; j0 += AHEAD * waves * 16) {
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
         const int j = j0 + i * waves * 16;
-        if (j < a.blocks) compute(x[i], j);
-        load(x[i], j + AHEAD * waves * 16);
+        if (j < stop) compute(x[i], j);
+        if (N != kPart || j + AHEAD * waves * 16 < stop) load(x[i], j + AHEAD * waves * 16);
       }
     }
   }
   __syncthreads();
-  for (int r = wave; r < rows && t0 + r < a.queries; r += waves)
-    select_row<N>(score + r * pitch, a.blocks, a.keep, a.first, a.local, own_block(r),
-                  ids + (((int64_t)b * a.queries + t0 + r) * a.kv_heads + g) * a.keep);
+  if constexpr (N == kPart) {
+    const int each = (stop - begin + 15) / 16 * 4;  // float4 of a row
+    const int last = min(rows, from + parts.rows - t0);  // the launch's may be fewer than the queries
+    for (int i = threadIdx.x; i < min(last, a.queries - t0) * each; i += blockDim.x) {
+      const int r = i / each, j = i % each * 4;
+      *(float4*)(parts.scores + (unit * parts.rows + t0 - from + r) * parts.pitch + begin + j) = *(float4*)&score[r * pitch + j];
+    }
+  } else {
+    for (int r = wave; r < rows && t0 + r < a.queries; r += waves)
+      select_row<N>(score + r * pitch, score + r * pitch, N, a.blocks, a.keep, a.first, a.local, own_block(a, b, t0 + r),
+                    ids + (((int64_t)b * a.queries + t0 + r) * a.kv_heads + g) * a.keep);
+  }
+}
+
+// A wave a row of scores in global memory.
+template <int N>
+__global__ __launch_bounds__(64) void pick_kernel(BlockArgs a, int from, Parts parts, int32_t* ids) {
+  extern __shared__ __attribute__((aligned(16))) float score[];  // chunks times 64; N = 0: 256 more
+  const int t = from + blockIdx.x, g = blockIdx.y, b = blockIdx.z, chunks = N ? N : (a.blocks + 63) / 64;
+  const float* row = parts.scores + (((int64_t)b * a.kv_heads + g) * parts.rows + blockIdx.x) * parts.pitch;
+#pragma unroll N ? N : 8
+  for (int i = 0; i < chunks; ++i) {
+    const int j = i * 64 + threadIdx.x;
+    score[j] = j < parts.pitch ? row[j] : NAN;
+  }
+  __syncthreads();
+  select_row<N>(score, N ? score : score + chunks * 64, chunks, a.blocks, a.keep, a.first, a.local,
+                own_block(a, b, t), ids + (((int64_t)b * a.queries + t) * a.kv_heads + g) * a.keep);
+}
+
+// Rows of many blocks, or few rows of much work: the scores by parts of a row, a workgroup each, to
+// global memory, then a wave a row picks.
+struct SelectPlan {
+  bool split;
+  int chunks, rows, pitch;  // of the kernel that forms scores: 64 blocks each, queries of a workgroup, LDS row
+  int queries;              // of a launch
+  Parts parts;
+  size_t bytes;
+};
+
+SelectPlan plan_selection(const nnx_block_config& c) {
+  SelectPlan p{};
+  const int blocks = (int)ceil_div(c.keys, c.block), group = c.heads / c.kv_heads;
+  const int64_t units = (int64_t)c.kv_heads * c.batch, tiles = ceil_div(c.queries, 16) * units;
+  p.chunks = 1;
+  while (p.chunks * 64 < blocks) p.chunks *= 2;
+  p.rows = std::min(16, c.queries);
+  p.split = blocks > kWholeBlocks ||
+            (tiles <= kFewTiles && (int64_t)blocks * group * (c.head_dim > 64 ? 2 : 1) >= kMuchWork);
+  if (!p.split) {
+    const size_t codes = (size_t)std::min(group, kScoreHeads) * 2048;
+    p.pitch = p.chunks * 64 + 4;
+    while (p.rows > 1 && (size_t)p.rows * p.pitch * 4 + codes > 160 * 1024 - 1024) p.rows /= 2;
+    return p;
+  }
+  p.parts.pitch = (int)ceil_div(blocks, 16) * 16;
+  p.queries = (int)std::min<int64_t>(c.queries, std::max<int64_t>(16, kScoreBudget / (units * p.parts.pitch * 4) / 16 * 16));
+  p.parts.rows = p.queries;
+  const double want = (double)blocks * ceil_div(p.queries, 16) * units / 256;
+  p.parts.blocks = (int)std::min(1024.0, std::max(1.0, std::ceil(want / 64)) * 64);
+  p.parts.count = (int)ceil_div(blocks, p.parts.blocks);
+  p.pitch = p.parts.blocks + 4;
+  p.bytes = (size_t)units * p.queries * p.parts.pitch * 4;
+  return p;
 }
 
 // ---- the attention ---------------------------------------------------------------------
@@ -661,10 +701,10 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
 // the lists of many launches are formed at once.
 constexpr size_t kPartialBudget = (size_t)160 << 20;
 constexpr int64_t kListPairs = (int64_t)1 << 27;
-// Pairs go one by one while they and the keys and values that they read come to no more than this: 5120
-// pairs of 16 KiB took 28 us one by one and 16 + 16 us by block (lists, partials), 8192 of 32 KiB 71
-// and 19 + 21, 1280 of 16 KiB 13 and 16 + 15.
-constexpr double kDirectPairs = 8192, kDirectBytes = 80e6;
+// Pairs go one by one up to so many, and so many bytes of keys and values.  One by one against by block
+// (lists and partials): 1280 of 16 KiB 13 us and 16 + 15, 5120 28 and 16 + 16, 8192 of 32 KiB 71 and
+// 19 + 21; 19200 of 4 KiB 45 and 25 + 30, 40000 of 1 KiB 67 and 25 + 24.
+constexpr double kDirectPairs = 20000, kDirectBytes = 80e6;
 
 struct AttentionPlan {
   bool by_block;
@@ -743,39 +783,72 @@ void block_summarize(const nnx_block_config& c, const void* k, const int32_t* le
 }
 
 void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
-                  const float* scales, const int32_t* start, int32_t* ids, hipStream_t st) {
+                  const float* scales, const int32_t* start, int32_t* ids, void* ws, size_t ws_bytes,
+                  hipStream_t st) {
   check_config(c, "block selection", true);
   require(q && codes && scales && ids, "block selection: null pointer");
+  const SelectPlan plan = plan_selection(c);
+  require(!plan.split || (ws && ws_bytes >= plan.bytes && reinterpret_cast<uintptr_t>(ws) % 16 == 0),
+          "block selection: the workspace is too small or not 16-byte aligned");
   const BlockArgs a = make_args(c, start, nullptr, nullptr);
   const double products = (double)c.batch * c.queries * c.heads * c.head_dim;
   ProfScope prof("block_select", 2.0 * products * a.blocks, products * type_bytes(c.type), st);
-  // As many queries a workgroup as the products take, while their scores fit the LDS; rows of up to
-  // 2048 blocks are picked from registers.  Few workgroups take twice the waves.
-  int n = 1;
-  while (n < 32 && n * 64 < a.blocks) n *= 2;
-  if (n * 64 < a.blocks) n = 0;
-  const int pitch = (n ? n * 64 : (int)ceil_div(a.blocks, 16) * 16) + 4;
-  const size_t heads = (size_t)std::min(a.group, kScoreHeads) * 2048;
-  int rows = 16;
-  while (rows > 1 && (size_t)rows * pitch * 4 + heads > 160 * 1024 - 1024) rows /= 2;
-  const dim3 grid((unsigned)ceil_div(c.queries, rows), c.kv_heads, c.batch);
+  using std::integral_constant;
+  const size_t codes_bytes = (size_t)std::min(a.group, kScoreHeads) * 2048;
+  const size_t shared = plan.rows * plan.pitch * sizeof(float) + codes_bytes;
+  if (plan.split) {
+    Parts parts = plan.parts;
+    parts.scores = (float*)ws;
+    for (int from = 0; from < c.queries; from += parts.rows) {
+      const int queries = std::min(parts.rows, c.queries - from);
+      const dim3 grid((unsigned)ceil_div(queries, plan.rows) * parts.count, c.kv_heads, c.batch);
+      with_type(c.type, [&](auto t) {
+        using T = decltype(t);
+        select_kernel<T, kPart><<<grid, 256, shared, st>>>(a, (const T*)q, codes, scales, ids, plan.rows, plan.pitch,
+                                                           from, parts);
+      });
+      launch_check("block_select");
+      auto go = [&](auto k) {
+        constexpr int N = decltype(k)::value;
+        const size_t places = N ? N * 64 : ceil_div(a.blocks, 64) * 64 + 256;
+        pick_kernel<N><<<dim3(queries, c.kv_heads, c.batch), 64, places * sizeof(float), st>>>(a, from, parts, ids);
+      };
+      if (plan.chunks <= 16) go(integral_constant<int, 16>{});
+      else if (plan.chunks == 32) go(integral_constant<int, 32>{});
+      else if (plan.chunks == 64) go(integral_constant<int, 64>{});
+      else if (plan.chunks == 128) go(integral_constant<int, 128>{});
+      else go(integral_constant<int, 0>{});
+      launch_check("block_select");
+    }
+    return;
+  }
+  // As many queries a workgroup as the products take, while their scores fit the LDS.  Few workgroups
+  // take twice the waves.
+  const dim3 grid((unsigned)ceil_div(c.queries, plan.rows), c.kv_heads, c.batch);
   const int threads = (double)grid.x * grid.y * grid.z < 2 * compute_units() ? 1024 : 512;
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto k) {
-      select_kernel<T, decltype(k)::value><<<grid, threads, rows * pitch * sizeof(float) + heads, st>>>(
-          a, (const T*)q, codes, scales, ids, rows, pitch);
+      select_kernel<T, decltype(k)::value><<<grid, threads, shared, st>>>(
+          a, (const T*)q, codes, scales, ids, plan.rows, plan.pitch, 0, Parts{});
     };
-    using std::integral_constant;
-    if (n == 1) return go(integral_constant<int, 1>{});
-    if (n == 2) return go(integral_constant<int, 2>{});
-    if (n == 4) return go(integral_constant<int, 4>{});
-    if (n == 8) return go(integral_constant<int, 8>{});
-    if (n == 16) return go(integral_constant<int, 16>{});
-    if (n == 32) return go(integral_constant<int, 32>{});
-    go(integral_constant<int, 0>{});
+    if (plan.chunks == 1) return go(integral_constant<int, 1>{});
+    if (plan.chunks == 2) return go(integral_constant<int, 2>{});
+    if (plan.chunks == 4) return go(integral_constant<int, 4>{});
+    if (plan.chunks == 8) return go(integral_constant<int, 8>{});
+    if (plan.chunks == 16) return go(integral_constant<int, 16>{});
+    go(integral_constant<int, 32>{});
   });
   launch_check("block_select");
+}
+
+size_t block_select_workspace(const nnx_block_config& c) {
+  try {
+    check_config(c, "block selection", true);
+    return plan_selection(c).bytes;
+  } catch (const Error&) {
+    return 0;
+  }
 }
 
 size_t block_attention_workspace(const nnx_block_config& c) {

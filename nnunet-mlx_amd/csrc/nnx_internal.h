@@ -348,8 +348,9 @@ void residual_norm(const nnx_residual_norm_config& c, const void* x, const void*
 void block_summarize(const nnx_block_config& c, const void* k, const int32_t* lengths,
                      const uint8_t* mask, int first_block, int blocks, int8_t* codes,
                      float* scales, hipStream_t st);
+size_t block_select_workspace(const nnx_block_config& c);
 void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
-                  const float* scales, const int32_t* start, int32_t* ids, hipStream_t st);
+                  const float* scales, const int32_t* start, int32_t* ids, void* ws, size_t ws_bytes, hipStream_t st);
 size_t block_attention_workspace(const nnx_block_config& c);
 void block_attention(const nnx_block_config& c, const void* q, const void* k, const void* v,
                      const int32_t* ids, const int32_t* start, const int32_t* lengths,

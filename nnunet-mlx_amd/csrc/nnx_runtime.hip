@@ -1641,11 +1641,17 @@ int nnx_block_summarize(const nnx_block_config* config, const void* d_k, const i
   });
 }
 
+size_t nnx_block_select_workspace(const nnx_block_config* config) {
+  return config ? block_select_workspace(*config) : 0;
+}
+
 int nnx_block_select(const nnx_block_config* config, const void* d_q, const int8_t* d_codes,
-                     const float* d_scales, const int32_t* d_start, int32_t* d_ids, void* stream) {
+                     const float* d_scales, const int32_t* d_start, int32_t* d_ids,
+                     void* d_workspace, size_t workspace_bytes, void* stream) {
   return guarded([&] {
     require(config, "block selection: null config");
-    block_select(*config, d_q, d_codes, d_scales, d_start, d_ids, as_stream(stream));
+    block_select(*config, d_q, d_codes, d_scales, d_start, d_ids, d_workspace, workspace_bytes,
+                 as_stream(stream));
   });
 }
 

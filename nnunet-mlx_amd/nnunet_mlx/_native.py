@@ -366,9 +366,11 @@ _SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [ctypes.POINTER(NnxBlockConfig), c_void_p, c_void_p, c_void_p, ctypes.c_int, ctypes.c_int,
          c_void_p, c_void_p, c_void_p],
     ),
+    "nnx_block_select_workspace": (ctypes.c_size_t, [ctypes.POINTER(NnxBlockConfig)]),
     "nnx_block_select": (
         ctypes.c_int,
-        [ctypes.POINTER(NnxBlockConfig), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+        [ctypes.POINTER(NnxBlockConfig), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         ctypes.c_size_t, c_void_p],
     ),
     "nnx_block_attention_workspace": (ctypes.c_size_t, [ctypes.POINTER(NnxBlockConfig)]),
     "nnx_block_attention": (

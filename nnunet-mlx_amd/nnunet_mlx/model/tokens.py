@@ -404,20 +404,23 @@ def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int,
     placed = isinstance(start, torch.Tensor)
     key = ("select", _signature(q, *summary, start if placed else None), block, keep, causal,
            None if placed else start, first, local)
-    config = _checked.get(key)
-    if config is None:
-        config = _remember(key, _selection_config(q, summary, block, keep, causal, start, first, local))
+    known = _checked.get(key)
+    if known is None:
+        known = _remember(key, _selection_config(q, summary, block, keep, causal, start, first, local))
+    config, size = known
     ids = torch.empty((q.shape[0], q.shape[1], summary.codes.shape[1], keep), dtype=torch.int32, device=q.device)
     if config:
+        work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         _launch(q.device, "nnx_block_select", config, q.data_ptr(), summary.codes.data_ptr(),
-                summary.scales.data_ptr(), start.data_ptr() if placed else None, ids.data_ptr())
+                summary.scales.data_ptr(), start.data_ptr() if placed else None, ids.data_ptr(), _address(work), size)
     elif ids.numel():
         ids.fill_(-1)
     return ids
 
 
 def _selection_config(q, summary, block, keep, causal, start, first, local):
-    """The checked configuration of a selection, False where there is nothing to select from."""
+    """The checked configuration of a selection (False where there is nothing to select from) and its workspace's
+    bytes."""
     _check("q", q, 4)
     batch, queries, heads, dim = q.shape
     _need(summary.codes.dim() == 4, f"summary codes need 4 axes, got shape {tuple(summary.codes.shape)}")
@@ -429,7 +432,9 @@ def _selection_config(q, summary, block, keep, causal, start, first, local):
     config = _block_config(q, block, batch, queries, blocks * block, heads, kv_heads, keep=keep, first=first,
                            local=local, causal=causal, start=start if isinstance(start, int) else 0,
                            q=q.stride()[:3])
-    return config if q.numel() and blocks else False
+    if q.numel() == 0 or blocks == 0:
+        return False, 0
+    return config, _native.load().nnx_block_select_workspace(config)
 
 
 def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torch.Tensor, block: int, *,

@@ -103,6 +103,7 @@ def select(q: np.ndarray, codes: np.ndarray, scales: np.ndarray, block: int, kee
             dots = whole[b, :, mine] @ codes[b, g].astype(np.int64).T  # (T, group, blocks)
             with np.errstate(over="ignore"):
                 score = (dots.astype(F32) * top[b, :, mine] * scales[b, g]).max(1)
+            score = np.clip(score, np.finfo(F32).min, np.finfo(F32).max)
             for t in range(queries):
                 own = ((0 if start is None else int(start[b])) + t) // block
                 row = score[t].copy()

@@ -445,6 +445,48 @@ def test_selection_with_equal_scores(device, blocks, keep, first, local, levels)
         assert np.array_equal(got.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("dim,heads", [(40, 6), (128, 20)])
+@pytest.mark.parametrize("blocks,keep,first,local", [
+    (255, 9, 1, 1), (256, 128, 0, 1), (257, 129, 2, 1), (512, 32, 0, 1), (700, 256, 5, 70), (1500, 100, 90, 90),
+    (2048, 128, 0, 1), (2100, 40, 1, 2), (4096, 20, 0, 0), (4099, 130, 1, 40), (8192, 64, 30, 1), (8200, 7, 1, 1)])
+def test_selection_alone_and_among_many(device, blocks, keep, first, local, dim, heads):
+    """Scores formed by parts for few queries and by whole rows for many: both as the formulas', among equals."""
+    gen = _gen(blocks + keep + dim)
+    codes = torch.randint(-9, 10, (1, 2, blocks, dim), generator=gen, dtype=torch.int8)
+    codes[..., 5:-1] = 0
+    scales = torch.randint(0, 9, (1, 2, blocks), generator=gen).float() * 0.5
+    scales[torch.rand(1, 2, blocks, generator=gen) < 0.1] = -1
+    q = torch.randint(-2, 3, (1, 1100, heads, dim), generator=gen).float()
+    summary = tokens.BlockSummary(codes.cuda(), scales.cuda())
+    for causal in (False, True):
+        begin = blocks * 16 - 900
+        start = torch.tensor([begin], dtype=torch.int32)
+        args = dict(first=first, local=local, causal=causal)
+        many = tokens.select_blocks(q.cuda(), summary, 16, keep, start=start.cuda(), **args)
+        for t in (0, 3, 517, 1083):
+            few = tokens.select_blocks(q[:, t:t + 17].cuda(), summary, 16, keep, start=begin + t, **args)
+            assert torch.equal(few, many[:, t:t + 17])
+        want = ot.select(q[:, 517:522].numpy(), codes.numpy(), scales.numpy(), 16, keep,
+                         start=np.array([begin + 517]), **args)
+        assert np.array_equal(many[:, 517:522].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("blocks", [60, 200, 300, 2500, 9000])
+@pytest.mark.parametrize("queries", [3, 2100])
+def test_selection_of_scores_that_overflow(device, blocks, queries):
+    gen = _gen(blocks)
+    codes = torch.randint(-127, 128, (1, 1, blocks, 32), generator=gen, dtype=torch.int8)
+    scales = torch.rand(1, 1, blocks, generator=gen) * 100
+    scales[torch.rand(1, 1, blocks, generator=gen) < 0.5] = -1
+    q = torch.randn(1, queries, 2, 32, generator=gen).sign() * torch.tensor([1e37, 1.0])[None, None, :, None]
+    q[0, 1] = 1e38
+    start = torch.tensor([blocks * 16 - 40], dtype=torch.int32)
+    got = tokens.select_blocks(q.cuda(), tokens.BlockSummary(codes.cuda(), scales.cuda()), 16, 20,
+                               start=start.cuda(), first=3, local=2)
+    want = ot.select(q[:, :3].numpy(), codes.numpy(), scales.numpy(), 16, 20, start=start.numpy(), first=3, local=2)
+    assert np.array_equal(got[:, :3].cpu().numpy(), want)
+
+
 def test_attention_skips_entries_that_are_no_blocks(device):
     case = (1, 70, 100, 2, 2, 64, 32, 4, 0, 0, False, False, False)
     q, k, v = _attention_inputs(case, torch.float16)

@@ -63,7 +63,7 @@ def test_residual_norm(change, text):
     (dict(first=-1), "first"), ({}, "null pointer")])
 def test_blocks(change, text):
     lib, config = _native.load(), _block(**change)
-    _refused(lib.nnx_block_select(config, *[None] * 6), text)
+    _refused(lib.nnx_block_select(config, *[None] * 6, 0, None), text)
     _refused(lib.nnx_block_attention(config, *[None] * 9, 0, None), text)
     if change:
         assert lib.nnx_block_attention_workspace(config) == 0
@@ -81,5 +81,5 @@ def test_summaries():
 def test_null_configs():
     lib = _native.load()
     none = ctypes.POINTER(_native.NnxBlockConfig)()
-    _refused(lib.nnx_block_select(none, *[None] * 6), "null config")
+    _refused(lib.nnx_block_select(none, *[None] * 6, 0, None), "null config")
     assert lib.nnx_block_attention_workspace(none) == 0
