@@ -624,6 +624,11 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
     t = vt - span * c.nt;
     s = span_of(c, c.span0 + span);
   };
+  // partials lie by query, slot and head
+  const auto partial_of = [&](int64_t row) {
+    const int vt = c.by_group((int)row);
+    return (int64_t)vt * a.keep * a.group + (int)row - vt * a.group;
+  };
   for (int i = threadIdx.x; i < here * a.keep; i += 256) {
     const int r = c.by_keep(i), slot = i - r * a.keep;
     Span s;
@@ -632,7 +637,7 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
     int j = -1;
     if (t < s.queries)
       j = c.ids[(((int64_t)s.b * a.queries + s.t0 + t) * a.kv_heads + s.g) * a.keep + slot];
-    weight[i] = (unsigned)j < (unsigned)a.blocks ? c.meta[(row0 + r) * a.keep + slot]
+    weight[i] = (unsigned)j < (unsigned)a.blocks ? c.meta[partial_of(row0 + r) + (int64_t)slot * a.group]
                                                  : make_float2(-INFINITY, 0.f);
   }
   const int lanes = a.dim / 8, sub = threadIdx.x / lanes, u = threadIdx.x - sub * lanes;
@@ -640,11 +645,11 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
   const bool live = own < here;
   // Partials of entries that are no block were never written: whatever is there is left out below.
   constexpr int AHEAD = 8;
-  const P* part = (const P*)c.part + (row0 + (live ? own : 0)) * a.keep * a.dim + 8 * u;
+  const P* part = (const P*)c.part + partial_of(row0 + (live ? own : 0)) * a.dim + 8 * u;
   Vec<P, 8> x[AHEAD];
   const auto fetch = [&](int s0) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) x[i] = load_vec<8>(part + (int64_t)min(s0 + i * share, a.keep - 1) * a.dim);
+    for (int i = 0; i < AHEAD; ++i) x[i] = load_vec<8>(part + (int64_t)min(s0 + i * share, a.keep - 1) * a.group * a.dim);
   };
   fetch(part0);
   __syncthreads();

@@ -389,7 +389,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
       const int rows = (c.start[held + 1] - c.start[held]) * a.group;
       const int64_t start = item_start(a, s.b) + s.t0;
       const T* queries = (const T*)c.q + s.b * a.qs[0] + s.t0 * a.qs[1] + (int64_t)s.g * a.group * a.qs[2];
-      const uint32_t partials = (uint32_t)span * c.nt * a.group;
+      const uint32_t first = (uint32_t)span * c.nt;
       // a row of the tile: its list entry a tile ahead, its query a tile ahead of its products
       struct Row {
         int entry, h;
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
       for (; tile < to; ++tile) {
         Row after = locate(tile + 2);
         const int t = c.by_keep(row.entry), slot = row.entry - t * a.keep;
-        const uint32_t partial = (partials + t * a.group + row.h) * a.keep + slot;
+        const uint32_t partial = ((first + t) * a.keep + slot) * a.group + row.h;
         // The next tile's queries take the registers of this one's after its scores, and are waited for
         // before its stores: accesses end in order, and a wait behind the stores would be one for
         // them too.
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
       load_query<T, DP>(q, (const T*)c.q + s.b * a.qs[0] + (s.t0 + t) * a.qs[1] +
                                (int64_t)(s.g * a.group + h) * a.qs[2],
                         a.dim);
-      const uint32_t partial = (vt * a.group + h) * a.keep + slot;
+      const uint32_t partial = item * a.group + h;
       attend_rows<T, DP, BK>(c, lk, lv, bias, out_lds, part, metas, q, last, c2, block,
                              live ? partial : kNowhere, [] {}, [] {});
     }
