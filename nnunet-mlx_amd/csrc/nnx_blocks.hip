@@ -56,8 +56,13 @@ __device__ __forceinline__ float finite_or_zero(float v) { return fabsf(v) < INF
 
 // ---- summaries -------------------------------------------------------------------------
 
-// A workgroup a block of keys, L = dim / 8 threads a key, each 8 channels of every RP-th key.  The
-// keys are read once for the largest magnitude and stay in registers for the whole-number sums.
+// The mean key of a block as 8-bit codes under one scale: s = sum of the keys in 15 bits of the block's
+// largest magnitude, the codes s in 7 bits of its own largest.  Sums of whole numbers have no order, so
+// the codes, and the choices made by them, are the same however the keys are dealt to threads.
+// Bound by the launch and one read of the keys: 2560 blocks of 64 keys of 64 bfloat16 (21 MB) take
+// 11 us, 4 us of it the read at a large copy's rate.  A workgroup a block, dim / 8 threads a key: whole
+// rows of memory, and as many loads in flight as a thread has keys (BK / 16); the keys stay in
+// registers between the search for the largest magnitude and the sums.
 template <class T, int BK>
 __global__ __launch_bounds__(256) void summarize_kernel(BlockArgs a, const T* k, int first,
                                                         int8_t* codes, float* scales) {
@@ -130,13 +135,14 @@ __global__ __launch_bounds__(256) void summarize_kernel(BlockArgs a, const T* k,
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// The kept blocks of one row of scores, written by a wave: those of `forced` and the highest scores,
+// The kept blocks of one row of scores, written by a wave: the forced ones and the highest scores,
 // equal ones by the lower index.  A score that is no candidate is NaN, which no comparison takes.
 // A cut is searched by halving until exactly as many scores as are wanted lie above it: of the
 // values at first, which ends in some 9 steps for scores with gaps, then of their order as whole
-// numbers, which ends in 32 at a value whose equals are taken from the lowest index on.  (Steps
-// aimed by a line through the counts' logarithms took longer, 214 us against 185 for 163840 rows
-// of 512: the scores have more than one hump.)
+// numbers, which ends in 32 at a value whose equals are taken from the lowest index on.  A step is
+// a comparison, a count and an addition for each register, and bound by their issue.  (Steps aimed
+// by a line through the counts' logarithms were fewer and took longer, 214 us against 185 for 163840
+// rows of 512: the scores have more than one hump.)
 struct Cut {
   float above;  // kept: scores above it, and the first `ties` that equal it
   int ties;
@@ -301,6 +307,12 @@ __device__ __forceinline__ void select_row(float* score, float* spare, int chunk
 // products in whole numbers, kept in LDS; then a wave a query picks.  Heads that share the key
 // head are taken kScoreHeads at a time (their codes in LDS) and meet in the largest score.  A
 // wave's next AHEAD times 16 blocks are on their way while it scores the ones before.
+// Bound by the issue of instructions: 163840 rows against 512 blocks
+// of 64 channels take 150 us, 84 million scores of which 5.2 million are kept; the codes of a key head
+// (32 KB) come from the L2, and the scores never leave the CU.  8 queries a workgroup leave half of a
+// product unused (240 us against 190), 4 or 16 waves a workgroup fill the CU less evenly than 8 (209
+// and 269 against 190) unless there are too few workgroups for the CUs; four tiles of codes in flight
+// instead of two spill (40 against 33 us for 12 rows against 2048 blocks).
 constexpr int kScoreHeads = 8;
 // Rows of up to 2048 blocks (32 registers a lane) are scored and picked from by one workgroup, a tile
 // of 16 queries each, unless there are few tiles and each has much to score (blocks times heads, twice
@@ -517,6 +529,10 @@ SelectPlan plan_selection(const nnx_block_config& c) {
 // keep different ones.  So the pairs (query, kept block) are gathered by block: dense tiles of
 // rows against a block that stays in LDS, one partial softmax a pair, and a last pass that joins
 // each row's partials.  Few pairs skip the gathering: a workgroup each.
+//
+// The lists of 5.2 million pairs (163840 rows of 32 blocks) take 50 us: totals cleared 5, counted 17,
+// summed 5, placed 25.  The ids are read twice (42 MB) and 21 MB of entries written in runs of a few;
+// counting and placing are bound by their additions in LDS, two for a pair.
 
 // Calls body(entry, block) for the pairs of `per` queries of a span (grid: groups, spans).
 template <class F>
@@ -604,8 +620,10 @@ __global__ __launch_bounds__(256) void place_pairs_kernel(ChunkArgs c, int per, 
 }
 
 // out = sum_s w_s O_s / sum_s w_s with w_s = 2^(log2 sum_s - largest), O_s a partial under its
-// factor.  A workgroup forms the weights of its rows together, then dim / 8 lanes a row add up
-// (`share` groups of them a row, each every share-th partial, where rows are few or have many).
+// factor, in the order of the slots.  A workgroup forms the weights of its rows together, then dim / 8
+// lanes a row add up (`share` groups of them a row, each every share-th partial, where rows are few
+// or have many).  Bound by its reads: 143 MB of partials in 26 us (5.5 TB/s, mostly from the
+// last-level cache), 8 partials in flight a lane.
 constexpr int kJoinWeights = 4096;
 
 template <class T>
@@ -923,7 +941,8 @@ void block_attention(const nnx_block_config& c, const void* q, const void* k, co
       }
       const int64_t rows = (int64_t)m.spans * p.nt * a.group;
       const int lanes = a.dim / 8;
-      // groups of lanes a row: more while rows are too few for the CUs or their weights for the LDS
+      // groups of lanes a row: more while rows are too few for the CUs (65536 threads are one wave a
+      // SIMD) or a workgroup's weights too many for its LDS
       int share = 1;
       const auto each = [&] { return 256 / (lanes * share); };
       while (lanes * share * 2 <= 256 &&

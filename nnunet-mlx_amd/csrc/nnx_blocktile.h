@@ -142,6 +142,9 @@ struct RowWriter {
   }
 };
 
+// The partial softmax of rows over one block: m = max x, l = sum 2^(x - m), O = sum 2^(x - m) v / l, of
+// which log2 l + m and O are kept (x the scores in units of log 2; weights, sums and O in float32,
+// weights rounded to the type's bits only as operands of the second product).
 // 32 query rows, a lane pair (l, l + 32) each: S^T = K Q^T leaves a row's scores in its two
 // lanes' registers, so the softmax needs one exchange between halves, and its weights are
 // already the second operand of O^T = V^T P^T (the order of keys is that of the registers; values
@@ -351,8 +354,14 @@ __device__ __forceinline__ int last_seen(const BlockArgs& a, int64_t at, int fir
   return a.causal ? (int)min(max(at - first_key, (int64_t)-1), (int64_t)1 << 20) : 1 << 20;
 }
 
-// Registers for two waves a SIMD where that leaves nothing in memory (accumulators then stay
-// where vector instructions reach them).
+// Bound by the partials' stores: 1.05 million pairs with blocks of 64 keys of 64 bfloat16 channels, a
+// fifth of 32768 queries by 5 heads by 32 blocks, take 59 us: 17 GFLOP, and 134 MB of partials with 8 MB
+// of sums, which leave in pieces of 128 and 8 bytes at 2.4 TB/s.  The products would take 14 us at a
+// large product's rate, the queries' 134 MB are read from the L2.  Two tiles of queries in registers,
+// keys and values held in registers, sums by products of ones, and four waves a SIMD were all measured
+// and made nothing faster (297 to 365 us for the five launches against 300).  Registers for two waves a
+// SIMD where that leaves nothing in memory (accumulators then stay where vector instructions reach
+// them); larger tiles take one.
 template <class T, int DP, int BK>
 constexpr int kWaves = (sizeof(T) == 2 ? DP * BK < 128 * 128 : DP + BK <= 128) ? 2 : 1;
 
@@ -458,7 +467,8 @@ template <class T, int DP, int BK>
 void launch_partials(const ChunkArgs& c, bool by_block, int grid, hipStream_t st) {
   constexpr size_t bytes = Tile<T, DP, BK>::LDS;
   if (by_block) {
-    // as many workgroups as run at once: they share the tiles evenly
+    // as many workgroups as run at once: they share the tiles evenly, and a block's keys are staged
+    // once for a run of its tiles
     static const int per_cu = [] {
       int n = 0;
       hip_check(hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, block_partials_kernel<T, DP, BK, true>, 256, bytes),
