@@ -189,7 +189,7 @@ __device__ __forceinline__ int lanes_before(uint64_t lanes, int from) {
 }
 
 // The row lies in LDS, `chunks` times 64 filled up with NaN; N > 0: N = chunks, held in N registers a
-// lane; N = 0: read again for every step.  `spare`: 256 places, for N > 0 the row's own.
+// lane; N = 0: a multiple of 8 chunks, read again for every step.  `spare`: 256 places, for N > 0 the row's own.
 template <int N>
 __device__ __forceinline__ void select_row(float* score, float* spare, int chunks, int blocks, int keep,
                                            int first, int local, int own, int32_t* out) {
@@ -214,7 +214,13 @@ __device__ __forceinline__ void select_row(float* score, float* spare, int chunk
 #pragma unroll
       for (int i = 0; i < N; ++i) body(i, v[i]);
     } else {
-      for (int i = 0; i < chunks; ++i) body(i, score[i * 64 + lane]);
+      for (int i = 0; i < chunks; i += 8) {
+        float y[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = score[(i + k) * 64 + lane];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) body(i + k, y[k]);
+      }
     }
   };
   const auto above = [&](float x) {
@@ -312,13 +318,16 @@ __device__ __forceinline__ void select_row(float* score, float* spare, int chunk
 // (32 KB) come from the L2, and the scores never leave the CU.  8 queries a workgroup leave half of a
 // product unused (240 us against 190), 4 or 16 waves a workgroup fill the CU less evenly than 8 (209
 // and 269 against 190) unless there are too few workgroups for the CUs; four tiles of codes in flight
-// instead of two spill (40 against 33 us for 12 rows against 2048 blocks).
+// instead of two spill (40 against 33 us for 12 rows against 2048 blocks of 8 heads of 128).
 constexpr int kScoreHeads = 8;
 // Rows of up to 2048 blocks (32 registers a lane) are scored and picked from by one workgroup, a tile
-// of 16 queries each, unless there are few tiles and each has much to score (blocks times heads, twice
-// for more than 64 channels).  One kernel against parts, 4 tiles: 8192 15 us and 17, 16384 20 to 29 and
-// 17 to 21, 32768 32 and 23; 32768 at 32 tiles 32 and 32, at 128 34 and 57.
-constexpr int kWholeBlocks = 2048, kFewTiles = 16, kMuchWork = 16384;
+// of 16 queries each, unless the tiles are few for the chip.  One kernel against scores by parts and
+// picking, with 64 channels: 4 tiles of 256 blocks 6.9 us and 8.1, 16 of 512 8.4 and 8.1, 32 of 512 8.2
+// and 9.3, 32 of 1024 10.8 and 10.7, 4 of 2048 16.5 and 11.8, 64 of 2048 16.6 and 19.7; with 8 heads
+// of 128 channels 4 tiles of 256 10.9 and 12.2, 4 of 2048 30 and 17, 32 of 2048 31 and 24, 64 31 and 34.
+// Longer rows always go by parts (8192 blocks: 16 queries of 32 key heads 324 us in one kernel that
+// read its scores again for every step, 8 tiles 32 us by parts).
+constexpr int kWholeBlocks = 2048, kPartBlocks = 512, kPartTiles = 32;
 constexpr int64_t kScoreBudget = (int64_t)128 << 20;
 
 struct Parts {
@@ -471,24 +480,25 @@ __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, c
   }
 }
 
-// A wave a row of scores in global memory.
-template <int N>
-__global__ __launch_bounds__(64) void pick_kernel(BlockArgs a, int from, Parts parts, int32_t* ids) {
-  extern __shared__ __attribute__((aligned(16))) float score[];  // chunks times 64; N = 0: 256 more
-  const int t = from + blockIdx.x, g = blockIdx.y, b = blockIdx.z, chunks = N ? N : (a.blocks + 63) / 64;
+// Picks from a row of scores in global memory: a workgroup brings it to LDS, a wave searches.  (Rows of
+// up to 8192 blocks held in registers took as long.)
+__global__ __launch_bounds__(256) void pick_kernel(BlockArgs a, int from, Parts parts, int32_t* ids) {
+  extern __shared__ __attribute__((aligned(16))) float score[];  // 64 a chunk and 256 more
+  const int t = from + blockIdx.x, g = blockIdx.y, b = blockIdx.z, chunks = (a.blocks + 511) / 512 * 8;
   const float* row = parts.scores + (((int64_t)b * a.kv_heads + g) * parts.rows + blockIdx.x) * parts.pitch;
-#pragma unroll N ? N : 8
-  for (int i = 0; i < chunks; ++i) {
-    const int j = i * 64 + threadIdx.x;
-    score[j] = j < parts.pitch ? row[j] : NAN;
+#pragma unroll 4
+  for (int j = threadIdx.x * 4; j < chunks * 64; j += 1024) {
+    const float4 v = *(const float4*)&row[min(j, parts.pitch - 4)];
+    *(float4*)&score[j] = j < parts.pitch ? v : make_float4(NAN, NAN, NAN, NAN);
   }
   __syncthreads();
-  select_row<N>(score, N ? score : score + chunks * 64, chunks, a.blocks, a.keep, a.first, a.local,
-                own_block(a, b, t), ids + (((int64_t)b * a.queries + t) * a.kv_heads + g) * a.keep);
+  if (threadIdx.x >= 64) return;
+  select_row<0>(score, score + chunks * 64, chunks, a.blocks, a.keep, a.first, a.local, own_block(a, b, t),
+                ids + (((int64_t)b * a.queries + t) * a.kv_heads + g) * a.keep);
 }
 
-// Rows of many blocks, or few rows of much work: the scores by parts of a row, a workgroup each, to
-// global memory, then a wave a row picks.
+// Rows of many blocks, or few rows: the scores by parts of a row, a workgroup each, to global memory,
+// then a wave a row picks.
 struct SelectPlan {
   bool split;
   int chunks, rows, pitch;  // of the kernel that forms scores: 64 blocks each, queries of a workgroup, LDS row
@@ -504,8 +514,7 @@ SelectPlan plan_selection(const nnx_block_config& c) {
   p.chunks = 1;
   while (p.chunks * 64 < blocks) p.chunks *= 2;
   p.rows = std::min(16, c.queries);
-  p.split = blocks > kWholeBlocks ||
-            (tiles <= kFewTiles && (int64_t)blocks * group * (c.head_dim > 64 ? 2 : 1) >= kMuchWork);
+  p.split = blocks > kWholeBlocks || (blocks >= kPartBlocks && tiles <= std::min(kPartTiles, blocks / 32));
   if (!p.split) {
     const size_t codes = (size_t)std::min(group, kScoreHeads) * 2048;
     p.pitch = p.chunks * 64 + 4;
@@ -831,16 +840,8 @@ void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
                                                            from, parts);
       });
       launch_check("block_select");
-      auto go = [&](auto k) {
-        constexpr int N = decltype(k)::value;
-        const size_t places = N ? N * 64 : ceil_div(a.blocks, 64) * 64 + 256;
-        pick_kernel<N><<<dim3(queries, c.kv_heads, c.batch), 64, places * sizeof(float), st>>>(a, from, parts, ids);
-      };
-      if (plan.chunks <= 16) go(integral_constant<int, 16>{});
-      else if (plan.chunks == 32) go(integral_constant<int, 32>{});
-      else if (plan.chunks == 64) go(integral_constant<int, 64>{});
-      else if (plan.chunks == 128) go(integral_constant<int, 128>{});
-      else go(integral_constant<int, 0>{});
+      pick_kernel<<<dim3(queries, c.kv_heads, c.batch), 256, (ceil_div(a.blocks, 512) * 512 + 256) * sizeof(float), st>>>(
+          a, from, parts, ids);
       launch_check("block_select");
     }
     return;
