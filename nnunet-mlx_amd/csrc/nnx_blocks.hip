@@ -325,8 +325,8 @@ constexpr int kScoreHeads = 8;
 // picking, with 64 channels: 4 tiles of 256 blocks 6.9 us and 8.1, 16 of 512 8.4 and 8.1, 32 of 512 8.2
 // and 9.3, 32 of 1024 10.8 and 10.7, 4 of 2048 16.5 and 11.8, 64 of 2048 16.6 and 19.7; with 8 heads
 // of 128 channels 4 tiles of 256 10.9 and 12.2, 4 of 2048 30 and 17, 32 of 2048 31 and 24, 64 31 and 34.
-// Longer rows always go by parts (8192 blocks: 16 queries of 32 key heads 324 us in one kernel that
-// read its scores again for every step, 8 tiles 32 us by parts).
+// Longer rows always go by parts (8192 blocks: 6 tiles 167 us in one kernel, which has to read its
+// scores again for every step, 8 tiles 32 us by parts).
 constexpr int kWholeBlocks = 2048, kPartBlocks = 512, kPartTiles = 32;
 constexpr int64_t kScoreBudget = (int64_t)128 << 20;
 
