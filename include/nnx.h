@@ -613,7 +613,8 @@ int nnx_block_summarize(const nnx_block_config* config, const void* d_k, const i
  * heads sharing the key head of (float(codes . codes) * m) * scale, at most the largest finite
  * value in magnitude.  Kept are the `first` leading blocks and the `local` ones ending at the
  * query's own, then the highest scores, equal ones by the lower index; blocks without valid keys
- * (scale < 0) never, nor blocks behind a causal query's own.  A workspace of 0 bytes may be null;
+ * (scale < 0) never, nor blocks behind a causal query's own.  d_codes must be 8-byte aligned, a
+ * workspace 16-byte; a workspace of 0 bytes may be null;
  * the workspace query answers 0 for what the entry refuses, too. */
 size_t nnx_block_select_workspace(const nnx_block_config* config);
 int nnx_block_select(const nnx_block_config* config, const void* d_q, const int8_t* d_codes,

@@ -313,9 +313,10 @@ __device__ __forceinline__ void select_row(float* score, float* spare, int chunk
 // products in whole numbers, kept in LDS; then a wave a query picks.  Heads that share the key
 // head are taken kScoreHeads at a time (their codes in LDS) and meet in the largest score.  A
 // wave's next AHEAD times 16 blocks are on their way while it scores the ones before.
-// Bound by the issue of instructions: 163840 rows against 512 blocks
-// of 64 channels take 150 us, 84 million scores of which 5.2 million are kept; the codes of a key head
-// (32 KB) come from the L2, and the scores never leave the CU.  8 queries a workgroup leave half of a
+// Bound by the issue of instructions: 163840 rows against 512 blocks of 64 channels take 150 us, the
+// vector and the scalar units busy for 71 and 73 % of it (380 and 385 instructions a row), for 84
+// million scores of which 5.2 million are kept; the codes of a key head (32 KB) come from the L2, and
+// the scores never leave the CU.  8 queries a workgroup leave half of a
 // product unused (240 us against 190), 4 or 16 waves a workgroup fill the CU less evenly than 8 (209
 // and 269 against 190) unless there are too few workgroups for the CUs; four tiles of codes in flight
 // instead of two spill (40 against 33 us for 12 rows against 2048 blocks of 8 heads of 128).
@@ -541,7 +542,8 @@ SelectPlan plan_selection(const nnx_block_config& c) {
 //
 // The lists of 5.2 million pairs (163840 rows of 32 blocks) take 50 us: totals cleared 5, counted 17,
 // summed 5, placed 25.  The ids are read twice (42 MB) and 21 MB of entries written in runs of a few;
-// counting and placing are bound by their additions in LDS, two for a pair.
+// counting and placing wait for most of their time, for the ids and the additions in LDS and memory.
+// (Sums formed by every placing workgroup, for one launch less, took as long: 58 us against 54.)
 
 // Calls body(entry, block) for the pairs of `per` queries of a span (grid: groups, spans).
 template <class F>
@@ -819,6 +821,8 @@ void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
                   hipStream_t st) {
   check_config(c, "block selection", true);
   require(q && codes && scales && ids, "block selection: null pointer");
+  require(reinterpret_cast<uintptr_t>(codes) % 8 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0,
+          "block selection: codes must be 8-byte and scales 4-byte aligned");
   const SelectPlan plan = plan_selection(c);
   require(!plan.split || (ws && ws_bytes >= plan.bytes && reinterpret_cast<uintptr_t>(ws) % 16 == 0),
           "block selection: the workspace is too small or not 16-byte aligned");

@@ -78,6 +78,25 @@ def test_summaries():
     _refused(lib.nnx_block_summarize(_block(), None, None, None, 0, 7, None, None, None), "null pointer")
 
 
+def test_selection_places():
+    """Codes and workspaces that do not fit are refused before anything runs on a device."""
+    lib = _native.load()
+    few, many = _block(), _block(keys=32 * 3000)
+    assert lib.nnx_block_select_workspace(few) == 0
+    size = lib.nnx_block_select_workspace(many)
+    assert size > 0
+    assert lib.nnx_block_select_workspace(_block(keys=32 * 3000, keep=0)) == 0
+    assert lib.nnx_block_select_workspace(ctypes.POINTER(_native.NnxBlockConfig)()) == 0
+    place = 1 << 20
+    for codes, scales in ((place + 4, place), (place, place + 2)):
+        _refused(lib.nnx_block_select(few, place, codes, scales, None, place, None, 0, None), "aligned")
+    for work, given in ((None, size), (place, size - 1), (place + 8, size)):
+        _refused(lib.nnx_block_select(many, place, place, place, None, place, work, given, None), "workspace")
+    size = lib.nnx_block_attention_workspace(many)
+    for work, given in ((place, size - 1), (place + 8, size)):
+        _refused(lib.nnx_block_attention(many, *[place] * 4, None, None, None, place, work, given, None), "workspace")
+
+
 def test_null_configs():
     lib = _native.load()
     none = ctypes.POINTER(_native.NnxBlockConfig)()
