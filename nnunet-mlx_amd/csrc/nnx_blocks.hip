@@ -545,23 +545,25 @@ SelectPlan plan_selection(const nnx_block_config& c) {
 // counting and placing wait for most of their time, for the ids and the additions in LDS and memory.
 // (Sums formed by every placing workgroup, for one launch less, took as long: 58 us against 54.)
 
-// Calls body(entry, block) for the pairs of `per` queries of a span (grid: groups, spans).
+// Calls body(entry, block) for the pairs of `per` queries of a span (grid: groups, spans), 16 ids a thread on
+// their way at a time (4: 56 us against 52 for the lists above).
 template <class F>
 __device__ __forceinline__ void each_pair(const ChunkArgs& c, int per, F&& body) {
+  constexpr int AHEAD = 16;
   const BlockArgs& a = c.a;
   const Span s = span_of(c, c.span0 + blockIdx.y);
   const int t_lo = blockIdx.x * per, t_hi = min(t_lo + per, s.queries);
   const int32_t* ids = c.ids + (((int64_t)s.b * a.queries + s.t0) * a.kv_heads + s.g) * a.keep;
   const int end = t_hi * a.keep;
-  for (int e0 = t_lo * a.keep + threadIdx.x; e0 < end; e0 += 4 * 256) {
-    int j[4];
+  for (int e0 = t_lo * a.keep + threadIdx.x; e0 < end; e0 += AHEAD * 256) {
+    int j[AHEAD];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < AHEAD; ++i) {
       const int e = min(e0 + i * 256, end - 1), t = c.by_keep(e);
       j[i] = ids[(int64_t)t * a.kv_heads * a.keep + e - t * a.keep];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < AHEAD; ++i)
       if (e0 + i * 256 < end && (unsigned)j[i] < (unsigned)a.blocks) body(e0 + i * 256, j[i]);
   }
 }
