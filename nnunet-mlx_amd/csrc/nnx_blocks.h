@@ -66,7 +66,8 @@ __device__ __forceinline__ Span span_of(const ChunkArgs& c, int v) {
 
 constexpr int kTileRows = 128;
 
-// Buffer accesses take 32-bit offsets, and past the buffer's end load 0 and store nothing.
+// Buffer accesses take 32-bit offsets, and past the buffer's end load 0 and store nothing; the check is of
+// the lane's offset, so all of it goes there and the scalar offset is 0.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, size_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)(uint32_t)bytes, 0x00027000);
 }

@@ -369,17 +369,18 @@ __global__ __launch_bounds__(1024) void select_kernel(BlockArgs a, const T* q, c
     int scale[4];
   };
   // Past the last block all is 0 and not kept; past the head's end lie the next block's codes, and the
-  // queries' codes are 0.
+  // queries' codes are 0.  The whole offset is the lane's: the scalar one is left out of the bounds check.
   const uint32_t code_at = (uint32_t)(col * a.dim + quad * 16), scale_at = (uint32_t)(quad * 16);
   const auto load = [&](Blocks& x, int j0) {
+    const uint32_t ca = code_at + (uint32_t)(j0 * a.dim), sa = scale_at + (uint32_t)(j0 * 4);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       if (s > 1 && !wide) break;
-      x.k[s] = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(
-                                             cu, code_at + s / 2 * 64 + s % 2 * 8, j0 * a.dim, 0));
+      x.k[s] = __builtin_bit_cast(
+          i32x2, __builtin_amdgcn_raw_buffer_load_b64(cu, ca + s / 2 * 64 + s % 2 * 8, 0, 0));
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x.scale[r] = (int)__builtin_amdgcn_raw_buffer_load_b32(su, scale_at + 4 * r, j0 * 4, 0);
+    for (int r = 0; r < 4; ++r) x.scale[r] = (int)__builtin_amdgcn_raw_buffer_load_b32(su, sa + 4 * r, 0, 0);
   };
   if (N > 0) {
     const int full = (a.blocks + 15) / 16 * 16, rest = N * 64 - full;
