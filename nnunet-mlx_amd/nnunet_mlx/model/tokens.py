@@ -234,11 +234,17 @@ Affine = tuple[torch.Tensor | None, torch.Tensor | None]
 
 
 def _rows(name: str, tensor: torch.Tensor) -> int:
-    """Stride of the rows of a (..., channels) tensor whose leading axes step evenly."""
-    step = tensor.stride(-2) if tensor.dim() > 1 else tensor.shape[-1]
-    for axis in range(tensor.dim() - 2, 0, -1):
-        if tensor.shape[axis - 1] > 1 and tensor.stride(axis - 1) != tensor.stride(axis) * tensor.shape[axis]:
+    """Stride of the rows of a (..., channels) tensor whose leading axes step evenly; an axis of one
+    element takes no step, whatever its stride."""
+    step, following = tensor.shape[-1], None  # of a single row, any
+    for size, stride in zip(reversed(tensor.shape[:-1]), reversed(tensor.stride()[:-1])):
+        if size == 1:
+            continue
+        if following is None:
+            step = stride
+        elif stride != following:
             raise ContractError(f"{name}: the axes before the last must step evenly")
+        following = stride * size
     return step
 
 

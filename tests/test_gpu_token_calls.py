@@ -1,0 +1,28 @@
+"""How the token operators take their arguments: views, numbers and positions, on the device."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from nnunet_mlx.model import tokens
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+@pytest.mark.parametrize("cut", [
+    lambda x: x[:, :1, 2:3], lambda x: x[:1, 3:4], lambda x: x[1:2, 2:3, ::2], lambda x: x[:, :, 4], lambda x: x[:1, :1],
+    lambda x: x[:, -1:, -1:, 5:]])
+def test_residual_norm_of_views_with_single_elements(device, cut):
+    """Axes of one element at any place: the rows are the view's own, for x, residual and gate."""
+    x, residual, gate = (cut(torch.randn(3, 5, 8, 24, generator=_gen(seed)).cuda()) for seed in range(3))
+    got = tokens.residual_norm(x, residual, gate=gate, post=(None, None), pre=(None, None))
+    want = tokens.residual_norm(x.contiguous(), residual.contiguous(), gate=gate.contiguous(), post=(None, None),
+                                pre=(None, None))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert torch.equal(tokens.residual_norm(x, residual)[0], residual + x)
