@@ -12,6 +12,7 @@ other strides.  No reference counterpart.
 from __future__ import annotations
 
 import math
+import operator
 import struct
 from typing import NamedTuple
 
@@ -47,6 +48,18 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 def _need(ok: bool, message: str) -> None:
     if not ok:
         raise ContractError(message)
+
+
+def _whole(name: str, value) -> int:
+    """The int of any whole number.  A tensor is none: its value would have to be waited for."""
+    if type(value) is int:
+        return value
+    if not isinstance(value, torch.Tensor):
+        try:
+            return operator.index(value)
+        except TypeError:
+            pass
+    raise ContractError(f"{name} must be a whole number, got {type(value).__name__}")
 
 
 def _check(name: str, tensor: torch.Tensor, dims: int, like: torch.Tensor | None = None) -> None:
@@ -324,21 +337,35 @@ _NO_STRIDES = (0, 0, 0)
 
 def _block_config(like: torch.Tensor, block: int, batch: int, queries: int, keys: int, heads: int,
                   kv_heads: int, *, keep: int = 1, first: int = 0, local: int = 0, causal: bool = False,
-                  start: int = 0, scale: float = 1.0, q=_NO_STRIDES, k=_NO_STRIDES, v=_NO_STRIDES,
+                  scale: float = 1.0, q=_NO_STRIDES, k=_NO_STRIDES, v=_NO_STRIDES,
                   out=_NO_STRIDES, mask_stride: int = 0) -> _native.NnxBlockConfig:
     if block not in BLOCK_SIZES:
         raise ContractError(f"block must be one of {BLOCK_SIZES}, got {block}")
     try:
         return _native.packed(_native.NnxBlockConfig, _BLOCK, _TYPES[like.dtype], batch, queries, keys, heads,
-                              kv_heads, like.shape[-1], block, keep, first, local, bool(causal), start, scale,
+                              kv_heads, like.shape[-1], block, keep, first, local, bool(causal), 0, scale,
                               *q, *k, *v, *out, mask_stride)
     except struct.error as error:
         raise ContractError(f"a block argument is no 32-bit whole number: {error}") from error
 
 
-def _check_start(start: torch.Tensor | int | None, batch: int, device: torch.device) -> None:
-    if isinstance(start, torch.Tensor):
-        _check_side("start", start, torch.int32, (batch,), device)
+def _split_start(start: torch.Tensor | int | None) -> tuple[torch.Tensor | None, int]:
+    """The items' positions, and one for them all."""
+    if start is None or isinstance(start, torch.Tensor):
+        return start, 0
+    at = _whole("start", start)
+    _need(0 <= at < 1 << 40, f"start must be 0..2^40, got {at}")
+    return None, at
+
+
+def _placed(config: _native.NnxBlockConfig, start: int) -> _native.NnxBlockConfig:
+    """The checked configuration for queries from ``start`` on.  A decoder moves it at every step, so it is
+    no part of what is remembered."""
+    if not start:
+        return config
+    config = _native.NnxBlockConfig.from_buffer_copy(config)
+    config.start = start
+    return config
 
 
 def _check_lengths_mask(lengths: torch.Tensor | None, mask: torch.Tensor | None, batch: int, keys: int,
@@ -407,24 +434,23 @@ def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int,
     product of the summary with the query heads that share the key head; equal scores go to the
     lower index.  The scores are formed in whole numbers, so they do not depend on how the work is
     split.  ``causal`` leaves out the blocks behind the query's own."""
-    placed = isinstance(start, torch.Tensor)
-    key = ("select", _signature(q, *summary, start if placed else None), block, keep, causal,
-           None if placed else start, first, local)
+    starts, at = _split_start(start)
+    key = ("select", _signature(q, *summary, starts), block, keep, causal, first, local)
     known = _checked.get(key)
     if known is None:
-        known = _remember(key, _selection_config(q, summary, block, keep, causal, start, first, local))
+        known = _remember(key, _selection_config(q, summary, block, keep, causal, starts, first, local))
     config, size = known
     ids = torch.empty((q.shape[0], q.shape[1], summary.codes.shape[1], keep), dtype=torch.int32, device=q.device)
     if config:
         work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        _launch(q.device, "nnx_block_select", config, q.data_ptr(), summary.codes.data_ptr(),
-                summary.scales.data_ptr(), start.data_ptr() if placed else None, ids.data_ptr(), _address(work), size)
+        _launch(q.device, "nnx_block_select", _placed(config, at), q.data_ptr(), summary.codes.data_ptr(),
+                summary.scales.data_ptr(), _address(starts), ids.data_ptr(), _address(work), size)
     elif ids.numel():
         ids.fill_(-1)
     return ids
 
 
-def _selection_config(q, summary, block, keep, causal, start, first, local):
+def _selection_config(q, summary, block, keep, causal, starts, first, local):
     """The checked configuration of a selection (False where there is nothing to select from) and its workspace's
     bytes."""
     _check("q", q, 4)
@@ -433,11 +459,11 @@ def _selection_config(q, summary, block, keep, causal, start, first, local):
     kv_heads, blocks = summary.codes.shape[1:3]
     _check_side("summary.codes", summary.codes, torch.int8, (batch, kv_heads, blocks, dim), q.device)
     _check_side("summary.scales", summary.scales, torch.float32, (batch, kv_heads, blocks), q.device)
-    _check_start(start, batch, q.device)
+    if starts is not None:
+        _check_side("start", starts, torch.int32, (batch,), q.device)
     _need(keep >= 1, f"keep must be positive, got {keep}")
     config = _block_config(q, block, batch, queries, blocks * block, heads, kv_heads, keep=keep, first=first,
-                           local=local, causal=causal, start=start if isinstance(start, int) else 0,
-                           q=q.stride()[:3])
+                           local=local, causal=causal, q=q.stride()[:3])
     if q.numel() == 0 or blocks == 0:
         return False, 0
     return config, _native.load().nnx_block_select_workspace(config)
@@ -452,26 +478,25 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torc
 
     ``scale`` defaults to head_dim^-0.5; ``causal``, ``start``, ``lengths`` and ``key_mask`` as in
     ``select_blocks`` and ``summarize_blocks``.  A query that sees no key gets zeros."""
-    placed = isinstance(start, torch.Tensor)
-    key = ("attention", _signature(q, k, v, ids, start if placed else None, lengths, key_mask, out), block, scale,
-           causal, None if placed else start)
+    starts, at = _split_start(start)
+    key = ("attention", _signature(q, k, v, ids, starts, lengths, key_mask, out), block, scale, causal)
     known = _checked.get(key)
     if known is None:
-        known = _remember(key, _attention_config(q, k, v, ids, block, scale, causal, start, lengths, key_mask, out))
+        known = _remember(key, _attention_config(q, k, v, ids, block, scale, causal, starts, lengths, key_mask, out))
     config, size = known
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if config:
         work = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _launch(q.device, "nnx_block_attention", config, q.data_ptr(), k.data_ptr(), v.data_ptr(), ids.data_ptr(),
-                start.data_ptr() if placed else None, _address(lengths), _address(key_mask), out.data_ptr(),
+        _launch(q.device, "nnx_block_attention", _placed(config, at), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                ids.data_ptr(), _address(starts), _address(lengths), _address(key_mask), out.data_ptr(),
                 work.data_ptr(), size)
     elif out.numel():
         out.zero_()
     return out
 
 
-def _attention_config(q, k, v, ids, block, scale, causal, start, lengths, key_mask, out):
+def _attention_config(q, k, v, ids, block, scale, causal, starts, lengths, key_mask, out):
     """The checked configuration (False where there is nothing to attend to) and workspace bytes."""
     _check("q", q, 4)
     _check("k", k, 4, q)
@@ -483,14 +508,15 @@ def _attention_config(q, k, v, ids, block, scale, causal, start, lengths, key_ma
     _need(ids.dim() == 4, f"ids need 4 axes, got shape {tuple(ids.shape)}")
     keep = ids.shape[3]
     _check_side("ids", ids, torch.int32, (batch, queries, kv_heads, keep), q.device)
-    _check_start(start, batch, q.device)
+    if starts is not None:
+        _check_side("start", starts, torch.int32, (batch,), q.device)
     mask_stride = _check_lengths_mask(lengths, key_mask, batch, keys, q.device)
     if out is not None:
         _check("out", out, 4, q)
         _need(out.shape == q.shape, f"out {tuple(out.shape)} does not match q {tuple(q.shape)}")
     config = _block_config(
         q, block, batch, queries, keys, heads, kv_heads, keep=keep, causal=causal,
-        start=start if isinstance(start, int) else 0, scale=dim**-0.5 if scale is None else scale,
+        scale=dim**-0.5 if scale is None else scale,
         q=q.stride()[:3], k=k.stride()[:3], v=v.stride()[:3],
         out=_contiguous_strides(q.shape) if out is None else out.stride()[:3], mask_stride=mask_stride)
     if q.numel() == 0 or keys == 0:

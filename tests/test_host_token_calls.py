@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import itertools
 
+import numpy as np
 import pytest
 import torch
 
@@ -51,3 +52,43 @@ def test_rows_that_do_not():
                  base[0].expand(4, 6, 10, 8), base[:, :, :, :4].transpose(0, 2)):
         with pytest.raises(ContractError, match="evenly"):
             tokens._rows("x", view)
+
+
+# ---- numbers and positions ------------------------------------------------------------
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """What the library would be told, on a host without a device."""
+    told = []
+    monkeypatch.setattr(tokens, "_check", lambda *args: None)
+    monkeypatch.setattr(tokens, "_launch", lambda device, entry, config, *rest: told.append((entry, config, rest)))
+    monkeypatch.setattr(tokens, "_checked", {})
+    return told
+
+
+def _selection():
+    return torch.zeros(1, 4, 2, 16), tokens.BlockSummary(torch.zeros(1, 2, 8, 16, dtype=torch.int8), torch.zeros(1, 2, 8))
+
+
+@pytest.mark.parametrize("order", list(itertools.permutations((40, np.int64(40), None, 7))))
+def test_start_whatever_was_called_before(launches, order):
+    q, summary = _selection()
+    k, ids = torch.zeros(1, 128, 2, 16), torch.zeros(1, 4, 2, 1, dtype=torch.int32)
+    for start in order:
+        tokens.select_blocks(q, summary, 16, 1, start=start)
+        tokens.block_attention(q, k, k, ids, 16, start=start)
+        for _, config, _ in launches[-2:]:
+            assert config.start == (0 if start is None else int(start))
+    assert len(tokens._checked) == 2  # a position that moves is checked once
+
+
+@pytest.mark.parametrize("start", [40.0, "x", np.float64(3), 1 << 40, -1, -(1 << 63), 1 << 64])
+def test_start_that_is_no_position(launches, start):
+    q, summary = _selection()
+    for known in (False, True):
+        with pytest.raises(ContractError, match="start"):
+            tokens.select_blocks(q, summary, 16, 1, start=start)
+        if not known:
+            tokens.select_blocks(q, summary, 16, 1, start=40)
+    assert [config.start for _, config, _ in launches] == [40]
