@@ -12,6 +12,7 @@ other strides.  No reference counterpart.
 from __future__ import annotations
 
 import math
+import numbers
 import operator
 import struct
 from typing import NamedTuple
@@ -60,6 +61,32 @@ def _whole(name: str, value) -> int:
         except TypeError:
             pass
     raise ContractError(f"{name} must be a whole number, got {type(value).__name__}")
+
+
+def _number(name: str, value) -> float:
+    """The float of any real number in float32's range; of a tensor not, as above."""
+    if type(value) is not float:
+        if not isinstance(value, numbers.Real):
+            raise ContractError(f"{name} must be a number, got {type(value).__name__}")
+        value = float(value)
+    if abs(value) <= 3.4028235e38:
+        return value
+    raise ContractError(f"{name} must be a finite float32, got {value}")
+
+
+def _flag(name: str, value) -> bool:
+    if type(value) is bool:
+        return value
+    if isinstance(value, torch.Tensor):
+        raise ContractError(f"{name} must be true or false, got a tensor")
+    return bool(value)
+
+
+def _packed(structure, layout: struct.Struct, *values):
+    try:
+        return _native.packed(structure, layout, *values)
+    except struct.error as error:
+        raise ContractError(f"an argument does not fit its 32 or 64 bits: {error}") from error
 
 
 def _check(name: str, tensor: torch.Tensor, dims: int, like: torch.Tensor | None = None) -> None:
@@ -184,11 +211,11 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
     with i + rotary_dim / 2 ("half") or 2i with 2i + 1 ("interleaved"); elements past the plan's
     pairs are copied.  ``inverse`` turns back, which is also the gradient of the forward turn.
     ``out`` may hold the results, ``(q, k)`` itself to rotate in place."""
-    key = ("rotate", _signature(q, k, positions, plan.steps, plan.axes, *(out or (None,))), plan.amplitude,
-           layout, inverse)
+    amplitude, inverse = _number("plan.amplitude", plan.amplitude), _flag("inverse", inverse)
+    key = ("rotate", _signature(q, k, positions, plan.steps, plan.axes, *(out or (None,))), amplitude, layout, inverse)
     config = _checked.get(key)
     if config is None:
-        config = _remember(key, _rotary_config(q, k, positions, plan, layout, inverse, out))
+        config = _remember(key, _rotary_config(q, k, positions, plan, amplitude, layout, inverse, out))
     if out is None:
         yq = torch.empty_like(q, memory_format=torch.contiguous_format)
         yk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
@@ -204,7 +231,7 @@ def _contiguous_strides(shape: torch.Size) -> tuple[int, int, int]:
     return (shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3])
 
 
-def _rotary_config(q, k, positions, plan, layout, inverse, out):
+def _rotary_config(q, k, positions, plan, amplitude, layout, inverse, out):
     """The checked configuration of a rotation, False where there is nothing to do."""
     _check("q", q, 4)
     batch, tokens, heads, dim = q.shape
@@ -234,9 +261,9 @@ def _rotary_config(q, k, positions, plan, layout, inverse, out):
         strides = [none if y is None else y.stride()[:3] for y in out]
     if q.numel() == 0 and (k is None or k.numel() == 0):
         return False
-    return _native.packed(
+    return _packed(
         _native.NnxRotaryConfig, _ROTARY, _TYPES[q.dtype], batch, tokens, heads, 0 if k is None else k.shape[2],
-        dim, rotary_dim, axes, _LAYOUTS[layout], int(inverse), plan.amplitude,
+        dim, rotary_dim, axes, _LAYOUTS[layout], int(inverse), amplitude,
         *q.stride()[:3], *(none if k is None else k.stride()[:3]), *strides[0], *strides[1],
         *((0, positions.stride(0)) if positions.dim() == 2 else positions.stride()[:2]))
 
@@ -277,6 +304,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, *, kind: str =
     ``gate`` is like x; ``scale`` float32 (channels,).  ``post`` and ``pre`` are (weight, bias),
     float32 (channels,) or None each.  ``kind`` is "layer" or "rms"; y is the norm of r' before
     it is rounded to its dtype."""
+    residual_scale, eps = _number("residual_scale", residual_scale), _number("eps", eps)
     vectors = (scale, *(post or (None, None)), *(pre or (None, None)))
     key = ("norm", _signature(x, residual, gate, *vectors), kind, post is None, pre is None, gate_activation,
            residual_scale, eps)
@@ -314,7 +342,7 @@ def _norm_config(x, residual, gate, vectors, kind, post, gate_activation, residu
     if rows == 0:
         return False
     wide = _TYPES[x.dtype if residual is None else residual.dtype]
-    return _native.packed(
+    return _packed(
         _native.NnxResidualNormConfig, _NORM, _TYPES[x.dtype], wide, rows, channels, _KINDS[kind], int(post),
         _GATES[gate_activation], residual_scale, eps, _rows("x", x),
         0 if residual is None else _rows("residual", residual), 0 if gate is None else _rows("gate", gate),
@@ -341,12 +369,8 @@ def _block_config(like: torch.Tensor, block: int, batch: int, queries: int, keys
                   out=_NO_STRIDES, mask_stride: int = 0) -> _native.NnxBlockConfig:
     if block not in BLOCK_SIZES:
         raise ContractError(f"block must be one of {BLOCK_SIZES}, got {block}")
-    try:
-        return _native.packed(_native.NnxBlockConfig, _BLOCK, _TYPES[like.dtype], batch, queries, keys, heads,
-                              kv_heads, like.shape[-1], block, keep, first, local, bool(causal), 0, scale,
-                              *q, *k, *v, *out, mask_stride)
-    except struct.error as error:
-        raise ContractError(f"a block argument is no 32-bit whole number: {error}") from error
+    return _packed(_native.NnxBlockConfig, _BLOCK, _TYPES[like.dtype], batch, queries, keys, heads, kv_heads,
+                   like.shape[-1], block, keep, first, local, causal, 0, scale, *q, *k, *v, *out, mask_stride)
 
 
 def _split_start(start: torch.Tensor | int | None) -> tuple[torch.Tensor | None, int]:
@@ -391,6 +415,8 @@ def summarize_blocks(k: torch.Tensor, block: int, *, lengths: torch.Tensor | Non
     ones that are seen.  ``first`` and ``count`` with ``out`` refresh those blocks of a summary
     that is kept, as after appending keys."""
     codes, scales = out or (None, None)
+    block, first = _whole("block", block), _whole("first", first)
+    count = None if count is None else _whole("count", count)
     key = ("summarize", _signature(k, lengths, key_mask, codes, scales), block, first, count)
     known = _checked.get(key)
     if known is None:
@@ -421,6 +447,8 @@ def _summary_config(k, block, lengths, key_mask, first, count, out):
     else:
         _check_side("out.codes", out.codes, torch.int8, (batch, kv_heads, blocks, dim), k.device)
         _check_side("out.scales", out.scales, torch.float32, (batch, kv_heads, blocks), k.device)
+        _need(first >= 0 and count >= 0 and first + count <= blocks,
+              f"blocks {first} to {first + count} are not blocks of the keys, which have {blocks}")
     return config if k.numel() else False, blocks, count
 
 
@@ -435,6 +463,8 @@ def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int,
     lower index.  The scores are formed in whole numbers, so they do not depend on how the work is
     split.  ``causal`` leaves out the blocks behind the query's own."""
     starts, at = _split_start(start)
+    block, keep, causal = _whole("block", block), _whole("keep", keep), _flag("causal", causal)
+    first, local = _whole("first", first), _whole("local", local)
     key = ("select", _signature(q, *summary, starts), block, keep, causal, first, local)
     known = _checked.get(key)
     if known is None:
@@ -479,6 +509,8 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torc
     ``scale`` defaults to head_dim^-0.5; ``causal``, ``start``, ``lengths`` and ``key_mask`` as in
     ``select_blocks`` and ``summarize_blocks``.  A query that sees no key gets zeros."""
     starts, at = _split_start(start)
+    block, causal = _whole("block", block), _flag("causal", causal)
+    scale = None if scale is None else _number("scale", scale)
     key = ("attention", _signature(q, k, v, ids, starts, lengths, key_mask, out), block, scale, causal)
     known = _checked.get(key)
     if known is None:

@@ -92,3 +92,56 @@ def test_start_that_is_no_position(launches, start):
         if not known:
             tokens.select_blocks(q, summary, 16, 1, start=40)
     assert [config.start for _, config, _ in launches] == [40]
+
+
+def _norm(**kw):
+    x = torch.zeros(3, 8)
+    return tokens.residual_norm(x, x, **kw)
+
+
+def _rotate(**kw):
+    plan = tokens.rotary_plan(16, device="cpu")._replace(amplitude=kw.pop("amplitude", 1.0))
+    return tokens.rotate(torch.zeros(1, 4, 2, 16), None, torch.zeros(4, 1, dtype=torch.int32), plan, **kw)
+
+
+def _select(**kw):
+    q, summary = _selection()
+    return tokens.select_blocks(q, summary, kw.pop("block", 16), kw.pop("keep", 1), **kw)
+
+
+def _attend(**kw):
+    k, ids = torch.zeros(1, 128, 2, 16), torch.zeros(1, 4, 2, 1, dtype=torch.int32)
+    return tokens.block_attention(_selection()[0], k, k, ids, kw.pop("block", 16), **kw)
+
+
+def _summarize(**kw):
+    return tokens.summarize_blocks(torch.zeros(1, 128, 2, 16), kw.pop("block", 16), out=_selection()[1], **kw)
+
+
+@pytest.mark.parametrize("call,name,value", [
+    (_norm, "residual_scale", 0.5), (_norm, "eps", 0.25), (_rotate, "amplitude", 1.5), (_attend, "scale", 0.125),
+    (_rotate, "inverse", True), (_select, "causal", True), (_attend, "causal", True), (_select, "block", 16),
+    (_select, "keep", 3), (_select, "first", 2), (_select, "local", 2), (_attend, "block", 16), (_summarize, "block", 16),
+    (_summarize, "first", 2), (_summarize, "count", 3)])
+def test_numbers_that_tensors_hold(launches, call, name, value):
+    """A tensor's value can change behind a remembered call and would have to be waited for; a NumPy number is
+    as good as Python's."""
+    with pytest.raises(ContractError, match=name):
+        call(**{name: torch.tensor(value)})
+    call(**{name: value})
+    call(**{name: np.array([value])[0]})
+    one, two = ((entry, bytes(config), [a for a in rest if isinstance(a, int) and a < 1 << 20])
+                for entry, config, rest in launches)
+    assert one == two and len(tokens._checked) == 1
+
+
+@pytest.mark.parametrize("call,kw", [
+    (_norm, dict(residual_scale="1")), (_norm, dict(residual_scale=1e39)), (_norm, dict(eps=None)), (_rotate, dict(amplitude=-1e40)),
+    (_attend, dict(scale=1e300)), (_attend, dict(scale="0.1")), (_select, dict(keep=1.0)), (_select, dict(keep=1 << 32)),
+    (_select, dict(first=1 << 31)), (_select, dict(local=1.5)), (_summarize, dict(first=1 << 32, count=1)),
+    (_summarize, dict(first=0, count=1 << 32)), (_summarize, dict(first=0.0)), (_summarize, dict(count=9)),
+    (_summarize, dict(first=-1, count=2))])
+def test_numbers_that_are_none_or_do_not_fit(launches, call, kw):
+    with pytest.raises(ContractError):
+        call(**kw)
+    assert not launches
