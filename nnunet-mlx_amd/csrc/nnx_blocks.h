@@ -40,8 +40,8 @@ __device__ __forceinline__ int64_t item_start(const BlockArgs& a, int b) {
 // The queries of each key head of each item are cut into `splits` spans of `nt`; span v = (item *
 // kv_heads + key head) * splits + split.  A launch covers spans [span0, span0 + spans).  Row =
 // (span, query of the span, head of the group), counted from span0; every row has `keep`
-// partials, one a kept block: `dim` values (float32, or for 16-bit types int16 in 32767ths of a
-// common factor) and (log2 of the sum of its weights, factor of the values over that sum).
+// partials, one a kept block: `dim` values (Partial<T>) and (log2 of the sum of its weights, factor
+// of the values over that sum).
 struct ChunkArgs {
   BlockArgs a;
   const void *q, *k, *v;
@@ -54,6 +54,23 @@ struct ChunkArgs {
   // rows (pairs * group heads), tiles[u] of them before block u = (span - span0) * blocks + block
   const int32_t *list, *start, *tiles;
 };
+
+// What the values of a partial result are held in.  bfloat16's are float16 times a power of two that
+// puts the row's largest below 2^15: 11 bits for every channel down to 2^-29 of it, where the result
+// keeps 8, so an error of 2^-12 of a channel's own partials.  float16's result keeps 11 itself, and its
+// partials are float32.
+template <class T>
+struct PartialOf {
+  using type = float;
+};
+template <>
+struct PartialOf<bf16> {
+  using type = f16;
+};
+template <class T>
+using Partial = typename PartialOf<T>::type;
+
+inline int partial_bytes(int type) { return type == NNX_TYPE_BF16 ? 2 : 4; }
 
 struct Span {
   int b, g, t0, queries;

@@ -642,8 +642,7 @@ constexpr int kJoinWeights = 4096;
 
 template <class T>
 __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out, int share, int each) {
-  using P = typename std::conditional<sizeof(T) == 2, int16_t, float>::type;
-  constexpr float kUnit = sizeof(T) == 2 ? 1.f / 32767.f : 1.f;
+  using P = Partial<T>;
   // by row and slot the weight of the sum and the factor of the values; then the shares' sums
   extern __shared__ float2 weight[];
   float(*sums)[9] = (float(*)[9])(weight + each * c.a.keep);
@@ -698,14 +697,12 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
       for (int i = 0; i < AHEAD; ++i) {
         const int s = s0 + i * share;
         const float2 m = s < a.keep ? w[s] : make_float2(-INFINITY, 0.f);
-        const float ws = __builtin_amdgcn_exp2f(m.x - top), f = ws * m.y * kUnit;
+        const float ws = __builtin_amdgcn_exp2f(m.x - top), f = ws * m.y;
         const bool written = !(m.x == -INFINITY);
         l += ws;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float v = (float)x[i].v[e];
-          if (sizeof(T) == 4) v = written ? v : 0.f;  // whole numbers times 0 are 0 anyway
-          o[e] = fmaf(f, v, o[e]);
+          o[e] = fmaf(f, written ? to_float(x[i].v[e]) : 0.f, o[e]);
         }
       }
     }
@@ -755,7 +752,7 @@ AttentionPlan make_plan(const nnx_block_config& c) {
   AttentionPlan p;
   const int64_t group = c.heads / c.kv_heads, blocks = ceil_div(c.keys, c.block);
   // bytes of the partials of a query and key head: at most 256 * 130 * 4 a head
-  const int64_t query = group * c.keep * (8 + (int64_t)c.head_dim * type_bytes(c.type));
+  const int64_t query = group * c.keep * (8 + (int64_t)c.head_dim * partial_bytes(c.type));
   const int64_t fit = std::max<int64_t>(1, kPartialBudget / query);
   p.nt = (int)ceil_div(c.queries, ceil_div(c.queries, fit));
   p.splits = (int)ceil_div(c.queries, p.nt);
@@ -786,7 +783,7 @@ AttentionPlan make_plan(const nnx_block_config& c) {
   p.tiles = take((lists + 1) * 4);
   p.list = take(p.by_block ? (size_t)p.listed * p.nt * c.keep * 4 : 0);
   p.meta = take(rows * 8);
-  p.part = take(rows * c.head_dim * type_bytes(c.type));
+  p.part = take(rows * c.head_dim * partial_bytes(c.type));
   p.bytes = at;
   return p;
 }
@@ -958,7 +955,7 @@ void block_attention(const nnx_block_config& c, const void* q, const void* k, co
         share *= 2;
       const int here = std::min(each(), kJoinWeights / c.keep);
       ProfScope prof("block_join", 2.0 * rows * c.keep * c.head_dim,
-                     (double)rows * c.keep * (8 + c.head_dim * type_bytes(c.type)), st);
+                     (double)rows * c.keep * (8 + c.head_dim * partial_bytes(c.type)), st);
       with_type(c.type, [&](auto z) {
         using T = decltype(z);
         const size_t bytes = (size_t)here * c.keep * 8 + (share > 1 ? 256 * 9 * 4 : 0);

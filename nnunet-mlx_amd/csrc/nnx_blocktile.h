@@ -277,25 +277,26 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
   const float sum = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);  // 0: nothing seen; NaN stays
   before_stores();
   float2 meta = make_float2(l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l), sum);
-  if constexpr (sizeof(T) == 2) {
-    // In whole 2^-15ths of the row's largest magnitude: an error of 2^-16 of it, a tenth of what
-    // float16 would leave.  An infinite magnitude makes the row NaN; NaN alone hides from the
-    // maximum and is looked for where the block's values hold any.
+  if constexpr (sizeof(Partial<T>) == 2) {
+    // The power of two: of the largest finite magnitude, at least 2^-96, so that both factors are normal.
+    // Infinities and NaN stay what they are; they hide from the largest or would be it, so they are left
+    // out where the block's values hold any.
     float big = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) big = fmaxf(fmaxf(big, fabsf(o[dt][r])), fabsf(o[dt][r + 1]));
     if (block.odd) {
+      big = 0.f;
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) big = o[dt][r] == o[dt][r] ? big : INFINITY;
+        for (int r = 0; r < 16; ++r) big = fabsf(o[dt][r]) < INFINITY ? fmaxf(big, fabsf(o[dt][r])) : big;
     }
     const float2 bh = both_halves(big);
-    big = fmaxf(fmaxf(bh.x, bh.y), 7.52e-37f);  // 2^-120, where the reciprocal is finite
-    const float down = __builtin_amdgcn_rcpf(big);
-    meta.y *= big;
+    const int exponent = max(__builtin_amdgcn_frexp_expf(fmaxf(bh.x, bh.y)), -96) - 15;
+    const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
+    meta.y *= __uint_as_float((uint32_t)(127 + exponent) << 23);
     const uint32_t bytes = c.a.dim * 2;
     const RowWriter writer{out_lds, part, partial == kNowhere ? kNowhere : partial * bytes, bytes};
 #pragma unroll
@@ -305,8 +306,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
         uint32_t w[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const auto pair = __builtin_amdgcn_cvt_pknorm_i16(o[dt][8 * i + 2 * r] * down,
-                                                            o[dt][8 * i + 2 * r + 1] * down);
+          const Vec<f16, 2> pair{(f16)(o[dt][8 * i + 2 * r] * down), (f16)(o[dt][8 * i + 2 * r + 1] * down)};
           __builtin_memcpy(&w[r], &pair, 4);
         }
         // channels 8 apart, 4 a half, become 8 neighbours a half
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP, BK>)) void block_partials_kerne
   const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-35f);
   const bool negate = a.scale < 0.f;
   const size_t partials_all = (size_t)c.spans * c.nt * a.group * a.keep;
-  const auto part = buffer_of(c.part, partials_all * a.dim * (sizeof(T) == 2 ? 2 : 4));
+  const auto part = buffer_of(c.part, partials_all * a.dim * sizeof(Partial<T>));
   const auto metas = buffer_of(c.meta, partials_all * 8);
   if constexpr (BY_BLOCK) {
     const int all = c.spans * a.blocks, tile0 = c.tiles[0];

@@ -1,0 +1,69 @@
+"""What attention over selected blocks keeps of its values: every channel by itself, at any magnitude.
+
+Tolerances.  U is a type's unit roundoff (half the spacing at 1).  Each channel is judged against the mean
+over its own weights of |v|, which is what an error of the weights can move it by.  Weights may be off by
+U where they are rounded to the type, and by 5e-4 through a float32 logit of up to 130 terms that sum to
+less than 20 in magnitude (130 * 2^-24 * 20 = 1.6e-4, a weight by twice that); partials and the result are
+rounded by at most U each: 3 U + 5e-4."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from nnunet_mlx.model import tokens
+from oracle import tokens as ot
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}
+TYPES = list(U)
+
+
+def _f64(t: torch.Tensor) -> np.ndarray:
+    return t.detach().double().cpu().numpy()
+
+
+def _attention(q, k, v, see, scale):
+    """Float64 attention over the seen keys and the same of |v|, by channel."""
+    q, k, v = map(_f64, (q, k, v))
+    group = q.shape[2] // k.shape[2]
+    k, v, see = (np.repeat(a, group, 2) for a in (k, v, see))
+    logits = np.einsum("bthd,bshd->bths", q, k) * scale
+    logits = np.where(see, logits, -np.inf)
+    top = logits.max(-1, keepdims=True)
+    p = np.exp(logits - np.where(np.isfinite(top), top, 0))
+    p /= np.maximum(p.sum(-1, keepdims=True), 1e-300)
+    return np.einsum("bths,bshd->bthd", p, v), np.einsum("bths,bshd->bthd", p, np.abs(v))
+
+
+def _inputs(seed, dtype, queries, keys, heads=4, kv_heads=2, dim=64):
+    gen = torch.Generator().manual_seed(seed)
+    q, k, v = (torch.randn(1, n, h, dim, generator=gen) for n, h in ((queries, heads), (keys, kv_heads), (keys, kv_heads)))
+    return q.to(dtype).cuda(), k.to(dtype).cuda(), v.to(dtype).cuda()
+
+
+def _ids(queries, kv_heads, blocks, keep, seed):
+    gen = torch.Generator().manual_seed(seed)
+    ids = torch.rand(1, queries, kv_heads, blocks, generator=gen).topk(keep).indices.sort(-1).values
+    return ids.to(torch.int32).cuda()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", [3, 1500])
+@pytest.mark.parametrize("dim,block", [(64, 32), (40, 16), (128, 128)])
+def test_channels_of_very_different_size(device, dtype, queries, dim, block):
+    """A few channels 64 to 4096 times larger than the others, which keep their own precision."""
+    keys, keep = 8 * block - 5, 4
+    q, k, v = _inputs(queries + dim, dtype, queries, keys, dim=dim)
+    sizes = torch.full((dim,), 2.0**-4)
+    sizes[3], sizes[dim // 2], sizes[dim - 1], sizes[1] = 4.0, 32.0, 256.0, 2.0**-10
+    v = (v.float() * sizes.cuda()).to(dtype)
+    ids = _ids(queries, 2, 8, keep, queries)
+    got = _f64(tokens.block_attention(q, k, v, ids, block))
+    see = ot.seen(ids.cpu().numpy(), keys, block, np.ones((1, keys), bool))
+    want, size = _attention(q, k, v, see, dim**-0.5)
+    # float16 has no finer spacing than 2^-24 below 2^-14
+    bound = (3 * U[dtype] + 5e-4) * size + (2.0**-24 if dtype == torch.float16 else 0)
+    assert (np.abs(got - want) <= bound).all()
