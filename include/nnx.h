@@ -623,8 +623,8 @@ int nnx_block_select(const nnx_block_config* config, const void* d_q, const int8
 
 /* out[q] = softmax(scale q . k) v over the valid keys of the blocks in d_ids (batch, queries,
  * kv_heads, keep; entries outside [0, nb) are skipped, the others of a row are distinct).  A
- * query without a valid key gets zeros.  In 16-bit types a value that is not finite, weighed by a
- * query, makes its row NaN.  The workspace query answers 0 for what the entry refuses. */
+ * query without a valid key gets zeros.  A value that is not finite reaches its own channel, of the
+ * queries that see its key.  The workspace query answers 0 for what the entry refuses. */
 size_t nnx_block_attention_workspace(const nnx_block_config* config);
 int nnx_block_attention(const nnx_block_config* config, const void* d_q, const void* d_k,
                         const void* d_v, const int32_t* d_ids, const int32_t* d_start,

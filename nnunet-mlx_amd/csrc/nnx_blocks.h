@@ -41,7 +41,8 @@ __device__ __forceinline__ int64_t item_start(const BlockArgs& a, int b) {
 // kv_heads + key head) * splits + split.  A launch covers spans [span0, span0 + spans).  Row =
 // (span, query of the span, head of the group), counted from span0; every row has `keep`
 // partials, one a kept block: `dim` values (Partial<T>) and (log2 of the sum of its weights, factor
-// of the values over that sum).
+// of the values over that sum; negative where the block holds values that are not finite, which count
+// as 0 in the partial).
 struct ChunkArgs {
   BlockArgs a;
   const void *q, *k, *v;

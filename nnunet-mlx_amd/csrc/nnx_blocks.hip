@@ -633,6 +633,27 @@ __global__ __launch_bounds__(256) void place_pairs_kernel(ChunkArgs c, int per, 
   each_pair(c, per, [&](int e, int j) { list[atomicAdd(&next[j], 1)] = e; });
 }
 
+// Adds what of block j's values is not finite and seen by query t of a span: the sum becomes the infinity or
+// NaN that it is by definition, in the channels that hold one.
+template <class T>
+__device__ __forceinline__ void add_odd_values(const ChunkArgs& c, const T* v, Span s, int t, int j,
+                                                         float (&o)[8]) {
+  const BlockArgs& a = c.a;
+  const uint8_t* mask = a.mask ? a.mask + s.b * a.ms : nullptr;
+  const int64_t first = (int64_t)j * a.block, at = item_start(a, s.b) + s.t0 + t;
+  int64_t end = min(first + a.block, (int64_t)item_length(a, s.b));
+  if (a.causal) end = min(end, at + 1);
+  for (int64_t key = first; key < end; ++key) {
+    if (mask && !mask[key]) continue;
+    const Vec<T, 8> x = load_vec<8>(v + s.b * a.vs[0] + key * a.vs[1] + s.g * a.vs[2]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = to_float(x.v[e]);
+      if (!(fabsf(y) < INFINITY)) o[e] += y;
+    }
+  }
+}
+
 // out = sum_s w_s O_s / sum_s w_s with w_s = 2^(log2 sum_s - largest), O_s a partial under its
 // factor, in the order of the slots.  A workgroup forms the weights of its rows together, then dim / 8
 // lanes a row add up (`share` groups of them a row, each every share-th partial, where rows are few
@@ -677,6 +698,7 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
   // Partials of entries that are no block were never written: whatever is there is left out below.
   constexpr int AHEAD = 8;
   const P* part = (const P*)c.part + partial_of(row0 + (live ? own : 0)) * a.dim + 8 * u;
+  bool odd = false;  // some partial leaves out values that are not finite
   Vec<P, 8> x[AHEAD];
   const auto fetch = [&](int s0) {
 #pragma unroll
@@ -697,7 +719,8 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
       for (int i = 0; i < AHEAD; ++i) {
         const int s = s0 + i * share;
         const float2 m = s < a.keep ? w[s] : make_float2(-INFINITY, 0.f);
-        const float ws = __builtin_amdgcn_exp2f(m.x - top), f = ws * m.y;
+        const float ws = __builtin_amdgcn_exp2f(m.x - top), f = ws * fabsf(m.y);
+        odd |= m.y < 0.f;
         const bool written = !(m.x == -INFINITY);
         l += ws;
 #pragma unroll
@@ -705,6 +728,16 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
           o[e] = fmaf(f, written ? to_float(x[i].v[e]) : 0.f, o[e]);
         }
       }
+    }
+  }
+  if (odd) {
+    Span s;
+    int t, h;
+    place(row0 + own, s, t, h);
+    for (int slot = part0; slot < a.keep; slot += share) {
+      if (!(weight[own * a.keep + slot].y < 0.f)) continue;
+      const int j = c.ids[(((int64_t)s.b * a.queries + s.t0 + t) * a.kv_heads + s.g) * a.keep + slot];
+      add_odd_values(c, (const T*)c.v + 8 * u, s, t, j, o);
     }
   }
   if (share > 1) {

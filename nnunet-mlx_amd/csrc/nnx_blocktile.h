@@ -54,11 +54,12 @@ struct Tile {
 
 struct Staged {
   bool full;  // every key is valid
-  bool odd;   // some value is not finite (looked for in 16-bit types)
+  bool odd;   // some value is not finite
 };
 
-// The block's keys and values into LDS, zeros for those that are not valid, and what is added to
-// their scores: 0, or -inf for keys that are not valid.
+// The block's keys and values into LDS, zeros for those that are not valid and for values that are not
+// finite (a weight of 0 would not keep them out of a product; the join takes them from the rows that see
+// them), and what is added to the keys' scores: 0, or -inf for keys that are not valid.
 template <class T, int DP, int BK>
 __device__ __forceinline__ Staged stage_block(const ChunkArgs& c, int b, int g, int j, T* lk, T* lv,
                                             float* bias, bool negate) {
@@ -83,10 +84,15 @@ __device__ __forceinline__ Staged stage_block(const ChunkArgs& c, int b, int g, 
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int n = threadIdx.x + i * 256;
-    if constexpr (sizeof(T) == 2) {
+    bool here = false;
 #pragma unroll
-      for (int e = 0; e < G::CH; ++e) odd |= !(fabsf(to_float(vr[i].v[e])) < INFINITY);
+    for (int e = 0; e < G::CH; ++e) here |= !(fabsf(to_float(vr[i].v[e])) < INFINITY);
+    if (here) {
+#pragma unroll
+      for (int e = 0; e < G::CH; ++e)
+        vr[i].v[e] = fabsf(to_float(vr[i].v[e])) < INFINITY ? vr[i].v[e] : from_float<T>(0.f);
     }
+    odd |= here;
     if (negate) {
 #pragma unroll
       for (int e = 0; e < G::CH; ++e) kr[i].v[e] = -kr[i].v[e];
@@ -278,21 +284,13 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
   before_stores();
   float2 meta = make_float2(l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l), sum);
   if constexpr (sizeof(Partial<T>) == 2) {
-    // The power of two: of the largest finite magnitude, at least 2^-96, so that both factors are normal.
-    // Infinities and NaN stay what they are; they hide from the largest or would be it, so they are left
-    // out where the block's values hold any.
+    // The power of two: of the largest magnitude, at least 2^-96, so that both factors are normal.  NaN, of
+    // the weights, hides from the largest and stays NaN.
     float big = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) big = fmaxf(fmaxf(big, fabsf(o[dt][r])), fabsf(o[dt][r + 1]));
-    if (block.odd) {
-      big = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) big = fabsf(o[dt][r]) < INFINITY ? fmaxf(big, fabsf(o[dt][r])) : big;
-    }
     const float2 bh = both_halves(big);
     const int exponent = max(__builtin_amdgcn_frexp_expf(fmaxf(bh.x, bh.y)), -96) - 15;
     const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
@@ -331,6 +329,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
       writer.flush(dt);
     }
   }
+  if (block.odd) meta.y = -meta.y;  // the join looks
   const u32x2 words{__float_as_uint(meta.x), __float_as_uint(meta.y)};
   __builtin_amdgcn_raw_buffer_store_b64(words, metas, half || partial == kNowhere ? kNowhere : partial * 8, 0, 0);
 }

@@ -67,3 +67,36 @@ def test_channels_of_very_different_size(device, dtype, queries, dim, block):
     # float16 has no finer spacing than 2^-24 below 2^-14
     bound = (3 * U[dtype] + 5e-4) * size + (2.0**-24 if dtype == torch.float16 else 0)
     assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("queries,heads,dim,block", [(5, 4, 64, 32), (250, 2, 40, 16), (255, 4, 128, 128), (90, 260, 8, 32)])
+def test_values_that_are_not_finite_stay_in_their_channel(device, dtype, causal, queries, heads, dim, block):
+    """An infinity or NaN reaches the channel it is in, of the rows that see its key; a key behind the query
+    shares a block with keys before it and may hold anything."""
+    keys, blocks = 256, 256 // block
+    q, k, v = _inputs(queries + dim, dtype, queries, keys, heads, 2, dim)
+    start = keys - queries - 1
+    keep = max(1, blocks // 2)
+    ids = _ids(queries, 2, blocks, keep, 5)
+    ids[..., -1] = blocks - 1  # the block that holds the last keys, in every row
+    odd = torch.zeros(1, keys, 2, dim)
+    odd[0, keys - 3, :, 1], odd[0, keys - 2, 0, 2], odd[0, keys - 1, 1, 2] = float("inf"), float("-inf"), float("nan")
+    odd[0, keys - 4, 0, 5], odd[0, keys - 2, 0, 5], odd[0, 40, 1, 7] = float("inf"), float("-inf"), float("-inf")
+    v = torch.where(odd == 0, v.cpu(), odd.to(dtype)).cuda()
+    got = tokens.block_attention(q, k, v, ids, block, causal=causal, start=start)
+    see = ot.seen(ids.cpu().numpy(), keys, block, np.ones((1, keys), bool), causal=causal, start=np.array([start]))
+    want, size = _attention(q, k, torch.where(odd.cuda() == 0, v, 0), see, dim**-0.5)
+    # what a row sees of the odd ones adds up to an infinity or NaN, or to 0
+    group = heads // 2
+    with np.errstate(invalid="ignore"):
+        poison = np.zeros((1, queries, 2, dim))
+        for _, key, head, channel in np.argwhere(odd.numpy() != 0):
+            poison[:, :, head, channel] += np.where(see[:, :, head, key], odd[0, key, head, channel].item(), 0)
+    poison = poison.repeat(group, 2)
+    got = _f64(got)
+    assert np.array_equal(got[poison != 0], poison[poison != 0], equal_nan=True)
+    assert (poison != 0).any() and (poison == 0).any()
+    clean = poison == 0
+    assert (np.abs(got - want)[clean] <= (3 * U[dtype] + 5e-4) * size[clean]).all()
