@@ -713,6 +713,7 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
 #pragma unroll 8
     for (int s = 0; s < a.keep; ++s) top = fmaxf(top, w[s].x);
     if (top == -INFINITY) top = 0.f;
+    top += (float)(32 - __clz(a.keep - 1));  // weights that sum to 1 at most keep the sum in the values' range
     for (int s0 = part0; s0 < a.keep; s0 += AHEAD * share) {
       if (s0 != part0) fetch(s0);
 #pragma unroll

@@ -148,8 +148,8 @@ struct RowWriter {
   }
 };
 
-// The partial softmax of rows over one block: m = max x, l = sum 2^(x - m), O = sum 2^(x - m) v / l, of
-// which log2 l + m and O are kept (x the scores in units of log 2; weights, sums and O in float32,
+// The partial softmax of rows over one block: m = max x up to a constant, l = sum 2^(x - m), O = sum
+// 2^(x - m) v / l, of which log2 l + m and O are kept (x the scores in units of log 2; weights, sums and O in float32,
 // weights rounded to the type's bits only as operands of the second product).
 // 32 query rows, a lane pair (l, l + 32) each: S^T = K Q^T leaves a row's scores in its two
 // lanes' registers, so the softmax needs one exchange between halves, and its weights are
@@ -229,7 +229,10 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
     for (int r = 0; r < G::REGS; ++r) m = fmaxf(m, acc[kt][r]);
   const float2 mh = both_halves(m);
   m = fmaxf(mh.x, mh.y);
-  const float top = m == -INFINITY ? 0.f : m * c2;  // nothing seen: all weights 2^-inf
+  // Weights of at most 2^-kDown, so that the block's values add up to no more than the largest of them
+  // (float16's do not reach float32's end).  Nothing seen: all weights 2^-inf.
+  constexpr float kDown = std::is_same<T, f16>::value ? 0 : BK == 16 ? 4 : BK == 32 ? 5 : BK == 64 ? 6 : 7;
+  const float top = m == -INFINITY ? 0.f : m * c2 + kDown;
   float l = 0.f;
 #pragma unroll
   for (int kt = 0; kt < G::KT; ++kt)

@@ -100,3 +100,23 @@ def test_values_that_are_not_finite_stay_in_their_channel(device, dtype, causal,
     assert (poison != 0).any() and (poison == 0).any()
     clean = poison == 0
     assert (np.abs(got - want)[clean] <= (3 * U[dtype] + 5e-4) * size[clean]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", [3, 700])
+@pytest.mark.parametrize("block,keep", [(16, 30), (64, 7), (128, 3)])
+def test_values_at_the_end_of_their_type(device, dtype, queries, block, keep):
+    """Sums of such values pass the type's range, and float32's, on the way to a mean within it."""
+    blocks = keep + 1
+    keys = blocks * block - 3
+    q, k, v = _inputs(queries + block, dtype, queries, keys)
+    top = 65504.0 if dtype == torch.float16 else 3.38e38
+    v = ((0.5 + 0.5 * torch.rand(v.shape, generator=torch.Generator().manual_seed(2))) * top).to(dtype).cuda()
+    v[..., 1::2] *= -1
+    ids = _ids(queries, 2, blocks, keep, 6)
+    for size_of_k in (0, 1):
+        got = tokens.block_attention(q, k * size_of_k, v, ids, block)
+        see = ot.seen(ids.cpu().numpy(), keys, block, np.ones((1, keys), bool))
+        want, size = _attention(q, k * size_of_k, v, see, 64**-0.5)
+        assert torch.isfinite(got).all()
+        assert (np.abs(_f64(got) - want) <= (3 * U[dtype] + 5e-4) * size).all()
