@@ -149,8 +149,10 @@ struct RowWriter {
 };
 
 // The partial softmax of rows over one block: m = max x up to a constant, l = sum 2^(x - m), O = sum
-// 2^(x - m) v / l, of which log2 l + m and O are kept (x the scores in units of log 2; weights, sums and O in float32,
-// weights rounded to the type's bits only as operands of the second product).
+// 2^(x - m) v / l, of which log2 l + m and O are kept (x the scores in units of log 2; weights, sums and O
+// in float32).  In 16-bit types a weight is two operands of the second product, its rounded value and the
+// rest: 16 bits of it for bfloat16, 22 for float16, so that the result's own rounding is the only one that
+// shows (1.3 times the error with one operand; 329 us of partials against 314 for 32768 queries of 32 blocks).
 // 32 query rows, a lane pair (l, l + 32) each: S^T = K Q^T leaves a row's scores in its two
 // lanes' registers, so the softmax needs one exchange between halves, and its weights are
 // already the second operand of O^T = V^T P^T (the order of keys is that of the registers; values
@@ -251,9 +253,14 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int i = 0; i < BK / 16; ++i) {
-      Frag<T> p;
+      // each weight as two operands, its rounded value and what that leaves
+      Frag<T> p, rest;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) p[r] = from_float<T>(acc[i / 2][8 * (i % 2) + r]);
+      for (int r = 0; r < 8; ++r) {
+        const float w = acc[i / 2][8 * (i % 2) + r];
+        p[r] = from_float<T>(w);
+        rest[r] = from_float<T>(w - to_float(p[r]));
+      }
       const int row = 16 * i + 4 * half + lane % 16 / 4;
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
@@ -267,6 +274,7 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
         vt.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lv + G::at(row, d / 8) + d % 8));
         vt.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lv + G::at(row + 8, d / 8) + d % 8));
         o[dt] = mfma(vt.f, p, o[dt]);
+        o[dt] = mfma(vt.f, rest, o[dt]);
       }
     }
   } else {

@@ -120,3 +120,21 @@ def test_values_at_the_end_of_their_type(device, dtype, queries, block, keep):
         want, size = _attention(q, k * size_of_k, v, see, 64**-0.5)
         assert torch.isfinite(got).all()
         assert (np.abs(_f64(got) - want) <= (3 * U[dtype] + 5e-4) * size).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("queries", [6, 900])
+@pytest.mark.parametrize("dim,block", [(64, 64), (80, 16), (128, 32)])
+def test_no_rounding_but_the_results_own(device, dtype, queries, dim, block):
+    """The distance to float64 is that of the float64 result rounded once: rounding errors are independent
+    and add in squares, and bfloat16's partials, an eighth of its unit, add less than a hundredth; float32
+    sums and exponents add some 1e-6 of the size of the terms."""
+    blocks, keep = 12, 5
+    keys = blocks * block - 7
+    q, k, v = _inputs(queries + dim + block, dtype, queries, keys, dim=dim)
+    ids = _ids(queries, 2, blocks, keep, 7)
+    got = _f64(tokens.block_attention(q, k, v, ids, block))
+    see = ot.seen(ids.cpu().numpy(), keys, block, np.ones((1, keys), bool))
+    want, size = _attention(q, k, v, see, dim**-0.5)
+    once = _f64(torch.from_numpy(want).to(dtype)) - want
+    assert np.linalg.norm(got - want) <= 1.05 * np.linalg.norm(once) + 1e-5 * np.linalg.norm(size)
