@@ -43,7 +43,7 @@ struct Tile {
   static constexpr int ROW_BYTES = DP * sizeof(T);
   static constexpr int PER = ROW_BYTES >= 256 ? 1 : 256 / ROW_BYTES;  // rows in 256 bytes
   static constexpr int TURNS = CHUNKS & -CHUNKS;   // a power of two that divides CHUNKS
-  // keys, values, what is added to their scores, and for each wave 32 rows of 128 bytes on their way out
+  // keys, values, what their scores are replaced by, and for each wave 32 rows of 128 bytes on their way out
   static constexpr int OUT = 32 * 128;
   static constexpr size_t LDS = (size_t)2 * ROWS * ROW_BYTES + ROWS * sizeof(float) + 16 + 4 * OUT;
   static __device__ __forceinline__ int at(int row, int chunk) {
@@ -59,7 +59,7 @@ struct Staged {
 
 // The block's keys and values into LDS, zeros for those that are not valid and for values that are not
 // finite (a weight of 0 would not keep them out of a product; the join takes them from the rows that see
-// them), and what is added to the keys' scores: 0, or -inf for keys that are not valid.
+// them), and the scores of keys that are not valid: -inf, 0 for the others.
 template <class T, int DP, int BK>
 __device__ __forceinline__ Staged stage_block(const ChunkArgs& c, int b, int g, int j, T* lk, T* lv,
                                             float* bias, bool negate) {
@@ -212,8 +212,12 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
     for (int kt = 0; kt < G::KT; ++kt)
 #pragma unroll
       for (int r = 0; r < G::REGS; r += 4) {
+        // chosen, not added: a query that is not finite has NaN for the zeros of such keys
         const float4 z = *(const float4*)&bias[kt * 32 + 2 * r + 4 * half];
-        acc[kt][r] += z.x, acc[kt][r + 1] += z.y, acc[kt][r + 2] += z.z, acc[kt][r + 3] += z.w;
+        acc[kt][r] = z.x < 0.f ? z.x : acc[kt][r];
+        acc[kt][r + 1] = z.y < 0.f ? z.y : acc[kt][r + 1];
+        acc[kt][r + 2] = z.z < 0.f ? z.z : acc[kt][r + 2];
+        acc[kt][r + 3] = z.w < 0.f ? z.w : acc[kt][r + 3];
       }
   }
   if (__any(last < BK - 1)) {  // the query's own block, or one behind it

@@ -138,3 +138,17 @@ def test_no_rounding_but_the_results_own(device, dtype, queries, dim, block):
     want, size = _attention(q, k, v, see, dim**-0.5)
     once = _f64(torch.from_numpy(want).to(dtype)) - want
     assert np.linalg.norm(got - want) <= 1.05 * np.linalg.norm(once) + 1e-5 * np.linalg.norm(size)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", [2, 400])
+def test_a_query_without_keys_gets_zeros_whatever_it_holds(device, dtype, queries):
+    """Rows of infinities and NaN over blocks of masked keys: zeros, as any row that sees nothing."""
+    q, k, v = _inputs(queries, dtype, queries, 200)
+    q[0, 0, 0], q[0, 1, 1, 3], q[0, 1, 2] = float("inf"), float("nan"), float("-inf")
+    mask = torch.zeros(1, 200, dtype=torch.bool, device="cuda")
+    mask[0, 32:64] = True
+    ids = torch.tensor([0, 3, 6], dtype=torch.int32).expand(1, queries, 2, 3).contiguous().cuda()
+    for args in (dict(key_mask=mask), dict(lengths=torch.zeros(1, dtype=torch.int32, device="cuda")),
+                 dict(key_mask=mask, causal=True, start=3)):
+        assert not tokens.block_attention(q, k, v, ids, 32, **args).any()
