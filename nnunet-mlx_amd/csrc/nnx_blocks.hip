@@ -276,6 +276,7 @@ __device__ __forceinline__ void select_row(float* score, float* spare, int chunk
       }
       if (over <= room) {
         if (forced) restore();
+        wave_sync();
         int n = 0;
         each([&](int i, float y) {
           const bool take = y > low;
@@ -284,6 +285,7 @@ __device__ __forceinline__ void select_row(float* score, float* spare, int chunk
           if (take && to < 128) spare[to] = y, spare[128 + to] = __int_as_float(i * 64 + lane);
           n += __popcll(taken);
         });
+        wave_sync();
         float w[2];
         int32_t at[2];
 #pragma unroll

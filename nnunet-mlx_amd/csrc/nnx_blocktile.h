@@ -138,6 +138,7 @@ struct RowWriter {
   __device__ __forceinline__ void flush(int pass) const {
     const int lane = threadIdx.x % 64, chunk = lane % 8;
     const uint32_t at = pass * 128 + chunk * 16;
+    wave_sync();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 8 * i + lane / 8;
@@ -145,6 +146,7 @@ struct RowWriter {
       const uint32_t to = __shfl(row, r);
       __builtin_amdgcn_raw_buffer_store_b128(v, part, at < bytes && to != kNowhere ? to + at : kNowhere, 0, 0);
     }
+    wave_sync();
   }
 };
 

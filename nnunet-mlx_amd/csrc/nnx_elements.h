@@ -53,6 +53,14 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& r) {
   __builtin_memcpy(p, &r, sizeof(r));
 }
 
+// Stands between what lanes of a wave write to LDS and what other lanes of it read there, and before they
+// write there again.  LDS serves a wave's accesses in order, so this costs no instruction: it holds the
+// compiler to that order.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Value of another lane of the same 16 (CTRL: a DPP control word) without a trip through LDS.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {

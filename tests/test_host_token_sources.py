@@ -33,3 +33,22 @@ def test_bounds_checked_offsets(name):
     for match in re.finditer(r"__builtin_amdgcn_raw_buffer_(load|store)_\w+\(", text):
         arguments = _arguments(text, match.end() - 1)
         assert arguments[-2] == "0", (match.group(), arguments)
+
+
+def _body(text: str, opening: str) -> str:
+    at = text.index(opening)
+    depth = 0
+    for i in range(text.index("{", at), len(text)):
+        depth += (text[i] == "{") - (text[i] == "}")
+        if depth == 0:
+            return text[at:i]
+    raise AssertionError("unbalanced body")
+
+
+def test_lanes_that_exchange_through_lds():
+    """What lanes of one wave leave for each other in LDS is fenced off on both sides."""
+    flush = _body((CSRC / "nnx_blocktile.h").read_text(), "void flush(int pass) const {")
+    assert flush.index("wave_sync()") < flush.index("*(const u32x4*)") < flush.rindex("wave_sync()")
+    packing = _body((CSRC / "nnx_blocks.hip").read_text(), "if (over <= room) {")
+    write, read = packing.index("spare[to] = y"), packing.index("in ? spare[")
+    assert packing.index("wave_sync()") < write < packing.rindex("wave_sync()") < read
