@@ -34,7 +34,7 @@ struct RotaryArgs {
 // cos(pi z / 4) end below 2e-9.
 __device__ __forceinline__ void sincos_turns(int32_t turns, float& s, float& c) {
   const int quarter = (int)((uint32_t)turns + 0x20000000u) >> 30;
-  const float z = (float)(turns - (int)((uint32_t)quarter << 30)) * 1.862645149230957e-09f;  // 2^-29
+  const float z = (float)(int32_t)((uint32_t)turns - ((uint32_t)quarter << 30)) * 1.862645149230957e-09f;  // 2^-29
   const float zz = z * z;
   const float ps = z * fmaf(zz, fmaf(zz, fmaf(zz, fmaf(zz, 3.1336162e-07f, -3.6576204e-05f),
                                              2.4903946e-03f), -8.0745512e-02f), 7.8539816e-01f);
