@@ -513,16 +513,14 @@ struct SelectPlan {
 
 SelectPlan plan_selection(const nnx_block_config& c) {
   SelectPlan p{};
-  const int blocks = (int)ceil_div(c.keys, c.block), group = c.heads / c.kv_heads;
+  const int blocks = (int)ceil_div(c.keys, c.block);
   const int64_t units = (int64_t)c.kv_heads * c.batch, tiles = ceil_div(c.queries, 16) * units;
   p.chunks = 1;
   while (p.chunks * 64 < blocks) p.chunks *= 2;
   p.rows = std::min(16, c.queries);
   p.split = blocks > kWholeBlocks || (blocks >= kPartBlocks && tiles <= std::min(kPartTiles, blocks / 32));
   if (!p.split) {
-    const size_t codes = (size_t)std::min(group, kScoreHeads) * 2048;
-    p.pitch = p.chunks * 64 + 4;
-    while (p.rows > 1 && (size_t)p.rows * p.pitch * 4 + codes > 160 * 1024 - 1024) p.rows /= 2;
+    p.pitch = p.chunks * 64 + 4;  // with the codes at most 16 * 2052 * 4 + 8 * 2048 bytes of LDS, 144 KB
     return p;
   }
   p.parts.pitch = (int)ceil_div(blocks, 16) * 16;
@@ -886,7 +884,7 @@ void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
     }
     return;
   }
-  // As many queries a workgroup as the products take, while their scores fit the LDS.  Few workgroups
+  // As many queries a workgroup as the products take.  Few workgroups
   // take twice the waves; up to 128 blocks give work to 4 (40960 rows of 64: 23 us against 26 with 8).
   const dim3 grid((unsigned)ceil_div(c.queries, plan.rows), c.kv_heads, c.batch);
   const int threads = (double)grid.x * grid.y * grid.z < 2 * compute_units() ? 1024 : plan.chunks <= 2 ? 256 : 512;

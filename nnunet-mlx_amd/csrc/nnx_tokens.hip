@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int units, in
       sn[p] *= a.amp_sin;
       cs[p] *= a.amp;
     }
-    const int e0 = INTERLEAVED ? u * W : u * W, e1 = e0 + a.half;
+    const int e0 = u * W, e1 = e0 + a.half;
     for (int h = h0; h < h1; h += HB) {
       Vec<T, W> v[HB], w[INTERLEAVED ? 1 : HB];
 #pragma unroll

@@ -145,10 +145,6 @@ def _launch(device: torch.device, entry: str, *arguments) -> None:
         _native.check(status, entry)
 
 
-def _address(tensor: torch.Tensor | None) -> int | None:
-    return None if tensor is None else tensor.data_ptr()
-
-
 # ---- rotary positions -----------------------------------------------------------------
 
 
