@@ -150,11 +150,14 @@ def _launch(device: torch.device, entry: str, *arguments) -> None:
 
 class RotaryPlan(NamedTuple):
     """Rotation of the pairs of a head: ``steps`` int64 in 2^-64 turns a position, ``axes`` int32
-    the position axis of each pair, ``amplitude`` the factor on the rotated elements."""
+    the position axis of each pair, ``amplitude`` the factor on the rotated elements and
+    ``position_axes`` how many axes a position has at least (0: not checked; a pair whose axis a
+    position lacks is turned by the last it has)."""
 
     steps: torch.Tensor
     axes: torch.Tensor
     amplitude: float
+    position_axes: int = 0
 
 
 def rotary_plan(rotary_dim: int, *, axes: int = 1, base: float = 10000.0, scaling: str | None = None,
@@ -194,7 +197,7 @@ def rotary_plan(rotary_dim: int, *, axes: int = 1, base: float = 10000.0, scalin
             owners.append(axis)
     amplitude = 0.1 * math.log(factor) + 1.0 if scaling == "ramp" else 1.0
     return RotaryPlan(torch.tensor(steps, dtype=torch.int64, device=device),
-                      torch.tensor(owners, dtype=torch.int32, device=device), amplitude)
+                      torch.tensor(owners, dtype=torch.int32, device=device), amplitude, axes)
 
 
 def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, plan: RotaryPlan, *,
@@ -208,7 +211,8 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
     pairs are copied.  ``inverse`` turns back, which is also the gradient of the forward turn.
     ``out`` may hold the results, ``(q, k)`` itself to rotate in place."""
     amplitude, inverse = _number("plan.amplitude", plan.amplitude), _flag("inverse", inverse)
-    key = ("rotate", _signature(q, k, positions, plan.steps, plan.axes, *(out or (None,))), amplitude, layout, inverse)
+    key = ("rotate", _signature(q, k, positions, plan.steps, plan.axes, *(out or (None,))), amplitude,
+           plan.position_axes, layout, inverse)
     config = _checked.get(key)
     if config is None:
         config = _remember(key, _rotary_config(q, k, positions, plan, amplitude, layout, inverse, out))
@@ -242,6 +246,7 @@ def _rotary_config(q, k, positions, plan, amplitude, layout, inverse, out):
           f"positions must be int32 (tokens, axes) or (batch, tokens, axes) on {q.device}, got "
           f"{positions.dtype} {tuple(positions.shape)} on {positions.device}")
     axes = positions.shape[-1]
+    _need(axes >= plan.position_axes, f"the plan turns by {plan.position_axes} position axes, positions have {axes}")
     _need(axes == 1 or positions.stride(-1) == 1, "positions need a contiguous last axis")
     _check_side("plan.steps", plan.steps, torch.int64, (rotary_dim // 2,), q.device)
     _check_side("plan.axes", plan.axes, torch.int32, (rotary_dim // 2,), q.device)

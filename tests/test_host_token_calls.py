@@ -145,3 +145,20 @@ def test_numbers_that_are_none_or_do_not_fit(launches, call, kw):
     with pytest.raises(ContractError):
         call(**kw)
     assert not launches
+
+
+# ---- what a call cannot do ------------------------------------------------------------
+
+
+def test_positions_of_too_few_axes(launches):
+    """A plan knows how many position axes its pairs turn by."""
+    q, plan = torch.zeros(1, 4, 2, 16), tokens.rotary_plan(12, axes=3, device="cpu")
+    made = tokens.RotaryPlan(plan.steps, plan.axes, 1.0)
+    for known in (made, plan):  # the check of one plan does not stand for another of the same shapes
+        for axes in (3, 4):
+            tokens.rotate(q, None, torch.zeros(4, axes, dtype=torch.int32), known)
+    tokens.rotate(q, None, torch.zeros(4, 2, dtype=torch.int32), made)
+    for axes in (1, 2):
+        with pytest.raises(ContractError, match="axes"):
+            tokens.rotate(q, None, torch.zeros(4, axes, dtype=torch.int32), plan)
+    assert len(launches) == 5
