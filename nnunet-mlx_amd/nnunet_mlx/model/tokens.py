@@ -5,8 +5,9 @@ rotary positions (``rotary_plan``, ``rotate``), attention over blocks of keys th
 score selects for each query (``summarize_blocks``, ``select_blocks``, ``block_attention``, all
 three in ``sparse_attention``) and the norms around the block with its gate and residual sum
 (``residual_norm``).  Everything runs in libnnunet_hip.so on the current stream of the tensors'
-device, forward only; float32, float16 and bfloat16 tensors with a contiguous last axis and any
-other strides.  No reference counterpart.
+device, forward only (a gradient asked of a result raises ``ContractError``; a selection has
+none); float32, float16 and bfloat16 tensors with a contiguous last axis and any other strides.
+No reference counterpart.
 """
 
 from __future__ import annotations
@@ -145,6 +146,28 @@ def _launch(device: torch.device, entry: str, *arguments) -> None:
         _native.check(status, entry)
 
 
+class _ForwardOnly(torch.autograd.Function):
+    """Results whose gradient is refused rather than lost."""
+
+    @staticmethod
+    def forward(ctx, name, results, *inputs):
+        ctx.name = name
+        return results
+
+    @staticmethod
+    def backward(ctx, *gradients):
+        raise ContractError(f"{ctx.name} is forward only and has no gradient")
+
+
+def _gradient_asked(*tensors: torch.Tensor | None) -> bool:
+    return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
+
+
+def _no_gradient_into(name: str, *tensors: torch.Tensor | None) -> None:
+    if _gradient_asked(*tensors):
+        raise ContractError(f"{name} is forward only and writes no results into place where a gradient is kept")
+
+
 # ---- rotary positions -----------------------------------------------------------------
 
 
@@ -220,11 +243,12 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
         yq = torch.empty_like(q, memory_format=torch.contiguous_format)
         yk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
+        _no_gradient_into("rotate", q, k, *out)
         yq, yk = out
     if config:
         _launch(q.device, "nnx_rotary", config, q.data_ptr(), _address(k), positions.data_ptr(),
                 plan.steps.data_ptr(), plan.axes.data_ptr(), yq.data_ptr(), _address(yk))
-    return yq, yk
+    return _ForwardOnly.apply("rotate", (yq, yk), q, k) if _gradient_asked(q, k) else (yq, yk)
 
 
 def _contiguous_strides(shape: torch.Size) -> tuple[int, int, int]:
@@ -318,6 +342,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, *, kind: str =
     if config:
         _launch(x.device, "nnx_residual_norm", config, x.data_ptr(), _address(residual), _address(gate),
                 *[None if v is None else v.data_ptr() for v in vectors], total.data_ptr(), _address(y))
+    if _gradient_asked(x, residual, gate, *vectors):
+        return _ForwardOnly.apply("residual_norm", (total, y), x, residual, gate, *vectors)
     return total, y
 
 
@@ -517,7 +543,9 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torc
     if known is None:
         known = _remember(key, _attention_config(q, k, v, ids, block, scale, causal, starts, lengths, key_mask, out))
     config, size = known
-    if out is None:
+    if out is not None:
+        _no_gradient_into("block_attention", q, k, v, out)
+    else:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if config:
         work = torch.empty(size, dtype=torch.uint8, device=q.device)
@@ -526,7 +554,7 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torc
                 work.data_ptr(), size)
     elif out.numel():
         out.zero_()
-    return out
+    return _ForwardOnly.apply("block_attention", (out,), q, k, v)[0] if _gradient_asked(q, k, v) else out
 
 
 def _attention_config(q, k, v, ids, block, scale, causal, starts, lengths, key_mask, out):

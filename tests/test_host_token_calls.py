@@ -162,3 +162,38 @@ def test_positions_of_too_few_axes(launches):
         with pytest.raises(ContractError, match="axes"):
             tokens.rotate(q, None, torch.zeros(4, axes, dtype=torch.int32), plan)
     assert len(launches) == 5
+
+
+@pytest.mark.parametrize("call", [
+    lambda x, w: tokens.rotate(x, None, torch.zeros(4, 1, dtype=torch.int32), tokens.rotary_plan(16, device="cpu"))[0],
+    lambda x, w: tokens.residual_norm(x, None, pre=(w, None))[1],
+    lambda x, w: tokens.residual_norm(torch.zeros(3, 16), None, post=(None, w))[0],
+    lambda x, w: tokens.residual_norm(torch.zeros_like(x), torch.zeros_like(x), gate=x)[0],
+    lambda x, w: tokens.block_attention(torch.zeros_like(x), x, torch.zeros_like(x), torch.zeros(1, 4, 2, 1, dtype=torch.int32), 16),
+    lambda x, w: tokens.sparse_attention(x, torch.zeros_like(x), torch.zeros_like(x), 16, 1)[0]])
+def test_a_gradient_that_is_asked_for_is_refused(launches, call):
+    """Forward only: results of inputs that require a gradient are there, but say so in the backward pass
+    instead of losing it."""
+    x, w = torch.zeros(1, 4, 2, 16, requires_grad=True), torch.zeros(16, requires_grad=True)
+    y = call(x, w)
+    with pytest.raises(ContractError, match="forward only"):
+        (y + x.sum() + w.sum()).sum().backward()
+    with torch.no_grad():
+        assert not call(x, w).requires_grad
+    assert not call(x.detach(), w.detach()).requires_grad
+
+
+def test_no_results_into_place_where_a_gradient_is_kept(launches):
+    q = torch.zeros(1, 4, 2, 16, requires_grad=True)
+    plan, positions = tokens.rotary_plan(16, device="cpu"), torch.zeros(4, 1, dtype=torch.int32)
+    ids, out = torch.zeros(1, 4, 2, 1, dtype=torch.int32), torch.zeros(1, 4, 2, 16)
+    for call in (lambda: tokens.rotate(q, None, positions, plan, out=(q, None)),
+                 lambda: tokens.rotate(out, None, positions, plan, out=(q, None)),
+                 lambda: tokens.rotate(q, None, positions, plan, out=(out, None)),
+                 lambda: tokens.block_attention(q, out, out, ids, 16, out=out)):
+        with pytest.raises(ContractError, match="forward only"):
+            call()
+    assert not launches
+    with torch.no_grad():
+        assert tokens.rotate(q, None, positions, plan, out=(q, None))[0] is q
+    assert len(launches) == 1
