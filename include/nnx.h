@@ -521,8 +521,9 @@ int nnx_sw_fold_finalize(const void* d_total, int num_classes, int64_t voxels, i
  * or (x[2i], x[2i + 1]) when `interleaved`; it is turned by position[pair_axes[i]] * steps[i]
  * turns, with steps in units of 2^-64 turns, so the product's low 64 bits are the exact
  * fraction of a turn at any position: (a, b) -> amplitude * (a c - b s, b c + a s), s negated
- * when `inverse`.  A pair axis outside [0, axes) counts as the nearest.  Elements from rotary_dim
- * on are copied.  y may be x itself (same pointer and strides). */
+ * when `inverse` (the transpose; it undoes the turn where amplitude is 1).  A pair axis outside
+ * [0, axes) counts as the nearest.  Elements from rotary_dim on are copied.  y may be x itself
+ * (same pointer and strides). */
 typedef struct nnx_rotary_config {
   int type;
   int batch, tokens;

@@ -231,7 +231,9 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
 
     ``positions`` is int32 (tokens, axes) or (batch, tokens, axes).  ``layout`` pairs element i
     with i + rotary_dim / 2 ("half") or 2i with 2i + 1 ("interleaved"); elements past the plan's
-    pairs are copied.  ``inverse`` turns back, which is also the gradient of the forward turn.
+    pairs are copied.  ``inverse`` turns by the opposite angles, the amplitude included: it is the
+    gradient of the forward turn, and undoes it where the amplitude is 1.  A scaled turn is undone with
+    ``plan._replace(amplitude=1 / plan.amplitude)``.
     ``out`` may hold the results, ``(q, k)`` itself to rotate in place."""
     amplitude, inverse = _number("plan.amplitude", plan.amplitude), _flag("inverse", inverse)
     key = ("rotate", _signature(q, k, positions, plan.steps, plan.axes, *(out or (None,))), amplitude,

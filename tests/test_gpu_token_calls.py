@@ -26,3 +26,17 @@ def test_residual_norm_of_views_with_single_elements(device, cut):
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     assert torch.equal(tokens.residual_norm(x, residual)[0], residual + x)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_a_scaled_turn_is_undone(device, layout):
+    """By the opposite turn under the amplitude's reciprocal.  Each turn errs by 2e-6 of a pair's size."""
+    x = torch.randn(1, 50, 3, 96, generator=_gen(3)).cuda()
+    positions = torch.randint(0, 1 << 20, (50, 1), generator=_gen(4), dtype=torch.int32).cuda()
+    plan = tokens.rotary_plan(96, scaling="ramp", factor=8.0)
+    turned, _ = tokens.rotate(x, None, positions, plan, layout=layout)
+    back, _ = tokens.rotate(turned, None, positions, plan._replace(amplitude=1 / plan.amplitude), layout=layout, inverse=True)
+    assert plan.amplitude > 1.2
+    assert float((back - x).abs().max()) <= 4e-6 * float(x.abs().max()) * 2**0.5
+    again, _ = tokens.rotate(turned, None, positions, plan, layout=layout, inverse=True)
+    assert float((again - plan.amplitude**2 * x).abs().max()) <= 4e-6 * plan.amplitude**2 * float(x.abs().max()) * 2**0.5
