@@ -615,9 +615,10 @@ int nnx_block_summarize(const nnx_block_config* config, const void* d_k, const i
  * heads sharing the key head of (float(codes . codes) * m) * scale, at most the largest finite
  * value in magnitude.  Kept are the `first` leading blocks and the `local` ones ending at the
  * query's own, then the highest scores, equal ones by the lower index; blocks without valid keys
- * (scale < 0) never, nor blocks behind a causal query's own.  d_codes must be 8-byte aligned, a
- * workspace 16-byte; a workspace of 0 bytes may be null;
- * the workspace query answers 0 for what the entry refuses, too. */
+ * (scale < 0) never, nor blocks behind a causal query's own.  A causal query's own block has the
+ * score of all its valid keys, later ones too; with local >= 1 it is kept whatever they are.
+ * d_codes must be 8-byte aligned, a workspace 16-byte; a workspace of 0 bytes may be null; the
+ * workspace query answers 0 for what the entry refuses, too. */
 size_t nnx_block_select_workspace(const nnx_block_config* config);
 int nnx_block_select(const nnx_block_config* config, const void* d_q, const int8_t* d_codes,
                      const float* d_scales, const int32_t* d_start, int32_t* d_ids,

@@ -490,7 +490,9 @@ def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int,
     position is ``start``, an int or int32 (batch,), plus its index), and the best by the largest
     product of the summary with the query heads that share the key head; equal scores go to the
     lower index.  The scores are formed in whole numbers, so they do not depend on how the work is
-    split.  ``causal`` leaves out the blocks behind the query's own."""
+    split.  ``causal`` leaves out the blocks behind the query's own.  A block's score is of all its
+    valid keys, so with ``local`` 0 a causal query's own block is kept or not by keys behind the query
+    too; with ``local`` 1 or more it is kept always, and no later key shows."""
     starts, at = _split_start(start)
     block, keep, causal = _whole("block", block), _whole("keep", keep), _flag("causal", causal)
     first, local = _whole("first", first), _whole("local", local)

@@ -40,3 +40,28 @@ def test_a_scaled_turn_is_undone(device, layout):
     assert float((back - x).abs().max()) <= 4e-6 * float(x.abs().max()) * 2**0.5
     again, _ = tokens.rotate(turned, None, positions, plan, layout=layout, inverse=True)
     assert float((again - plan.amplitude**2 * x).abs().max()) <= 4e-6 * plan.amplitude**2 * float(x.abs().max()) * 2**0.5
+
+
+@pytest.mark.parametrize("block", [16, 128])
+def test_a_causal_selection_does_not_see_later_keys(device, block):
+    """With the query's own block kept for every query, what later keys hold changes neither the kept blocks
+    nor the result."""
+    k, v = (torch.randn(1, 700, 2, 32, generator=_gen(seed)).cuda() for seed in (5, 6))
+    q = torch.randn(1, 700, 4, 32, generator=_gen(7)).cuda()
+    want, ids = tokens.sparse_attention(q, k, v, block, 3, causal=True, local=1)
+    for at in (1, 130, 255, 256, 500):
+        later = k.clone()
+        later[:, at:] = torch.randn(1, 700 - at, 2, 32, generator=_gen(at)).cuda() * 5
+        got, again = tokens.sparse_attention(q, later, v, block, 3, causal=True, local=1)
+        assert torch.equal(again[:, :at], ids[:, :at])
+        # the same operations on the same numbers: the order of rows in a tile does not show
+        assert torch.equal(got[:, :at], want[:, :at])
+
+
+def test_one_position_for_all_items_and_each_its_own(device):
+    q, k, v = (torch.randn(2, n, 2, 16, generator=_gen(n)).cuda() for n in (6, 90, 90))
+    for start in (0, 7, 77):
+        each = torch.full((2,), start, dtype=torch.int32, device="cuda")
+        for a, b in zip(tokens.sparse_attention(q, k, v, 16, 2, causal=True, start=start),
+                        tokens.sparse_attention(q, k, v, 16, 2, causal=True, start=each)):
+            assert torch.equal(a, b)
