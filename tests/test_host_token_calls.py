@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import itertools
+import threading
 
 import numpy as np
 import pytest
@@ -197,3 +198,19 @@ def test_no_results_into_place_where_a_gradient_is_kept(launches):
     with torch.no_grad():
         assert tokens.rotate(q, None, positions, plan, out=(q, None))[0] is q
     assert len(launches) == 1
+
+
+def test_threads_that_share_what_has_been_checked(launches):
+    """Eight threads with more signatures than are remembered: every call is told its own shape."""
+    def work(seed):
+        for i in range(400):
+            n = 1 + (seed * 400 + i) % 1500
+            tokens.residual_norm(torch.zeros(n, 4), None)
+
+    threads = [threading.Thread(target=work, args=(seed,)) for seed in range(8)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert sorted(config.rows for _, config, _ in launches) == sorted(1 + n % 1500 for n in range(3200))
+    assert len(tokens._checked) <= 1024 + 8
