@@ -772,6 +772,12 @@ constexpr int64_t kListPairs = (int64_t)1 << 27;
 // Pairs go one by one up to so many, and so many bytes of keys and values.  One by one against by block
 // (lists and partials): 1280 of 16 KiB 13 us and 16 + 15, 5120 28 and 16 + 16, 8192 of 32 KiB 71 and
 // 19 + 21; 19200 of 4 KiB 45 and 25 + 30, 40000 of 1 KiB 67 and 25 + 24.
+// More than that go by block where there are more of them than blocks that they may keep (of every item
+// and key head): the sums over the blocks' totals cost 1 us a thousand, and a block that few pairs keep is
+// staged for little.  A whole call, one by one against by block: 32768 pairs over 2097152 blocks of 4 KiB
+// 80 us and 1964, over 1048576 79 and 1079; 16384 over 262144 of 32 KiB 262 and 526, over 32768 246 and
+// 282; 32768 over 32768 505 and 424, over 8192 454 and 161; 65536 over 4096 858 and 97; of 8 KiB 32768
+// over 16384 90 and 131, 65536 over 16384 167 and 145.
 constexpr double kDirectPairs = 20000, kDirectBytes = 80e6;
 
 struct AttentionPlan {
@@ -794,7 +800,8 @@ AttentionPlan make_plan(const nnx_block_config& c) {
   require(spans < (int64_t)1 << 31, "block attention: too many queries and key heads");
   p.spans = (int)spans;
   const double pairs = (double)c.batch * c.kv_heads * c.queries * c.keep;
-  p.by_block = pairs > kDirectPairs || pairs * c.block * c.head_dim * 2 * type_bytes(c.type) > kDirectBytes;
+  p.by_block = pairs > (double)c.batch * c.kv_heads * blocks &&
+               (pairs > kDirectPairs || pairs * c.block * c.head_dim * 2 * type_bytes(c.type) > kDirectBytes);
   p.at_once = (int)std::max<int64_t>(1, std::min(spans, fit / p.nt));
   // counts and tiles are 32-bit, and spans a grid axis
   const int64_t most = std::min<int64_t>({spans, 65535, ((int64_t)1 << 30) / blocks, kListPairs / ((int64_t)p.nt * c.keep)});

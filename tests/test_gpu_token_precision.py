@@ -152,3 +152,22 @@ def test_a_query_without_keys_gets_zeros_whatever_it_holds(device, dtype, querie
     for args in (dict(key_mask=mask), dict(lengths=torch.zeros(1, dtype=torch.int32, device="cuda")),
                  dict(key_mask=mask, causal=True, start=3)):
         assert not tokens.block_attention(q, k, v, ids, 32, **args).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_items_of_few_queries(device, dtype):
+    """Single tokens of many items: more pairs than blocks of one item, fewer than all blocks, in more than
+    one launch."""
+    batch, keys, heads, kv_heads, dim, block, keep = 40, 300 * 16, 64, 4, 128, 16, 130
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    q, k, v = (torch.randn(batch, n, h, dim, generator=gen, device="cuda").to(dtype)
+               for n, h in ((1, heads), (keys, kv_heads), (keys, kv_heads)))
+    lengths = torch.arange(batch, dtype=torch.int32, device="cuda") * (keys // batch) + 5
+    ids = torch.rand(batch, 1, kv_heads, 300, generator=gen, device="cuda").topk(keep).indices.sort(-1).values.to(torch.int32)
+    got = tokens.block_attention(q, k, v, ids, block, lengths=lengths)
+    for item in (0, 1, 19, 20, 21, 39):
+        one = slice(item, item + 1)
+        valid = np.arange(keys)[None] < int(lengths[item])
+        see = ot.seen(ids[one].cpu().numpy(), keys, block, valid)
+        want, size = _attention(q[one], k[one], v[one], see, dim**-0.5)
+        assert (np.abs(_f64(got[one]) - want) <= (3 * U[dtype] + 5e-4) * size).all()
