@@ -506,10 +506,20 @@ __global__ __launch_bounds__(256) void residual_norm_narrow_kernel(NormArgs a, i
     if (c < a.channels) ((T*)a.y)[row * a.ys + c] = from_float<T>(u[c]);
 }
 
-// The fewest lanes that hold a row in at most 24 channels a thread, the fewest runs a thread that do:
-// 16 lanes put four rows in a wave and keep its sums within 16 lanes (262144 rows of 320: 161 us
-// against 215 with a wave a row, of 64: 47 against 162), but leave few rows too few waves to hide
-// their loads (4096 of 320: 10.4 us against 7.7; even at 8192).
+// The fewest lanes that hold a row in at most 24 channels a thread, the fewest runs a thread that do.
+// 16 lanes put four rows in a wave and keep its sums within 16 lanes, but leave few rows too few waves
+// to hide their loads.  16 lanes against 64, in us (one norm; both):
+//   bf16, bf16 residual, 256 channels   4096 rows 3.9 and 4.2   8192 4.9 and 6.2    262144 99, 104 and 128, 175
+//                        320            4.7 and 4.4             6.0 and 6.7         120, 139 and 137, 184
+//                        384            4.8 and 4.5             6.3 and 6.6         146, 153 and 150, 194
+//   bf16, float32        256            4.4 and 4.5             6.1 and 6.9         142, 154 and 158, 196
+//                        320            5.2 and 4.8             7.6 and 7.9         190, 198 and 186, 210
+//                        384            5.5 and 5.1             8.4 and 8.7         223, 230 and 216, 237
+//   float32              256            5.2 and 5.2             7.2 and 7.9         193, 194 and 199, 229
+//                        320            6.3 and 5.6             9.5 and 9.5         282, 268 and 241, 274
+//                        384            6.7 and 6.0             10.5 and 10.5       327, 304 and 278, 298
+// so from 8192 rows on, up to 384 channels, of float32 up to 256; fewer channels gain more (136: 262144
+// rows 63 and 116).
 constexpr int64_t kManyRows = 8192;
 
 template <class T, class R>
@@ -535,7 +545,8 @@ void residual_norm_launch(const NormArgs& a, int rms, hipStream_t st) {
     if (need <= 2) return go(g, two);
     go(g, three);
   };
-  if (a.channels <= 128 || (a.channels <= 16 * 24 && a.rows >= kManyRows)) return lanes(integral_constant<int, 16>{});
+  constexpr int kMost = sizeof(T) == 4 ? 256 : 16 * 24;
+  if (a.channels <= 128 || (a.channels <= kMost && a.rows >= kManyRows)) return lanes(integral_constant<int, 16>{});
   if (a.channels <= 64 * 24) return lanes(integral_constant<int, 64>{});
   if (a.channels <= 256 * 24) return lanes(integral_constant<int, 256>{});
   go(integral_constant<int, 1024>{}, two);

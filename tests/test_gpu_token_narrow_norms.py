@@ -1,5 +1,5 @@
 """Norms over rows of few channels: fewer than a wide access holds, and just above, where nearly every
-access is moved back to end with its row.
+access is moved back to end with its row; and over many rows, which fewer lanes share.
 
 Tolerances: a row is a few float32 sums (1e-5 of its largest result) and one rounding.  A LayerNorm of few
 channels can divide by a small deviation: with eps 0.25 its square root is 0.5 at least, so an error of
@@ -49,3 +49,19 @@ def test_one_channel_has_no_deviation(device, dtype):
     weight, bias = torch.full((1,), 3.0, device="cuda"), torch.full((1,), -0.5, device="cuda")
     total, y = tokens.residual_norm(x, x, post=(weight, bias), pre=(weight, bias), eps=1e-5)
     assert torch.equal(total, (x.float() - 0.5).to(dtype)) and (y == -0.5).all()
+
+
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("channels", [129, 256, 257, 320, 384, 385])
+def test_many_rows(device, channels, dtype):
+    """Rows about the 8192 from which 16 lanes take a row: each as it is among few, up to the order of sums."""
+    gen = torch.Generator().manual_seed(channels)
+    x, residual = (torch.randn(8200, channels, generator=gen).to(dtype).cuda() for _ in range(2))
+    affine = (torch.randn(channels, generator=gen).cuda(), torch.randn(channels, generator=gen).cuda())
+    total, y = tokens.residual_norm(x, residual, post=affine, pre=affine, eps=1e-3)
+    for rows in (slice(0, 70), slice(8130, 8200)):
+        want, want_y = ot.residual_norm(_f64(x[rows]), _f64(residual[rows]), post=[_f64(a) for a in affine],
+                                        pre=[_f64(a) for a in affine], eps=1e-3)
+        for got, expected in ((total[rows], want), (y[rows], want_y)):
+            size = np.abs(expected).max(-1, keepdims=True)
+            assert (np.abs(_f64(got) - expected) <= U[dtype] * np.abs(expected) + 1e-5 * size).all()
