@@ -891,10 +891,16 @@ void block_select(const nnx_block_config& c, const void* q, const int8_t* codes,
     }
     return;
   }
-  // As many queries a workgroup as the products take.  Few workgroups
-  // take twice the waves; up to 128 blocks give work to 4 (40960 rows of 64: 23 us against 26 with 8).
+  // As many queries a workgroup as the products take, and waves by how many workgroups a CU has.  16 waves
+  // while CUs would idle: of 64 blocks 190 workgroups 6.0 us against 6.5 with 8 waves, 375 8.8 and 7.6; of
+  // 400 8.3 and 10.1, 12.2 and 11.6; of 1000 10.6 and 13.3, 17.0 and 16.3; of 2000 14.7 and 19.3, 26.8 and
+  // 35.6, where a workgroup's LDS leaves room for one alone.  4 waves for up to 128 blocks where there are
+  // workgroups enough: of 64 blocks 5120 workgroups 29.9 against 35.4 with 8, 1024 14.7 and 15.9, 375 8.6
+  // and 7.6; of 128 37.7 and 43.7, 19.2 and 18.1; of 256 49.6 and 54.2, 23.5 and 23.0; of 512 74.5 and
+  // 66.4, 39.7 and 29.4.
   const dim3 grid((unsigned)ceil_div(c.queries, plan.rows), c.kv_heads, c.batch);
-  const int threads = (double)grid.x * grid.y * grid.z < 2 * compute_units() ? 1024 : plan.chunks <= 2 ? 256 : 512;
+  const double each = (double)grid.x * grid.y * grid.z / compute_units();
+  const int threads = each < (plan.chunks > 16 ? 2 : 1) ? 1024 : plan.chunks <= 2 && each >= 2 ? 256 : 512;
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto k) {
