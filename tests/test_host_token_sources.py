@@ -52,3 +52,10 @@ def test_lanes_that_exchange_through_lds():
     packing = _body((CSRC / "nnx_blocks.hip").read_text(), "if (over <= room) {")
     write, read = packing.index("spare[to] = y"), packing.index("in ? spare[")
     assert packing.index("wave_sync()") < write < packing.rindex("wave_sync()") < read
+
+
+@pytest.mark.parametrize("name", ["block_select_workspace", "block_attention_workspace"])
+def test_no_exception_leaves_a_size_query(name):
+    """Refusals are built as strings, which may fail to be allocated: everything is caught."""
+    body = _body((CSRC / "nnx_blocks.hip").read_text(), f"size_t {name}(")
+    assert "catch (...)" in body
