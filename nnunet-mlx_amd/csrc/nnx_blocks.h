@@ -40,9 +40,9 @@ __device__ __forceinline__ int64_t item_start(const BlockArgs& a, int b) {
 // The queries of each key head of each item are cut into `splits` spans of `nt`; span v = (item *
 // kv_heads + key head) * splits + split.  A launch covers spans [span0, span0 + spans).  Row =
 // (span, query of the span, head of the group), counted from span0; every row has `keep`
-// partials, one a kept block: `dim` values (Partial<T>) and (log2 of the sum of its weights, factor
-// of the values over that sum; negative where the block holds values that are not finite, which count
-// as 0 in the partial).
+// partials, one a kept block: `dim` values (Partial<T>), sums over the block's keys with weights 2^(x - m),
+// and (m, l), l the sum of the weights.  A negative l: the block holds values that are not finite, which
+// count as 0 in the partial.
 struct ChunkArgs {
   BlockArgs a;
   const void *q, *k, *v;
@@ -58,8 +58,8 @@ struct ChunkArgs {
 
 // What the values of a partial result are held in.  bfloat16's are float16 times a power of two that
 // puts the row's largest below 2^15: 11 bits for every channel down to 2^-29 of it, where the result
-// keeps 8, so an error of 2^-12 of a channel's own partials.  float16's result keeps 11 itself, and its
-// partials are float32.
+// keeps 8, so an error of 2^-12 of a channel's own partials; the power's exponent is kept in the last 8
+// bits of l, which leaves l 16.  float16's result keeps 11 bits itself, and its partials are float32.
 template <class T>
 struct PartialOf {
   using type = float;
@@ -70,6 +70,8 @@ struct PartialOf<bf16> {
 };
 template <class T>
 using Partial = typename PartialOf<T>::type;
+
+constexpr uint32_t kExponentBits = 255, kExponentZero = 128;
 
 inline int partial_bytes(int type) { return type == NNX_TYPE_BF16 ? 2 : 4; }
 

@@ -654,7 +654,7 @@ __device__ __forceinline__ void add_odd_values(const ChunkArgs& c, const T* v, S
   }
 }
 
-// out = sum_s w_s O_s / sum_s w_s with w_s = 2^(log2 sum_s - largest), O_s a partial under its
+// out = sum_s w_s O_s / sum_s w_s l_s with w_s = 2^(m_s - largest), O_s a partial under its
 // factor, in the order of the slots.  A workgroup forms the weights of its rows together, then dim / 8
 // lanes a row add up (`share` groups of them a row, each every share-th partial, where rows are few
 // or have many).  Bound by its reads: 143 MB of partials in 26 us (5.5 TB/s, mostly from the
@@ -664,7 +664,8 @@ constexpr int kJoinWeights = 4096;
 template <class T>
 __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out, int share, int each) {
   using P = Partial<T>;
-  // by row and slot the weight of the sum and the factor of the values; then the shares' sums
+  const float2 nothing = make_float2(-INFINITY, __uint_as_float(kExponentZero));
+  // by row and slot (m, l); then the shares' sums
   extern __shared__ float2 weight[];
   float(*sums)[9] = (float(*)[9])(weight + each * c.a.keep);
   const BlockArgs& a = c.a;
@@ -690,7 +691,7 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
     if (t < s.queries)
       j = c.ids[(((int64_t)s.b * a.queries + s.t0 + t) * a.kv_heads + s.g) * a.keep + slot];
     weight[i] = (unsigned)j < (unsigned)a.blocks ? c.meta[partial_of(row0 + r) + (int64_t)slot * a.group]
-                                                 : make_float2(-INFINITY, 0.f);
+                                                 : nothing;
   }
   const int lanes = a.dim / 8, sub = threadIdx.x / lanes, u = threadIdx.x - sub * lanes;
   const int own = sub / share, part0 = sub - own * share;
@@ -719,11 +720,17 @@ __global__ __launch_bounds__(256) void join_partials_kernel(ChunkArgs c, T* out,
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
         const int s = s0 + i * share;
-        const float2 m = s < a.keep ? w[s] : make_float2(-INFINITY, 0.f);
-        const float ws = __builtin_amdgcn_exp2f(m.x - top), f = ws * fabsf(m.y);
-        odd |= m.y < 0.f;
+        const float2 m = s < a.keep ? w[s] : nothing;
+        const float ws = __builtin_amdgcn_exp2f(m.x - top);
         const bool written = !(m.x == -INFINITY);
-        l += ws;
+        float f = ws, sum = fabsf(m.y);
+        if constexpr (sizeof(P) == 2) {
+          const uint32_t bits = __float_as_uint(sum);
+          f *= __uint_as_float(((bits & kExponentBits) + 127 - kExponentZero) << 23);
+          sum = __uint_as_float(bits & ~kExponentBits);
+        }
+        odd |= m.y < 0.f;
+        l = fmaf(ws, sum, l);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           o[e] = fmaf(f, written ? to_float(x[i].v[e]) : 0.f, o[e]);

@@ -151,7 +151,7 @@ struct RowWriter {
 };
 
 // The partial softmax of rows over one block: m = max x up to a constant, l = sum 2^(x - m), O = sum
-// 2^(x - m) v / l, of which log2 l + m and O are kept (x the scores in units of log 2; weights, sums and O
+// 2^(x - m) v (x the scores in units of log 2; weights, sums and O
 // in float32).  In 16-bit types a weight is two operands of the second product, its rounded value and the
 // rest: 16 bits of it for bfloat16, 22 for float16, so that the result's own rounding is the only one that
 // shows (1.3 times the error with one operand; 329 us of partials against 314 for 32768 queries of 32 blocks).
@@ -297,9 +297,8 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
       }
   }
   // Registers 4i .. 4i + 3 of o[dt] are channels 32 dt + 8 i + 4 half + 0..3 of the lane's row.
-  const float sum = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);  // 0: nothing seen; NaN stays
   before_stores();
-  float2 meta = make_float2(l == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(l), sum);
+  float2 meta = make_float2(l == 0.f ? -INFINITY : top, l);  // 0: nothing seen; NaN stays
   if constexpr (sizeof(Partial<T>) == 2) {
     // The power of two: of the largest magnitude, at least 2^-96, so that both factors are normal.  NaN, of
     // the weights, hides from the largest and stays NaN.
@@ -311,7 +310,8 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
     const float2 bh = both_halves(big);
     const int exponent = max(__builtin_amdgcn_frexp_expf(fmaxf(bh.x, bh.y)), -96) - 15;
     const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
-    meta.y *= __uint_as_float((uint32_t)(127 + exponent) << 23);
+    meta.y = __uint_as_float(((__float_as_uint(l) + (kExponentBits + 1) / 2) & ~kExponentBits) |
+                             (uint32_t)(exponent + (int)kExponentZero));
     const uint32_t bytes = c.a.dim * 2;
     const RowWriter writer{out_lds, part, partial == kNowhere ? kNowhere : partial * bytes, bytes};
 #pragma unroll

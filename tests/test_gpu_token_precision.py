@@ -171,3 +171,24 @@ def test_many_items_of_few_queries(device, dtype):
         see = ot.seen(ids[one].cpu().numpy(), keys, block, valid)
         want, size = _attention(q[one], k[one], v[one], see, dim**-0.5)
         assert (np.abs(_f64(got[one]) - want) <= (3 * U[dtype] + 5e-4) * size).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", [3, 800])
+def test_blocks_that_count_alike_at_any_logit(device, dtype, queries):
+    """Equal keys under logits of tens of thousands: every key counts the same however many its block has, so
+    the result is the mean of the values seen.  A sum of a block's, then the blocks', and a division err by at
+    most one unit of 2^-24 a term (bfloat16's l and partials by 2^-16 and 2^-12), the result by U."""
+    block, blocks, keep = 32, 9, 6
+    keys = blocks * block - 11
+    _, _, v = _inputs(queries, dtype, queries, keys)
+    k = torch.ones(1, keys, 2, 64, dtype=dtype, device="cuda")
+    q = (1.0 + torch.arange(queries, device="cuda").remainder(100) / 128).to(dtype)[None, :, None, None].expand(1, queries, 4, 64).contiguous()
+    mask = torch.rand(1, keys, generator=torch.Generator().manual_seed(8)) < 0.6
+    ids = _ids(queries, 2, blocks, keep, 9)
+    see = ot.seen(ids.cpu().numpy(), keys, block, mask.numpy())
+    for scale in (1e-3, 777.7, -7919.0):
+        got = _f64(tokens.block_attention(q, k, v, ids, block, scale=scale, key_mask=mask.cuda()))
+        want, size = _attention(torch.zeros_like(q), k, v, see, 1.0)
+        bound = U[dtype] + (block + keep + 4) * 2.0**-24 + (2.0**-12 + 2.0**-16 if dtype == torch.bfloat16 else 0)
+        assert (np.abs(got - want) <= bound * size).all()
