@@ -194,19 +194,24 @@ __device__ __forceinline__ void attend_rows(const ChunkArgs& c, const T* lk, con
       for (int kt = 0; kt < G::KT; ++kt)
         acc[kt] = mfma(*(const Frag<T>*)(lk + G::at(kt * 32 + col, 2 * s + half)), qf[s], acc[kt]);
   } else {
+    // 32 channels at a time: a sum of 128 in one chain errs by twice as much
 #pragma unroll
-    for (int s = 0; s < DP / 8; ++s) {
-      Vec<float, 4> qf;
-      __builtin_memcpy(&qf, &q.v[s], 16);
+    for (int kt = 0; kt < G::KT; ++kt)
 #pragma unroll
-      for (int kt = 0; kt < G::KT; ++kt) {
-        const float4 kf = *(const float4*)(lk + G::at(kt * 32 + col, 2 * s + half));
-        acc[kt] = mfma(kf.x, qf.v[0], acc[kt]);
-        acc[kt] = mfma(kf.y, qf.v[1], acc[kt]);
-        acc[kt] = mfma(kf.z, qf.v[2], acc[kt]);
-        acc[kt] = mfma(kf.w, qf.v[3], acc[kt]);
+      for (int s0 = 0; s0 < DP / 8; s0 += 4) {
+        f32x16 part = {};
+#pragma unroll
+        for (int s = s0; s < s0 + 4; ++s) {
+          Vec<float, 4> qf;
+          __builtin_memcpy(&qf, &q.v[s], 16);
+          const float4 kf = *(const float4*)(lk + G::at(kt * 32 + col, 2 * s + half));
+          part = mfma(kf.x, qf.v[0], part);
+          part = mfma(kf.y, qf.v[1], part);
+          part = mfma(kf.z, qf.v[2], part);
+          part = mfma(kf.w, qf.v[3], part);
+        }
+        acc[kt] = s0 ? acc[kt] + part : part;
       }
-    }
   }
   after_scores();
   if (!block.full) {

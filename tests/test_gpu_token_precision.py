@@ -192,3 +192,25 @@ def test_blocks_that_count_alike_at_any_logit(device, dtype, queries):
         want, size = _attention(torch.zeros_like(q), k, v, see, 1.0)
         bound = U[dtype] + (block + keep + 4) * 2.0**-24 + (2.0**-12 + 2.0**-16 if dtype == torch.bfloat16 else 0)
         assert (np.abs(got - want) <= bound * size).all()
+
+
+@pytest.mark.parametrize("dim", [96, 128])
+@pytest.mark.parametrize("queries", [2, 700])
+def test_logits_whose_channels_cancel(device, dim, queries):
+    """float32 logits are summed 32 channels at a time: what small channels add up to is not lost to large ones
+    that cancel in the end.  The small ones, 1 or 3 each, add up to even numbers, which 2^24 can hold beside
+    it, so the logits are exact."""
+    keys, block = 200, 64
+    gen = torch.Generator().manual_seed(dim)
+    q, k = torch.zeros(1, queries, 4, dim), torch.zeros(1, keys, 2, dim)
+    q[..., 0], q[..., dim - 1], k[..., 0], k[..., dim - 1] = 2.0**12, -(2.0**12), 2.0**12, 2.0**12
+    q[..., 32:64] = 1.0 + 2 * torch.randint(0, 2, (1, queries, 4, 1), generator=gen)
+    k[..., 32:63] = torch.randint(0, 2, (1, keys, 2, 31), generator=gen).float()
+    k[..., 63] = k[..., 32:63].sum(-1) % 2
+    v = torch.randn(1, keys, 2, dim, generator=gen)
+    ids = _ids(queries, 2, 4, 3, 10)
+    got = _f64(tokens.block_attention(q.cuda(), k.cuda(), v.cuda(), ids, block, scale=0.25))
+    see = ot.seen(ids.cpu().numpy(), keys, block, np.ones((1, keys), bool))
+    want, size = _attention(q, k, v, see, 0.25)
+    # exponents of at most 24 log2(e), each a product rounded once, weights and their sums
+    assert (np.abs(got - want) <= (64 + 70) * 2.0**-24 * size).all()
