@@ -117,14 +117,14 @@ def _address(tensor: torch.Tensor | None) -> int | None:
     return None if tensor is None else tensor.data_ptr()
 
 
-# What calls have been checked and how the library is told of them, by the shapes, strides, types and
-# devices of their tensors and their other arguments (never by what the tensors hold or where):
+# What calls have been checked and how the library is told of them, by the shapes, strides, types, devices
+# and asked-for gradients of their tensors and their other arguments (never by what the tensors hold or where):
 # checking again would be half of what the smallest calls cost.
 _checked: dict = {}
 
 
 def _signature(*tensors: torch.Tensor | None) -> tuple:
-    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors])
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.requires_grad) for t in tensors])
 
 
 def _remember(key: tuple, value):
@@ -159,13 +159,17 @@ class _ForwardOnly(torch.autograd.Function):
         raise ContractError(f"{ctx.name} is forward only and has no gradient")
 
 
-def _gradient_asked(*tensors: torch.Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
+def _gradients(*tensors: torch.Tensor | None) -> bool:
+    return any([t is not None and t.requires_grad for t in tensors])
 
 
-def _no_gradient_into(name: str, *tensors: torch.Tensor | None) -> None:
-    if _gradient_asked(*tensors):
+def _without_gradient(name: str, results: tuple, given: bool, *inputs: torch.Tensor | None) -> tuple:
+    """The results of inputs some of which require a gradient; ``given``: written into place."""
+    if not torch.is_grad_enabled():
+        return results
+    if given:
         raise ContractError(f"{name} is forward only and writes no results into place where a gradient is kept")
+    return _ForwardOnly.apply(name, results, *inputs)
 
 
 # ---- rotary positions -----------------------------------------------------------------
@@ -235,22 +239,28 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
     gradient of the forward turn, and undoes it where the amplitude is 1.  A scaled turn is undone with
     ``plan._replace(amplitude=1 / plan.amplitude)``.
     ``out`` may hold the results, ``(q, k)`` itself to rotate in place."""
-    amplitude, inverse = _number("plan.amplitude", plan.amplitude), _flag("inverse", inverse)
+    amplitude = plan.amplitude
+    if type(amplitude) is not float or type(inverse) is not bool:
+        amplitude, inverse = _number("plan.amplitude", amplitude), _flag("inverse", inverse)
     key = ("rotate", _signature(q, k, positions, plan.steps, plan.axes, *(out or (None,))), amplitude,
            plan.position_axes, layout, inverse)
-    config = _checked.get(key)
-    if config is None:
-        config = _remember(key, _rotary_config(q, k, positions, plan, amplitude, layout, inverse, out))
+    known = _checked.get(key)
+    if known is None:
+        known = _remember(key, (_rotary_config(q, k, positions, plan, amplitude, layout, inverse, out),
+                                _gradients(q, k, *(out or ()))))
+    config, gradients = known
     if out is None:
         yq = torch.empty_like(q, memory_format=torch.contiguous_format)
         yk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
-        _no_gradient_into("rotate", q, k, *out)
         yq, yk = out
+    results = (yq, yk)
+    if gradients:
+        results = _without_gradient("rotate", results, out is not None, q, k)
     if config:
         _launch(q.device, "nnx_rotary", config, q.data_ptr(), _address(k), positions.data_ptr(),
                 plan.steps.data_ptr(), plan.axes.data_ptr(), yq.data_ptr(), _address(yk))
-    return _ForwardOnly.apply("rotate", (yq, yk), q, k) if _gradient_asked(q, k) else (yq, yk)
+    return results
 
 
 def _contiguous_strides(shape: torch.Size) -> tuple[int, int, int]:
@@ -259,6 +269,7 @@ def _contiguous_strides(shape: torch.Size) -> tuple[int, int, int]:
 
 def _rotary_config(q, k, positions, plan, amplitude, layout, inverse, out):
     """The checked configuration of a rotation, False where there is nothing to do."""
+    _number("plan.amplitude", amplitude)
     _check("q", q, 4)
     batch, tokens, heads, dim = q.shape
     rotary_dim = 2 * plan.steps.numel()
@@ -331,26 +342,30 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, *, kind: str =
     ``gate`` is like x; ``scale`` float32 (channels,).  ``post`` and ``pre`` are (weight, bias),
     float32 (channels,) or None each.  ``kind`` is "layer" or "rms"; y is the norm of r' before
     it is rounded to its dtype."""
-    residual_scale, eps = _number("residual_scale", residual_scale), _number("eps", eps)
+    if type(residual_scale) is not float or type(eps) is not float:
+        residual_scale, eps = _number("residual_scale", residual_scale), _number("eps", eps)
     vectors = (scale, *(post or (None, None)), *(pre or (None, None)))
     key = ("norm", _signature(x, residual, gate, *vectors), kind, post is None, pre is None, gate_activation,
            residual_scale, eps)
-    config = _checked.get(key)
-    if config is None:
-        config = _remember(key, _norm_config(x, residual, gate, vectors, kind, post is not None,
-                                             gate_activation, residual_scale, eps))
+    known = _checked.get(key)
+    if known is None:
+        known = _remember(key, (_norm_config(x, residual, gate, vectors, kind, post is not None, gate_activation,
+                                             residual_scale, eps), _gradients(x, residual, gate, *vectors)))
+    config, gradients = known
     total = torch.empty_like(x if residual is None else residual, memory_format=torch.contiguous_format)
     y = None if pre is None else torch.empty_like(x, memory_format=torch.contiguous_format)
+    results = (total, y)
+    if gradients:
+        results = _without_gradient("residual_norm", results, False, x, residual, gate, *vectors)
     if config:
         _launch(x.device, "nnx_residual_norm", config, x.data_ptr(), _address(residual), _address(gate),
                 *[None if v is None else v.data_ptr() for v in vectors], total.data_ptr(), _address(y))
-    if _gradient_asked(x, residual, gate, *vectors):
-        return _ForwardOnly.apply("residual_norm", (total, y), x, residual, gate, *vectors)
-    return total, y
+    return results
 
 
 def _norm_config(x, residual, gate, vectors, kind, post, gate_activation, residual_scale, eps):
     """The checked configuration of a residual norm, False where there is nothing to do."""
+    _number("residual_scale", residual_scale), _number("eps", eps)
     _check("x", x, max(1, x.dim()))
     channels = x.shape[-1]
     rows = x.numel() // channels if channels else 0
@@ -402,20 +417,16 @@ def _block_config(like: torch.Tensor, block: int, batch: int, queries: int, keys
                    like.shape[-1], block, keep, first, local, causal, 0, scale, *q, *k, *v, *out, mask_stride)
 
 
-def _split_start(start: torch.Tensor | int | None) -> tuple[torch.Tensor | None, int]:
-    """The items' positions, and one for them all."""
-    if start is None or isinstance(start, torch.Tensor):
-        return start, 0
+def _one_start(start: int) -> int:
+    """One position for all items."""
     at = _whole("start", start)
     _need(0 <= at < 1 << 40, f"start must be 0..2^40, got {at}")
-    return None, at
+    return at
 
 
 def _placed(config: _native.NnxBlockConfig, start: int) -> _native.NnxBlockConfig:
     """The checked configuration for queries from ``start`` on.  A decoder moves it at every step, so it is
     no part of what is remembered."""
-    if not start:
-        return config
     config = _native.NnxBlockConfig.from_buffer_copy(config)
     config.start = start
     return config
@@ -444,8 +455,10 @@ def summarize_blocks(k: torch.Tensor, block: int, *, lengths: torch.Tensor | Non
     ones that are seen.  ``first`` and ``count`` with ``out`` refresh those blocks of a summary
     that is kept, as after appending keys."""
     codes, scales = out or (None, None)
-    block, first = _whole("block", block), _whole("first", first)
-    count = None if count is None else _whole("count", count)
+    if type(block) is not int or type(first) is not int:
+        block, first = _whole("block", block), _whole("first", first)
+    if count is not None and type(count) is not int:
+        count = _whole("count", count)
     key = ("summarize", _signature(k, lengths, key_mask, codes, scales), block, first, count)
     known = _checked.get(key)
     if known is None:
@@ -493,9 +506,12 @@ def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int,
     split.  ``causal`` leaves out the blocks behind the query's own.  A block's score is of all its
     valid keys, so with ``local`` 0 a causal query's own block is kept or not by keys behind the query
     too; with ``local`` 1 or more it is kept always, and no later key shows."""
-    starts, at = _split_start(start)
-    block, keep, causal = _whole("block", block), _whole("keep", keep), _flag("causal", causal)
-    first, local = _whole("first", first), _whole("local", local)
+    starts, at = start, 0
+    if start is not None and not isinstance(start, torch.Tensor):
+        starts, at = None, _one_start(start)
+    if not type(block) is type(keep) is type(first) is type(local) is int or type(causal) is not bool:
+        block, keep, causal = _whole("block", block), _whole("keep", keep), _flag("causal", causal)
+        first, local = _whole("first", first), _whole("local", local)
     key = ("select", _signature(q, *summary, starts), block, keep, causal, first, local)
     known = _checked.get(key)
     if known is None:
@@ -504,7 +520,7 @@ def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int,
     ids = torch.empty((q.shape[0], q.shape[1], summary.codes.shape[1], keep), dtype=torch.int32, device=q.device)
     if config:
         work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        _launch(q.device, "nnx_block_select", _placed(config, at), q.data_ptr(), summary.codes.data_ptr(),
+        _launch(q.device, "nnx_block_select", _placed(config, at) if at else config, q.data_ptr(), summary.codes.data_ptr(),
                 summary.scales.data_ptr(), _address(starts), ids.data_ptr(), _address(work), size)
     elif ids.numel():
         ids.fill_(-1)
@@ -539,30 +555,39 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torc
 
     ``scale`` defaults to head_dim^-0.5; ``causal``, ``start``, ``lengths`` and ``key_mask`` as in
     ``select_blocks`` and ``summarize_blocks``.  A query that sees no key gets zeros."""
-    starts, at = _split_start(start)
-    block, causal = _whole("block", block), _flag("causal", causal)
-    scale = None if scale is None else _number("scale", scale)
+    starts, at = start, 0
+    if start is not None and not isinstance(start, torch.Tensor):
+        starts, at = None, _one_start(start)
+    if type(block) is not int or type(causal) is not bool:
+        block, causal = _whole("block", block), _flag("causal", causal)
+    if scale is not None and type(scale) is not float:
+        scale = _number("scale", scale)
     key = ("attention", _signature(q, k, v, ids, starts, lengths, key_mask, out), block, scale, causal)
     known = _checked.get(key)
     if known is None:
-        known = _remember(key, _attention_config(q, k, v, ids, block, scale, causal, starts, lengths, key_mask, out))
-    config, size = known
-    if out is not None:
-        _no_gradient_into("block_attention", q, k, v, out)
-    else:
+        known = _remember(key, (*_attention_config(q, k, v, ids, block, scale, causal, starts, lengths, key_mask, out),
+                                _gradients(q, k, v, out)))
+    config, size, gradients = known
+    given = out is not None
+    if not given:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    results = (out,)
+    if gradients:
+        results = _without_gradient("block_attention", results, given, q, k, v)
     if config:
         work = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _launch(q.device, "nnx_block_attention", _placed(config, at), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        _launch(q.device, "nnx_block_attention", _placed(config, at) if at else config, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 ids.data_ptr(), _address(starts), _address(lengths), _address(key_mask), out.data_ptr(),
                 work.data_ptr(), size)
     elif out.numel():
-        out.zero_()
-    return _ForwardOnly.apply("block_attention", (out,), q, k, v)[0] if _gradient_asked(q, k, v) else out
+        out.detach().zero_()
+    return results[0]
 
 
 def _attention_config(q, k, v, ids, block, scale, causal, starts, lengths, key_mask, out):
     """The checked configuration (False where there is nothing to attend to) and workspace bytes."""
+    if scale is not None:
+        _number("scale", scale)
     _check("q", q, 4)
     _check("k", k, 4, q)
     _check("v", v, 4, q)
