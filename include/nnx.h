@@ -509,9 +509,9 @@ int nnx_sw_fold_finalize(const void* d_total, int num_classes, int64_t voxels, i
  * Steps of a transformer block over the tokens of a volume (one token a cube of voxels),
  * between its plain matrix products.  No reference counterpart.  Element types are
  * NNX_TYPE_*; sums, softmax statistics and norms are held in float32 and every result is
- * rounded once to its type (bfloat16 attention holds the mean over each kept block with an error of
- * 2^-12 of every channel).  Innermost axes are contiguous, other strides (in elements) and row
- * addresses are free. */
+ * rounded once to its type (bfloat16 attention holds each kept block's share of a row to 2^-12
+ * of every channel).  Innermost axes are contiguous, other strides (in elements) are free, rows
+ * start at any element. */
 #define NNX_TYPE_F32 0
 #define NNX_TYPE_F16 1
 #define NNX_TYPE_BF16 2

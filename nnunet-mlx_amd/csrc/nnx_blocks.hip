@@ -316,7 +316,7 @@ __device__ __forceinline__ void select_row(float* score, float* spare, int chunk
 // head are taken kScoreHeads at a time (their codes in LDS) and meet in the largest score.  A
 // wave's next AHEAD times 16 blocks are on their way while it scores the ones before.
 // Bound by the issue of instructions: 163840 rows against 512 blocks of 64 channels take 150 us, the
-// vector and the scalar units busy for 71 and 73 % of it (380 and 385 instructions a row), for 84
+// vector and the scalar units busy for 72 % of it (389 and 383 instructions a row), for 84
 // million scores of which 5.2 million are kept; the codes of a key head (32 KB) come from the L2, and
 // the scores never leave the CU.  8 queries a workgroup leave half of a
 // product unused (240 us against 190), 4 or 16 waves a workgroup fill the CU less evenly than 8 (209
@@ -654,10 +654,10 @@ __device__ __forceinline__ void add_odd_values(const ChunkArgs& c, const T* v, S
   }
 }
 
-// out = sum_s w_s O_s / sum_s w_s l_s with w_s = 2^(m_s - largest), O_s a partial under its
-// factor, in the order of the slots.  A workgroup forms the weights of its rows together, then dim / 8
+// out = sum_s w_s O_s / sum_s w_s l_s with w_s = 2^(m_s - largest), O_s a partial times its power of
+// two, in the order of the slots.  A workgroup forms the weights of its rows together, then dim / 8
 // lanes a row add up (`share` groups of them a row, each every share-th partial, where rows are few
-// or have many).  Bound by its reads: 143 MB of partials in 26 us (5.5 TB/s, mostly from the
+// or have many).  Bound by its reads: 143 MB of partials in 27 us (5.3 TB/s, mostly from the
 // last-level cache), 8 partials in flight a lane.
 constexpr int kJoinWeights = 4096;
 

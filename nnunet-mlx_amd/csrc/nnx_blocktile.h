@@ -376,11 +376,12 @@ __device__ __forceinline__ int last_seen(const BlockArgs& a, int64_t at, int fir
 }
 
 // Bound by the partials' stores: 1.05 million pairs with blocks of 64 keys of 64 bfloat16 channels, a
-// fifth of 32768 queries by 5 heads by 32 blocks, take 59 us: 17 GFLOP, and 134 MB of partials with 8 MB
-// of sums, which leave in pieces of 128 and 8 bytes at 2.4 TB/s.  The products would take 14 us at a
-// large product's rate, the queries' 134 MB are read from the L2.  Two tiles of queries in registers,
-// keys and values held in registers, sums by products of ones, and four waves a SIMD were all measured
-// and made nothing faster (297 to 365 us for the five launches against 300).  Registers for two waves a
+// fifth of 32768 queries by 5 heads by 32 blocks, take 61 to 69 us: 26 GFLOP with both operands of the
+// weights, and 134 MB of partials with 8 MB of sums, which leave in pieces of 128 and 8 bytes at 2.1 TB/s.
+// The products would take 21 us at a large product's rate, the queries' 134 MB are read from the L2.  Two
+// tiles of queries in registers, keys and values held in registers, sums by products of ones, and four
+// waves a SIMD were all measured, with one operand of the weights, and made nothing faster (297 to 365 us
+// for the five launches against 300).  Registers for two waves a
 // SIMD where that leaves nothing in memory (accumulators then stay where vector instructions reach
 // them); larger tiles take one.
 template <class T, int DP, int BK>

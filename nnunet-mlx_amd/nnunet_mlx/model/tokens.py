@@ -520,8 +520,8 @@ def select_blocks(q: torch.Tensor, summary: BlockSummary, block: int, keep: int,
     ids = torch.empty((q.shape[0], q.shape[1], summary.codes.shape[1], keep), dtype=torch.int32, device=q.device)
     if config:
         work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        _launch(q.device, "nnx_block_select", _placed(config, at) if at else config, q.data_ptr(), summary.codes.data_ptr(),
-                summary.scales.data_ptr(), _address(starts), ids.data_ptr(), _address(work), size)
+        _launch(q.device, "nnx_block_select", _placed(config, at) if at else config, q.data_ptr(),
+                summary.codes.data_ptr(), summary.scales.data_ptr(), _address(starts), ids.data_ptr(), _address(work), size)
     elif ids.numel():
         ids.fill_(-1)
     return ids
@@ -576,8 +576,8 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ids: torc
         results = _without_gradient("block_attention", results, given, q, k, v)
     if config:
         work = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _launch(q.device, "nnx_block_attention", _placed(config, at) if at else config, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                ids.data_ptr(), _address(starts), _address(lengths), _address(key_mask), out.data_ptr(),
+        _launch(q.device, "nnx_block_attention", _placed(config, at) if at else config, q.data_ptr(), k.data_ptr(),
+                v.data_ptr(), ids.data_ptr(), _address(starts), _address(lengths), _address(key_mask), out.data_ptr(),
                 work.data_ptr(), size)
     elif out.numel():
         out.detach().zero_()

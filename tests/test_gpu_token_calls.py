@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from nnunet_mlx.errors import ContractError
 from nnunet_mlx.model import tokens
 
 pytestmark = pytest.mark.gpu
@@ -65,3 +66,26 @@ def test_one_position_for_all_items_and_each_its_own(device):
         for a, b in zip(tokens.sparse_attention(q, k, v, 16, 2, causal=True, start=start),
                         tokens.sparse_attention(q, k, v, 16, 2, causal=True, start=each)):
             assert torch.equal(a, b)
+
+
+def test_results_of_inputs_that_require_a_gradient(device):
+    """The same results, whose backward pass is refused."""
+    q, k, v = (torch.randn(1, n, 2, 16, generator=_gen(n)).cuda() for n in (6, 90, 91))
+    v = v[:, :90]
+    weight = torch.ones(32, device="cuda")
+    plan, positions = tokens.rotary_plan(16), torch.arange(6, dtype=torch.int32, device="cuda")[:, None].contiguous()
+
+    def run(q, v, weight):
+        turned, _ = tokens.rotate(q, None, positions, plan)
+        mixed, _ = tokens.sparse_attention(turned, k, v, 16, 3)
+        return tokens.residual_norm(mixed.flatten(2), None, pre=(weight, None))[1]
+
+    want = run(q, v, weight)
+    for which in range(3):
+        inputs = [t.clone().requires_grad_(i == which) for i, t in enumerate((q, v, weight))]
+        got = run(*inputs)
+        assert torch.equal(got.detach(), want)
+        with pytest.raises(ContractError, match="forward only"):
+            got.sum().backward()
+        with torch.no_grad():
+            assert torch.equal(run(*inputs), want)
