@@ -1,6 +1,6 @@
 """What attention over selected blocks keeps of its values: every channel by itself, at any magnitude.
 
-Tolerances.  U is a type's unit roundoff (half the spacing at 1).  Each channel is judged against the mean
+Tolerances.  U is a type's unit roundoff (half the spacing at 1).  Each channel is held against the mean
 over its own weights of |v|, which is what an error of the weights can move it by.  Weights may be off by
 U where they are rounded to the type, and by 5e-4 through a float32 logit of up to 130 terms that sum to
 less than 20 in magnitude (130 * 2^-24 * 20 = 1.6e-4, a weight by twice that); partials and the result are
