@@ -634,6 +634,85 @@ int nnx_block_attention(const nnx_block_config* config, const void* d_q, const v
                         const int32_t* d_lengths, const uint8_t* d_mask, void* d_out,
                         void* d_workspace, size_t workspace_bytes, void* stream);
 
+/* Keys and values held in 8 bits, quantised as they are written.  Row x (a token's head_dim
+ * elements under one key head), step by step in float32: m = max |x|; an element that is not
+ * finite: scale NaN, codes 0; m < 2^-60: scale and codes 0; else code = rint(x * (127 / m)),
+ * scale = min(m, 3.4028233e38) / 127.  Such a row stands for code * scale; every step is
+ * elementwise, so nothing depends on how the work is split.
+ *
+ * An item has `slots` rows a key head.  d_k_codes (batch, kv_heads, slots, head_dim); d_v_codes
+ * (batch, kv_heads, slots / 64, head_dim, 64), slot 16 t + 4 g + i of 64 at place 16 g + 4 t + i;
+ * d_k_scales and d_v_scales float32 (batch, kv_heads, slots); all four contiguous and 16-byte
+ * aligned. */
+typedef struct nnx_held_config {
+  int type;      /* of k, v, q and out */
+  int batch;     /* 1..65535 */
+  int tokens;    /* of k and v, or queries */
+  int slots;     /* a multiple of 64 */
+  int keys;      /* attention: slots from here on are not seen, 1..slots */
+  int heads;     /* attention: a multiple of kv_heads */
+  int kv_heads;
+  int head_dim;  /* a multiple of 16, 16..128 */
+  int causal;    /* attention: a query sees the slots up to its position */
+  float scale;   /* attention: of the logits */
+  int64_t start; /* the first token's slot or the first query's position */
+  int64_t strides[2][3]; /* (batch, token, head) of k and v, or of q and out */
+  int64_t mask_stride;
+} nnx_held_config;
+
+/* Writes token t < d_lengths[b] (NULL: all) of item b into slot start + d_start[b] (NULL: 0) + t;
+ * tokens without such a slot are left out, slots without a token as they were. */
+int nnx_hold_tokens(const nnx_held_config* config, const void* d_k, const void* d_v,
+                    const int32_t* d_start, const int32_t* d_lengths, int8_t* d_k_codes,
+                    float* d_k_scales, int8_t* d_v_codes, float* d_v_scales, void* stream);
+
+/* Slots start, ..., start + tokens - 1 of every item as `type`: code * scale, rounded once. */
+int nnx_read_held(const nnx_held_config* config, const int8_t* d_k_codes, const float* d_k_scales,
+                  const int8_t* d_v_codes, const float* d_v_scales, void* d_k, void* d_v,
+                  void* stream);
+
+/* out[q] = softmax(scale q . k) v over the held slots before min(keys, d_lengths[b]) with a nonzero
+ * d_mask[b * mask_stride + slot] (NULL: all), and with `causal` up to position start + d_start[b]
+ * + t of query t.  What other slots hold is never used.  A query that sees no slot gets zeros.
+ * Logits, softmax and sums are float32.  The workspace query answers 0 for what the entry refuses;
+ * the workspace is 16-byte aligned, of 0 bytes it may be null; `start` does not change its size. */
+size_t nnx_held_attention_workspace(const nnx_held_config* config);
+int nnx_held_attention(const nnx_held_config* config, const void* d_q, const int8_t* d_k_codes,
+                       const float* d_k_scales, const int8_t* d_v_codes, const float* d_v_scales,
+                       const int32_t* d_start, const int32_t* d_lengths, const uint8_t* d_mask,
+                       void* d_out, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Products with 4-bit weights.  `group` consecutive inputs of an output share a float32 scale; a
+ * code's low three bits stand for 0, 0.5, 1, 1.5, 2, 3, 4 or 6, its fourth for the sign (E2M1), and
+ * a weight is that times the scale.  Packed, m = max |w| of a group (not finite: scale NaN, codes
+ * 0; below 2^-60: scale and codes 0): the value nearest |w| * (6 / m), half-way values to the even
+ * code, scale = min(m, 3.4028233e38) / 6.
+ *
+ * d_codes (ceil(outputs / 16), ceil(inputs / 128), 64, 16) bytes: byte 4 j + b of place 16 g + n
+ * holds inputs 32 j + 8 g + 2 b (low four bits) and the next of output n of 16; d_scales float32
+ * (ceil(outputs / 16), ceil(inputs / 128) * 128 / group, 16); both 16-byte aligned.  Codes and
+ * scales past the matrix are zero. */
+typedef struct nnx_packed_config {
+  int type;    /* of x and y, or of the unpacked weights */
+  int inputs;  /* 1..2^20 */
+  int outputs; /* 1..2^20 */
+  int group;   /* 32, 64 or 128 */
+  int gate_activation; /* NNX_GATE_*, with a gate */
+  int64_t rows;        /* 1..2^31 - 1, of x and y */
+  int64_t x_stride, y_stride; /* of rows; of weights (outputs, inputs) x_stride */
+} nnx_packed_config;
+int nnx_pack_weight(const nnx_packed_config* config, const void* d_w, uint8_t* d_codes,
+                    float* d_scales, void* stream);
+int nnx_unpack_weight(const nnx_packed_config* config, const uint8_t* d_codes,
+                      const float* d_scales, void* d_w, void* stream);
+
+/* y = x W^T + bias, or act(x G^T) * (x W^T + bias) with a gate G of W's sizes, rounded once: products
+ * and sums are float32 of the exact codes, scaled by group.  d_bias float32 (outputs) or NULL; a
+ * NULL gate is none. */
+int nnx_packed_linear(const nnx_packed_config* config, const void* d_x, const uint8_t* d_codes,
+                      const float* d_scales, const float* d_bias, const uint8_t* d_gate_codes,
+                      const float* d_gate_scales, void* d_y, void* stream);
+
 /* ---- kernel timing (no reference counterpart: measurement support) ----------------
  * Between nnx_profile_begin and nnx_profile_end every kernel launch of the library is
  * bracketed by HIP events on its own stream and attributed to a class (kernel name and

@@ -356,4 +356,23 @@ void block_attention(const nnx_block_config& c, const void* q, const void* k, co
                      const int32_t* ids, const int32_t* start, const int32_t* lengths,
                      const uint8_t* mask, void* out, void* ws, size_t ws_bytes, hipStream_t st);
 
+// Held tokens and packed weights (nnx_held.hip, nnx_packed.hip).
+void hold_tokens(const nnx_held_config& c, const void* k, const void* v, const int32_t* start,
+                 const int32_t* lengths, int8_t* k_codes, float* k_scales, int8_t* v_codes,
+                 float* v_scales, hipStream_t st);
+void read_held(const nnx_held_config& c, const int8_t* k_codes, const float* k_scales,
+               const int8_t* v_codes, const float* v_scales, void* k, void* v, hipStream_t st);
+size_t held_attention_workspace(const nnx_held_config& c);
+void held_attention(const nnx_held_config& c, const void* q, const int8_t* k_codes,
+                    const float* k_scales, const int8_t* v_codes, const float* v_scales,
+                    const int32_t* start, const int32_t* lengths, const uint8_t* mask, void* out,
+                    void* ws, size_t ws_bytes, hipStream_t st);
+void pack_weight(const nnx_packed_config& c, const void* w, uint8_t* codes, float* scales,
+                 hipStream_t st);
+void unpack_weight(const nnx_packed_config& c, const uint8_t* codes, const float* scales, void* w,
+                   hipStream_t st);
+void packed_linear(const nnx_packed_config& c, const void* x, const uint8_t* codes,
+                   const float* scales, const float* bias, const uint8_t* gate_codes,
+                   const float* gate_scales, void* y, hipStream_t st);
+
 }  // namespace nnx

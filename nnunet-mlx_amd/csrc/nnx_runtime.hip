@@ -1670,4 +1670,64 @@ int nnx_block_attention(const nnx_block_config* config, const void* d_q, const v
   });
 }
 
+int nnx_hold_tokens(const nnx_held_config* config, const void* d_k, const void* d_v,
+                    const int32_t* d_start, const int32_t* d_lengths, int8_t* d_k_codes,
+                    float* d_k_scales, int8_t* d_v_codes, float* d_v_scales, void* stream) {
+  return guarded([&] {
+    require(config, "hold tokens: null config");
+    hold_tokens(*config, d_k, d_v, d_start, d_lengths, d_k_codes, d_k_scales, d_v_codes, d_v_scales,
+                as_stream(stream));
+  });
+}
+
+int nnx_read_held(const nnx_held_config* config, const int8_t* d_k_codes, const float* d_k_scales,
+                  const int8_t* d_v_codes, const float* d_v_scales, void* d_k, void* d_v,
+                  void* stream) {
+  return guarded([&] {
+    require(config, "read held: null config");
+    read_held(*config, d_k_codes, d_k_scales, d_v_codes, d_v_scales, d_k, d_v, as_stream(stream));
+  });
+}
+
+size_t nnx_held_attention_workspace(const nnx_held_config* config) {
+  return config ? held_attention_workspace(*config) : 0;
+}
+
+int nnx_held_attention(const nnx_held_config* config, const void* d_q, const int8_t* d_k_codes,
+                       const float* d_k_scales, const int8_t* d_v_codes, const float* d_v_scales,
+                       const int32_t* d_start, const int32_t* d_lengths, const uint8_t* d_mask,
+                       void* d_out, void* d_workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    require(config, "held attention: null config");
+    held_attention(*config, d_q, d_k_codes, d_k_scales, d_v_codes, d_v_scales, d_start, d_lengths,
+                   d_mask, d_out, d_workspace, workspace_bytes, as_stream(stream));
+  });
+}
+
+int nnx_pack_weight(const nnx_packed_config* config, const void* d_w, uint8_t* d_codes,
+                    float* d_scales, void* stream) {
+  return guarded([&] {
+    require(config, "pack weight: null config");
+    pack_weight(*config, d_w, d_codes, d_scales, as_stream(stream));
+  });
+}
+
+int nnx_unpack_weight(const nnx_packed_config* config, const uint8_t* d_codes,
+                      const float* d_scales, void* d_w, void* stream) {
+  return guarded([&] {
+    require(config, "unpack weight: null config");
+    unpack_weight(*config, d_codes, d_scales, d_w, as_stream(stream));
+  });
+}
+
+int nnx_packed_linear(const nnx_packed_config* config, const void* d_x, const uint8_t* d_codes,
+                      const float* d_scales, const float* d_bias, const uint8_t* d_gate_codes,
+                      const float* d_gate_scales, void* d_y, void* stream) {
+  return guarded([&] {
+    require(config, "packed linear: null config");
+    packed_linear(*config, d_x, d_codes, d_scales, d_bias, d_gate_codes, d_gate_scales, d_y,
+                  as_stream(stream));
+  });
+}
+
 }  // extern "C"

@@ -160,6 +160,37 @@ class NnxBlockConfig(ctypes.Structure):
     ]
 
 
+class NnxHeldConfig(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int),
+        ("batch", ctypes.c_int),
+        ("tokens", ctypes.c_int),
+        ("slots", ctypes.c_int),
+        ("keys", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("causal", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("start", ctypes.c_int64),
+        ("strides", ctypes.c_int64 * 6),
+        ("mask_stride", ctypes.c_int64),
+    ]
+
+
+class NnxPackedConfig(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int),
+        ("inputs", ctypes.c_int),
+        ("outputs", ctypes.c_int),
+        ("group", ctypes.c_int),
+        ("gate_activation", ctypes.c_int),
+        ("rows", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64),
+    ]
+
+
 FORWARD_FN = ctypes.CFUNCTYPE(
     ctypes.c_int, c_void_p, c_void_p, c_void_p, ctypes.c_int, c_int_p, c_void_p
 )
@@ -378,6 +409,15 @@ _SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [ctypes.POINTER(NnxBlockConfig), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
          c_void_p, c_void_p, c_void_p, ctypes.c_size_t, c_void_p],
     ),
+    "nnx_hold_tokens": (ctypes.c_int, [ctypes.POINTER(NnxHeldConfig), *[c_void_p] * 9]),
+    "nnx_read_held": (ctypes.c_int, [ctypes.POINTER(NnxHeldConfig), *[c_void_p] * 7]),
+    "nnx_held_attention_workspace": (ctypes.c_size_t, [ctypes.POINTER(NnxHeldConfig)]),
+    "nnx_held_attention": (
+        ctypes.c_int, [ctypes.POINTER(NnxHeldConfig), *[c_void_p] * 10, ctypes.c_size_t, c_void_p]
+    ),
+    "nnx_pack_weight": (ctypes.c_int, [ctypes.POINTER(NnxPackedConfig), *[c_void_p] * 4]),
+    "nnx_unpack_weight": (ctypes.c_int, [ctypes.POINTER(NnxPackedConfig), *[c_void_p] * 4]),
+    "nnx_packed_linear": (ctypes.c_int, [ctypes.POINTER(NnxPackedConfig), *[c_void_p] * 8]),
     "nnx_profile_begin": (ctypes.c_int, []),
     "nnx_profile_end": (ctypes.c_int, [c_int_p]),
     "nnx_profile_read": (

@@ -4,7 +4,10 @@ A volume cut into cubes is a sequence of tokens.  Between a block's plain matrix
 rotary positions (``rotary_plan``, ``rotate``), attention over blocks of keys that a cheap
 score selects for each query (``summarize_blocks``, ``select_blocks``, ``block_attention``, all
 three in ``sparse_attention``) and the norms around the block with its gate and residual sum
-(``residual_norm``).  Everything runs in libnnunet_hip.so on the current stream of the tensors'
+(``residual_norm``).  Points are answered against a volume that stays on the GPU: its keys and
+values in 8 bits (``held_tokens``, ``hold_tokens``, ``read_held``), the attention that reads them
+so (``held_attention``) and products of few rows with 4-bit weights (``pack_weight``,
+``unpack_weight``, ``packed_linear``).  Everything runs in libnnunet_hip.so on the current stream of the tensors'
 device, forward only (a gradient asked of a result raises ``ContractError``; a selection has
 none); float32, float16 and bfloat16 tensors with a contiguous last axis and any other strides.
 No reference counterpart.
@@ -41,6 +44,8 @@ BLOCK_SIZES = (16, 32, 64, 128)
 _ROTARY = struct.Struct("@10if4x14q")
 _NORM = struct.Struct("@2iq4i2f5q")
 _BLOCK = struct.Struct("@12iqf4x13q")
+_HELD = struct.Struct("@9if8q")
+_PACKED = struct.Struct("@5i4x3q")
 
 # the current stream of a device index, as torch's own launches ask for it
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
@@ -424,11 +429,13 @@ def _one_start(start: int) -> int:
     return at
 
 
-def _placed(config: _native.NnxBlockConfig, start: int) -> _native.NnxBlockConfig:
-    """The checked configuration for queries from ``start`` on.  A decoder moves it at every step, so it is
-    no part of what is remembered."""
-    config = _native.NnxBlockConfig.from_buffer_copy(config)
+def _placed(config, start: int, keys: int | None = None):
+    """The checked configuration for queries or tokens from ``start`` on, of ``keys`` slots.  A decoder moves
+    both at every step, so they are no part of what is remembered."""
+    config = type(config).from_buffer_copy(config)
     config.start = start
+    if keys is not None:
+        config.keys = keys
     return config
 
 
@@ -627,3 +634,335 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block: i
     ids = select_blocks(q, summary, block, keep, causal=causal, start=start, first=first, local=local)
     return block_attention(q, k, v, ids, block, scale=scale, causal=causal, start=start, lengths=lengths,
                            key_mask=key_mask), ids
+
+
+# ---- tokens held in 8 bits --------------------------------------------------------------
+
+
+class HeldTokens(NamedTuple):
+    """Keys and values of every item's slots in 8 bits, a scale for each slot and key head; a row
+    stands for code * scale.
+
+    ``k_codes`` int8 (batch, kv_heads, slots, head_dim); ``v_codes`` int8 (batch, kv_heads, slots / 64,
+    head_dim, 64), in which slot 16 t + 4 g + i of 64 stands at place 16 g + 4 t + i (what the attention's
+    products take together lies together); ``k_scales`` and ``v_scales`` float32 (batch, kv_heads, slots)."""
+
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+
+
+def held_tokens(batch: int, slots: int, kv_heads: int, head_dim: int, *,
+                device: torch.device | str = "cuda") -> HeldTokens:
+    """Slots for at least ``slots`` tokens of each item (a multiple of 64), all zero."""
+    batch, slots, kv_heads, head_dim = (_whole(name, value) for name, value in (
+        ("batch", batch), ("slots", slots), ("kv_heads", kv_heads), ("head_dim", head_dim)))
+    _need(batch >= 0 and slots >= 0 and kv_heads >= 1 and head_dim >= 1,
+          f"no tokens of {batch} items, {slots} slots, {kv_heads} key heads of {head_dim} can be held")
+    tiles = -(-slots // 64)
+
+    def zeros(*shape: int, dtype: torch.dtype) -> torch.Tensor:
+        return torch.zeros((batch, kv_heads, *shape), dtype=dtype, device=device)
+
+    return HeldTokens(zeros(64 * tiles, head_dim, dtype=torch.int8), zeros(64 * tiles, dtype=torch.float32),
+                      zeros(tiles, head_dim, 64, dtype=torch.int8), zeros(64 * tiles, dtype=torch.float32))
+
+
+def _check_held(held: HeldTokens, device: torch.device) -> tuple[int, int, int, int]:
+    """Batch, key heads, slots and head_dim of what is held."""
+    _need(held.k_codes.dim() == 4, f"held codes need 4 axes, got shape {tuple(held.k_codes.shape)}")
+    batch, kv_heads, slots, dim = held.k_codes.shape
+    _need(slots % 64 == 0, f"slots must be a multiple of 64, got {slots}")
+    _check_side("k_codes", held.k_codes, torch.int8, (batch, kv_heads, slots, dim), device)
+    _check_side("k_scales", held.k_scales, torch.float32, (batch, kv_heads, slots), device)
+    _check_side("v_codes", held.v_codes, torch.int8, (batch, kv_heads, slots // 64, dim, 64), device)
+    _check_side("v_scales", held.v_scales, torch.float32, (batch, kv_heads, slots), device)
+    return batch, kv_heads, slots, dim
+
+
+def _held_config(like: torch.dtype, batch: int, tokens: int, slots: int, kv_heads: int, dim: int, first, second, *,
+                 keys: int = 1, heads: int = 1, causal: bool = False, scale: float = 1.0, start: int = 0,
+                 mask_stride: int = 0) -> _native.NnxHeldConfig:
+    return _packed(_native.NnxHeldConfig, _HELD, _TYPES[like], batch, tokens, slots, keys, heads, kv_heads, dim,
+                   causal, scale, start, *first, *second, mask_stride)
+
+
+def _addresses(held: HeldTokens) -> tuple[int, int, int, int]:
+    return (held.k_codes.data_ptr(), held.k_scales.data_ptr(), held.v_codes.data_ptr(), held.v_scales.data_ptr())
+
+
+def hold_tokens(held: HeldTokens, k: torch.Tensor, v: torch.Tensor, *, start: torch.Tensor | int = 0,
+                lengths: torch.Tensor | None = None) -> HeldTokens:
+    """Writes keys and values (batch, tokens, kv_heads, head_dim) into slots ``start``, ``start`` + 1, ...
+
+    ``start`` is an int or int32 (batch,); ``lengths`` int32 (batch,) counts the tokens that each item has.
+    Each row is held as whole numbers -127 to 127 times its largest magnitude / 127; a row with an
+    element that is not finite is held as NaN, one below 2^-60 as zero.  Slots that no token is
+    written to stay as they were; where ``start`` is a tensor, tokens past the slots are left out.
+    Returns ``held``."""
+    starts, at = (start, 0) if isinstance(start, torch.Tensor) else (None, _one_start(start))
+    key = ("hold", _signature(*held, k, v, starts, lengths))
+    known = _checked.get(key)
+    if known is None:
+        known = _remember(key, _hold_config(held, k, v, starts, lengths))
+    config, most = known
+    if at > most:
+        raise ContractError(f"tokens from slot {at} on pass the slots, the last place for them is {most}")
+    if config:
+        _launch(k.device, "nnx_hold_tokens", _placed(config, at) if at else config, k.data_ptr(), v.data_ptr(),
+                _address(starts), _address(lengths), *_addresses(held))
+    return held
+
+
+def _hold_config(held, k, v, starts, lengths):
+    """The checked configuration (False where there is nothing to do) and the last start that has slots for all."""
+    _check("k", k, 4)
+    _check("v", v, 4, k)
+    batch, kv_heads, slots, dim = _check_held(held, k.device)
+    tokens = k.shape[1]
+    _need(k.shape == (batch, tokens, kv_heads, dim) and v.shape == k.shape,
+          f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match {batch} items held with {kv_heads} key heads of {dim}")
+    for name, side in (("start", starts), ("lengths", lengths)):
+        if side is not None:
+            _check_side(name, side, torch.int32, (batch,), k.device)
+    _need(tokens <= slots, f"{tokens} tokens do not fit into {slots} slots")
+    if k.numel() == 0:
+        return False, slots
+    return _held_config(k.dtype, batch, tokens, slots, kv_heads, dim, k.stride()[:3], v.stride()[:3]), slots - tokens
+
+
+def read_held(held: HeldTokens, dtype: torch.dtype, *, first: int = 0, count: int | None = None,
+              out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values (batch, count, kv_heads, head_dim) of slots ``first`` on as ``dtype``: code * scale,
+    rounded once.  ``out`` may hold the results."""
+    slots = held.k_scales.shape[-1]
+    if type(first) is not int:
+        first = _whole("first", first)
+    if count is None:
+        count = slots - first
+    elif type(count) is not int:
+        count = _whole("count", count)
+    if not 0 <= first <= first + count <= slots:
+        raise ContractError(f"first {first} and count {count} leave the {slots} slots")
+    yk, yv = out or (None, None)
+    key = ("read", _signature(*held, yk, yv), dtype, count)
+    known = _checked.get(key)
+    if known is None:
+        known = _remember(key, (*_read_config(held, dtype, count, out), _gradients(yk, yv)))
+    config, shape, gradients = known
+    if gradients:
+        _without_gradient("read_held", (), True)
+    if out is None:
+        yk, yv = (torch.empty(shape, dtype=dtype, device=held.k_codes.device) for _ in range(2))
+    if config:
+        _launch(yk.device, "nnx_read_held", _placed(config, first) if first else config, *_addresses(held),
+                yk.data_ptr(), yv.data_ptr())
+    return yk, yv
+
+
+def _read_config(held, dtype, count, out):
+    """The checked configuration of a reading (False where there is nothing to do) and its results' shape."""
+    _need(dtype in _TYPES, f"dtype must be float32, float16 or bfloat16, not {dtype}")
+    batch, kv_heads, slots, dim = _check_held(held, held.k_codes.device)
+    shape = torch.Size((batch, count, kv_heads, dim))
+    strides = [_contiguous_strides(shape)] * 2
+    if out is not None:
+        for name, y in zip(("out[0]", "out[1]"), out):
+            _check(name, y, 4)
+            _need(y.shape == shape and y.dtype == dtype and y.device == held.k_codes.device,
+                  f"{name} must be {dtype} {tuple(shape)} on {held.k_codes.device}, got {y.dtype} {tuple(y.shape)} "
+                  f"on {y.device}")
+        strides = [y.stride()[:3] for y in out]
+    if shape.numel() == 0:
+        return False, shape
+    return _held_config(dtype, batch, count, slots, kv_heads, dim, *strides), shape
+
+
+def held_attention(q: torch.Tensor, held: HeldTokens, lengths: torch.Tensor | int, *, scale: float | None = None,
+                   causal: bool = False, start: torch.Tensor | int | None = None,
+                   key_mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Softmax attention of q (batch, queries, heads, head_dim) over held keys and values.
+
+    ``lengths``, an int or int32 (batch,), counts the slots from the first on that each item's queries
+    see; ``key_mask`` (batch, n) marks which of the first n are seen, those behind them are not.
+    ``scale`` defaults to head_dim^-0.5.  With ``causal`` a query sees the slots up to its position, which
+    is ``start`` (an int or int32 (batch,)) plus its index.  A query that sees no slot gets zeros."""
+    starts, at, counts, keys = start, 0, lengths, None
+    if start is not None and not isinstance(start, torch.Tensor):
+        starts, at = None, _one_start(start)
+    if not isinstance(lengths, torch.Tensor):
+        counts, keys = None, _whole("lengths", lengths)
+    if type(causal) is not bool:
+        causal = _flag("causal", causal)
+    if scale is not None and type(scale) is not float:
+        scale = _number("scale", scale)
+    key = ("held", _signature(q, *held, counts, starts, key_mask, out), scale, causal)
+    known = _checked.get(key)
+    if known is None:
+        known = _remember(key, (*_held_attention_config(q, held, counts, scale, causal, starts, key_mask, out),
+                                _gradients(q, out)))
+    config, size, slots, gradients = known
+    if keys is not None and not 0 <= keys <= slots:
+        raise ContractError(f"lengths must be 0 to the {slots} slots, got {keys}")
+    given = out is not None
+    if not given:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    results = (out,)
+    if gradients:
+        results = _without_gradient("held_attention", results, given, q)
+    if config and keys != 0:
+        if keys is not None:
+            config = _placed(config, at, min(keys, config.keys))
+            size = _native.load().nnx_held_attention_workspace(config)
+        elif at:
+            config = _placed(config, at)
+        work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        _launch(q.device, "nnx_held_attention", config, q.data_ptr(), *_addresses(held), _address(starts),
+                _address(counts), _address(key_mask), out.data_ptr(), _address(work), size)
+    elif out.numel():
+        out.detach().zero_()
+    return results[0]
+
+
+def _held_attention_config(q, held, counts, scale, causal, starts, mask, out):
+    """The checked configuration (False where there is nothing to attend to), workspace bytes and slots."""
+    if scale is not None:
+        _number("scale", scale)
+    _check("q", q, 4)
+    batch, kv_heads, slots, dim = _check_held(held, q.device)
+    _need(q.shape[0] == batch and q.shape[3] == dim,
+          f"q {tuple(q.shape)} does not match {batch} items held with {kv_heads} key heads of {dim}")
+    queries, heads = q.shape[1:3]
+    for name, side in (("lengths", counts), ("start", starts)):
+        if side is not None:
+            _check_side(name, side, torch.int32, (batch,), q.device)
+    keys, mask_stride = slots, 0
+    if mask is not None:
+        keys = mask.shape[-1]
+        _need(keys <= slots, f"key_mask is of {keys} slots, {slots} are held")
+        mask_stride = _check_lengths_mask(None, mask, batch, keys, q.device)
+    if out is not None:
+        _check("out", out, 4, q)
+        _need(out.shape == q.shape, f"out {tuple(out.shape)} does not match q {tuple(q.shape)}")
+    if q.numel() == 0 or keys == 0:
+        return False, 0, slots
+    config = _held_config(
+        q.dtype, batch, queries, slots, kv_heads, dim, q.stride()[:3],
+        _contiguous_strides(q.shape) if out is None else out.stride()[:3], keys=keys, heads=heads, causal=causal,
+        scale=dim**-0.5 if scale is None else scale, mask_stride=mask_stride)
+    return config, _native.load().nnx_held_attention_workspace(config), slots
+
+
+# ---- products with 4-bit weights ------------------------------------------------------
+
+
+class PackedWeight(NamedTuple):
+    """A matrix (outputs, inputs) in 4 bits: each ``group`` consecutive inputs of an output share a
+    scale, and a code stands for 0, 0.5, 1, 1.5, 2, 3, 4 or 6 (its low three bits; the fourth is the
+    sign) times it.
+
+    ``codes`` uint8 (tiles, blocks, 64, 16) of 16 outputs and 128 inputs each: byte 4 j + b of place
+    16 g + n holds inputs 32 j + 8 g + 2 b (low four bits) and the next of the tile's output n;
+    ``scales`` float32 (tiles, blocks * 128 / group, 16).  What is past the matrix is zero."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    outputs: int
+    inputs: int
+    group: int
+
+
+GROUP_SIZES = (32, 64, 128)
+
+
+def _packed_shapes(outputs: int, inputs: int, group: int) -> tuple[tuple[int, ...], tuple[int, ...]]:
+    _need(group in GROUP_SIZES, f"group must be one of {GROUP_SIZES}, got {group}")
+    tiles, blocks = -(-outputs // 16), -(-inputs // 128)
+    return (tiles, blocks, 64, 16), (tiles, blocks * 128 // group, 16)
+
+
+def _check_packed(name: str, weight: PackedWeight, device: torch.device) -> None:
+    codes, scales = _packed_shapes(*(_whole("outputs, inputs and group", size) for size in weight[2:]))
+    _check_side(f"{name} codes", weight.codes, torch.uint8, codes, device)
+    _check_side(f"{name} scales", weight.scales, torch.float32, scales, device)
+
+
+def _packed_config(dtype: torch.dtype, outputs: int, inputs: int, group: int, *, activation: int = 0, rows: int = 1,
+                   x_stride: int = 0, y_stride: int = 0) -> _native.NnxPackedConfig:
+    return _packed(_native.NnxPackedConfig, _PACKED, _TYPES[dtype], inputs, outputs, group, activation, rows, x_stride,
+                   y_stride)
+
+
+def pack_weight(w: torch.Tensor, group: int = 64) -> PackedWeight:
+    """A matrix (outputs, inputs) in 4 bits: each group's scale is its largest magnitude / 6, each weight
+    the nearest of the codes' values, half-way ones the even code's.  A group with a weight that is not
+    finite is NaN, one below 2^-60 zero."""
+    group = _whole("group", group)
+    _check("w", w, 2)
+    outputs, inputs = w.shape
+    _need(outputs >= 1 and inputs >= 1, f"a matrix of {outputs} x {inputs} cannot be packed")
+    shapes = _packed_shapes(outputs, inputs, group)
+    config = _packed_config(w.dtype, outputs, inputs, group, x_stride=w.stride(0))
+    codes = torch.empty(shapes[0], dtype=torch.uint8, device=w.device)
+    scales = torch.empty(shapes[1], dtype=torch.float32, device=w.device)
+    _launch(w.device, "nnx_pack_weight", config, w.data_ptr(), codes.data_ptr(), scales.data_ptr())
+    return PackedWeight(codes, scales, outputs, inputs, group)
+
+
+def unpack_weight(weight: PackedWeight, dtype: torch.dtype) -> torch.Tensor:
+    """The matrix (outputs, inputs) that packed weights stand for, each rounded once to ``dtype``."""
+    _need(dtype in _TYPES, f"dtype must be float32, float16 or bfloat16, not {dtype}")
+    _need(weight.codes.is_cuda, "the HIP path needs device tensors")
+    _check_packed("weight", weight, weight.codes.device)
+    config = _packed_config(dtype, weight.outputs, weight.inputs, weight.group, x_stride=weight.inputs)
+    w = torch.empty((weight.outputs, weight.inputs), dtype=dtype, device=weight.codes.device)
+    _launch(w.device, "nnx_unpack_weight", config, weight.codes.data_ptr(), weight.scales.data_ptr(), w.data_ptr())
+    return w
+
+
+def packed_linear(x: torch.Tensor, weight: PackedWeight, *, bias: torch.Tensor | None = None,
+                  gate: PackedWeight | None = None, gate_activation: str = "none") -> torch.Tensor:
+    """x (..., inputs) times a packed matrix's transpose plus ``bias`` (float32 (outputs,)), times
+    activation(x gate^T) where a ``gate`` of the matrix's sizes and group is given, in one pass.
+
+    Sums are of the exact codes in float32, each group's times its scale; the result is rounded once to
+    x's dtype.  Made for few rows, where the weights' bytes are what a product costs."""
+    codes, scales, *sizes = weight
+    gate_codes, gate_scales, *gate_sizes = gate or (None, None)
+    for size in (*sizes, *gate_sizes):
+        if type(size) is not int:
+            _whole("outputs, inputs and group", size)
+    key = ("linear", _signature(x, codes, scales, bias, gate_codes, gate_scales), *sizes, *gate_sizes, gate_activation)
+    known = _checked.get(key)
+    if known is None:
+        known = _remember(key, (*_linear_config(x, weight, bias, gate, gate_activation), _gradients(x, bias)))
+    config, shape, gradients = known
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    results = (y,)
+    if gradients:
+        results = _without_gradient("packed_linear", results, False, x, bias)
+    if config:
+        _launch(x.device, "nnx_packed_linear", config, x.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+                _address(bias), _address(gate_codes), _address(gate_scales), y.data_ptr())
+    return results[0]
+
+
+def _linear_config(x, weight, bias, gate, gate_activation):
+    """The checked configuration of a product (False where there is nothing to do) and its result's shape."""
+    _check("x", x, max(1, x.dim()))
+    _check_packed("weight", weight, x.device)
+    _need(x.shape[-1] == weight.inputs, f"x {tuple(x.shape)} does not match a matrix of {weight.inputs} inputs")
+    _need(gate_activation in _GATES, f"unknown gate activation {gate_activation!r}")
+    _need(gate is not None or gate_activation == "none", "a gate activation needs a gate")
+    if gate is not None:
+        _need(gate[2:] == weight[2:], f"a gate of {gate[2:]} outputs, inputs and group does not match {weight[2:]}")
+        _check_packed("gate", gate, x.device)
+    if bias is not None:
+        _check_side("bias", bias, torch.float32, (weight.outputs,), x.device)
+    shape = x.shape[:-1] + (weight.outputs,)
+    rows = x.numel() // weight.inputs
+    if rows == 0:
+        return False, shape
+    return _packed_config(x.dtype, weight.outputs, weight.inputs, weight.group, activation=_GATES[gate_activation],
+                          rows=rows, x_stride=_rows("x", x), y_stride=weight.outputs), shape

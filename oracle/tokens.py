@@ -150,3 +150,66 @@ def attention(q: np.ndarray, k: np.ndarray, v: np.ndarray, see: np.ndarray,
         out[b, t, h] = p @ vv
         size[b, t, h] = p @ np.abs(vv).max(1)
     return out, size
+
+
+# ---- tokens held in 8 bits, weights in 4 -----------------------------------------------
+
+
+def _scales(top: np.ndarray, steps: int) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+    """Of largest magnitudes: the factor to codes of up to ``steps``, the scale, and where codes are zero."""
+    zero = ~np.isfinite(top) | (top < TINY)
+    safe = np.where(zero, F32(1), top).astype(F32)
+    scale = np.minimum(safe, F32(3.4028233e38)) / F32(steps)
+    scale = np.where(zero, np.where(np.isfinite(top), F32(0), F32(np.nan)), scale)
+    return F32(steps) / safe, scale.astype(F32), zero
+
+
+def hold(x: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """Rows (..., D) float32 -> codes int8 (..., D) and scales (...)."""
+    up, scale, zero = _scales(np.abs(x).max(-1, keepdims=True), 127)
+    with np.errstate(invalid="ignore", over="ignore"):
+        codes = np.where(zero, F32(0), np.rint(x * up))
+    return codes.astype(np.int8), scale[..., 0]
+
+
+def place_values(codes: np.ndarray) -> np.ndarray:
+    """Codes (B, G, slots, D) in the order in which values are held, slot by slot."""
+    b, g, slots, d = codes.shape
+    out = np.zeros((b, g, slots // 64, d, 64), np.int8)
+    for s in range(64):
+        out[..., 16 * (s // 4 % 4) + 4 * (s // 16) + s % 4] = codes[:, :, s::64]
+    return out
+
+
+LEVELS = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+
+
+def pack(w: np.ndarray, group: int) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+    """A matrix (O, I) float32 -> packed codes and scales and the matrix that they stand for, weight by weight."""
+    outputs, inputs = w.shape
+    tiles, blocks = -(-outputs // 16), -(-inputs // 128)
+    codes = np.zeros((tiles, blocks, 64, 16), np.uint8)
+    scales = np.zeros((tiles, blocks * 128 // group, 16), F32)
+    stands = np.zeros(w.shape)
+    for o in range(outputs):
+        for i0 in range(0, inputs, group):
+            part = w[o, i0:i0 + group]
+            up, scale, zero = _scales(np.abs(part).max(), 6)
+            scales[o // 16, i0 // group, o % 16] = scale
+            for n, x in enumerate(part):
+                size, i = 0.0 if zero else float(F32(abs(x)) * up), i0 + n
+                # the nearest value, of two as near the one with the even code
+                code = min(range(8), key=lambda c: (abs(LEVELS[c] - size), c % 2))
+                stands[o, i] = np.copysign(LEVELS[code], x) * float(scale)
+                if code and x < 0:
+                    code += 8
+                place, byte = i % 32 // 8 * 16 + o % 16, i % 128 // 32 * 4 + i % 8 // 2
+                codes[o // 16, i // 128, place, byte] |= code << (4 if i % 2 else 0)
+    return codes, scales, stands
+
+
+def gated(u: np.ndarray, g: np.ndarray | None, activation: str) -> np.ndarray:
+    if g is None:
+        return u
+    open_ = 1.0 / (1.0 + np.exp(-g))
+    return u * {"none": g, "sigmoid": open_, "silu": g * open_}[activation]
