@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "nnx_elements.h"
+#include "nnx_held.h"
 
 namespace nnx {
 
@@ -11,15 +11,6 @@ namespace {
 
 constexpr float kTiny = 8.673617379884035e-19f;  // 2^-60
 constexpr float kMost = 3.4028233e38f;           // 127 * (kMost / 127) is finite
-
-struct HeldArgs {
-  int batch, tokens, slots, keys, heads, kv_heads, dim, causal;
-  float scale;
-  int64_t start0;
-  int64_t s[2][3], ms;
-  const int32_t *start, *lengths;
-  const uint8_t* mask;
-};
 
 HeldArgs make_args(const nnx_held_config& c, const int32_t* start, const int32_t* lengths, const uint8_t* mask) {
   HeldArgs a;
@@ -93,55 +84,34 @@ __global__ __launch_bounds__(256) void read_kernel(HeldArgs a, const int8_t* k_c
   y[d] = from_float<T>(stands_for(code, (which ? v_scales : k_scales)[item * a.slots + slot]));
 }
 
-// A workgroup a query and head: 256 slots at a time, their logits a thread each, then a thread a channel.
+// The parts of rows: weighted by their largest logits and added up in order, a thread four channels.
 template <class T>
-__global__ __launch_bounds__(256) void attend_kernel(HeldArgs a, float down, const T* q, const int8_t* k_codes,
-                                                     const float* k_scales, const int8_t* v_codes,
-                                                     const float* v_scales, T* out) {
-  __shared__ float qs[128], ws[256], red[4];
-  const int h = blockIdx.x % a.heads;
-  const int64_t bt = blockIdx.x / a.heads;
-  const int b = (int)(bt / a.tokens), t = (int)(bt - (int64_t)b * a.tokens);
-  const int64_t item = (int64_t)b * a.kv_heads + h / (a.heads / a.kv_heads);
-  const T* row = q + b * a.s[0][0] + t * a.s[0][1] + h * a.s[0][2];
-  if (threadIdx.x < a.dim) qs[threadIdx.x] = to_float(row[threadIdx.x]) * 0x1p-14f;  // products with codes stay finite
-  int64_t n = a.lengths ? min(a.lengths[b], a.keys) : a.keys;
-  if (a.causal) n = min(n, a.start0 + (a.start ? a.start[b] : 0) + t + 1);
-  const float c2 = a.scale * (1.4426950408889634f * 0x1p14f), unit = exp2f(-down);
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int s0 = 0; s0 < n; s0 += 256) {
-    __syncthreads();
-    const int slot = s0 + threadIdx.x;
-    const bool seen = slot < n && (!a.mask || a.mask[b * a.ms + slot]);
-    float x = -INFINITY;
-    if (seen) {
-      const int8_t* key = k_codes + (item * a.slots + slot) * a.dim;
-      float dot = 0.f;
-      for (int d = 0; d < a.dim; ++d) dot = fmaf(qs[d], (float)key[d], dot);
-      x = dot * k_scales[item * a.slots + slot] * c2;
-    }
-    const float most = lanes_reduce<64>(x, [](float p, float r) { return fmaxf(p, r); });
-    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = most;
-    __syncthreads();
-    const float next = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float top = next == -INFINITY ? 0.f : next;
-    const float back = m == -INFINITY ? 0.f : exp2f(m - next);
-    m = next;
-    ws[threadIdx.x] = seen ? exp2f(x - top) : -1.f;
-    __syncthreads();
-    float ls = 0.f, os = 0.f;  // of 256 slots: sums of sums lose less
-    for (int j = 0; j < 256 && s0 + j < n; ++j) {
-      const float w = ws[j];
-      if (w < 0.f) continue;  // not seen
-      ls += w;
-      if (threadIdx.x < a.dim)
-        os = fmaf(w * (v_scales[item * a.slots + s0 + j] * unit),
-                 (float)v_codes[item * a.slots * a.dim + value_at(s0 + j, threadIdx.x, a.dim)], os);
-    }
-    l = fmaf(l, back, ls), o = fmaf(o, back, os);
+__global__ __launch_bounds__(256) void join_kernel(HeldAttention h) {
+  const int quads = h.a.dim / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / quads;
+  if (row >= (int64_t)h.a.batch * h.a.kv_heads * h.rows) return;
+  const int d = (int)(i - row * quads) * 4;
+  const int64_t bg = row / h.rows;
+  const int b = (int)(bg / h.a.kv_heads), kh = (int)(bg - (int64_t)b * h.a.kv_heads), mine = (int)(row - bg * h.rows);
+  const int64_t first = bg * h.splits * h.rows + mine;
+  float top = -INFINITY, l = 0.f, o[4] = {};
+  for (int s = 0; s < h.splits; ++s) top = fmaxf(top, h.meta[first + (int64_t)s * h.rows].x);
+  for (int s = 0; s < h.splits; ++s) {
+    const int64_t at = first + (int64_t)s * h.rows;
+    const float2 m = h.meta[at];
+    const float4 v = *(const float4*)__builtin_assume_aligned(h.part + at * h.a.dim + d, 16);
+    // nothing seen: sums of zero, or of NaN logits
+    const float w = m.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m.x - top);
+    l = fmaf(m.y, w, l);
+    o[0] = fmaf(v.x, w, o[0]), o[1] = fmaf(v.y, w, o[1]), o[2] = fmaf(v.z, w, o[2]), o[3] = fmaf(v.w, w, o[3]);
   }
-  if (threadIdx.x < a.dim)
-    (out + b * a.s[1][0] + t * a.s[1][1] + h * a.s[1][2])[threadIdx.x] = from_float<T>(l == 0.f ? 0.f : o / l / unit);
+  const int t = mine / h.group, hd = mine - t * h.group;
+  T* out = (T*)h.out + b * h.a.s[1][0] + t * h.a.s[1][1] + (int64_t)(kh * h.group + hd) * h.a.s[1][2] + d;
+  const float whole = l == 0.f && top == -INFINITY ? 0.f : 1.f / l;  // nothing seen: zeros
+  Vec<T, 4> y;
+  for (int k = 0; k < 4; ++k) y.v[k] = from_float<T>(o[k] * whole * h.back);
+  store_vec(out, y);
 }
 
 void check_config(const nnx_held_config& c, const char* name, bool attention) {
@@ -208,10 +178,33 @@ void read_held(const nnx_held_config& c, const int8_t* k_codes, const float* k_s
   launch_check("read_held");
 }
 
+namespace {
+
+HeldPlan make_plan(const nnx_held_config& c) {
+  HeldPlan p;
+  p.group = c.heads / c.kv_heads;
+  p.rows = c.tokens * p.group;
+  p.r = p.rows <= 16 ? 1 : 2;
+  p.tiles = (int)ceil_div(p.rows, 16 * p.r);
+  p.units = (int64_t)c.batch * c.kv_heads * p.tiles;
+  // parts of at least 4 tiles of 64 slots, a wave each, while two workgroups a CU are not reached
+  p.splits = (int)std::max<int64_t>(1, std::min(512 / p.units, ceil_div(c.keys, 256)));
+  require(p.units * p.splits < 1 << 24, "held attention: fewer than 2^24 items times key heads times tiles of 32 rows");
+  p.meta = p.bytes = 0;
+  if (p.splits > 1) {
+    const size_t rows = (size_t)c.batch * c.kv_heads * p.splits * p.rows;
+    p.meta = rows * c.head_dim * 4;
+    p.bytes = p.meta + rows * 8;
+  }
+  return p;
+}
+
+}  // namespace
+
 size_t held_attention_workspace(const nnx_held_config& c) {
   try {
     check_config(c, "held attention", true);
-    return 0;
+    return make_plan(c).bytes;
   } catch (...) {  // nothing may leave a C entry
     return 0;
   }
@@ -222,21 +215,40 @@ void held_attention(const nnx_held_config& c, const void* q, const int8_t* k_cod
                     const int32_t* start, const int32_t* lengths, const uint8_t* mask, void* out,
                     void* ws, size_t ws_bytes, hipStream_t st) {
   check_config(c, "held attention", true);
+  const HeldPlan p = make_plan(c);
   require(q && out, "held attention: null pointer");
   check_held(k_codes, k_scales, v_codes, v_scales, "held attention");
-  const HeldArgs a = make_args(c, start, lengths, mask);
+  require(p.bytes == 0 || (ws && ws_bytes >= p.bytes && reinterpret_cast<uintptr_t>(ws) % 16 == 0),
+          "held attention: the workspace is too small or not 16-byte aligned");
+  // The keys' scales are multiplied by at most 64, which none of them overflows by, and the queries by the
+  // rest: their products with codes are finite below 2^122 and so are logits up to the type's end.  A float16
+  // query is taken as it is.
+  const float factor = c.scale * 1.4426950408889634f;
+  const float query = c.type == NNX_TYPE_F16 || factor == 0.f
+                          ? 1.f : std::exp2(std::min(20.f, std::max(-16.f, std::ceil(std::log2(std::fabs(factor) / 64.f)))));
+  const float many = std::ceil(std::log2((float)c.keys));
+  HeldAttention h{make_args(c, start, lengths, mask), q, k_codes, v_codes, k_scales, v_scales, out, (float*)ws,
+                  (float2*)((char*)ws + p.meta), p.group, p.rows, p.tiles, p.splits,
+                  query, factor / query, std::exp2(-many), std::exp2(many)};
   const double rows = (double)c.batch * c.tokens * c.heads;
   ProfScope prof("held_attention", 4.0 * rows * c.keys * c.head_dim,
                  2.0 * rows * c.head_dim * type_bytes(c.type) +
                      2.0 * c.batch * c.kv_heads * c.keys * (c.head_dim + 4.0),
                  st);
-  const float down = ceilf(log2f((float)c.keys));
+  if (c.type == NNX_TYPE_F32) {
+    held_units_f32(h, p, st);
+  } else if (c.type == NNX_TYPE_F16) {
+    held_units_f16(h, p, st);
+  } else {
+    held_units_bf16(h, p, st);
+  }
+  if (p.splits == 1) return;
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    attend_kernel<T><<<(unsigned)(int64_t)rows, 256, 0, st>>>(a, down, (const T*)q, k_codes, k_scales, v_codes,
-                                                             v_scales, (T*)out);
+    const int64_t threads = (int64_t)rows * (c.head_dim / 4);
+    join_kernel<T><<<(unsigned)ceil_div(threads, 256), 256, 0, st>>>(h);
   });
-  launch_check("held_attention");
+  launch_check("held_join");
 }
 
 }  // namespace nnx
