@@ -23,40 +23,106 @@ HeldArgs make_args(const nnx_held_config& c, const int32_t* start, const int32_t
   return a;
 }
 
-// Place of a value's code among those of its item and key head.
-__device__ __forceinline__ int64_t value_at(int slot, int d, int dim) {
-  const int s = slot % 64;
-  return ((int64_t)(slot / 64) * dim + d) * 64 + s / 4 % 4 * 16 + s / 16 * 4 + s % 4;
+// Where slot s of 64 stands among the 64 places of a value channel's codes.
+__device__ __forceinline__ int place_of(int s) { return s / 4 % 4 * 16 + s / 16 * 4 + s % 4; }
+
+// A workgroup a tile of 64 slots of one key head's keys or values.  Threads take 8 channels of a row, rows
+// follow each other: whole rows in and out, 16 bytes a thread and more.  Value tiles pass through LDS, where
+// they change between rows of channels and rows of places.
+constexpr int kPlaces = 80;  // bytes from channel to channel there: 64 and a turn of the banks
+
+struct Unit {
+  int which, b, g, tile;
+};
+
+__device__ __forceinline__ Unit unit_of(const HeldArgs& a, int64_t u, int tiles) {
+  Unit r;
+  const int64_t rest = u / tiles;
+  r.tile = (int)(u - rest * tiles);
+  r.which = (int)(rest % 2);
+  r.g = (int)(rest / 2 % a.kv_heads);
+  r.b = (int)(rest / 2 / a.kv_heads);
+  return r;
 }
 
 template <class T>
 __global__ __launch_bounds__(256) void hold_kernel(HeldArgs a, const T* k, const T* v, int8_t* k_codes,
-                                                   float* k_scales, int8_t* v_codes, float* v_scales) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t rows = (int64_t)a.batch * a.tokens * a.kv_heads;
-  if (i >= 2 * rows) return;
-  const int which = i >= rows;
-  const int64_t r = which ? i - rows : i, bt = r / a.kv_heads;
-  const int g = (int)(r - bt * a.kv_heads), b = (int)(bt / a.tokens), t = (int)(bt - (int64_t)b * a.tokens);
-  const int64_t slot = a.start0 + (a.start ? a.start[b] : 0) + t;
-  if (slot < 0 || slot >= a.slots || (a.lengths && t >= a.lengths[b])) return;
-  const T* x = (which ? v : k) + b * a.s[which][0] + t * a.s[which][1] + g * a.s[which][2];
-  float top = 0.f;
-  bool odd = false;
-  for (int d = 0; d < a.dim; ++d) {
-    const float e = fabsf(to_float(x[d]));
-    top = fmaxf(top, e);
-    odd |= !(e < INFINITY);
+                                                   float* k_scales, int8_t* v_codes, float* v_scales, int tiles,
+                                                   int64_t units) {
+  __shared__ float tops[64 * 16];
+  __shared__ float ups[64];
+  __shared__ __attribute__((aligned(16))) int8_t placed[128 * kPlaces];
+  const int chunks = a.dim / 8, all = 64 * chunks;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const Unit w = unit_of(a, u, tiles);
+    const int64_t start = a.start0 + (a.start ? a.start[w.b] : 0);
+    const int64_t slot0 = ((start >> 6) + w.tile) * 64;  // of the tile; may lie outside the slots
+    const int given = a.lengths ? min(max(a.lengths[w.b], 0), a.tokens) : a.tokens;
+    // tokens of the tile: rows r0 to r1, row r token slot0 - start + r
+    const int r0 = (int)max((int64_t)0, start - slot0);
+    const int r1 = slot0 < 0 || slot0 >= a.slots ? 0 : (int)max((int64_t)0, min((int64_t)64, start + given - slot0));
+    if (r0 >= r1) continue;
+    const T* x = (w.which ? v : k) + w.b * a.s[w.which][0] + w.g * a.s[w.which][2];
+    const int64_t ts = a.s[w.which][1], t0 = slot0 - start;
+    const int64_t item = (int64_t)w.b * a.kv_heads + w.g;
+    Vec<T, 8> rows[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int i = n * 256 + threadIdx.x, r = i / chunks, c = i - r * chunks;
+      if (i >= all || r < r0 || r >= r1) continue;
+      rows[n] = load_vec<8>(x + (t0 + r) * ts + c * 8);
+      float top = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float m = fabsf(to_float(rows[n].v[e]));
+        top = m < INFINITY ? fmaxf(top, m) : INFINITY;  // stays there
+      }
+      tops[r * 16 + c] = top;
+    }
+    __syncthreads();
+    const int mine = threadIdx.x;
+    if (mine >= r0 && mine < r1) {
+      float top = 0.f;
+      for (int c = 0; c < chunks; ++c) top = fmaxf(top, tops[mine * 16 + c]);
+      const bool odd = !(top < INFINITY), zero = odd || top < kTiny;
+      ups[mine] = zero ? 0.f : 127.f / top;  // codes of 0 where it is 0
+      (w.which ? v_scales : k_scales)[item * a.slots + slot0 + mine] = odd ? NAN : zero ? 0.f : fminf(top, kMost) / 127.f;
+    }
+    __syncthreads();
+    int8_t* codes = (w.which ? v_codes : k_codes) + (item * a.slots + slot0) * a.dim;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int i = n * 256 + threadIdx.x, r = i / chunks, c = i - r * chunks;
+      if (i >= all || r < r0 || r >= r1) continue;
+      const float up = ups[r];
+      Vec<int8_t, 8> y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y.v[e] = up == 0.f ? 0 : (int8_t)(int)rintf(to_float(rows[n].v[e]) * up);
+      if (w.which) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) placed[(c * 8 + e) * kPlaces + place_of(r)] = y.v[e];
+      } else {
+        store_vec(codes + i * 8, y);
+      }
+    }
+    if (!w.which) continue;  // the next unit's first barrier is before what this one reads last
+    __syncthreads();
+    const bool whole = r0 == 0 && r1 == 64;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int i = n * 256 + threadIdx.x, d = i / 4, p = i % 4;
+      if (d >= a.dim) break;
+      const Vec<int8_t, 16> y = *(const Vec<int8_t, 16>*)__builtin_assume_aligned(placed + d * kPlaces + p * 16, 16);
+      if (whole) {
+        store_vec(codes + d * 64 + p * 16, y);
+        continue;
+      }
+      for (int e = 0; e < 16; ++e) {  // others' bytes stay as they are
+        const int slot = e / 4 * 16 + p * 4 + e % 4;
+        if (slot >= r0 && slot < r1) codes[d * 64 + p * 16 + e] = y.v[e];
+      }
+    }
   }
-  const bool zero = odd || top < kTiny;
-  const float up = zero ? 0.f : 127.f / top;
-  const int64_t item = (int64_t)b * a.kv_heads + g;
-  int8_t* codes = (which ? v_codes : k_codes) + item * a.slots * a.dim;
-  for (int d = 0; d < a.dim; ++d) {
-    const int8_t code = zero ? 0 : (int8_t)(int)rintf(to_float(x[d]) * up);
-    codes[which ? value_at((int)slot, d, a.dim) : slot * a.dim + d] = code;
-  }
-  (which ? v_scales : k_scales)[item * a.slots + slot] = odd ? NAN : zero ? 0.f : fminf(top, kMost) / 127.f;
 }
 
 // code * scale in float32.  Kept apart from its conversion: the two as one instruction round a float16 from
@@ -69,19 +135,49 @@ __device__ __forceinline__ float stands_for(float code, float scale) {
 
 template <class T>
 __global__ __launch_bounds__(256) void read_kernel(HeldArgs a, const int8_t* k_codes, const float* k_scales,
-                                                   const int8_t* v_codes, const float* v_scales, T* k, T* v) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t all = (int64_t)a.batch * a.tokens * a.kv_heads * a.dim;
-  if (i >= 2 * all) return;
-  const int which = i >= all;
-  const int64_t e = which ? i - all : i, r = e / a.dim, bt = r / a.kv_heads;
-  const int d = (int)(e - r * a.dim), g = (int)(r - bt * a.kv_heads);
-  const int b = (int)(bt / a.tokens), t = (int)(bt - (int64_t)b * a.tokens), slot = (int)a.start0 + t;
-  const int64_t item = (int64_t)b * a.kv_heads + g;
-  const int8_t* codes = (which ? v_codes : k_codes) + item * a.slots * a.dim;
-  const float code = (float)codes[which ? value_at(slot, d, a.dim) : (int64_t)slot * a.dim + d];
-  T* y = (which ? v : k) + b * a.s[which][0] + t * a.s[which][1] + g * a.s[which][2];
-  y[d] = from_float<T>(stands_for(code, (which ? v_scales : k_scales)[item * a.slots + slot]));
+                                                   const int8_t* v_codes, const float* v_scales, T* k, T* v, int tiles,
+                                                   int64_t units) {
+  __shared__ __attribute__((aligned(16))) int8_t placed[128 * kPlaces];
+  const int chunks = a.dim / 8, all = 64 * chunks;
+  const int first = (int)a.start0, end = first + a.tokens;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const Unit w = unit_of(a, u, tiles);
+    const int slot0 = (first / 64 + w.tile) * 64;
+    if (slot0 >= end) continue;
+    const int r0 = max(0, first - slot0), r1 = min(64, end - slot0);
+    const int64_t item = (int64_t)w.b * a.kv_heads + w.g;
+    const int8_t* codes = (w.which ? v_codes : k_codes) + (item * a.slots + slot0) * a.dim;
+    const float* scales = (w.which ? v_scales : k_scales) + item * a.slots + slot0;
+    T* y = (w.which ? v : k) + w.b * a.s[w.which][0] + w.g * a.s[w.which][2];
+    const int64_t ts = a.s[w.which][1];
+    if (w.which) {
+      __syncthreads();  // the unit before has been read
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int i = n * 256 + threadIdx.x, d = i / 4, p = i % 4;
+        if (d >= a.dim) break;
+        *(Vec<int8_t, 16>*)__builtin_assume_aligned(placed + d * kPlaces + p * 16, 16) = load_vec<16>(codes + d * 64 + p * 16);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int i = n * 256 + threadIdx.x, r = i / chunks, c = i - r * chunks;
+      if (i >= all || r < r0 || r >= r1) continue;
+      const float scale = scales[r];
+      Vec<int8_t, 8> x;
+      if (w.which) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x.v[e] = placed[(c * 8 + e) * kPlaces + place_of(r)];
+      } else {
+        x = load_vec<8>(codes + i * 8);
+      }
+      Vec<T, 8> o;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o.v[e] = from_float<T>(stands_for((float)x.v[e], scale));
+      store_vec(y + (int64_t)(slot0 + r - first) * ts + c * 8, o);
+    }
+  }
 }
 
 // The parts of rows: weighted by their largest logits and added up in order, a thread four channels.
@@ -151,11 +247,13 @@ void hold_tokens(const nnx_held_config& c, const void* k, const void* v, const i
   require(k && v, "hold tokens: null pointer");
   check_held(k_codes, k_scales, v_codes, v_scales, "hold tokens");
   const HeldArgs a = make_args(c, start, lengths, nullptr);
+  const int tiles = (int)ceil_div((int64_t)c.tokens + (start || c.start % 64 ? 63 : 0), 64);  // that tokens may lie in
+  const int64_t units = 2ll * c.batch * c.kv_heads * tiles;
   ProfScope prof("hold_tokens", 4.0 * rows * c.head_dim, rows * (c.head_dim * (type_bytes(c.type) + 1.0) + 4.0), st);
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    hold_kernel<T><<<(unsigned)ceil_div((int64_t)rows, 256), 256, 0, st>>>(
-        a, (const T*)k, (const T*)v, k_codes, k_scales, v_codes, v_scales);
+    hold_kernel<T><<<(unsigned)std::min<int64_t>(units, 1 << 20), 256, 0, st>>>(
+        a, (const T*)k, (const T*)v, k_codes, k_scales, v_codes, v_scales, tiles, units);
   });
   launch_check("hold_tokens");
 }
@@ -169,11 +267,13 @@ void read_held(const nnx_held_config& c, const int8_t* k_codes, const float* k_s
   require(k && v, "read held: null pointer");
   check_held(k_codes, k_scales, v_codes, v_scales, "read held");
   const HeldArgs a = make_args(c, nullptr, nullptr, nullptr);
+  const int tiles = (int)ceil_div(c.start % 64 + c.tokens, 64);
+  const int64_t units = 2ll * c.batch * c.kv_heads * tiles;
   ProfScope prof("read_held", rows * c.head_dim, rows * (c.head_dim * (type_bytes(c.type) + 1.0) + 4.0), st);
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    read_kernel<T><<<(unsigned)ceil_div((int64_t)rows * c.head_dim, 256), 256, 0, st>>>(
-        a, k_codes, k_scales, v_codes, v_scales, (T*)k, (T*)v);
+    read_kernel<T><<<(unsigned)std::min<int64_t>(units, 1 << 20), 256, 0, st>>>(
+        a, k_codes, k_scales, v_codes, v_scales, (T*)k, (T*)v, tiles, units);
   });
   launch_check("read_held");
 }
