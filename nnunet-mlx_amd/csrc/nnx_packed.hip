@@ -1,6 +1,7 @@
 // Products with 4-bit weights under group scales, and their packing.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "nnx_elements.h"
 
@@ -80,28 +81,198 @@ __device__ __forceinline__ float open_gate(float g, int act) {
   return act == NNX_GATE_SIGMOID ? s : g * s;
 }
 
-// A wave an output and row, a group at a time.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <class T>
-__global__ __launch_bounds__(64) void linear_kernel(PackedArgs a, const T* x, const uint8_t* codes, const float* scales,
-                                                    const float* bias, const uint8_t* gate_codes,
-                                                    const float* gate_scales, T* y) {
-  const int o = blockIdx.x;
-  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    auto product = [&](const uint8_t* codes, const float* scales) {
-      float sum = 0.f;
-      for (int g = 0; g * a.group < a.inputs; ++g) {
-        float part = 0.f;
-        for (int i = g * a.group + threadIdx.x; i < min((g + 1) * a.group, a.inputs); i += 64)
-          part = fmaf(to_float(x[row * a.xs + i]), level(codes[code_at(a, o, i)] >> (i % 2 * 4) & 15), part);
-        sum = fmaf(part, scales[scale_at(a, o, g)], sum);
+using Frag = T __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x4 mfma(Frag<f16> a, Frag<f16> b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(Frag<bf16> a, Frag<bf16> b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// What x is multiplied in: 16-bit types as they are, float32 in three bfloat16 operands that add up to it.
+template <class T>
+struct Operand {
+  using E = T;
+  static constexpr int kTerms = 1;
+};
+template <>
+struct Operand<float> {
+  using E = bf16;
+  static constexpr int kTerms = 3;
+};
+
+template <class T>
+__device__ __forceinline__ void split(const Vec<T, 8>& x, Frag<typename Operand<T>::E> (&q)[Operand<T>::kTerms]) {
+  if constexpr (sizeof(T) == 2) {
+    __builtin_memcpy(&q[0], &x, 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float left = x.v[e];
+#pragma unroll
+      for (int term = 0; term < 3; ++term) {
+        // cut, not rounded: the next bits, eight at a time
+        const float part = __uint_as_float(__float_as_uint(left) & 0xffff0000u);
+        q[term][e] = from_float<bf16>(part);
+        left -= part;
       }
-      return lanes_reduce<64>(sum, [](float p, float r) { return p + r; });
-    };
-    float u = product(codes, scales);
-    if (bias) u += bias[o];
-    if (gate_codes) u *= open_gate(product(gate_codes, gate_scales), a.act);
-    if (threadIdx.x == 0) y[row * a.ys + o] = from_float<T>(u);
+    }
   }
+}
+
+// Eight codes as E, exactly.
+template <class E>
+__device__ __forceinline__ Frag<E> decode(uint32_t w) {
+  u32x4 r;
+  if constexpr (std::is_same<E, bf16>::value) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 0));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 1));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 2));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 3));
+  } else {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.f, 0));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.f, 1));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.f, 2));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.f, 3));
+  }
+  Frag<E> f;
+  __builtin_memcpy(&f, &r, 16);
+  return f;
+}
+
+struct LinearArgs {
+  PackedArgs a;
+  const void* x;
+  const uint8_t* codes[2];
+  const float* scales[2];
+  const float* bias;
+  void* y;
+};
+
+// Eight elements of a row from `at` on, zeros past its end.
+template <class T>
+__device__ __forceinline__ Vec<T, 8> load_row(const T* row, int at, int end) {
+  if (at + 8 <= end) return load_vec<8>(row + at);
+  Vec<T, 8> x{};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (at + e < end) x.v[e] = row[at + e];
+  return x;
+}
+
+// A workgroup 16 outputs of 16 R rows, its waves blocks of 128 inputs in turn.  Weights are the matrix
+// instruction's rows, x its columns: a lane's 16 bytes of codes are its operands of four instructions, and
+// its results four neighbouring outputs of one row, which a group's scales multiply as they stand.
+template <class T, int R, int G32, int MATRICES>
+__global__ __launch_bounds__(512) void linear_few_kernel(LinearArgs h, int row_tiles, int64_t units) {
+  using E = typename Operand<T>::E;
+  constexpr int TERMS = Operand<T>::kTerms;
+  __shared__ __attribute__((aligned(16))) f32x4 sums[8][MATRICES * R][64];
+  const PackedArgs& a = h.a;
+  const int lane = threadIdx.x % 64, n16 = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int tile = (int)(u / row_tiles);
+    const int64_t row0 = (u - (int64_t)tile * row_tiles) * 16 * R;
+    const T* x[R];
+    bool live[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      live[r] = row0 + 16 * r + n16 < a.rows;
+      x[r] = (const T*)h.x + (live[r] ? row0 + 16 * r + n16 : 0) * a.xs;
+    }
+    f32x4 sum[MATRICES][R];
+#pragma unroll
+    for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+      for (int r = 0; r < R; ++r) sum[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int kb = wave; kb < a.blocks; kb += waves) {
+      u32x4 c[MATRICES];
+      f32x4 sc[MATRICES][4 / G32];
+#pragma unroll
+      for (int m = 0; m < MATRICES; ++m) {
+        const int64_t block = (int64_t)tile * a.blocks + kb;
+        c[m] = *(const u32x4*)__builtin_assume_aligned(h.codes[m] + block * 1024 + lane * 16, 16);
+#pragma unroll
+        for (int s = 0; s < 4 / G32; ++s)
+          sc[m][s] = *(const f32x4*)__builtin_assume_aligned(h.scales[m] + (block * (4 / G32) + s) * 16 + 4 * g, 16);
+      }
+      Vec<T, 8> xv[R][4];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          xv[r][j] = Vec<T, 8>{};
+          if (live[r]) xv[r][j] = load_row(x[r], kb * 128 + 32 * j + 8 * g, a.inputs);
+        }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        Frag<E> q[4][TERMS];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split(xv[r][j], q[j]);
+#pragma unroll
+        for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+          for (int s = 0; s < 4 / G32; ++s) {
+            f32x4 part{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = s * G32; j < (s + 1) * G32; ++j) {
+              const Frag<E> w = decode<E>(c[m][j]);
+#pragma unroll
+              for (int term = 0; term < TERMS; ++term) part = mfma(w, q[j][term], part);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[m][r][i] = fmaf(part[i], sc[m][s][i], sum[m][r][i]);
+          }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+      for (int r = 0; r < R; ++r) sums[wave][m * R + r][lane] = sum[m][r];
+    __syncthreads();
+    for (int r = wave; r < R; r += waves) {
+      const int64_t row = row0 + 16 * r + n16;
+      if (row >= a.rows) continue;
+      f32x4 u[MATRICES];
+#pragma unroll
+      for (int m = 0; m < MATRICES; ++m) {
+        u[m] = sums[0][m * R + r][lane];
+        for (int w = 1; w < waves; ++w) u[m] += sums[w][m * R + r][lane];
+      }
+      T* y = (T*)h.y + row * a.ys;
+      const int o = tile * 16 + 4 * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (o + i >= a.outputs) break;
+        float v = u[0][i];
+        if (h.bias) v += h.bias[o + i];
+        if constexpr (MATRICES == 2) v *= open_gate(u[1][i], a.act);
+        y[o + i] = from_float<T>(v);
+      }
+    }
+    __syncthreads();  // sums are read before the next unit's
+  }
+}
+
+template <class T, int G32, int MATRICES>
+void linear_launch(const LinearArgs& h, hipStream_t st) {
+  using std::integral_constant;
+  const int tiles = (int)ceil_div(h.a.outputs, 16);
+  auto go = [&](auto r) {
+    constexpr int R = decltype(r)::value;
+    const int waves = std::min(h.a.blocks, 8), row_tiles = (int)ceil_div(h.a.rows, 16 * R);
+    const int64_t units = (int64_t)tiles * row_tiles;
+    linear_few_kernel<T, R, G32, MATRICES>
+        <<<(unsigned)std::min<int64_t>(units, 1 << 20), 64 * waves, 0, st>>>(h, row_tiles, units);
+  };
+  if (h.a.rows <= 16) return go(integral_constant<int, 1>{});
+  if (h.a.rows <= 32) return go(integral_constant<int, 2>{});
+  go(integral_constant<int, 4>{});
 }
 
 void check_config(const nnx_packed_config& c, const char* name) {
@@ -165,8 +336,15 @@ void packed_linear(const nnx_packed_config& c, const void* x, const uint8_t* cod
                  n * (0.5 + 4.0 / c.group) + (double)c.rows * (c.inputs + c.outputs) * type_bytes(c.type), st);
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    const dim3 grid((unsigned)c.outputs, (unsigned)std::min<int64_t>(c.rows, 65535));
-    linear_kernel<T><<<grid, 64, 0, st>>>(a, (const T*)x, codes, scales, bias, gate_codes, gate_scales, (T*)y);
+    LinearArgs h{a, x, {codes, gate_codes}, {scales, gate_scales}, bias, y};
+    auto groups = [&](auto m) {
+      constexpr int M = decltype(m)::value;
+      if (c.group == 32) return linear_launch<T, 1, M>(h, st);
+      if (c.group == 64) return linear_launch<T, 2, M>(h, st);
+      linear_launch<T, 4, M>(h, st);
+    };
+    if (gate_codes) return groups(std::integral_constant<int, 2>{});
+    groups(std::integral_constant<int, 1>{});
   });
   launch_check("packed_linear");
 }
