@@ -19,7 +19,7 @@ struct HeldArgs {
 struct HeldPlan {
   int group, rows, r, tiles, splits;
   int64_t units;  // batch * kv_heads * tiles
-  size_t meta, bytes;  // the workspace: sums of values, then (largest logit, sum of weights) by unit, part and row
+  size_t meta, bytes;  // the workspace: results, then (reference logit, sum of weights), by key head, row and part
 };
 
 struct HeldAttention {
@@ -32,8 +32,12 @@ struct HeldAttention {
   float2* meta;
   int group, rows, tiles, splits;
   float query, c2;   // factors of the queries, a power of two, and of the keys' scales: scale * log2 e together
-  float unit, back;  // of the values: 2^-n, so that the sum of 2^n slots does not overflow, and 2^n
 };
+
+// 16 rows a wave or 32: two share what a code's conversion costs, where a wave's registers hold them beside two
+// waves a SIMD.
+constexpr bool held_pairs(int type, int dim) { return type != NNX_TYPE_F32 && dim <= 96; }
+inline int held_rows(int type, int dim, int rows) { return rows > 16 && held_pairs(type, dim) ? 2 : 1; }
 
 void held_units_f32(const HeldAttention& h, const HeldPlan& p, hipStream_t st);
 void held_units_f16(const HeldAttention& h, const HeldPlan& p, hipStream_t st);

@@ -11,6 +11,7 @@ namespace {
 
 constexpr float kTiny = 8.673617379884035e-19f;  // 2^-60
 constexpr float kMost = 3.4028233e38f;           // 127 * (kMost / 127) is finite
+constexpr int kMostSplits = 512;
 
 HeldArgs make_args(const nnx_held_config& c, const int32_t* start, const int32_t* lengths, const uint8_t* mask) {
   HeldArgs a;
@@ -180,34 +181,55 @@ __global__ __launch_bounds__(256) void read_kernel(HeldArgs a, const int8_t* k_c
   }
 }
 
-// The parts of rows: weighted by their largest logits and added up in order, a thread four channels.
+// The parts' results of rows, weighted by their sums relative to the largest reference and added up in order:
+// a workgroup a row, its threads four channels of every 1024 / dim-th part.
 template <class T>
 __global__ __launch_bounds__(256) void join_kernel(HeldAttention h) {
-  const int quads = h.a.dim / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / quads;
-  if (row >= (int64_t)h.a.batch * h.a.kv_heads * h.rows) return;
-  const int d = (int)(i - row * quads) * 4;
-  const int64_t bg = row / h.rows;
-  const int b = (int)(bg / h.a.kv_heads), kh = (int)(bg - (int64_t)b * h.a.kv_heads), mine = (int)(row - bg * h.rows);
-  const int64_t first = bg * h.splits * h.rows + mine;
-  float top = -INFINITY, l = 0.f, o[4] = {};
-  for (int s = 0; s < h.splits; ++s) top = fmaxf(top, h.meta[first + (int64_t)s * h.rows].x);
-  for (int s = 0; s < h.splits; ++s) {
-    const int64_t at = first + (int64_t)s * h.rows;
-    const float2 m = h.meta[at];
-    const float4 v = *(const float4*)__builtin_assume_aligned(h.part + at * h.a.dim + d, 16);
-    // nothing seen: sums of zero, or of NaN logits
-    const float w = m.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m.x - top);
-    l = fmaf(m.y, w, l);
-    o[0] = fmaf(v.x, w, o[0]), o[1] = fmaf(v.y, w, o[1]), o[2] = fmaf(v.z, w, o[2]), o[3] = fmaf(v.w, w, o[3]);
+  __shared__ float weights[kMostSplits], reds[8];
+  __shared__ __attribute__((aligned(16))) float4 sums[256];
+  const int quads = h.a.dim / 4, lanes = 256 / quads;
+  const int64_t bg = blockIdx.x / h.rows;
+  const int mine = (int)(blockIdx.x - bg * h.rows);
+  const int b = (int)(bg / h.a.kv_heads), kh = (int)(bg - (int64_t)b * h.a.kv_heads);
+  const int64_t first = (int64_t)blockIdx.x * h.splits;
+  float top = -INFINITY, l = 0.f;
+  for (int s = threadIdx.x; s < h.splits; s += 256) top = fmaxf(top, h.meta[first + s].x);
+  top = lanes_reduce<64>(top, [](float u, float v) { return fmaxf(u, v); });
+  if (threadIdx.x % 64 == 0) reds[threadIdx.x / 64] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(reds[0], reds[1]), fmaxf(reds[2], reds[3]));
+  for (int s = threadIdx.x; s < h.splits; s += 256) {
+    const float2 m = h.meta[first + s];
+    // nothing seen: a sum of 0, or of NaN logits
+    const float w = m.x == -INFINITY ? m.y : m.y * __builtin_amdgcn_exp2f(m.x - top);
+    weights[s] = w;
+    l += w;
+  }
+  l = lanes_reduce<64>(l, [](float u, float v) { return u + v; });
+  if (threadIdx.x % 64 == 0) reds[4 + threadIdx.x / 64] = l;
+  __syncthreads();
+  l = (reds[4] + reds[5]) + (reds[6] + reds[7]);
+  const float share = l == 0.f ? 0.f : 1.f / l;
+  const int part = threadIdx.x / quads, d = (threadIdx.x - part * quads) * 4;
+  float4 o{0.f, 0.f, 0.f, 0.f};
+  if (part < lanes) {
+#pragma unroll 4
+    for (int s = part; s < h.splits; s += lanes) {
+      const float w = weights[s] * share;
+      const float4 v = *(const float4*)__builtin_assume_aligned(h.part + (first + s) * h.a.dim + d, 16);
+      o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
+    }
+  }
+  sums[threadIdx.x] = o;
+  __syncthreads();
+  if (part != 0) return;
+  for (int i = 1; i < lanes; ++i) {
+    const float4 v = sums[i * quads + threadIdx.x];
+    o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
   }
   const int t = mine / h.group, hd = mine - t * h.group;
   T* out = (T*)h.out + b * h.a.s[1][0] + t * h.a.s[1][1] + (int64_t)(kh * h.group + hd) * h.a.s[1][2] + d;
-  const float whole = l == 0.f && top == -INFINITY ? 0.f : 1.f / l;  // nothing seen: zeros
-  Vec<T, 4> y;
-  for (int k = 0; k < 4; ++k) y.v[k] = from_float<T>(o[k] * whole * h.back);
-  store_vec(out, y);
+  store_vec(out, Vec<T, 4>{from_float<T>(o.x), from_float<T>(o.y), from_float<T>(o.z), from_float<T>(o.w)});
 }
 
 void check_config(const nnx_held_config& c, const char* name, bool attention) {
@@ -284,12 +306,12 @@ HeldPlan make_plan(const nnx_held_config& c) {
   HeldPlan p;
   p.group = c.heads / c.kv_heads;
   p.rows = c.tokens * p.group;
-  p.r = p.rows <= 16 ? 1 : 2;
+  p.r = held_rows(c.type, c.head_dim, p.rows);
   p.tiles = (int)ceil_div(p.rows, 16 * p.r);
   p.units = (int64_t)c.batch * c.kv_heads * p.tiles;
   // parts of at least 4 tiles of 64 slots, a wave each, while two workgroups a CU are not reached
-  p.splits = (int)std::max<int64_t>(1, std::min(512 / p.units, ceil_div(c.keys, 256)));
-  require(p.units * p.splits < 1 << 24, "held attention: fewer than 2^24 items times key heads times tiles of 32 rows");
+  p.splits = (int)std::max<int64_t>(1, std::min(kMostSplits / p.units, ceil_div(c.keys, 256)));
+  require(p.units * p.splits < 1 << 24, "held attention: fewer than 2^24 items times key heads times tiles of rows");
   p.meta = p.bytes = 0;
   if (p.splits > 1) {
     const size_t rows = (size_t)c.batch * c.kv_heads * p.splits * p.rows;
@@ -326,10 +348,9 @@ void held_attention(const nnx_held_config& c, const void* q, const int8_t* k_cod
   const float factor = c.scale * 1.4426950408889634f;
   const float query = c.type == NNX_TYPE_F16 || factor == 0.f
                           ? 1.f : std::exp2(std::min(20.f, std::max(-16.f, std::ceil(std::log2(std::fabs(factor) / 64.f)))));
-  const float many = std::ceil(std::log2((float)c.keys));
   HeldAttention h{make_args(c, start, lengths, mask), q, k_codes, v_codes, k_scales, v_scales, out, (float*)ws,
                   (float2*)((char*)ws + p.meta), p.group, p.rows, p.tiles, p.splits,
-                  query, factor / query, std::exp2(-many), std::exp2(many)};
+                  query, factor / query};
   const double rows = (double)c.batch * c.tokens * c.heads;
   ProfScope prof("held_attention", 4.0 * rows * c.keys * c.head_dim,
                  2.0 * rows * c.head_dim * type_bytes(c.type) +
@@ -345,8 +366,7 @@ void held_attention(const nnx_held_config& c, const void* q, const int8_t* k_cod
   if (p.splits == 1) return;
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    const int64_t threads = (int64_t)rows * (c.head_dim / 4);
-    join_kernel<T><<<(unsigned)ceil_div(threads, 256), 256, 0, st>>>(h);
+    join_kernel<T><<<(unsigned)(int64_t)rows, 256, 0, st>>>(h);
   });
   launch_check("held_join");
 }

@@ -22,20 +22,27 @@ __device__ __forceinline__ f32x4 mfma(Frag<bf16> a, Frag<bf16> b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Eight codes as E, exactly.
+// Eight codes as E, exactly.  float16: a code's byte under 0x64 is 1024 + (code + 128), less 1152 in pairs: 5
+// instructions for 4 codes; bfloat16 takes 6, through float32.
 template <class E>
 __device__ __forceinline__ Frag<E> codes_to(uint32_t lo, uint32_t hi) {
   u32x4 r;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int w = (int)(i ? hi : lo);
-    const float f0 = (float)(int8_t)w, f1 = (float)(int8_t)(w >> 8), f2 = (float)(int8_t)(w >> 16), f3 = (float)(w >> 24);
+    const uint32_t w = i ? hi : lo;
     if constexpr (std::is_same<E, bf16>::value) {
+      const int v = (int)w;
+      const float f0 = (float)(int8_t)v, f1 = (float)(int8_t)(v >> 8), f2 = (float)(int8_t)(v >> 16), f3 = (float)(v >> 24);
       r[2 * i] = __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302);
       r[2 * i + 1] = __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302);
     } else {
-      r[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(f0, f1));
-      r[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(f2, f3));
+      typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+      const f16x2 less = {1152.f, 1152.f};
+      const uint32_t above = w ^ 0x80808080u;
+      const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, above, 0x04010400)) - less;
+      const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, above, 0x04030402)) - less;
+      r[2 * i] = __builtin_bit_cast(uint32_t, a);
+      r[2 * i + 1] = __builtin_bit_cast(uint32_t, b);
     }
   }
   Frag<E> f;
@@ -52,20 +59,29 @@ __device__ __forceinline__ float rows_reduce(float v, F op) {
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// What a query's element is multiplied in: float16 as it is, the others in bfloat16 operands that add up to it.
+// What a query's element is multiplied in: 16-bit types as they are, float32 in bfloat16 operands that add up to it.
 template <class T>
 struct Query {
-  using E = bf16;
-  static constexpr int kTerms = std::is_same<T, float>::value ? 3 : 1;
-};
-template <>
-struct Query<f16> {
-  using E = f16;
+  using E = T;
   static constexpr int kTerms = 1;
 };
-// A weight times its value's scale goes into the second product as two bfloat16 operands (16 bits), of float32 three.
+template <>
+struct Query<float> {
+  using E = bf16;
+  static constexpr int kTerms = 3;
+};
+
+// A weight times its value's scale is one float16 operand of the second product for bfloat16 results (2^-12 of
+// every weight, where the result keeps 2^-9), and for the others two, its rounded value and the rest (2^-23).
 template <class T>
-constexpr int kWeightTerms = std::is_same<T, float>::value ? 3 : 2;
+constexpr int kWeightTerms = std::is_same<T, bf16>::value ? 1 : 2;
+
+// Values' scales are taken relative to a power of two at or above the largest so far, and a row's weights to a
+// logit that a tile leaves alone while 16 slots' weights add up to kMostWeight at most (the largest is only looked for
+// when they do not).  2^kRoom puts their products in float16's range: they pass no kMostWeight 2^kRoom = 2^15,
+// and are normal down to 2^(-14 - kRoom).
+constexpr float kMostWeight = 32.f;
+constexpr int kRoom = 10;
 
 // A wave's rows: 16 to a matrix instruction's columns, R of those.  Lane l = 16 g + n has row n; of 64
 // slots the logits of 16 t + 4 g + i (t, i < 4), which are the second product's operand as they
@@ -75,8 +91,10 @@ struct Rows {
   static constexpr int KF = DP / 32, CT = DP / 16, QT = Query<T>::kTerms;
   Frag<typename Query<T>::E> q[R][QT][KF];
   f32x4 o[R][CT];
-  float m[R], l[R];  // l of the lane's slots only
-  int count[R];      // slots that the row sees, but for the mask
+  // the logit that weights are relative to, how much the weights of 16 slots may add up to before it moves (-1:
+  // nothing seen yet), and the sum of the weights of the lane's slots
+  float ref[R], most[R], l[R];
+  int count[R];  // slots that the row sees, but for the mask
 };
 
 // 64 slots' codes as a wave holds them.
@@ -85,13 +103,13 @@ struct Codes {
   static constexpr int K16 = DP / 64, K8 = DP % 64 / 32;
   u32x4 k[4][K16 ? K16 : 1];
   u32x2 k8[4];
-  f32x4 ks[4];
 };
-template <int DP>
-struct Values {
-  u32x4 v[DP / 16];
-  f32x4 vs[4];
-};
+
+// op over all 64 lanes.
+template <class F>
+__device__ __forceinline__ float wave_reduce(float v, F op) {
+  return rows_reduce(lanes_reduce<16>(v, op), op);
+}
 
 // First dimension of the eight that fragment s takes in lane group g: 16 bytes a lane in whole 64s, 8 in what is left.
 template <int DP>
@@ -100,13 +118,14 @@ __device__ __forceinline__ int dims_at(int s, int g) {
 }
 
 template <class T, int DP, int R>
-__global__ __launch_bounds__(256) void held_kernel(HeldAttention h) {
+__global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
   using Q = Query<T>;
   using E = typename Q::E;
   using Row = Rows<T, DP, R>;
   constexpr int KF = Row::KF, CT = Row::CT, WT = kWeightTerms<T>;
   __shared__ __attribute__((aligned(16))) f32x4 exchange[2][R * CT][64];
   __shared__ float exchange_ml[2][2 * R][64];
+  __shared__ __attribute__((aligned(16))) float slot_scales[4][128];
   const HeldArgs& a = h.a;
   const int lane = threadIdx.x % 64, n16 = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -139,17 +158,22 @@ __global__ __launch_bounds__(256) void held_kernel(HeldAttention h) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float left = to_float(x.v[e]) * h.query;
+        if constexpr (Q::kTerms == 1) {
+          w.q[r][0][s][e] = from_float<E>(left);
+        } else {
 #pragma unroll
-        for (int term = 0; term < Q::kTerms; ++term) {
-          const E part = from_float<E>(left);
-          w.q[r][term][s][e] = part;
-          left -= to_float(part);
+          for (int term = 0; term < Q::kTerms; ++term) {
+            // cut, not rounded: the next bits, eight at a time
+            const float part = __uint_as_float(__float_as_uint(left) & 0xffff0000u);
+            w.q[r][term][s][e] = from_float<E>(part);
+            left -= part;
+          }
         }
       }
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c) w.o[r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    w.m[r] = -INFINITY, w.l[r] = 0.f;
+    w.ref[r] = 0.f, w.most[r] = -1.f, w.l[r] = 0.f;
     w.count[r] = live ? sees(row) : 0;
   }
 
@@ -160,49 +184,72 @@ __global__ __launch_bounds__(256) void held_kernel(HeldAttention h) {
   const float* ks = h.k_scales + item * a.slots;
   const float* vs = h.v_scales + item * a.slots;
   const uint8_t* mask = a.mask ? a.mask + b * a.ms : nullptr;
-  auto load_keys = [&](Codes<DP>& c, int j) {
+  // Offsets of the lane in a tile of 64 slots, whose start is the wave's own.  Past the end of a row of keys: any
+  // codes, the query is zero there; of values: results that are not stored.
+  uint32_t key_at[Codes<DP>::K16 + 1];
+#pragma unroll
+  for (int s = 0; s <= Codes<DP>::K16; ++s) {
+    const int d = s < Codes<DP>::K16 ? 64 * s + 16 * g : DP / 64 * 64 + 8 * g;
+    key_at[s] = n16 * a.dim + (d < a.dim ? d : 0);
+  }
+  const uint32_t value_at = n16 * 64 + 16 * g;
+  const int last_channels = a.dim / 16 - 1;
+  // scales a lane a slot, spread to the lanes that need them through LDS
+  float* scales = slot_scales[wave];
+  Codes<DP> keys;
+  u32x4 values[CT];
+  float key_scale, value_scale;
+  bool shown = true;
+  auto load_keys = [&](int j) {
+    const int8_t* at = kc + (int64_t)j * 64 * a.dim;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int8_t* row = kc + ((int64_t)j * 64 + 16 * t + n16) * a.dim;
 #pragma unroll
-      for (int s = 0; s < Codes<DP>::K16; ++s) {
-        const int d = 64 * s + 16 * g;  // past the end: any codes, the query is zero there
-        c.k[t][s] = *(const u32x4*)__builtin_assume_aligned(row + (d < a.dim ? d : 0), 16);
-      }
-      if constexpr (Codes<DP>::K8) {
-        const int d = DP / 64 * 64 + 8 * g;
-        c.k8[t] = *(const u32x2*)__builtin_assume_aligned(row + (d < a.dim ? d : 0), 8);
-      }
-      c.ks[t] = *(const f32x4*)__builtin_assume_aligned(ks + (int64_t)j * 64 + 16 * t + 4 * g, 16);
+      for (int s = 0; s < Codes<DP>::K16; ++s)
+        keys.k[t][s] = *(const u32x4*)__builtin_assume_aligned(at + 16 * t * a.dim + key_at[s], 16);
+      if constexpr (Codes<DP>::K8 != 0)
+        keys.k8[t] = *(const u32x2*)__builtin_assume_aligned(at + 16 * t * a.dim + key_at[Codes<DP>::K16], 8);
     }
+    key_scale = ks[(int64_t)j * 64 + lane];
+    value_scale = vs[(int64_t)j * 64 + lane];
+    if (mask) shown = mask[min(64 * j + lane, a.keys - 1)];
   };
-  auto load_values = [&](Values<DP>& c, int j) {
+  auto load_values = [&](int j) {
+    const int8_t* at = vc + (int64_t)j * 64 * a.dim;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int channels = min(16 * ct, a.dim - 16);
-      c.v[ct] = *(const u32x4*)__builtin_assume_aligned(vc + (int64_t)j * 64 * a.dim + (channels + n16) * 64 + 16 * g, 16);
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-      c.vs[t] = *(const f32x4*)__builtin_assume_aligned(vs + (int64_t)j * 64 + 16 * t + 4 * g, 16);
+    for (int c = 0; c < CT; ++c)
+      values[c] = *(const u32x4*)__builtin_assume_aligned(at + min(c, last_channels) * 1024 + value_at, 16);
   };
 
-  Codes<DP> keys;
-  Values<DP> values;
+  int exponent = -70;  // of the values' power of two; held scales other than 0 are above it
+  const auto larger = [](float u, float v) { return fmaxf(u, v); };
   int j = j0 + wave;
   if (j < j1) {
-    load_keys(keys, j);
-    load_values(values, j);
+    load_keys(j);
+    load_values(j);
   }
   for (; j < j1; j += 4) {
     // which of the 64 slots are seen, but for each row's own end
-    uint64_t seen = ~0ull;
-    if (mask) seen = __ballot(64 * j + lane < a.keys && mask[min(64 * j + lane, a.keys - 1)]);
+    shown = shown && 64 * j + lane < most;
+    const uint64_t seen = __ballot(shown);
     const bool whole = seen == ~0ull && 64 * (j + 1) <= least;
-    f32x4 x[R][4];  // logits in units of log 2
+    const float mine = shown ? value_scale : 0.f;
+    if (__any(mine > __builtin_amdgcn_ldexpf(1.f, exponent))) {
+      const int next = __builtin_amdgcn_frexp_expf(wave_reduce(mine, larger));
+      const float back = __builtin_amdgcn_ldexpf(1.f, exponent - next);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) w.o[r][c] *= back;
+      exponent = __builtin_amdgcn_readfirstlane(next);
+    }
+    wave_sync();
+    scales[lane] = key_scale * h.c2;
+    scales[64 + lane] = __builtin_amdgcn_ldexpf(mine, kRoom - exponent);
+    wave_sync();
+    f32x4 x[R][4];  // logits in units of log 2, relative to the row's reference
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      keys.ks[t] *= h.c2;
 #pragma unroll
       for (int r = 0; r < R; ++r) x[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -218,72 +265,126 @@ __global__ __launch_bounds__(256) void held_kernel(HeldAttention h) {
 #pragma unroll
           for (int term = 0; term < Q::kTerms; ++term) x[r][t] = mfma(k, w.q[r][term][s], x[r][t]);
       }
-#pragma unroll
-      for (int r = 0; r < R; ++r) x[r][t] *= keys.ks[t];
     }
-    if (j + 4 < j1) load_keys(keys, j + 4);
+    __builtin_amdgcn_sched_barrier(0);
+    load_keys(min(j + 4, j1 - 1));  // the last again: no branch, which would double the registers
 #pragma unroll
-    for (int t = 0; t < 4; ++t) values.vs[t] *= h.unit;
-    Frag<bf16> p[R][WT][2];
+    for (int t = 0; t < 4; ++t) {
+      const f32x4 by = *(const f32x4*)__builtin_assume_aligned(scales + 16 * t + 4 * g, 16);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[r][t][i] = fmaf(x[r][t][i], by[i], -w.ref[r]);
+    }
+    // of the lane's four slots from 16 t + 4 g on, those that the row sees
+    const auto row_sees = [&](int r, int t) {
+      const int first = 16 * t + 4 * g, end = min(max(w.count[r] - 64 * j - first, 0), 4);
+      return (uint32_t)(seen >> first) & ((1u << end) - 1);
+    };
+    if (!whole) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t bits = row_sees(r, t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[r][t][i] = bits & (1u << i) ? x[r][t][i] : -INFINITY;
+        }
+    }
+    Frag<f16> p[R][WT][2];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int end = whole ? 64 : w.count[r] - 64 * j;
-      auto hidden = [&](int t, int i) {
-        const int slot = 16 * t + 4 * g + i;
-        return !((seen >> slot) & 1) || slot >= end;
-      };
-      if (!whole) {
+      f32x4 e[4];
+      const auto weights = [&] {
+        f32x4 sum{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[r][t][i] = hidden(t, i) ? -INFINITY : x[r][t][i];
-      }
-      float top = -INFINITY;
+          for (int i = 0; i < 4; ++i) {
+            e[t][i] = __builtin_amdgcn_exp2f(x[r][t][i]);
+            sum[i] += e[t][i];
+          }
+        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      };
+      float sum = weights();
+      if (__any(sum > w.most[r])) {
+        float top = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, x[r][t][i]);
-      top = fmaxf(w.m[r], rows_reduce(top, [](float u, float v) { return fmaxf(u, v); }));
-      if (__any(top > w.m[r])) {
-        const float back = w.m[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m[r] - top);
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, x[r][t][i]);
+        top = rows_reduce(top, larger);
+        // by the row's own weights: what other rows do does not show
+        const bool first = w.most[r] < 0.f;
+        const bool moves = rows_reduce(sum, larger) > w.most[r] && top > (first ? -INFINITY : 0.f);
+        const float next = moves ? w.ref[r] + top : w.ref[r], by = next - w.ref[r];
+        const float back = first ? 1.f : __builtin_amdgcn_exp2f(-by);
         w.l[r] *= back;
 #pragma unroll
         for (int c = 0; c < CT; ++c) w.o[r][c] *= back;
-        w.m[r] = top;
-      }
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[r][t][i] -= by;
+        w.ref[r] = next;
+        w.most[r] = moves ? kMostWeight : w.most[r];
+        sum = weights();
+      }
+      w.l[r] += sum;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const f32x4 by = *(const f32x4*)__builtin_assume_aligned(scales + 64 + 16 * t + 4 * g, 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(x[r][t][i] - base);
-          sum += e;
-          float left = e * values.vs[t][i];
-          if (!whole) left = hidden(t, i) ? 0.f : left;
+          float left = e[t][i] * by[i];
 #pragma unroll
           for (int term = 0; term < WT; ++term) {
-            const bf16 part = from_float<bf16>(left);
+            const f16 part = from_float<f16>(left);
             p[r][term][t / 2][t % 2 * 4 + i] = part;
             left -= to_float(part);
           }
         }
-      w.l[r] += sum;
+      }
     }
+    if (!whole) {  // a weight of 0 keeps out no value that is not a number
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t bits = row_sees(r, t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int term = 0; term < WT; ++term)
+              p[r][term][t / 2][t % 2 * 4 + i] = bits & (1u << i) ? p[r][term][t / 2][t % 2 * 4 + i] : (f16)0.f;
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const Frag<bf16> v = codes_to<bf16>(values.v[c][2 * u], values.v[c][2 * u + 1]);
+        const Frag<f16> v = codes_to<f16>(values[c][2 * u], values[c][2 * u + 1]);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int term = 0; term < WT; ++term) w.o[r][c] = mfma(v, p[r][term][u], w.o[r][c]);
       }
-    if (j + 4 < j1) load_values(values, j + 4);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(min(j + 4, j1 - 1));
   }
+  // the row's own result over its slots, with (reference, sum of weights) to join it by
+  float m[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) w.l[r] = rows_reduce(w.l[r], [](float u, float v) { return u + v; });
+  for (int r = 0; r < R; ++r) {
+    w.l[r] = rows_reduce(w.l[r], [](float u, float v) { return u + v; });
+    m[r] = w.most[r] < 0.f ? -INFINITY : w.ref[r];
+    const float whole = w.l[r] == 0.f ? 0.f : 1.f / w.l[r];
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w.o[r][c][i] = __builtin_amdgcn_ldexpf(w.o[r][c][i] * whole, exponent - kRoom);
+  }
 
   // waves 2 and 3 into 0 and 1, then 1 into 0; lanes hold the same places
 #pragma unroll
@@ -291,7 +392,7 @@ __global__ __launch_bounds__(256) void held_kernel(HeldAttention h) {
     if (wave >= step && wave < 2 * step) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        exchange_ml[wave - step][2 * r][lane] = w.m[r];
+        exchange_ml[wave - step][2 * r][lane] = m[r];
         exchange_ml[wave - step][2 * r + 1][lane] = w.l[r];
 #pragma unroll
         for (int c = 0; c < CT; ++c) exchange[wave - step][r * CT + c][lane] = w.o[r][c];
@@ -301,13 +402,15 @@ __global__ __launch_bounds__(256) void held_kernel(HeldAttention h) {
     if (wave < step) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float m = exchange_ml[wave][2 * r][lane], top = fmaxf(m, w.m[r]);
-        const float mine = w.m[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(w.m[r] - top);
-        const float theirs = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
-        w.l[r] = w.l[r] * mine + exchange_ml[wave][2 * r + 1][lane] * theirs;
+        const float m1 = exchange_ml[wave][2 * r][lane], l1 = exchange_ml[wave][2 * r + 1][lane], top = fmaxf(m1, m[r]);
+        // nothing seen: a sum of 0, or of NaN logits
+        const float mine = m[r] == -INFINITY ? w.l[r] : w.l[r] * __builtin_amdgcn_exp2f(m[r] - top);
+        const float theirs = m1 == -INFINITY ? l1 : l1 * __builtin_amdgcn_exp2f(m1 - top);
+        const float l = mine + theirs, share = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-        for (int c = 0; c < CT; ++c) w.o[r][c] = w.o[r][c] * mine + exchange[wave][r * CT + c][lane] * theirs;
-        w.m[r] = top;
+        for (int c = 0; c < CT; ++c)
+          w.o[r][c] = w.o[r][c] * (mine * share) + exchange[wave][r * CT + c][lane] * (theirs * share);
+        m[r] = top, w.l[r] = l;
       }
     }
     __syncthreads();
@@ -320,21 +423,20 @@ __global__ __launch_bounds__(256) void held_kernel(HeldAttention h) {
     if (h.splits == 1) {
       const int t = row / h.group, hd = row - t * h.group;
       T* out = (T*)h.out + b * a.s[1][0] + t * a.s[1][1] + (int64_t)(kh * h.group + hd) * a.s[1][2];
-      const float whole = w.l[r] == 0.f && w.m[r] == -INFINITY ? 0.f : 1.f / w.l[r];  // nothing seen: zeros
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         if (16 * c >= a.dim) break;
         Vec<T, 4> y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y.v[i] = from_float<T>(w.o[r][c][i] * whole * h.back);
+        for (int i = 0; i < 4; ++i) y.v[i] = from_float<T>(w.o[r][c][i]);
         store_vec(out + 16 * c + 4 * g, y);
       }
     } else {
-      const int64_t at = ((int64_t)bg * h.splits + split) * h.rows + row;
+      const int64_t at = ((int64_t)bg * h.rows + row) * h.splits + split;
 #pragma unroll
       for (int c = 0; c < CT; ++c)
         if (16 * c < a.dim) *(f32x4*)__builtin_assume_aligned(h.part + at * a.dim + 16 * c + 4 * g, 16) = w.o[r][c];
-      if (g == 0) h.meta[at] = make_float2(w.m[r], w.l[r]);
+      if (g == 0) h.meta[at] = make_float2(m[r], w.l[r]);
     }
   }
 }
@@ -350,8 +452,10 @@ void held_units(const HeldAttention& h, const HeldPlan& p, hipStream_t st) {
   using std::integral_constant;
   auto rows = [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    if (p.r == 1) return held_launch<T, DP, 1>(h, p, st);
-    held_launch<T, DP, 2>(h, p, st);
+    if constexpr (!std::is_same<T, float>::value && DP <= 96) {
+      if (p.r == 2) return held_launch<T, DP, 2>(h, p, st);
+    }
+    held_launch<T, DP, 1>(h, p, st);
   };
   if (h.a.dim <= 32) return rows(integral_constant<int, 32>{});
   if (h.a.dim <= 64) return rows(integral_constant<int, 64>{});

@@ -6,8 +6,9 @@ Codes and scales are elementwise float32 steps and compare exactly, and so does 
 Attention, U a type's unit roundoff, u = 2^-24.  A float32 logit of D products is off by at most
 (D + 4) u times the sum of their magnitudes; a weight's relative error is that of its own logit plus
 that of the others in the softmax's sum, at most twice the largest, plus 4 u for the power of two.  A
-16-bit type's weights may be held in two bfloat16 operands (2^-17), float32's in three (u); the sums
-over n slots are off by at most n u.  All of this moves an output by its relative size times the
+bfloat16 result's weights may be held in one float16 operand (half a step of 2^-11: 2^-12), the others'
+in two, the second of what the first leaves (2^-12 of 2^-12: u); the sums over n slots are off by at most
+n u.  All of this moves an output by its relative size times the
 weighted mean of the slots' largest |v|, twice where the weights' sum is off too; then the result is
 rounded once.  In relative L2 errors do not agree in sign, and n roundings of one size make sqrt(n) of
 them: D in a logit, of the logits' size L, twice in a weight; n in the sums; the weights' operands and 8
@@ -183,7 +184,8 @@ def _attend_check(q, held, n, dtype, *, lengths, scale=None, causal=False, start
         @ np.abs(k).transpose(0, 2, 3, 1) if n else np.zeros((batch, see.shape[2], queries * group, 1))
     largest = span.max(-1).reshape(batch, -1, queries, group).swapaxes(1, 2).reshape(batch, queries, heads)
     u = 2.0**-24
-    weight = 2 * ((dim + 4) * u * largest * abs(factor) + 4 * u) + (u if dtype == torch.float32 else 2.0**-17)
+    operands = 2.0**-12 if dtype == torch.bfloat16 else u
+    weight = 2 * ((dim + 4) * u * largest * abs(factor) + 4 * u) + operands
     bound = U[dtype] * np.abs(want) + (size * (2 * weight + 2 * n * u))[..., None] + 1e-30
     off = np.abs(_f64(got) - want)
     assert (off <= bound).all(), (off / bound).max()
@@ -191,7 +193,6 @@ def _attend_check(q, held, n, dtype, *, lengths, scale=None, causal=False, start
         rel = np.linalg.norm(_f64(got) - want) / np.linalg.norm(want)
         rows = _f64(q).reshape(batch, queries, -1, group, dim).swapaxes(1, 2).reshape(batch, -1, queries * group, dim)
         logit = np.abs(rows @ k.transpose(0, 2, 3, 1)).max() * abs(factor)
-        operands = u if dtype == torch.float32 else 2.0**-17
         most = U[dtype] + operands + (2 * dim**0.5 * logit + n**0.5 + 8) * u
         assert rel <= most, (rel, most)
 
