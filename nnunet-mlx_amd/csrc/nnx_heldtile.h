@@ -105,6 +105,16 @@ struct Codes {
   u32x2 k8[4];
 };
 
+// Units of one key head and part lie next to each other and read the same slots: kTogether of them run on one
+// XCD, then the next XCD's turn comes, so that heads of different lengths are spread over all.
+constexpr int kTogether = 4;
+__device__ __forceinline__ int unit_of_block(int block, int blocks) {
+  constexpr int kXcds = 8;
+  if (block >= blocks / (kXcds * kTogether) * (kXcds * kTogether)) return block;
+  const int xcd = block % kXcds, at = block / kXcds;
+  return (at / kTogether * kXcds + xcd) * kTogether + at % kTogether;
+}
+
 // op over all 64 lanes.
 template <class F>
 __device__ __forceinline__ float wave_reduce(float v, F op) {
@@ -129,9 +139,9 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
   const HeldArgs& a = h.a;
   const int lane = threadIdx.x % 64, n16 = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  // units of one key head and part next to each other, on one XCD: they read the same slots
-  const int unit = xcd_remap(blockIdx.x, gridDim.x);
-  const int tile = unit % h.tiles, rest = unit / h.tiles, split = rest % h.splits, bg = rest / h.splits;
+  const int unit = unit_of_block(blockIdx.x, gridDim.x);
+  const int rest = unit / h.tiles, split = rest % h.splits, bg = rest / h.splits;
+  const int tile = h.tiles - 1 - (unit - rest * h.tiles);  // causal rows: those that see most first
   const int b = bg / a.kv_heads, kh = bg - b * a.kv_heads;
   const int64_t item = bg;
 
