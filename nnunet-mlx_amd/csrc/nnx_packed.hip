@@ -259,6 +259,140 @@ __global__ __launch_bounds__(512) void linear_few_kernel(LinearArgs h, int row_t
   }
 }
 
+// A workgroup 64 outputs of 64 rows, a wave 32 of 32.  Blocks of 128 inputs of x go through LDS, split into
+// operands once; a block's weights are the waves' own, as above.  Chunk c (8 inputs) of row r lies at place
+// c * 64 + (r ^ c), so that neither the rows' chunks on their way in nor the chunks' rows on their way out meet
+// in a bank.
+template <class T, int G32, int MATRICES>
+__global__ __launch_bounds__(256) void linear_many_kernel(LinearArgs h, int row_tiles, int64_t units) {
+  using E = typename Operand<T>::E;
+  constexpr int TERMS = Operand<T>::kTerms, BUFFERS = TERMS == 1 ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) Frag<E> staged[BUFFERS][TERMS][16 * 64];
+  const PackedArgs& a = h.a;
+  const int lane = threadIdx.x % 64, n16 = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave % 2, wo = wave / 2;
+  const int last_tile = (a.outputs - 1) / 16;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int tile0 = (int)(u / row_tiles) * 4 + wo * 2;
+    const int64_t row0 = (u - u / row_tiles * row_tiles) * 64;
+    // the thread's chunks of x: chunk threadIdx % 16 of rows threadIdx / 16 + 16 n
+    const int chunk = threadIdx.x % 16;
+    Vec<T, 8> x[4];
+    u32x4 c[MATRICES][2];
+    f32x4 sc[MATRICES][2][4 / G32];
+    const auto load_x = [&](int kb) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int64_t row = row0 + threadIdx.x / 16 + 16 * n;
+        x[n] = Vec<T, 8>{};
+        if (row < a.rows) x[n] = load_row((const T*)h.x + row * a.xs, kb * 128 + chunk * 8, a.inputs);
+      }
+    };
+    const auto load_weights = [&](int kb) {
+#pragma unroll
+      for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int64_t block = (int64_t)min(tile0 + t, last_tile) * a.blocks + kb;
+          c[m][t] = *(const u32x4*)__builtin_assume_aligned(h.codes[m] + block * 1024 + lane * 16, 16);
+#pragma unroll
+          for (int s = 0; s < 4 / G32; ++s)
+            sc[m][t][s] = *(const f32x4*)__builtin_assume_aligned(h.scales[m] + (block * (4 / G32) + s) * 16 + 4 * g, 16);
+        }
+    };
+    const auto store_x = [&](int buffer) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        Frag<E> q[TERMS];
+        split(x[n], q);
+        const int at = chunk * 64 + ((threadIdx.x / 16 + 16 * n) ^ chunk);
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) staged[buffer][term][at] = q[term];
+      }
+    };
+    f32x4 sum[MATRICES][2][2];
+#pragma unroll
+    for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) sum[m][t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    load_x(0);
+    load_weights(0);
+    __syncthreads();  // the unit before has been read
+    store_x(0);
+    __syncthreads();
+    for (int kb = 0; kb < a.blocks; ++kb) {
+      const int next = min(kb + 1, a.blocks - 1), buffer = BUFFERS == 2 ? kb % 2 : 0;
+      u32x4 cc[MATRICES][2];
+      f32x4 cs[MATRICES][2][4 / G32];
+      __builtin_memcpy(cc, c, sizeof(c));
+      __builtin_memcpy(cs, sc, sizeof(sc));
+      load_x(next);
+      load_weights(next);
+#pragma unroll
+      for (int s = 0; s < 4 / G32; ++s) {
+        f32x4 part[MATRICES][2][2];
+#pragma unroll
+        for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) part[m][t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = s * G32; j < (s + 1) * G32; ++j) {
+          Frag<E> q[2][TERMS];
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term)
+              q[r][term] = staged[buffer][term][(4 * j + g) * 64 + ((wr * 32 + r * 16 + n16) ^ (4 * j + g))];
+#pragma unroll
+          for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const Frag<E> w = decode<E>(cc[m][t][j]);
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term) part[m][t][r] = mfma(w, q[r][term], part[m][t][r]);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum[m][t][r][i] = fmaf(part[m][t][r][i], cs[m][t][s][i], sum[m][t][r][i]);
+      }
+      if (BUFFERS == 1) __syncthreads();
+      if (kb + 1 < a.blocks) store_x(BUFFERS == 2 ? 1 - buffer : 0);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int64_t row = row0 + wr * 32 + r * 16 + n16;
+        if (row >= a.rows) continue;
+        T* y = (T*)h.y + row * a.ys;
+        const int o = (tile0 + t) * 16 + 4 * g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (o + i >= a.outputs) break;
+          float v = sum[0][t][r][i];
+          if (h.bias) v += h.bias[o + i];
+          if constexpr (MATRICES == 2) v *= open_gate(sum[1][t][r][i], a.act);
+          y[o + i] = from_float<T>(v);
+        }
+      }
+  }
+}
+
+constexpr int kManyRows = 64;
+
 template <class T, int G32, int MATRICES>
 void linear_launch(const LinearArgs& h, hipStream_t st) {
   using std::integral_constant;
@@ -270,6 +404,12 @@ void linear_launch(const LinearArgs& h, hipStream_t st) {
     linear_few_kernel<T, R, G32, MATRICES>
         <<<(unsigned)std::min<int64_t>(units, 1 << 20), 64 * waves, 0, st>>>(h, row_tiles, units);
   };
+  if (h.a.rows > kManyRows) {
+    const int row_tiles = (int)ceil_div(h.a.rows, 64);
+    const int64_t units = ceil_div(tiles, 4) * row_tiles;
+    linear_many_kernel<T, G32, MATRICES><<<(unsigned)std::min<int64_t>(units, 1 << 20), 256, 0, st>>>(h, row_tiles, units);
+    return;
+  }
   if (h.a.rows <= 16) return go(integral_constant<int, 1>{});
   if (h.a.rows <= 32) return go(integral_constant<int, 2>{});
   go(integral_constant<int, 4>{});
