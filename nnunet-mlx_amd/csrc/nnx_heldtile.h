@@ -209,7 +209,10 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
   Codes<DP> keys;
   u32x4 values[CT];
   float key_scale, value_scale;
-  bool shown = true;
+  // without a mask any byte is loaded and none looked at: a load under a condition would be waited for at once
+  const uint8_t* marks = mask ? mask : (const uint8_t*)ks;
+  const int last_mark = mask ? a.keys - 1 : 0;
+  uint8_t mark;
   auto load_keys = [&](int j) {
     const int8_t* at = kc + (int64_t)j * 64 * a.dim;
 #pragma unroll
@@ -222,7 +225,7 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
     }
     key_scale = ks[(int64_t)j * 64 + lane];
     value_scale = vs[(int64_t)j * 64 + lane];
-    if (mask) shown = mask[min(64 * j + lane, a.keys - 1)];
+    mark = marks[min(64 * j + lane, last_mark)];
   };
   auto load_values = [&](int j) {
     const int8_t* at = vc + (int64_t)j * 64 * a.dim;
@@ -240,7 +243,7 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
   }
   for (; j < j1; j += 4) {
     // which of the 64 slots are seen, but for each row's own end
-    shown = shown && 64 * j + lane < most;
+    const bool shown = (!mask || mark) && 64 * j + lane < most;
     const uint64_t seen = __ballot(shown);
     const bool whole = seen == ~0ull && 64 * (j + 1) <= least;
     const float mine = shown ? value_scale : 0.f;

@@ -153,6 +153,28 @@ struct LinearArgs {
   void* y;
 };
 
+// Four neighbouring outputs of a row from o on: bias, gate, one rounding.
+template <class T, int MATRICES>
+__device__ __forceinline__ void finish(const LinearArgs& h, int64_t row, int o, f32x4 u, f32x4 gate) {
+  const PackedArgs& a = h.a;
+  T* y = (T*)h.y + row * a.ys + o;
+  Vec<T, 4> v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float z = u[i];
+    if (h.bias) z += h.bias[min(o + i, a.outputs - 1)];
+    if constexpr (MATRICES == 2) z *= open_gate(gate[i], a.act);
+    v.v[i] = from_float<T>(z);
+  }
+  if (o + 4 <= a.outputs) {
+    store_vec(y, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (o + i < a.outputs) y[i] = v.v[i];
+  }
+}
+
 // Eight elements of a row from `at` on, zeros past its end.
 template <class T>
 __device__ __forceinline__ Vec<T, 8> load_row(const T* row, int at, int end) {
@@ -164,20 +186,22 @@ __device__ __forceinline__ Vec<T, 8> load_row(const T* row, int at, int end) {
   return x;
 }
 
-// A workgroup 16 outputs of 16 R rows, its waves blocks of 128 inputs in turn.  Weights are the matrix
-// instruction's rows, x its columns: a lane's 16 bytes of codes are its operands of four instructions, and
-// its results four neighbouring outputs of one row, which a group's scales multiply as they stand.
-template <class T, int R, int G32, int MATRICES>
-__global__ __launch_bounds__(512) void linear_few_kernel(LinearArgs h, int row_tiles, int64_t units) {
+// A workgroup 16 N outputs of 16 R rows, its W waves blocks of 128 inputs in turn, without a word to each other
+// until their sums are added up.  Weights are the matrix instruction's rows, x its columns: a lane's 16 bytes of
+// codes are its operands of four instructions, and its results four neighbouring outputs of one row, which a
+// group's scales multiply as they stand.
+template <class T, int G32, int MATRICES, int R, int N, int W>
+__global__ __launch_bounds__(64 * W) void linear_kernel(LinearArgs h, int row_tiles, int64_t units) {
   using E = typename Operand<T>::E;
-  constexpr int TERMS = Operand<T>::kTerms;
-  __shared__ __attribute__((aligned(16))) f32x4 sums[8][MATRICES * R][64];
+  constexpr int TERMS = Operand<T>::kTerms, S = 4 / G32, TILES = MATRICES * N * R, AT_ONCE = W < 4 ? W : 4;
+  __shared__ __attribute__((aligned(16))) f32x4 sums[AT_ONCE][TILES][64];
   const PackedArgs& a = h.a;
   const int lane = threadIdx.x % 64, n16 = lane % 16, g = lane / 16;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int last_tile = (a.outputs - 1) / 16;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int tile = (int)(u / row_tiles);
-    const int64_t row0 = (u - (int64_t)tile * row_tiles) * 16 * R;
+    const int tile0 = (int)(u / row_tiles) * N;
+    const int64_t row0 = (u - u / row_tiles * row_tiles) * 16 * R;
     const T* x[R];
     bool live[R];
 #pragma unroll
@@ -185,131 +209,135 @@ __global__ __launch_bounds__(512) void linear_few_kernel(LinearArgs h, int row_t
       live[r] = row0 + 16 * r + n16 < a.rows;
       x[r] = (const T*)h.x + (live[r] ? row0 + 16 * r + n16 : 0) * a.xs;
     }
-    f32x4 sum[MATRICES][R];
+    f32x4 sum[MATRICES][N][R];
 #pragma unroll
     for (int m = 0; m < MATRICES; ++m)
 #pragma unroll
-      for (int r = 0; r < R; ++r) sum[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wave; kb < a.blocks; kb += waves) {
-      u32x4 c[MATRICES];
-      f32x4 sc[MATRICES][4 / G32];
+      for (int t = 0; t < N; ++t)
 #pragma unroll
-      for (int m = 0; m < MATRICES; ++m) {
-        const int64_t block = (int64_t)tile * a.blocks + kb;
-        c[m] = *(const u32x4*)__builtin_assume_aligned(h.codes[m] + block * 1024 + lane * 16, 16);
+        for (int r = 0; r < R; ++r) sum[m][t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto take = [&](int kb, auto whole) {
+      u32x4 c[MATRICES][N];
+      f32x4 sc[MATRICES][N][S];
 #pragma unroll
-        for (int s = 0; s < 4 / G32; ++s)
-          sc[m][s] = *(const f32x4*)__builtin_assume_aligned(h.scales[m] + (block * (4 / G32) + s) * 16 + 4 * g, 16);
-      }
+      for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+          const int64_t block = (int64_t)min(tile0 + t, last_tile) * a.blocks + kb;
+          c[m][t] = *(const u32x4*)__builtin_assume_aligned(h.codes[m] + block * 1024 + lane * 16, 16);
+#pragma unroll
+          for (int s = 0; s < S; ++s)
+            sc[m][t][s] = *(const f32x4*)__builtin_assume_aligned(h.scales[m] + (block * S + s) * 16 + 4 * g, 16);
+        }
       Vec<T, 8> xv[R][4];
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          xv[r][j] = Vec<T, 8>{};
-          if (live[r]) xv[r][j] = load_row(x[r], kb * 128 + 32 * j + 8 * g, a.inputs);
+          const int at = kb * 128 + 32 * j + 8 * g;
+          if constexpr (decltype(whole)::value) {
+            xv[r][j] = load_vec<8>(x[r] + at);
+          } else {
+            xv[r][j] = load_row(x[r], at, a.inputs);
+          }
         }
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        Frag<E> q[4][TERMS];
+      for (int s = 0; s < S; ++s) {
+        Frag<E> q[G32][R][TERMS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split(xv[r][j], q[j]);
+        for (int j = 0; j < G32; ++j)
+#pragma unroll
+          for (int r = 0; r < R; ++r) split(xv[r][s * G32 + j], q[j][r]);
 #pragma unroll
         for (int m = 0; m < MATRICES; ++m)
 #pragma unroll
-          for (int s = 0; s < 4 / G32; ++s) {
-            f32x4 part{0.f, 0.f, 0.f, 0.f};
+          for (int t = 0; t < N; ++t) {
+            f32x4 part[R];
 #pragma unroll
-            for (int j = s * G32; j < (s + 1) * G32; ++j) {
-              const Frag<E> w = decode<E>(c[m][j]);
+            for (int r = 0; r < R; ++r) part[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int term = 0; term < TERMS; ++term) part = mfma(w, q[j][term], part);
+            for (int j = 0; j < G32; ++j) {
+              const Frag<E> w = decode<E>(c[m][t][s * G32 + j]);
+#pragma unroll
+              for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term) part[r] = mfma(w, q[j][r][term], part[r]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[m][r][i] = fmaf(part[i], sc[m][s][i], sum[m][r][i]);
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum[m][t][r][i] = fmaf(part[r][i], sc[m][t][s][i], sum[m][t][r][i]);
           }
       }
+    };
+    // whole blocks first: a load under a condition would be waited for at once
+    int kb = wave;
+    for (; kb < a.inputs / 128; kb += W) take(kb, std::true_type{});
+    if (kb < a.blocks) take(kb, std::false_type{});
+    // waves from the fourth on into those four before, then every wave some of the tiles
+    const auto put = [&](int to) {
+#pragma unroll
+      for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+          for (int r = 0; r < R; ++r) sums[to][(m * N + t) * R + r][lane] = sum[m][t][r];
+    };
+#pragma unroll
+    for (int w0 = W - 4; w0 >= 4; w0 -= 4) {
+      if (wave >= w0 && wave < w0 + 4) put(wave - w0);
+      __syncthreads();
+      if (wave >= w0 - 4 && wave < w0) {
+#pragma unroll
+        for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+          for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int r = 0; r < R; ++r) sum[m][t][r] += sums[wave - w0 + 4][(m * N + t) * R + r][lane];
+      }
+      __syncthreads();
     }
-#pragma unroll
-    for (int m = 0; m < MATRICES; ++m)
-#pragma unroll
-      for (int r = 0; r < R; ++r) sums[wave][m * R + r][lane] = sum[m][r];
+    if (wave < AT_ONCE) put(wave);
     __syncthreads();
-    for (int r = wave; r < R; r += waves) {
+    for (int at = wave; at < N * R; at += W) {
+      const int t = at / R, r = at % R;
       const int64_t row = row0 + 16 * r + n16;
+      const int o = (tile0 + t) * 16 + 4 * g;
       if (row >= a.rows) continue;
-      f32x4 u[MATRICES];
+      f32x4 v[MATRICES];
 #pragma unroll
       for (int m = 0; m < MATRICES; ++m) {
-        u[m] = sums[0][m * R + r][lane];
-        for (int w = 1; w < waves; ++w) u[m] += sums[w][m * R + r][lane];
-      }
-      T* y = (T*)h.y + row * a.ys;
-      const int o = tile * 16 + 4 * g;
+        v[m] = sums[0][m * N * R + at][lane];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (o + i >= a.outputs) break;
-        float v = u[0][i];
-        if (h.bias) v += h.bias[o + i];
-        if constexpr (MATRICES == 2) v *= open_gate(u[1][i], a.act);
-        y[o + i] = from_float<T>(v);
+        for (int w = 1; w < AT_ONCE; ++w) v[m] += sums[w][m * N * R + at][lane];
       }
+      finish<T, MATRICES>(h, row, o, v[0], v[MATRICES - 1]);
     }
     __syncthreads();  // sums are read before the next unit's
   }
 }
 
-// A workgroup 64 outputs of 64 rows, a wave 32 of 32.  Blocks of 128 inputs of x go through LDS, split into
-// operands once; a block's weights are the waves' own, as above.  Chunk c (8 inputs) of row r lies at place
-// c * 64 + (r ^ c), so that neither the rows' chunks on their way in nor the chunks' rows on their way out meet
-// in a bank.
+// A workgroup 64 outputs of 64 rows, a wave 32 of 32.  A block of 128 inputs of x goes through LDS, split into operands once; its weights are the waves' own, as above.  Chunk
+// c (8 inputs) of row r lies at place c * 64 + (r ^ c), so that neither the rows' chunks on their way in nor the
+// chunks' rows on their way out meet in a bank.  What bounds it is the way of a block from memory, so two are on
+// theirs while one is multiplied.
 template <class T, int G32, int MATRICES>
-__global__ __launch_bounds__(256) void linear_many_kernel(LinearArgs h, int row_tiles, int64_t units) {
+__global__ __launch_bounds__(256, 2) void linear_many_kernel(LinearArgs h, int row_tiles, int64_t units) {
   using E = typename Operand<T>::E;
-  constexpr int TERMS = Operand<T>::kTerms, BUFFERS = TERMS == 1 ? 2 : 1;
-  __shared__ __attribute__((aligned(16))) Frag<E> staged[BUFFERS][TERMS][16 * 64];
+  constexpr int TERMS = Operand<T>::kTerms, BUFFERS = TERMS == 1 ? 2 : 1, S = 4 / G32;
+  __shared__ __attribute__((aligned(16))) Frag<E> staged[BUFFERS * TERMS * 1024];  // [buffer][operand][place]
   const PackedArgs& a = h.a;
   const int lane = threadIdx.x % 64, n16 = lane % 16, g = lane / 16;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave % 2, wo = wave / 2;
-  const int last_tile = (a.outputs - 1) / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int wr = wave % 2, wo = wave / 2;
+  const int last_tile = (a.outputs - 1) / 16, whole = a.inputs / 128;
+  const int chunk = threadIdx.x % 16, first = threadIdx.x / 16;  // of x, of rows first + 16 n
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int tile0 = (int)(u / row_tiles) * 4 + wo * 2;
     const int64_t row0 = (u - u / row_tiles * row_tiles) * 64;
-    // the thread's chunks of x: chunk threadIdx % 16 of rows threadIdx / 16 + 16 n
-    const int chunk = threadIdx.x % 16;
-    Vec<T, 8> x[4];
-    u32x4 c[MATRICES][2];
-    f32x4 sc[MATRICES][2][4 / G32];
-    const auto load_x = [&](int kb) {
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const int64_t row = row0 + threadIdx.x / 16 + 16 * n;
-        x[n] = Vec<T, 8>{};
-        if (row < a.rows) x[n] = load_row((const T*)h.x + row * a.xs, kb * 128 + chunk * 8, a.inputs);
-      }
-    };
-    const auto load_weights = [&](int kb) {
-#pragma unroll
-      for (int m = 0; m < MATRICES; ++m)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int64_t block = (int64_t)min(tile0 + t, last_tile) * a.blocks + kb;
-          c[m][t] = *(const u32x4*)__builtin_assume_aligned(h.codes[m] + block * 1024 + lane * 16, 16);
-#pragma unroll
-          for (int s = 0; s < 4 / G32; ++s)
-            sc[m][t][s] = *(const f32x4*)__builtin_assume_aligned(h.scales[m] + (block * (4 / G32) + s) * 16 + 4 * g, 16);
-        }
-    };
-    const auto store_x = [&](int buffer) {
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        Frag<E> q[TERMS];
-        split(x[n], q);
-        const int at = chunk * 64 + ((threadIdx.x / 16 + 16 * n) ^ chunk);
-#pragma unroll
-        for (int term = 0; term < TERMS; ++term) staged[buffer][term][at] = q[term];
-      }
-    };
+    Vec<T, 8> x[2][4];
+    u32x4 c[2][MATRICES][2];
+    f32x4 sc[2][MATRICES][2][S];
     f32x4 sum[MATRICES][2][2];
 #pragma unroll
     for (int m = 0; m < MATRICES; ++m)
@@ -317,21 +345,39 @@ __global__ __launch_bounds__(256) void linear_many_kernel(LinearArgs h, int row_
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 2; ++r) sum[m][t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    load_x(0);
-    load_weights(0);
-    __syncthreads();  // the unit before has been read
-    store_x(0);
-    __syncthreads();
-    for (int kb = 0; kb < a.blocks; ++kb) {
-      const int next = min(kb + 1, a.blocks - 1), buffer = BUFFERS == 2 ? kb % 2 : 0;
-      u32x4 cc[MATRICES][2];
-      f32x4 cs[MATRICES][2][4 / G32];
-      __builtin_memcpy(cc, c, sizeof(c));
-      __builtin_memcpy(cs, sc, sizeof(sc));
-      load_x(next);
-      load_weights(next);
+    const T* rows[4];
 #pragma unroll
-      for (int s = 0; s < 4 / G32; ++s) {
+    for (int n = 0; n < 4; ++n)
+      rows[n] = (const T*)h.x + min(row0 + first + 16 * n, a.rows - 1) * a.xs + chunk * 8;
+    const auto load_x = [&](int which, int kb) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) x[which][n] = load_vec<8>(rows[n] + kb * 128);
+    };
+    const auto load_weights = [&](int which, int kb) {
+#pragma unroll
+      for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int64_t block = (int64_t)min(tile0 + t, last_tile) * a.blocks + kb;
+          c[which][m][t] = *(const u32x4*)__builtin_assume_aligned(h.codes[m] + block * 1024 + lane * 16, 16);
+#pragma unroll
+          for (int s = 0; s < S; ++s)
+            sc[which][m][t][s] = *(const f32x4*)__builtin_assume_aligned(h.scales[m] + (block * S + s) * 16 + 4 * g, 16);
+        }
+    };
+    const auto stage = [&](int which, int buffer) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        Frag<E> q[TERMS];
+        split(x[which][n], q);
+        const int at = chunk * 64 + ((first + 16 * n) ^ chunk);
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) staged[(buffer * TERMS + term) * 1024 + at] = q[term];
+      }
+    };
+    const auto multiply = [&](int which, int buffer) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
         f32x4 part[MATRICES][2][2];
 #pragma unroll
         for (int m = 0; m < MATRICES; ++m)
@@ -346,12 +392,12 @@ __global__ __launch_bounds__(256) void linear_many_kernel(LinearArgs h, int row_
           for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int term = 0; term < TERMS; ++term)
-              q[r][term] = staged[buffer][term][(4 * j + g) * 64 + ((wr * 32 + r * 16 + n16) ^ (4 * j + g))];
+              q[r][term] = staged[(buffer * TERMS + term) * 1024 + (4 * j + g) * 64 + ((wr * 32 + r * 16 + n16) ^ (4 * j + g))];
 #pragma unroll
           for (int m = 0; m < MATRICES; ++m)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              const Frag<E> w = decode<E>(cc[m][t][j]);
+              const Frag<E> w = decode<E>(c[which][m][t][j]);
 #pragma unroll
               for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -365,11 +411,43 @@ __global__ __launch_bounds__(256) void linear_many_kernel(LinearArgs h, int row_
 #pragma unroll
             for (int r = 0; r < 2; ++r)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) sum[m][t][r][i] = fmaf(part[m][t][r][i], cs[m][t][s][i], sum[m][t][r][i]);
+              for (int i = 0; i < 4; ++i)
+                sum[m][t][r][i] = fmaf(part[m][t][r][i], sc[which][m][t][s][i], sum[m][t][r][i]);
       }
-      if (BUFFERS == 1) __syncthreads();
-      if (kb + 1 < a.blocks) store_x(BUFFERS == 2 ? 1 - buffer : 0);
+    };
+    __syncthreads();  // the unit before has been read
+    // Whole blocks first: a load under a condition would be waited for at once.
+    if (whole > 0) {
+      const int second = min(1, whole - 1);
+      load_x(0, 0);
+      load_weights(0, 0);
+      load_x(1, second);
+      load_weights(1, second);
+      stage(0, 0);
       __syncthreads();
+    }
+    const auto round = [&](int which, int kb) {
+      const int next = min(kb + 2, whole - 1);  // past the last the last again
+      load_x(which, next);
+      multiply(which, BUFFERS == 2 ? which : 0);
+      load_weights(which, next);
+      if (BUFFERS == 1) __syncthreads();
+      stage(1 - which, BUFFERS == 2 ? 1 - which : 0);
+      __syncthreads();
+    };
+    int kb = 0;
+    for (; kb + 2 <= whole; kb += 2) {
+      round(0, kb);
+      round(1, kb + 1);
+    }
+    if (kb < whole) round(0, kb);
+    if (whole < a.blocks) {
+      load_weights(0, whole);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) x[0][n] = load_row(rows[n] - chunk * 8, whole * 128 + chunk * 8, a.inputs);
+      stage(0, 0);
+      __syncthreads();
+      multiply(0, 0);
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -377,16 +455,7 @@ __global__ __launch_bounds__(256) void linear_many_kernel(LinearArgs h, int row_
       for (int r = 0; r < 2; ++r) {
         const int64_t row = row0 + wr * 32 + r * 16 + n16;
         if (row >= a.rows) continue;
-        T* y = (T*)h.y + row * a.ys;
-        const int o = (tile0 + t) * 16 + 4 * g;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (o + i >= a.outputs) break;
-          float v = sum[0][t][r][i];
-          if (h.bias) v += h.bias[o + i];
-          if constexpr (MATRICES == 2) v *= open_gate(sum[1][t][r][i], a.act);
-          y[o + i] = from_float<T>(v);
-        }
+        finish<T, MATRICES>(h, row, (tile0 + t) * 16 + 4 * g, sum[0][t][r], sum[MATRICES - 1][t][r]);
       }
   }
 }
@@ -397,22 +466,19 @@ template <class T, int G32, int MATRICES>
 void linear_launch(const LinearArgs& h, hipStream_t st) {
   using std::integral_constant;
   const int tiles = (int)ceil_div(h.a.outputs, 16);
-  auto go = [&](auto r) {
+  auto few = [&](auto r) {
     constexpr int R = decltype(r)::value;
-    const int waves = std::min(h.a.blocks, 8), row_tiles = (int)ceil_div(h.a.rows, 16 * R);
+    const int row_tiles = (int)ceil_div(h.a.rows, 16 * R);
     const int64_t units = (int64_t)tiles * row_tiles;
-    linear_few_kernel<T, R, G32, MATRICES>
-        <<<(unsigned)std::min<int64_t>(units, 1 << 20), 64 * waves, 0, st>>>(h, row_tiles, units);
+    linear_kernel<T, G32, MATRICES, R, 1, 8>
+        <<<(unsigned)std::min<int64_t>(units, 1 << 20), 512, 0, st>>>(h, row_tiles, units);
   };
-  if (h.a.rows > kManyRows) {
-    const int row_tiles = (int)ceil_div(h.a.rows, 64);
-    const int64_t units = ceil_div(tiles, 4) * row_tiles;
-    linear_many_kernel<T, G32, MATRICES><<<(unsigned)std::min<int64_t>(units, 1 << 20), 256, 0, st>>>(h, row_tiles, units);
-    return;
-  }
-  if (h.a.rows <= 16) return go(integral_constant<int, 1>{});
-  if (h.a.rows <= 32) return go(integral_constant<int, 2>{});
-  go(integral_constant<int, 4>{});
+  if (h.a.rows <= 16) return few(integral_constant<int, 1>{});
+  if (h.a.rows <= 32) return few(integral_constant<int, 2>{});
+  if (h.a.rows <= kManyRows) return few(integral_constant<int, sizeof(T) == 2 ? 4 : 2>{});
+  const int row_tiles = (int)ceil_div(h.a.rows, 64);
+  const int64_t units = ceil_div(tiles, 4) * row_tiles;
+  linear_many_kernel<T, G32, MATRICES><<<(unsigned)std::min<int64_t>(units, 1 << 20), 256, 0, st>>>(h, row_tiles, units);
 }
 
 void check_config(const nnx_packed_config& c, const char* name) {
