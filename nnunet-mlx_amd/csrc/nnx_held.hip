@@ -24,13 +24,10 @@ HeldArgs make_args(const nnx_held_config& c, const int32_t* start, const int32_t
   return a;
 }
 
-// Where slot s of 64 stands among the 64 places of a value channel's codes.
-__device__ __forceinline__ int place_of(int s) { return s / 4 % 4 * 16 + s / 16 * 4 + s % 4; }
-
-// A workgroup a tile of 64 slots of one key head's keys or values.  Threads take 8 channels of a row, rows
-// follow each other: whole rows in and out, 16 bytes a thread and more.  Value tiles pass through LDS, where
-// they change between rows of channels and rows of places.
-constexpr int kPlaces = 80;  // bytes from channel to channel there: 64 and a turn of the banks
+// A workgroup a tile of 64 slots of one key head's keys or values, a thread 8 channels of four slots in a row:
+// rows come in and go out whole.  Four slots of a value channel are one word of its 64 places (slot 16 t + 4 g
+// + i at 16 g + 4 t + i), so value tiles change between rows of channels and rows of places by words, through LDS.
+constexpr int kPlaceWords = 17;  // from channel to channel there: 16 and a turn of the banks
 
 struct Unit {
   int which, b, g, tile;
@@ -46,14 +43,17 @@ __device__ __forceinline__ Unit unit_of(const HeldArgs& a, int64_t u, int tiles)
   return r;
 }
 
+inline int tile_threads(int dim) { return (16 * (dim / 8) + 63) / 64 * 64; }
+
 template <class T>
 __global__ __launch_bounds__(256) void hold_kernel(HeldArgs a, const T* k, const T* v, int8_t* k_codes,
                                                    float* k_scales, int8_t* v_codes, float* v_scales, int tiles,
                                                    int64_t units) {
-  __shared__ float tops[64 * 16];
+  __shared__ float tops[64 * kPlaceWords];
   __shared__ float ups[64];
-  __shared__ __attribute__((aligned(16))) int8_t placed[128 * kPlaces];
-  const int chunks = a.dim / 8, all = 64 * chunks;
+  __shared__ uint32_t placed[128 * kPlaceWords];
+  const int chunks = a.dim / 8, quad = threadIdx.x / chunks, c = threadIdx.x - quad * chunks;
+  const bool works = quad < 16;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const Unit w = unit_of(a, u, tiles);
     const int64_t start = a.start0 + (a.start ? a.start[w.b] : 0);
@@ -63,65 +63,78 @@ __global__ __launch_bounds__(256) void hold_kernel(HeldArgs a, const T* k, const
     const int r0 = (int)max((int64_t)0, start - slot0);
     const int r1 = slot0 < 0 || slot0 >= a.slots ? 0 : (int)max((int64_t)0, min((int64_t)64, start + given - slot0));
     if (r0 >= r1) continue;
-    const T* x = (w.which ? v : k) + w.b * a.s[w.which][0] + w.g * a.s[w.which][2];
+    const T* x = (w.which ? v : k) + w.b * a.s[w.which][0] + w.g * a.s[w.which][2] + c * 8;
     const int64_t ts = a.s[w.which][1], t0 = slot0 - start;
     const int64_t item = (int64_t)w.b * a.kv_heads + w.g;
     Vec<T, 8> rows[4];
+    if (works) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int i = n * 256 + threadIdx.x, r = i / chunks, c = i - r * chunks;
-      if (i >= all || r < r0 || r >= r1) continue;
-      rows[n] = load_vec<8>(x + (t0 + r) * ts + c * 8);
-      float top = 0.f;
+      for (int i = 0; i < 4; ++i)  // of rows that are none: a neighbour's
+        rows[i] = load_vec<8>(x + (t0 + min(max(quad * 4 + i, r0), r1 - 1)) * ts);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float m = fabsf(to_float(rows[n].v[e]));
-        top = m < INFINITY ? fmaxf(top, m) : INFINITY;  // stays there
+      for (int i = 0; i < 4; ++i) {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float m = fabsf(to_float(rows[i].v[e]));
+          top = m < INFINITY ? fmaxf(top, m) : INFINITY;  // stays there
+        }
+        tops[(quad * 4 + i) * kPlaceWords + c] = top;
       }
-      tops[r * 16 + c] = top;
     }
     __syncthreads();
-    const int mine = threadIdx.x;
-    if (mine >= r0 && mine < r1) {
+    for (int r = threadIdx.x; r < 64; r += blockDim.x) {
       float top = 0.f;
-      for (int c = 0; c < chunks; ++c) top = fmaxf(top, tops[mine * 16 + c]);
+      for (int n = 0; n < chunks; ++n) top = fmaxf(top, tops[r * kPlaceWords + n]);
       const bool odd = !(top < INFINITY), zero = odd || top < kTiny;
-      ups[mine] = zero ? 0.f : 127.f / top;  // codes of 0 where it is 0
-      (w.which ? v_scales : k_scales)[item * a.slots + slot0 + mine] = odd ? NAN : zero ? 0.f : fminf(top, kMost) / 127.f;
+      ups[r] = zero ? 0.f : 127.f / top;  // codes of 0 where it is 0
+      if (r >= r0 && r < r1)
+        (w.which ? v_scales : k_scales)[item * a.slots + slot0 + r] = odd ? NAN : zero ? 0.f : fminf(top, kMost) / 127.f;
     }
     __syncthreads();
     int8_t* codes = (w.which ? v_codes : k_codes) + (item * a.slots + slot0) * a.dim;
+    if (works) {
+      Vec<int8_t, 8> y[4];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int i = n * 256 + threadIdx.x, r = i / chunks, c = i - r * chunks;
-      if (i >= all || r < r0 || r >= r1) continue;
-      const float up = ups[r];
-      Vec<int8_t, 8> y;
+      for (int i = 0; i < 4; ++i) {
+        const float up = ups[quad * 4 + i];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y.v[e] = up == 0.f ? 0 : (int8_t)(int)rintf(to_float(rows[n].v[e]) * up);
+        for (int e = 0; e < 8; ++e) y[i].v[e] = up == 0.f ? 0 : (int8_t)(int)rintf(to_float(rows[i].v[e]) * up);
+      }
       if (w.which) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) placed[(c * 8 + e) * kPlaces + place_of(r)] = y.v[e];
+        for (int e = 0; e < 8; ++e) {
+          const Vec<int8_t, 4> word{y[0].v[e], y[1].v[e], y[2].v[e], y[3].v[e]};
+          placed[(c * 8 + e) * kPlaceWords + quad % 4 * 4 + quad / 4] = __builtin_bit_cast(uint32_t, word);
+        }
       } else {
-        store_vec(codes + i * 8, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = quad * 4 + i;
+          if (r >= r0 && r < r1) store_vec(codes + r * a.dim + c * 8, y[i]);
+        }
       }
     }
-    if (!w.which) continue;  // the next unit's first barrier is before what this one reads last
+    if (!w.which) continue;  // the next unit's first barrier is before what this one reads last is written
     __syncthreads();
     const bool whole = r0 == 0 && r1 == 64;
+    for (int n = threadIdx.x; n < a.dim * 4; n += blockDim.x) {
+      const int d = n / 4, g = n % 4;
+      Vec<uint32_t, 4> y;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int i = n * 256 + threadIdx.x, d = i / 4, p = i % 4;
-      if (d >= a.dim) break;
-      const Vec<int8_t, 16> y = *(const Vec<int8_t, 16>*)__builtin_assume_aligned(placed + d * kPlaces + p * 16, 16);
+      for (int t = 0; t < 4; ++t) y.v[t] = placed[d * kPlaceWords + g * 4 + t];
+      int8_t* to = codes + d * 64 + g * 16;
       if (whole) {
-        store_vec(codes + d * 64 + p * 16, y);
+        store_vec((uint32_t*)to, y);
         continue;
       }
-      for (int e = 0; e < 16; ++e) {  // others' bytes stay as they are
-        const int slot = e / 4 * 16 + p * 4 + e % 4;
-        if (slot >= r0 && slot < r1) codes[d * 64 + p * 16 + e] = y.v[e];
-      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // others' bytes stay as they are
+          const int slot = 16 * t + 4 * g + i;
+          if (slot >= r0 && slot < r1) to[t * 4 + i] = (int8_t)(y.v[t] >> (8 * i));
+        }
     }
   }
 }
@@ -138,8 +151,9 @@ template <class T>
 __global__ __launch_bounds__(256) void read_kernel(HeldArgs a, const int8_t* k_codes, const float* k_scales,
                                                    const int8_t* v_codes, const float* v_scales, T* k, T* v, int tiles,
                                                    int64_t units) {
-  __shared__ __attribute__((aligned(16))) int8_t placed[128 * kPlaces];
-  const int chunks = a.dim / 8, all = 64 * chunks;
+  __shared__ uint32_t placed[128 * kPlaceWords];
+  const int chunks = a.dim / 8, quad = threadIdx.x / chunks, c = threadIdx.x - quad * chunks;
+  const bool works = quad < 16;
   const int first = (int)a.start0, end = first + a.tokens;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const Unit w = unit_of(a, u, tiles);
@@ -149,34 +163,40 @@ __global__ __launch_bounds__(256) void read_kernel(HeldArgs a, const int8_t* k_c
     const int64_t item = (int64_t)w.b * a.kv_heads + w.g;
     const int8_t* codes = (w.which ? v_codes : k_codes) + (item * a.slots + slot0) * a.dim;
     const float* scales = (w.which ? v_scales : k_scales) + item * a.slots + slot0;
-    T* y = (w.which ? v : k) + w.b * a.s[w.which][0] + w.g * a.s[w.which][2];
+    T* y = (w.which ? v : k) + w.b * a.s[w.which][0] + w.g * a.s[w.which][2] + c * 8;
     const int64_t ts = a.s[w.which][1];
+    const Vec<float, 4> scale = load_vec<4>(scales + min(quad, 15) * 4);
+    Vec<int8_t, 8> x[4] = {};
     if (w.which) {
       __syncthreads();  // the unit before has been read
+      for (int n = threadIdx.x; n < a.dim * 4; n += blockDim.x) {
+        const Vec<uint32_t, 4> word = load_vec<4>((const uint32_t*)(codes + n * 16));
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int i = n * 256 + threadIdx.x, d = i / 4, p = i % 4;
-        if (d >= a.dim) break;
-        *(Vec<int8_t, 16>*)__builtin_assume_aligned(placed + d * kPlaces + p * 16, 16) = load_vec<16>(codes + d * 64 + p * 16);
+        for (int t = 0; t < 4; ++t) placed[n / 4 * kPlaceWords + n % 4 * 4 + t] = word.v[t];
       }
       __syncthreads();
-    }
+      if (works) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int i = n * 256 + threadIdx.x, r = i / chunks, c = i - r * chunks;
-      if (i >= all || r < r0 || r >= r1) continue;
-      const float scale = scales[r];
-      Vec<int8_t, 8> x;
-      if (w.which) {
+        for (int e = 0; e < 8; ++e) {
+          const Vec<int8_t, 4> word =
+              __builtin_bit_cast(Vec<int8_t, 4>, placed[(c * 8 + e) * kPlaceWords + quad % 4 * 4 + quad / 4]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x.v[e] = placed[(c * 8 + e) * kPlaces + place_of(r)];
-      } else {
-        x = load_vec<8>(codes + i * 8);
+          for (int i = 0; i < 4; ++i) x[i].v[e] = word.v[i];
+        }
       }
+    } else if (works) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = load_vec<8>(codes + (quad * 4 + i) * a.dim + c * 8);
+    }
+    if (!works) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = quad * 4 + i;
+      if (r < r0 || r >= r1) continue;
       Vec<T, 8> o;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o.v[e] = from_float<T>(stands_for((float)x.v[e], scale));
-      store_vec(y + (int64_t)(slot0 + r - first) * ts + c * 8, o);
+      for (int e = 0; e < 8; ++e) o.v[e] = from_float<T>(stands_for((float)x[i].v[e], scale.v[i]));
+      store_vec(y + (int64_t)(slot0 + r - first) * ts, o);
     }
   }
 }
@@ -274,7 +294,7 @@ void hold_tokens(const nnx_held_config& c, const void* k, const void* v, const i
   ProfScope prof("hold_tokens", 4.0 * rows * c.head_dim, rows * (c.head_dim * (type_bytes(c.type) + 1.0) + 4.0), st);
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    hold_kernel<T><<<(unsigned)std::min<int64_t>(units, 1 << 20), 256, 0, st>>>(
+    hold_kernel<T><<<(unsigned)std::min<int64_t>(units, 1 << 20), tile_threads(c.head_dim), 0, st>>>(
         a, (const T*)k, (const T*)v, k_codes, k_scales, v_codes, v_scales, tiles, units);
   });
   launch_check("hold_tokens");
@@ -294,7 +314,7 @@ void read_held(const nnx_held_config& c, const int8_t* k_codes, const float* k_s
   ProfScope prof("read_held", rows * c.head_dim, rows * (c.head_dim * (type_bytes(c.type) + 1.0) + 4.0), st);
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    read_kernel<T><<<(unsigned)std::min<int64_t>(units, 1 << 20), 256, 0, st>>>(
+    read_kernel<T><<<(unsigned)std::min<int64_t>(units, 1 << 20), tile_threads(c.head_dim), 0, st>>>(
         a, k_codes, k_scales, v_codes, v_scales, (T*)k, (T*)v, tiles, units);
   });
   launch_check("read_held");
@@ -311,6 +331,9 @@ HeldPlan make_plan(const nnx_held_config& c) {
   p.units = (int64_t)c.batch * c.kv_heads * p.tiles;
   // parts of at least 4 tiles of 64 slots, a wave each, while two workgroups a CU are not reached
   p.splits = (int)std::max<int64_t>(1, std::min(kMostSplits / p.units, ceil_div(c.keys, 256)));
+  // what one workgroup is done with before another launch would begin: one query of 5 heads of 64 over 2048 slots
+  // takes 12.4 us in one launch and 15.3 in two, over 3000 15.8 and 15.3 (of 128: 1536 14.3 and 15.2, 2048 17.0 and 15.6)
+  if ((int64_t)c.keys * c.head_dim <= 2048 * 64) p.splits = 1;
   require(p.units * p.splits < 1 << 24, "held attention: fewer than 2^24 items times key heads times tiles of rows");
   p.meta = p.bytes = 0;
   if (p.splits > 1) {

@@ -83,6 +83,10 @@ constexpr int kWeightTerms = std::is_same<T, bf16>::value ? 1 : 2;
 constexpr float kMostWeight = 32.f;
 constexpr int kRoom = 10;
 
+// Beyond this a logit's last place is more than the weights' own errors: there logits are rounded before the
+// reference is taken off, so that equal ones stay equal (one instruction more a logit).
+constexpr float kFar = 0x1p16f;
+
 // A wave's rows: 16 to a matrix instruction's columns, R of those.  Lane l = 16 g + n has row n; of 64
 // slots the logits of 16 t + 4 g + i (t, i < 4), which are the second product's operand as they
 // stand, and of the result channels 16 c + 4 g + i.
@@ -234,6 +238,7 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
       values[c] = *(const u32x4*)__builtin_assume_aligned(at + min(c, last_channels) * 1024 + value_at, 16);
   };
 
+  bool far = false;     // some row's reference is further from 0 than kFar
   int exponent = -70;  // of the values' power of two; held scales other than 0 are above it
   const auto larger = [](float u, float v) { return fmaxf(u, v); };
   int j = j0 + wave;
@@ -281,13 +286,27 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
     }
     __builtin_amdgcn_sched_barrier(0);
     load_keys(min(j + 4, j1 - 1));  // the last again: no branch, which would double the registers
+    if (!far) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const f32x4 by = *(const f32x4*)__builtin_assume_aligned(scales + 16 * t + 4 * g, 16);
+      for (int t = 0; t < 4; ++t) {
+        const f32x4 by = *(const f32x4*)__builtin_assume_aligned(scales + 16 * t + 4 * g, 16);
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[r][t][i] = fmaf(x[r][t][i], by[i], -w.ref[r]);
+          for (int i = 0; i < 4; ++i) x[r][t][i] = fmaf(x[r][t][i], by[i], -w.ref[r]);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const f32x4 by = *(const f32x4*)__builtin_assume_aligned(scales + 16 * t + 4 * g, 16);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float rounded = x[r][t][i] * by[i] - w.ref[r];
+            x[r][t][i] = fabsf(w.ref[r]) > kFar ? rounded : fmaf(x[r][t][i], by[i], -w.ref[r]);
+          }
+      }
     }
     // of the lane's four slots from 16 t + 4 g on, those that the row sees
     const auto row_sees = [&](int r, int t) {
@@ -340,6 +359,7 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[r][t][i] -= by;
         w.ref[r] = next;
+        far |= __any(fabsf(next) > kFar);
         w.most[r] = moves ? kMostWeight : w.most[r];
         sum = weights();
       }

@@ -754,7 +754,7 @@ def read_held(held: HeldTokens, dtype: torch.dtype, *, first: int = 0, count: in
     if gradients:
         _without_gradient("read_held", (), True)
     if out is None:
-        yk, yv = (torch.empty(shape, dtype=dtype, device=held.k_codes.device) for _ in range(2))
+        yk, yv = held.k_codes.new_empty(shape, dtype=dtype), held.k_codes.new_empty(shape, dtype=dtype)
     if config:
         _launch(yk.device, "nnx_read_held", _placed(config, first) if first else config, *_addresses(held),
                 yk.data_ptr(), yv.data_ptr())
@@ -817,7 +817,7 @@ def held_attention(q: torch.Tensor, held: HeldTokens, lengths: torch.Tensor | in
             size = _native.load().nnx_held_attention_workspace(config)
         elif at:
             config = _placed(config, at)
-        work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        work = held.k_codes.new_empty(size) if size else None
         _launch(q.device, "nnx_held_attention", config, q.data_ptr(), *_addresses(held), _address(starts),
                 _address(counts), _address(key_mask), out.data_ptr(), _address(work), size)
     elif out.numel():
@@ -938,7 +938,7 @@ def packed_linear(x: torch.Tensor, weight: PackedWeight, *, bias: torch.Tensor |
     if known is None:
         known = _remember(key, (*_linear_config(x, weight, bias, gate, gate_activation), _gradients(x, bias)))
     config, shape, gradients = known
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(shape)
     results = (y,)
     if gradients:
         results = _without_gradient("packed_linear", results, False, x, bias)
