@@ -11,7 +11,7 @@ namespace {
 
 constexpr float kTiny = 8.673617379884035e-19f;  // 2^-60
 constexpr float kMost = 3.4028233e38f;           // 127 * (kMost / 127) is finite
-constexpr int kMostSplits = 512;
+constexpr int kMostSplits = 512, kUnits = 256;  // a workgroup a CU
 
 HeldArgs make_args(const nnx_held_config& c, const int32_t* start, const int32_t* lengths, const uint8_t* mask) {
   HeldArgs a;
@@ -252,6 +252,46 @@ __global__ __launch_bounds__(256) void join_kernel(HeldAttention h) {
   store_vec(out, Vec<T, 4>{from_float<T>(o.x), from_float<T>(o.y), from_float<T>(o.z), from_float<T>(o.w)});
 }
 
+// The same for few parts of many rows: a thread four channels of a row.
+constexpr int kFewSplits = 8;
+template <class T>
+__global__ __launch_bounds__(256) void join_few_kernel(HeldAttention h, int rows) {
+  const int quads = h.a.dim / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / quads;
+  if (row >= rows) return;
+  const int d = (int)(i - row * quads) * 4;
+  const int64_t bg = row / h.rows, first = row * h.splits;
+  const int mine = (int)(row - bg * h.rows), b = (int)(bg / h.a.kv_heads), kh = (int)(bg - (int64_t)b * h.a.kv_heads);
+  float2 m[kFewSplits];
+  float4 v[kFewSplits];
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {  // past the last the last again, which then counts 0
+    const int64_t at = first + min(s, h.splits - 1);
+    m[s] = h.meta[at];
+    v[s] = *(const float4*)__builtin_assume_aligned(h.part + at * h.a.dim + d, 16);
+  }
+  float top = -INFINITY, l = 0.f, w[kFewSplits];
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) top = fmaxf(top, m[s].x);
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    w[s] = m[s].x == -INFINITY ? m[s].y : m[s].y * __builtin_amdgcn_exp2f(m[s].x - top);
+    if (s >= h.splits) w[s] = 0.f;
+    l += w[s];
+  }
+  const float share = l == 0.f ? 0.f : 1.f / l;
+  float4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    if (s >= h.splits) break;
+    const float by = w[s] * share;
+    o.x = fmaf(v[s].x, by, o.x), o.y = fmaf(v[s].y, by, o.y), o.z = fmaf(v[s].z, by, o.z), o.w = fmaf(v[s].w, by, o.w);
+  }
+  const int t = mine / h.group, hd = mine - t * h.group;
+  T* out = (T*)h.out + b * h.a.s[1][0] + t * h.a.s[1][1] + (int64_t)(kh * h.group + hd) * h.a.s[1][2] + d;
+  store_vec(out, Vec<T, 4>{from_float<T>(o.x), from_float<T>(o.y), from_float<T>(o.z), from_float<T>(o.w)});
+}
+
 void check_config(const nnx_held_config& c, const char* name, bool attention) {
   const std::string n(name);
   require(known_type(c.type), n + ": unknown type");
@@ -329,11 +369,23 @@ HeldPlan make_plan(const nnx_held_config& c) {
   p.r = held_rows(c.type, c.head_dim, p.rows);
   p.tiles = (int)ceil_div(p.rows, 16 * p.r);
   p.units = (int64_t)c.batch * c.kv_heads * p.tiles;
-  // parts of at least 4 tiles of 64 slots, a wave each, while two workgroups a CU are not reached
-  p.splits = (int)std::max<int64_t>(1, std::min(kMostSplits / p.units, ceil_div(c.keys, 256)));
-  // what one workgroup is done with before another launch would begin: one query of 5 heads of 64 over 2048 slots
-  // takes 12.4 us in one launch and 15.3 in two, over 3000 15.8 and 15.3 (of 128: 1536 14.3 and 15.2, 2048 17.0 and 15.6)
-  if ((int64_t)c.keys * c.head_dim <= 2048 * 64) p.splits = 1;
+  p.splits = 1;
+  if (p.units < kUnits) {
+    // Few units: parts of at least 4 tiles of 64 slots, a wave each, up to two workgroups a CU.  (4 queries of 3 items
+    // over up to 131072 slots 50 us, with four workgroups a CU 59.)  Not where one workgroup is done before another
+    // launch would begin: one query of 5 heads of 64 over 2048 slots takes 12.4 us in one launch and 15.3 in two, over
+    // 3000 15.8 and 15.3 (heads of 128: 1536 14.3 and 15.2, 2048 17.0 and 15.6).
+    if ((int64_t)c.keys * c.head_dim > 2048 * 64)
+      p.splits = (int)std::max<int64_t>(1, std::min(kMostSplits / p.units, ceil_div(c.keys, 256)));
+  } else {
+    // Many: parts that even out what the CUs get, in tiles a wave and with what a workgroup (6) and the join (8) cost.
+    // 640 units over 32768 slots: 380, 328, 357 and 350 us in 1 to 4 parts; 1280 units over 4096: 124 in 1, 143 in 2.
+    int64_t least = INT64_MAX;
+    for (int s = 1; s <= 4; ++s) {
+      const int64_t cost = ceil_div(p.units * s, kUnits) * (ceil_div(c.keys, 256 * s) + 6) + (s > 1 ? 8 : 0);
+      if (cost < least) least = cost, p.splits = s;
+    }
+  }
   require(p.units * p.splits < 1 << 24, "held attention: fewer than 2^24 items times key heads times tiles of rows");
   p.meta = p.bytes = 0;
   if (p.splits > 1) {
@@ -389,7 +441,12 @@ void held_attention(const nnx_held_config& c, const void* q, const int8_t* k_cod
   if (p.splits == 1) return;
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    join_kernel<T><<<(unsigned)(int64_t)rows, 256, 0, st>>>(h);
+    if (p.splits <= kFewSplits) {
+      const int64_t threads = (int64_t)rows * (c.head_dim / 4);
+      join_few_kernel<T><<<(unsigned)ceil_div(threads, 256), 256, 0, st>>>(h, (int)rows);
+    } else {
+      join_kernel<T><<<(unsigned)(int64_t)rows, 256, 0, st>>>(h);
+    }
   });
   launch_check("held_join");
 }
