@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
 #pragma unroll
     for (int c = 0; c < CT; ++c) w.o[r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     w.ref[r] = 0.f, w.most[r] = -1.f, w.l[r] = 0.f;
-    w.count[r] = live ? sees(row) : 0;
+    w.count[r] = live ? sees(row) : held;  // rows past the last see what there is, like others
   }
 
   const int all = (most + 63) / 64;
