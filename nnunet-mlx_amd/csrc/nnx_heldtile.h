@@ -268,8 +268,10 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
     f32x4 x[R][4];  // logits in units of log 2, relative to the row's reference
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
+      // A matrix instruction's sum loses up to a last place: what the lower operands add is small, and has sums of its own.
+      f32x4 rest[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r) x[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int r = 0; r < R; ++r) x[r][t] = rest[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < KF; ++s) {
         Frag<E> k;
@@ -279,9 +281,15 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
           k = codes_to<E>(keys.k8[t][0], keys.k8[t][1]);
         }
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+          x[r][t] = mfma(k, w.q[r][0][s], x[r][t]);
 #pragma unroll
-          for (int term = 0; term < Q::kTerms; ++term) x[r][t] = mfma(k, w.q[r][term][s], x[r][t]);
+          for (int term = 1; term < Q::kTerms; ++term) rest[r] = mfma(k, w.q[r][term][s], rest[r]);
+        }
+      }
+      if constexpr (Q::kTerms > 1) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) x[r][t] += rest[r];
       }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -370,6 +378,9 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float left = e[t][i] * by[i];
+          // one value for all operands: a product that is rounded to float16 at once may be another than the one that
+          // it is then taken from
+          if constexpr (WT > 1) asm("" : "+v"(left));
 #pragma unroll
           for (int term = 0; term < WT; ++term) {
             const f16 part = from_float<f16>(left);

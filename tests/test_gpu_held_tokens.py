@@ -503,3 +503,36 @@ def test_refusals(device):
             call()
     for a, b in zip(held, before):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths", [(3000, 1, 0, 900, 2999), (0, 0, 0), (5000, 5000), (1,) * 64, (700,) * 65 + (0,)])
+def test_items_that_share_the_parts(device, dtype, lengths):
+    """Items of very different lengths, whose parts of the work go by what they hold: each as if it were alone."""
+    batch, n = len(lengths), 5000
+    held = _held(batch, n, 1, 128, 27)
+    q = torch.randn(batch, 2, 3, 128, generator=_gen(28)).to(dtype).cuda()
+    for causal, start in ((False, None), (True, [max(0, length - 40) for length in lengths])):
+        starts = None if start is None else _int32(*start)
+        got = tokens.held_attention(q, held, _int32(*lengths), causal=causal, start=starts)
+        for b in range(0, batch, 1 if batch < 10 else 13):
+            alone = tokens.HeldTokens(*(t[b:b + 1].clone() for t in held))
+            _attend_check(q[b:b + 1], alone, n, dtype, lengths=lengths[b:b + 1], causal=causal,
+                          start=None if start is None else start[b:b + 1], got=got[b:b + 1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_operands_of_a_weight_belong_together(device, dtype):
+    """Of 16 million weights some lie next to half a step of their first operand's type.  Logits below 1 err by less
+    than (16 + 4) u, weights by twice that and 4 u, the operands and sums of 8 slots by 10 u: 58 u of the mean
+    |v| in all; an operand that is a step off, by 2^-11 / 8, a hundred times that."""
+    held = _held(1, 8, 4, 16, 29)
+    q = (0.05 * torch.randn(1, 500000, 4, 16, generator=_gen(30))).to(dtype).cuda()
+    got = tokens.held_attention(q, held, 8).double()
+    k, v = (x.double()[0].permute(1, 2, 0).contiguous() for x in tokens.read_held(held, torch.float32, count=8))
+    logits = torch.matmul(q.double()[0].permute(1, 0, 2).contiguous(), k) / 4  # (heads, queries, 8)
+    assert float(logits.abs().max()) < 1
+    p = torch.softmax(logits, -1)
+    want = torch.matmul(p, v.transpose(1, 2).contiguous()).permute(1, 0, 2)
+    size = torch.matmul(p, v.abs().amax(1)[..., None])[..., 0].t()[..., None]
+    assert bool(((got[0] - want).abs() <= U[dtype] * want.abs() + 58 * 2.0**-24 * size).all())
