@@ -43,10 +43,16 @@ __device__ __forceinline__ Unit unit_of(const HeldArgs& a, int64_t u, int tiles)
   return r;
 }
 
+// rint(v) in two's complement, |v| <= 127, in the lowest byte: beside 1.5 * 2^23 a float's last place is 1.
+__device__ __forceinline__ uint32_t code_of(float v) { return __float_as_uint(v + 12582912.f); }
+__device__ __forceinline__ uint32_t lowest_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400), __builtin_amdgcn_perm(b, a, 0x0c0c0400), 0x05040100);
+}
+
 inline int tile_threads(int dim) { return (16 * (dim / 8) + 63) / 64 * 64; }
 
 template <class T>
-__global__ __launch_bounds__(256) void hold_kernel(HeldArgs a, const T* k, const T* v, int8_t* k_codes,
+__global__ __launch_bounds__(256, 4) void hold_kernel(HeldArgs a, const T* k, const T* v, int8_t* k_codes,
                                                    float* k_scales, int8_t* v_codes, float* v_scales, int tiles,
                                                    int64_t units) {
   __shared__ float tops[64 * kPlaceWords];
@@ -94,24 +100,24 @@ __global__ __launch_bounds__(256) void hold_kernel(HeldArgs a, const T* k, const
     __syncthreads();
     int8_t* codes = (w.which ? v_codes : k_codes) + (item * a.slots + slot0) * a.dim;
     if (works) {
-      Vec<int8_t, 8> y[4];
+      uint32_t code[4][8];  // in the lowest byte
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float up = ups[quad * 4 + i];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[i].v[e] = up == 0.f ? 0 : (int8_t)(int)rintf(to_float(rows[i].v[e]) * up);
+        for (int e = 0; e < 8; ++e) code[i][e] = up == 0.f ? 0 : code_of(to_float(rows[i].v[e]) * up);
       }
       if (w.which) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const Vec<int8_t, 4> word{y[0].v[e], y[1].v[e], y[2].v[e], y[3].v[e]};
-          placed[(c * 8 + e) * kPlaceWords + quad % 4 * 4 + quad / 4] = __builtin_bit_cast(uint32_t, word);
-        }
+        for (int e = 0; e < 8; ++e)
+          placed[(c * 8 + e) * kPlaceWords + quad % 4 * 4 + quad / 4] = lowest_bytes(code[0][e], code[1][e], code[2][e], code[3][e]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = quad * 4 + i;
-          if (r >= r0 && r < r1) store_vec(codes + r * a.dim + c * 8, y[i]);
+          const Vec<uint32_t, 2> y{lowest_bytes(code[i][0], code[i][1], code[i][2], code[i][3]),
+                                   lowest_bytes(code[i][4], code[i][5], code[i][6], code[i][7])};
+          if (r >= r0 && r < r1) store_vec((uint32_t*)(codes + r * a.dim + c * 8), y);
         }
       }
     }
