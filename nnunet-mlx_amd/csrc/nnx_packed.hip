@@ -124,20 +124,23 @@ __device__ __forceinline__ void split(const Vec<T, 8>& x, Frag<typename Operand<
   }
 }
 
+// Products are formed 2^-10 times as large, by what a code stands for: 128 of them add up to no more than the largest of x.
+constexpr float kDown = 0x1p-10f, kUp = 0x1p10f;
+
 // Eight codes as E, exactly.
 template <class E>
 __device__ __forceinline__ Frag<E> decode(uint32_t w) {
   u32x4 r;
   if constexpr (std::is_same<E, bf16>::value) {
-    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 0));
-    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 1));
-    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 2));
-    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 3));
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, kDown, 0));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, kDown, 1));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, kDown, 2));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, kDown, 3));
   } else {
-    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.f, 0));
-    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.f, 1));
-    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.f, 2));
-    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.f, 3));
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, kDown, 0));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, kDown, 1));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, kDown, 2));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, kDown, 3));
   }
   Frag<E> f;
   __builtin_memcpy(&f, &r, 16);
@@ -161,9 +164,9 @@ __device__ __forceinline__ void finish(const LinearArgs& h, int64_t row, int o, 
   Vec<T, 4> v;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float z = u[i];
+    float z = u[i] * kUp;
     if (h.bias) z += h.bias[min(o + i, a.outputs - 1)];
-    if constexpr (MATRICES == 2) z *= open_gate(gate[i], a.act);
+    if constexpr (MATRICES == 2) z *= open_gate(gate[i] * kUp, a.act);
     v.v[i] = from_float<T>(z);
   }
   if (o + 4 <= a.outputs) {
@@ -186,22 +189,25 @@ __device__ __forceinline__ Vec<T, 8> load_row(const T* row, int at, int end) {
   return x;
 }
 
-// A workgroup 16 N outputs of 16 R rows, its W waves blocks of 128 inputs in turn, without a word to each other
+// A workgroup 16 outputs of 16 R rows, its eight waves blocks of 128 inputs in turn, without a word to each other
 // until their sums are added up.  Weights are the matrix instruction's rows, x its columns: a lane's 16 bytes of
 // codes are its operands of four instructions, and its results four neighbouring outputs of one row, which a
-// group's scales multiply as they stand.
-template <class T, int G32, int MATRICES, int R, int N, int W>
-__global__ __launch_bounds__(64 * W) void linear_kernel(LinearArgs h, int row_tiles, int64_t units) {
+// group's scales multiply as they stand.  Bound by memory: one row by two matrices of 16384 x 4096 in 13 us (71 MB,
+// 5.4 TB/s), by 4096 x 16384 in less than the call from Python takes (10 us); 64 rows by 4096 x 4096 take 18 us, bound
+// by how x is read, 16 rows of 64 bytes an access, 8 KB apart, by every workgroup.
+constexpr int kFewWaves = 8;
+
+template <class T, int G32, int MATRICES, int R>
+__global__ __launch_bounds__(64 * kFewWaves) void linear_kernel(LinearArgs h, int row_tiles, int64_t units) {
   using E = typename Operand<T>::E;
-  constexpr int TERMS = Operand<T>::kTerms, S = 4 / G32, TILES = MATRICES * N * R, AT_ONCE = W < 4 ? W : 4;
-  __shared__ __attribute__((aligned(16))) f32x4 sums[AT_ONCE][TILES][64];
+  constexpr int TERMS = Operand<T>::kTerms, S = 4 / G32;
+  __shared__ __attribute__((aligned(16))) f32x4 sums[4][MATRICES * R][64];
   const PackedArgs& a = h.a;
   const int lane = threadIdx.x % 64, n16 = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int last_tile = (a.outputs - 1) / 16;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int tile0 = (int)(u / row_tiles) * N;
-    const int64_t row0 = (u - u / row_tiles * row_tiles) * 16 * R;
+    const int tile = (int)(u / row_tiles);
+    const int64_t row0 = (u - (int64_t)tile * row_tiles) * 16 * R;
     const T* x[R];
     bool live[R];
 #pragma unroll
@@ -209,26 +215,22 @@ __global__ __launch_bounds__(64 * W) void linear_kernel(LinearArgs h, int row_ti
       live[r] = row0 + 16 * r + n16 < a.rows;
       x[r] = (const T*)h.x + (live[r] ? row0 + 16 * r + n16 : 0) * a.xs;
     }
-    f32x4 sum[MATRICES][N][R];
+    f32x4 sum[MATRICES][R];
 #pragma unroll
     for (int m = 0; m < MATRICES; ++m)
 #pragma unroll
-      for (int t = 0; t < N; ++t)
-#pragma unroll
-        for (int r = 0; r < R; ++r) sum[m][t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int r = 0; r < R; ++r) sum[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
     const auto take = [&](int kb, auto whole) {
-      u32x4 c[MATRICES][N];
-      f32x4 sc[MATRICES][N][S];
+      const int64_t block = (int64_t)tile * a.blocks + kb;
+      u32x4 c[MATRICES];
+      f32x4 sc[MATRICES][S];
 #pragma unroll
-      for (int m = 0; m < MATRICES; ++m)
+      for (int m = 0; m < MATRICES; ++m) {
+        c[m] = *(const u32x4*)__builtin_assume_aligned(h.codes[m] + block * 1024 + lane * 16, 16);
 #pragma unroll
-        for (int t = 0; t < N; ++t) {
-          const int64_t block = (int64_t)min(tile0 + t, last_tile) * a.blocks + kb;
-          c[m][t] = *(const u32x4*)__builtin_assume_aligned(h.codes[m] + block * 1024 + lane * 16, 16);
-#pragma unroll
-          for (int s = 0; s < S; ++s)
-            sc[m][t][s] = *(const f32x4*)__builtin_assume_aligned(h.scales[m] + (block * S + s) * 16 + 4 * g, 16);
-        }
+        for (int s = 0; s < S; ++s)
+          sc[m][s] = *(const f32x4*)__builtin_assume_aligned(h.scales[m] + (block * S + s) * 16 + 4 * g, 16);
+      }
       Vec<T, 8> xv[R][4];
 #pragma unroll
       for (int r = 0; r < R; ++r)
@@ -249,69 +251,58 @@ __global__ __launch_bounds__(64 * W) void linear_kernel(LinearArgs h, int row_ti
 #pragma unroll
           for (int r = 0; r < R; ++r) split(xv[r][s * G32 + j], q[j][r]);
 #pragma unroll
-        for (int m = 0; m < MATRICES; ++m)
+        for (int m = 0; m < MATRICES; ++m) {
+          f32x4 part[R];
 #pragma unroll
-          for (int t = 0; t < N; ++t) {
-            f32x4 part[R];
+          for (int r = 0; r < R; ++r) part[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < R; ++r) part[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < G32; ++j) {
-              const Frag<E> w = decode<E>(c[m][t][s * G32 + j]);
-#pragma unroll
-              for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int term = 0; term < TERMS; ++term) part[r] = mfma(w, q[j][r][term], part[r]);
-            }
+          for (int j = 0; j < G32; ++j) {
+            const Frag<E> w = decode<E>(c[m][s * G32 + j]);
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) sum[m][t][r][i] = fmaf(part[r][i], sc[m][t][s][i], sum[m][t][r][i]);
+              for (int term = 0; term < TERMS; ++term) part[r] = mfma(w, q[j][r][term], part[r]);
           }
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[m][r][i] = fmaf(part[r][i], sc[m][s][i], sum[m][r][i]);
+        }
       }
     };
     // whole blocks first: a load under a condition would be waited for at once
     int kb = wave;
-    for (; kb < a.inputs / 128; kb += W) take(kb, std::true_type{});
+    for (; kb < a.inputs / 128; kb += kFewWaves) take(kb, std::true_type{});
     if (kb < a.blocks) take(kb, std::false_type{});
-    // waves from the fourth on into those four before, then every wave some of the tiles
-    const auto put = [&](int to) {
+    // waves 4 to 7 into 0 to 3, then a wave a tile of rows
 #pragma unroll
-      for (int m = 0; m < MATRICES; ++m)
-#pragma unroll
-        for (int t = 0; t < N; ++t)
-#pragma unroll
-          for (int r = 0; r < R; ++r) sums[to][(m * N + t) * R + r][lane] = sum[m][t][r];
-    };
-#pragma unroll
-    for (int w0 = W - 4; w0 >= 4; w0 -= 4) {
-      if (wave >= w0 && wave < w0 + 4) put(wave - w0);
-      __syncthreads();
-      if (wave >= w0 - 4 && wave < w0) {
+    for (int w0 = 4; w0 >= 0; w0 -= 4) {
+      if (wave >= w0 && wave < w0 + 4) {
 #pragma unroll
         for (int m = 0; m < MATRICES; ++m)
 #pragma unroll
-          for (int t = 0; t < N; ++t)
+          for (int r = 0; r < R; ++r) sums[wave - w0][m * R + r][lane] = sum[m][r];
+      }
+      __syncthreads();
+      if (w0 == 0) break;
+      if (wave < 4) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) sum[m][t][r] += sums[wave - w0 + 4][(m * N + t) * R + r][lane];
+        for (int m = 0; m < MATRICES; ++m)
+#pragma unroll
+          for (int r = 0; r < R; ++r) sum[m][r] += sums[wave][m * R + r][lane];
       }
       __syncthreads();
     }
-    if (wave < AT_ONCE) put(wave);
-    __syncthreads();
-    for (int at = wave; at < N * R; at += W) {
-      const int t = at / R, r = at % R;
-      const int64_t row = row0 + 16 * r + n16;
-      const int o = (tile0 + t) * 16 + 4 * g;
-      if (row >= a.rows) continue;
+    const int64_t row = row0 + 16 * wave + n16;
+    if (wave < R && row < a.rows) {
       f32x4 v[MATRICES];
 #pragma unroll
       for (int m = 0; m < MATRICES; ++m) {
-        v[m] = sums[0][m * N * R + at][lane];
+        v[m] = sums[0][m * R + wave][lane];
 #pragma unroll
-        for (int w = 1; w < AT_ONCE; ++w) v[m] += sums[w][m * N * R + at][lane];
+        for (int w = 1; w < 4; ++w) v[m] += sums[w][m * R + wave][lane];
       }
-      finish<T, MATRICES>(h, row, o, v[0], v[MATRICES - 1]);
+      finish<T, MATRICES>(h, row, tile * 16 + 4 * g, v[0], v[MATRICES - 1]);
     }
     __syncthreads();  // sums are read before the next unit's
   }
@@ -320,7 +311,7 @@ __global__ __launch_bounds__(64 * W) void linear_kernel(LinearArgs h, int row_ti
 // A workgroup 64 outputs of 64 rows, a wave 32 of 32.  A block of 128 inputs of x goes through LDS, split into operands once; its weights are the waves' own, as above.  Chunk
 // c (8 inputs) of row r lies at place c * 64 + (r ^ c), so that neither the rows' chunks on their way in nor the
 // chunks' rows on their way out meet in a bank.  What bounds it is the way of a block from memory, so two are on
-// theirs while one is multiplied.
+// theirs while one is multiplied: 4096 rows by 320 x 1280 in float16 14 us, 512 rows by 4096 x 4096 32 us (540 TFLOP/s).
 template <class T, int G32, int MATRICES>
 __global__ __launch_bounds__(256, 2) void linear_many_kernel(LinearArgs h, int row_tiles, int64_t units) {
   using E = typename Operand<T>::E;
@@ -470,8 +461,8 @@ void linear_launch(const LinearArgs& h, hipStream_t st) {
     constexpr int R = decltype(r)::value;
     const int row_tiles = (int)ceil_div(h.a.rows, 16 * R);
     const int64_t units = (int64_t)tiles * row_tiles;
-    linear_kernel<T, G32, MATRICES, R, 1, 8>
-        <<<(unsigned)std::min<int64_t>(units, 1 << 20), 512, 0, st>>>(h, row_tiles, units);
+    linear_kernel<T, G32, MATRICES, R>
+        <<<(unsigned)std::min<int64_t>(units, 1 << 20), 64 * kFewWaves, 0, st>>>(h, row_tiles, units);
   };
   if (h.a.rows <= 16) return few(integral_constant<int, 1>{});
   if (h.a.rows <= 32) return few(integral_constant<int, 2>{});

@@ -252,3 +252,18 @@ def test_refusals(device):
     for call in bad:
         with pytest.raises(ContractError):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 100])
+def test_ends_of_the_type(device, dtype, rows):
+    """x near its type's end times small weights does not overflow on the way.  Weights of 6 codes' size, all equal:
+    each output is the row's sum times the weight, whose float32 sum of 256 errs by less than 256 u."""
+    top = torch.finfo(dtype).max
+    x = ((torch.rand(rows, 256, generator=_gen(12)) * 0.1 + 0.9) * top).to(dtype).cuda()
+    w = tokens.pack_weight(torch.full((40, 256), 2.0**-9, device="cuda"), 128)
+    got = tokens.packed_linear(x, w).double()
+    want = (x.double().sum(1, keepdim=True) * 2.0**-9).expand(rows, 40)
+    assert bool(((got - want).abs() <= (U[dtype] + 258 * 2.0**-24) * want).all())
+    assert torch.isfinite(tokens.packed_linear(x, w, gate=w)).logical_not().all()  # the product itself passes the end
+    assert torch.isfinite(tokens.packed_linear(x, w, gate=w, gate_activation="sigmoid")).all()

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -236,3 +237,10 @@ def test_oracle_places():
     for s in (0, 1, 5, 17, 63):
         assert np.array_equal(placed[1, 0, 1, :, 16 * (s // 4 % 4) + 4 * (s // 16) + s % 4],
                               (codes[1, 0, 64 + s] % 251 - 125).astype(np.int8))
+
+
+def test_no_exception_leaves_the_size_query():
+    """Refusals are built as strings, which may fail to be allocated: everything is caught."""
+    source = (Path(__file__).resolve().parents[1] / "nnunet-mlx_amd" / "csrc" / "nnx_held.hip").read_text()
+    query = source[source.index("size_t held_attention_workspace("):]
+    assert "catch (...)" in query[:query.index("\n}\n")]
