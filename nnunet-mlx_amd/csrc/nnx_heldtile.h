@@ -264,8 +264,8 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
     const uint64_t seen = __ballot(shown);
     const bool whole = seen == ~0ull && 64 * (j + 1) <= least;
     const float mine = shown ? value_scale : 0.f;
-    if (__any(mine > __builtin_amdgcn_ldexpf(1.f, exponent))) {
-      const int next = __builtin_amdgcn_frexp_expf(wave_reduce(mine, larger));
+    if (__any(fabsf(mine) > __builtin_amdgcn_ldexpf(1.f, exponent))) {
+      const int next = __builtin_amdgcn_frexp_expf(wave_reduce(fabsf(mine), larger));
       const float back = __builtin_amdgcn_ldexpf(1.f, exponent - next);
 #pragma unroll
       for (int r = 0; r < R; ++r)

@@ -39,40 +39,42 @@ __device__ __forceinline__ float level(int code) {
 // A thread a group.
 template <class T>
 __global__ __launch_bounds__(256) void pack_kernel(PackedArgs a, const T* w, uint8_t* codes, float* scales) {
-  const int groups = a.blocks * (128 / a.group), padded = (a.outputs + 15) / 16 * 16;
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= (int64_t)padded * groups) return;
-  const int o = (int)(n / groups), g = (int)(n - (int64_t)o * groups);
-  const int i0 = g * a.group, i1 = o < a.outputs ? min(i0 + a.group, a.inputs) : i0;
-  const T* row = w + o * a.xs;
-  float top = 0.f;
-  bool odd = false;
-  for (int i = i0; i < i1; ++i) {
-    const float e = fabsf(to_float(row[i]));
-    top = fmaxf(top, e);
-    odd |= !(e < INFINITY);
+  const int groups = a.blocks * (128 / a.group);
+  const int64_t all = (int64_t)((a.outputs + 15) / 16 * 16) * groups;
+  for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < all; n += (int64_t)gridDim.x * 256) {
+    const int o = (int)(n / groups), g = (int)(n - (int64_t)o * groups);
+    const int i0 = g * a.group, i1 = o < a.outputs ? min(i0 + a.group, a.inputs) : i0;
+    const T* row = w + o * a.xs;
+    float top = 0.f;
+    bool odd = false;
+    for (int i = i0; i < i1; ++i) {
+      const float e = fabsf(to_float(row[i]));
+      top = fmaxf(top, e);
+      odd |= !(e < INFINITY);
+    }
+    const bool zero = odd || top < kTiny;
+    const float up = zero ? 0.f : 6.f / top;
+    auto code_of = [&](int i) {
+      if (zero || i >= i1) return 0;
+      const float x = to_float(row[i]), s = fabsf(x) * up;
+      const int e = (s > 0.25f) + (s >= 0.75f) + (s > 1.25f) + (s >= 1.75f) + (s > 2.5f) + (s >= 3.5f) + (s > 5.f);
+      return e | (e && x < 0.f ? 8 : 0);
+    };
+    for (int i = i0; i < i0 + a.group; i += 2) codes[code_at(a, o, i)] = (uint8_t)(code_of(i) | code_of(i + 1) << 4);
+    scales[scale_at(a, o, g)] = odd ? NAN : zero ? 0.f : fminf(top, kMost) / 6.f;
   }
-  const bool zero = odd || top < kTiny;
-  const float up = zero ? 0.f : 6.f / top;
-  auto code_of = [&](int i) {
-    if (zero || i >= i1) return 0;
-    const float x = to_float(row[i]), s = fabsf(x) * up;
-    const int e = (s > 0.25f) + (s >= 0.75f) + (s > 1.25f) + (s >= 1.75f) + (s > 2.5f) + (s >= 3.5f) + (s > 5.f);
-    return e | (e && x < 0.f ? 8 : 0);
-  };
-  for (int i = i0; i < i0 + a.group; i += 2) codes[code_at(a, o, i)] = (uint8_t)(code_of(i) | code_of(i + 1) << 4);
-  scales[scale_at(a, o, g)] = odd ? NAN : zero ? 0.f : fminf(top, kMost) / 6.f;
 }
 
 template <class T>
 __global__ __launch_bounds__(256) void unpack_kernel(PackedArgs a, const uint8_t* codes, const float* scales, T* w) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= (int64_t)a.outputs * a.inputs) return;
-  const int o = (int)(n / a.inputs), i = (int)(n - (int64_t)o * a.inputs);
-  const int code = codes[code_at(a, o, i)] >> (i % 2 * 4) & 15;
-  float v = level(code) * scales[scale_at(a, o, i / a.group)];
-  asm("" : "+v"(v));  // one instruction with the conversion would round a float16 from the exact product
-  w[o * a.xs + i] = from_float<T>(v);
+  const int64_t all = (int64_t)a.outputs * a.inputs;
+  for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < all; n += (int64_t)gridDim.x * 256) {
+    const int o = (int)(n / a.inputs), i = (int)(n - (int64_t)o * a.inputs);
+    const int code = codes[code_at(a, o, i)] >> (i % 2 * 4) & 15;
+    float v = level(code) * scales[scale_at(a, o, i / a.group)];
+    asm("" : "+v"(v));  // one instruction with the conversion would round a float16 from the exact product
+    w[o * a.xs + i] = from_float<T>(v);
+  }
 }
 
 __device__ __forceinline__ float open_gate(float g, int act) {
@@ -497,7 +499,7 @@ void pack_weight(const nnx_packed_config& c, const void* w, uint8_t* codes, floa
   ProfScope prof("pack_weight", 0.0, (double)c.outputs * c.inputs * (type_bytes(c.type) + 0.5), st);
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    pack_kernel<T><<<(unsigned)ceil_div(groups, 256), 256, 0, st>>>(a, (const T*)w, codes, scales);
+    pack_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(groups, 256), 1 << 20), 256, 0, st>>>(a, (const T*)w, codes, scales);
   });
   launch_check("pack_weight");
 }
@@ -508,11 +510,10 @@ void unpack_weight(const nnx_packed_config& c, const uint8_t* codes, const float
   check_packed(codes, scales, "unpack weight");
   const PackedArgs a = make_args(c);
   const int64_t n = (int64_t)c.outputs * c.inputs;
-  require(n < (int64_t)1 << 38, "unpack weight: fewer than 2^38 weights");
   ProfScope prof("unpack_weight", 0.0, (double)n * (type_bytes(c.type) + 0.5), st);
   with_type(c.type, [&](auto t) {
     using T = decltype(t);
-    unpack_kernel<T><<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(a, codes, scales, (T*)w);
+    unpack_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(n, 256), 1 << 20), 256, 0, st>>>(a, codes, scales, (T*)w);
   });
   launch_check("unpack_weight");
 }

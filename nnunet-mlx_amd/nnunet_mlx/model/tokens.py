@@ -702,6 +702,8 @@ def hold_tokens(held: HeldTokens, k: torch.Tensor, v: torch.Tensor, *, start: to
     written to stay as they were; where ``start`` is a tensor, tokens past the slots are left out.
     Returns ``held``."""
     starts, at = (start, 0) if isinstance(start, torch.Tensor) else (None, _one_start(start))
+    if not isinstance(lengths, (torch.Tensor, type(None))):
+        raise ContractError(f"lengths must be int32 (batch,), got {type(lengths).__name__}")
     key = ("hold", _signature(*held, k, v, starts, lengths))
     known = _checked.get(key)
     if known is None:
@@ -764,7 +766,8 @@ def read_held(held: HeldTokens, dtype: torch.dtype, *, first: int = 0, count: in
 def _read_config(held, dtype, count, out):
     """The checked configuration of a reading (False where there is nothing to do) and its results' shape."""
     _need(dtype in _TYPES, f"dtype must be float32, float16 or bfloat16, not {dtype}")
-    batch, kv_heads, slots, dim = _check_held(held, held.k_codes.device)
+    _check("k_scales", held.k_scales, 3)
+    batch, kv_heads, slots, dim = _check_held(held, held.k_scales.device)
     shape = torch.Size((batch, count, kv_heads, dim))
     strides = [_contiguous_strides(shape)] * 2
     if out is not None:
@@ -839,8 +842,9 @@ def _held_attention_config(q, held, counts, scale, causal, starts, mask, out):
             _check_side(name, side, torch.int32, (batch,), q.device)
     keys, mask_stride = slots, 0
     if mask is not None:
-        keys = mask.shape[-1]
-        _need(keys <= slots, f"key_mask is of {keys} slots, {slots} are held")
+        _need(mask.dim() == 2 and mask.shape[1] <= slots,
+              f"key_mask must be (batch, n) of n up to the {slots} slots, got {tuple(mask.shape)}")
+        keys = mask.shape[1]
         mask_stride = _check_lengths_mask(None, mask, batch, keys, q.device)
     if out is not None:
         _check("out", out, 4, q)

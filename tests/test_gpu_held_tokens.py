@@ -187,10 +187,15 @@ def _attend_check(q, held, n, dtype, *, lengths, scale=None, causal=False, start
     operands = 2.0**-12 if dtype == torch.bfloat16 else u
     weight = 2 * ((dim + 4) * u * largest * abs(factor) + 4 * u) + operands
     bound = U[dtype] * np.abs(want) + (size * (2 * weight + 2 * n * u))[..., None] + 1e-30
-    off = np.abs(_f64(got) - want)
+    # what lies past the type's end, whichever way its bound takes it, is infinite; at the end either is right
+    end, got = float(torch.finfo(dtype).max), _f64(got)
+    past, inside = np.abs(want) - bound > end * (1 + 2 * U[dtype]), np.abs(want) + bound <= end
+    assert (got[past] == np.sign(want[past]) * np.inf).all()
+    got, want, bound = got[inside], want[inside], bound[inside]
+    off = np.abs(got - want)
     assert (off <= bound).all(), (off / bound).max()
     if np.linalg.norm(want):
-        rel = np.linalg.norm(_f64(got) - want) / np.linalg.norm(want)
+        rel = np.linalg.norm(got - want) / np.linalg.norm(want)
         rows = _f64(q).reshape(batch, queries, -1, group, dim).swapaxes(1, 2).reshape(batch, -1, queries * group, dim)
         logit = np.abs(rows @ k.transpose(0, 2, 3, 1)).max() * abs(factor)
         most = U[dtype] + operands + (2 * dim**0.5 * logit + n**0.5 + 8) * u
@@ -536,3 +541,18 @@ def test_operands_of_a_weight_belong_together(device, dtype):
     want = torch.matmul(p, v.transpose(1, 2).contiguous()).permute(1, 0, 2)
     size = torch.matmul(p, v.abs().amax(1)[..., None])[..., 0].t()[..., None]
     assert bool(((got[0] - want).abs() <= U[dtype] * want.abs() + 58 * 2.0**-24 * size).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scales_that_others_wrote(device, dtype):
+    """Codes and scales may come from elsewhere: -128 is a code, a scale may be negative, values may lie far apart, and
+    past float16's end (127 * 1e4 is 20 times that)."""
+    held = _filled(2, 128, 2, 48, 31)
+    held.v_scales[0] *= -1e4
+    held.v_scales[1, :, 60:] *= 2.0**-40
+    held.k_scales.mul_(0.01)
+    held.k_codes[:, :, 5] = -128
+    held.v_codes[..., 7] = -128
+    for queries in (1, 37):
+        q = torch.randn(2, queries, 4, 48, generator=_gen(32)).to(dtype).cuda()
+        _attend_check(q, held, 128, dtype, lengths=(128, 100), got=tokens.held_attention(q, held, _int32(128, 100)))

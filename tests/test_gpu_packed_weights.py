@@ -267,3 +267,17 @@ def test_ends_of_the_type(device, dtype, rows):
     assert bool(((got - want).abs() <= (U[dtype] + 258 * 2.0**-24) * want).all())
     assert torch.isfinite(tokens.packed_linear(x, w, gate=w)).logical_not().all()  # the product itself passes the end
     assert torch.isfinite(tokens.packed_linear(x, w, gate=w, gate_activation="sigmoid")).all()
+
+
+def test_large_matrix(device):
+    """More weights than a launch has threads."""
+    outputs, inputs = 8192, 600000
+    w = torch.zeros(outputs, inputs, dtype=torch.float16, device="cuda")
+    w[-1, -40:] = torch.arange(40, device="cuda") / 40
+    w[0, 0], w[-2, inputs // 2] = 3.0, -1.0
+    packed = tokens.pack_weight(w, 32)
+    back = tokens.unpack_weight(packed, torch.float16)
+    small = tokens.unpack_weight(tokens.pack_weight(w[-1:, -64:].contiguous(), 32), torch.float16)  # the same groups
+    assert torch.equal(back[-1, -64:], small[0])
+    assert float(back[0, 0]) == 3.0 and float(back[-2, inputs // 2]) == -1.0
+    assert int(torch.count_nonzero(back)) == 2 + int(torch.count_nonzero(small))

@@ -244,3 +244,20 @@ def test_no_exception_leaves_the_size_query():
     source = (Path(__file__).resolve().parents[1] / "nnunet-mlx_amd" / "csrc" / "nnx_held.hip").read_text()
     query = source[source.index("size_t held_attention_workspace("):]
     assert "catch (...)" in query[:query.index("\n}\n")]
+
+
+def test_arguments_of_the_wrong_kind(launches, monkeypatch):
+    held, x = _some()
+    for mask in (torch.tensor(True), torch.ones(5, dtype=torch.bool), torch.ones(2, 129, dtype=torch.bool),
+                 torch.ones(2, 2, 5, dtype=torch.bool), torch.ones(2, 5)):
+        with pytest.raises(ContractError, match="key_mask"):
+            tokens.held_attention(x, held, 5, key_mask=mask)
+    for lengths in (3, [1, 2], 1.0):
+        with pytest.raises(ContractError, match="lengths"):
+            tokens.hold_tokens(held, x, x, lengths=lengths)
+    monkeypatch.undo()
+    for call in (lambda: tokens.read_held(held, torch.float32), lambda: tokens.hold_tokens(held, x, x),
+                 lambda: tokens.held_attention(x, held, 5)):  # nothing of a host's memory reaches a kernel
+        with pytest.raises(ContractError, match="device"):
+            call()
+    assert not launches
