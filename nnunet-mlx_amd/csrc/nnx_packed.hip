@@ -195,8 +195,9 @@ __device__ __forceinline__ Vec<T, 8> load_row(const T* row, int at, int end) {
 // until their sums are added up.  Weights are the matrix instruction's rows, x its columns: a lane's 16 bytes of
 // codes are its operands of four instructions, and its results four neighbouring outputs of one row, which a
 // group's scales multiply as they stand.  Bound by memory: one row by two matrices of 16384 x 4096 in 13 us (71 MB,
-// 5.4 TB/s), by 4096 x 16384 in less than the call from Python takes (10 us); 64 rows by 4096 x 4096 take 18 us, bound
-// by how x is read, 16 rows of 64 bytes an access, 8 KB apart, by every workgroup.
+// 5.4 TB/s), by 4096 x 16384 in less than the call from Python takes (10 us).  More than 16 rows are read in
+// pieces of 256 bytes and more and turned in LDS (64 rows by 4096 x 4096 11 us; straight into the operands, 64 bytes of
+// 16 rows an access, 18 us); 128 rows take 19 us, bound by the L2, from which every workgroup reads its rows (268 MB).
 constexpr int kFewWaves = 8;
 
 template <class T, int G32, int MATRICES, int R>
@@ -204,6 +205,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_kernel(LinearArgs h, in
   using E = typename Operand<T>::E;
   constexpr int TERMS = Operand<T>::kTerms, S = 4 / G32;
   __shared__ __attribute__((aligned(16))) f32x4 sums[4][MATRICES * R][64];
+  extern __shared__ __attribute__((aligned(16))) char lds[];  // x of R > 1: 16 R rows of 128 elements a wave
   const PackedArgs& a = h.a;
   const int lane = threadIdx.x % 64, n16 = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -222,10 +224,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_kernel(LinearArgs h, in
     for (int m = 0; m < MATRICES; ++m)
 #pragma unroll
       for (int r = 0; r < R; ++r) sum[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const auto take = [&](int kb, auto whole) {
+    u32x4 c[MATRICES];
+    f32x4 sc[MATRICES][S];
+    const auto load_weights = [&](int kb) {
       const int64_t block = (int64_t)tile * a.blocks + kb;
-      u32x4 c[MATRICES];
-      f32x4 sc[MATRICES][S];
 #pragma unroll
       for (int m = 0; m < MATRICES; ++m) {
         c[m] = *(const u32x4*)__builtin_assume_aligned(h.codes[m] + block * 1024 + lane * 16, 16);
@@ -233,25 +235,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_kernel(LinearArgs h, in
         for (int s = 0; s < S; ++s)
           sc[m][s] = *(const f32x4*)__builtin_assume_aligned(h.scales[m] + (block * S + s) * 16 + 4 * g, 16);
       }
-      Vec<T, 8> xv[R][4];
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int at = kb * 128 + 32 * j + 8 * g;
-          if constexpr (decltype(whole)::value) {
-            xv[r][j] = load_vec<8>(x[r] + at);
-          } else {
-            xv[r][j] = load_row(x[r], at, a.inputs);
-          }
-        }
+    };
+    const auto multiply = [&](auto&& elements) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         Frag<E> q[G32][R][TERMS];
 #pragma unroll
         for (int j = 0; j < G32; ++j)
 #pragma unroll
-          for (int r = 0; r < R; ++r) split(xv[r][s * G32 + j], q[j][r]);
+          for (int r = 0; r < R; ++r) split(elements(r, s * G32 + j), q[j][r]);
 #pragma unroll
         for (int m = 0; m < MATRICES; ++m) {
           f32x4 part[R];
@@ -273,9 +265,52 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_kernel(LinearArgs h, in
       }
     };
     // whole blocks first: a load under a condition would be waited for at once
+    const int whole = a.inputs / 128;
     int kb = wave;
-    for (; kb < a.inputs / 128; kb += kFewWaves) take(kb, std::true_type{});
-    if (kb < a.blocks) take(kb, std::false_type{});
+    if constexpr (R == 1) {
+      for (; kb < whole; kb += kFewWaves) {
+        load_weights(kb);
+        Vec<T, 8> xv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xv[j] = load_vec<8>(x[0] + kb * 128 + 32 * j + 8 * g);
+        multiply([&](int, int j) { return xv[j]; });
+      }
+    } else if (kb < whole) {
+      // rows in pieces of 256 bytes and more, turned to the operands' 16 rows of 8 elements through the wave's own LDS:
+      // chunk k of row r at place 16 r + (k ^ r % 16)
+      Vec<T, 8>* staged = (Vec<T, 8>*)__builtin_assume_aligned(lds, 16) + wave * 16 * R * 16;
+      const T* rows[4 * R];
+#pragma unroll
+      for (int n = 0; n < 4 * R; ++n)
+        rows[n] = (const T*)h.x + min(row0 + 4 * n + g, a.rows - 1) * a.xs + n16 * 8;
+      Vec<T, 8> xv[4 * R];
+      const auto load_x = [&](int kb) {
+#pragma unroll
+        for (int n = 0; n < 4 * R; ++n) xv[n] = load_vec<8>(rows[n] + kb * 128);
+      };
+      load_x(kb);
+      for (; kb < whole; kb += kFewWaves) {
+        load_weights(kb);
+        wave_sync();
+#pragma unroll
+        for (int n = 0; n < 4 * R; ++n) {
+          const int r = 4 * n + g;
+          staged[r * 16 + (n16 ^ (r % 16))] = xv[n];
+        }
+        wave_sync();
+        load_x(min(kb + kFewWaves, whole - 1));
+        multiply([&](int r, int j) { return staged[(16 * r + n16) * 16 + ((4 * j + g) ^ n16)]; });
+      }
+    }
+    if (kb < a.blocks) {
+      load_weights(kb);
+      Vec<T, 8> xv[R][4];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xv[r][j] = load_row(x[r], kb * 128 + 32 * j + 8 * g, a.inputs);
+      multiply([&](int r, int j) { return xv[r][j]; });
+    }
     // waves 4 to 7 into 0 to 3, then a wave a tile of rows
 #pragma unroll
     for (int w0 = 4; w0 >= 0; w0 -= 4) {
@@ -310,9 +345,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_kernel(LinearArgs h, in
   }
 }
 
-// A workgroup 64 outputs of 64 rows, a wave 32 of 32.  A block of 128 inputs of x goes through LDS, split into operands once; its weights are the waves' own, as above.  Chunk
-// c (8 inputs) of row r lies at place c * 64 + (r ^ c), so that neither the rows' chunks on their way in nor the
-// chunks' rows on their way out meet in a bank.  What bounds it is the way of a block from memory, so two are on
+// A workgroup 64 outputs of 64 rows, a wave 32 of 32.  A block of 128 inputs of x goes through LDS, split into operands
+// once; its weights are the waves' own, as above.  Chunk c (8 inputs) of row r lies at place c * 64 + (r ^ c), so that
+// neither the rows' chunks on their way in nor the chunks' rows on their way out meet in a bank.  What bounds it is the way of a block from memory, so two are on
 // theirs while one is multiplied: 4096 rows by 320 x 1280 in float16 14 us, 512 rows by 4096 x 4096 32 us (540 TFLOP/s).
 template <class T, int G32, int MATRICES>
 __global__ __launch_bounds__(256, 2) void linear_many_kernel(LinearArgs h, int row_tiles, int64_t units) {
@@ -453,7 +488,11 @@ __global__ __launch_bounds__(256, 2) void linear_many_kernel(LinearArgs h, int r
   }
 }
 
-constexpr int kManyRows = 64;
+// Pieces of 64 rows by 64 outputs, half as many as CUs: with more of them waves that take a piece each are faster, with
+// fewer or as many waves that share the inputs of smaller pieces (us, shared and a piece each, bfloat16): 128 pieces of
+// 4096 inputs 19.3 and 24.0; 160 of 1280 inputs 13.4 and 10.8, 165 of 960 with a gate 22.9 and 14.5, 256 of 4096 inputs
+// 35.1 and 24.4.
+constexpr int kManyUnits = 128;
 
 template <class T, int G32, int MATRICES>
 void linear_launch(const LinearArgs& h, hipStream_t st) {
@@ -464,13 +503,14 @@ void linear_launch(const LinearArgs& h, hipStream_t st) {
     const int row_tiles = (int)ceil_div(h.a.rows, 16 * R);
     const int64_t units = (int64_t)tiles * row_tiles;
     linear_kernel<T, G32, MATRICES, R>
-        <<<(unsigned)std::min<int64_t>(units, 1 << 20), 64 * kFewWaves, 0, st>>>(h, row_tiles, units);
+        <<<(unsigned)std::min<int64_t>(units, 1 << 20), 64 * kFewWaves,
+            R > 1 ? kFewWaves * 16 * R * 128 * sizeof(T) : 0, st>>>(h, row_tiles, units);
   };
-  if (h.a.rows <= 16) return few(integral_constant<int, 1>{});
-  if (h.a.rows <= 32) return few(integral_constant<int, 2>{});
-  if (h.a.rows <= kManyRows) return few(integral_constant<int, sizeof(T) == 2 ? 4 : 2>{});
   const int row_tiles = (int)ceil_div(h.a.rows, 64);
   const int64_t units = ceil_div(tiles, 4) * row_tiles;
+  if (h.a.rows <= 16) return few(integral_constant<int, 1>{});
+  if (h.a.rows <= 32) return few(integral_constant<int, 2>{});
+  if (units <= kManyUnits) return few(integral_constant<int, sizeof(T) == 2 ? 4 : 2>{});
   linear_many_kernel<T, G32, MATRICES><<<(unsigned)std::min<int64_t>(units, 1 << 20), 256, 0, st>>>(h, row_tiles, units);
 }
 

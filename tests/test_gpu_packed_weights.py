@@ -110,7 +110,10 @@ def _check_product(got, x, w, bias, gate, activation, dtype):
             (np.abs(product) + off)
         product = product * opened
     got = _f64(got).reshape(product.shape)
-    bound = U[dtype] * np.abs(product) + off + 1e-30
+    # Below the type's least normal value tiny a result's steps no longer shrink with it: they stay tiny * eps, and a
+    # rounding is off by up to half of one, tiny * U (float16: 2^-14 * 2^-11 = 2^-25).  The exact products of 8300 rows
+    # by 17 with a gate, rounded to float16 by numpy, already pass U |product| in 4016 places, all of them below 2^-14.
+    bound = U[dtype] * np.abs(product) + U[dtype] * torch.finfo(dtype).tiny + off + 1e-30
     assert (np.abs(got - product) <= bound).all(), (np.abs(got - product) / bound).max()
     rel = np.linalg.norm(got - product) / np.linalg.norm(product)
     assert rel <= U[dtype] + ((2 if gate is None else 4) * k**0.5 + 10) * u, rel
@@ -281,3 +284,30 @@ def test_large_matrix(device):
     assert torch.equal(back[-1, -64:], small[0])
     assert float(back[0, 0]) == 3.0 and float(back[-2, inputs // 2]) == -1.0
     assert int(torch.count_nonzero(back)) == 2 + int(torch.count_nonzero(small))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", [
+    # rows, inputs, outputs, group, bias, gated, activation: enough pieces for waves that take one each
+    (1000, 257, 530, 128, True, False, "none"),
+    (2100, 333, 250, 64, True, True, "silu"),
+    (8300, 31, 17, 32, False, True, "sigmoid"),
+    (4161, 128, 130, 32, False, False, "none"),
+    (1025, 900, 513, 64, True, True, "none"),
+])
+def test_many_rows(device, case, dtype):
+    rows, inputs, outputs, group, with_bias, gated, activation = case
+    x = torch.randn(rows, inputs + 5, generator=_gen(rows)).to(dtype).cuda()[:, 3:-2]
+    w = tokens.pack_weight(_matrix(rows, outputs, inputs) * inputs**-0.5, group)
+    gate = tokens.pack_weight(_matrix(50 + rows, outputs, inputs) * inputs**-0.5, group) if gated else None
+    bias = torch.randn(outputs, generator=_gen(rows)).cuda() if with_bias else None
+    got = tokens.packed_linear(x, w, bias=bias, gate=gate, gate_activation=activation)
+    _check_product(got, x, _f64(tokens.unpack_weight(w, torch.float32)), bias,
+                   None if gate is None else _f64(tokens.unpack_weight(gate, torch.float32)), activation, dtype)
+    assert torch.equal(tokens.packed_linear(x.contiguous(), w, bias=bias, gate=gate, gate_activation=activation), got)
+    # what is not a number stays in its row, what lies behind a row stays out
+    wide = torch.full((rows, inputs + 5), math.nan, dtype=dtype, device="cuda")
+    wide[:, 3:-2] = x
+    wide[rows - 1, inputs + 2] = math.inf
+    odd = tokens.packed_linear(wide[:, 3:-2], w, bias=bias, gate=gate, gate_activation=activation)
+    assert torch.equal(odd[:-1], got[:-1]) and not torch.isfinite(odd[-1]).any()
