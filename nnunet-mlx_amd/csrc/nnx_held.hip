@@ -26,8 +26,9 @@ HeldArgs make_args(const nnx_held_config& c, const int32_t* start, const int32_t
 
 // Bound by memory: 32768 tokens of 5 heads of 64 in bfloat16 are written in 16 us (42 MB in, 22 out) and read back in
 // 11 (5.8 TB/s; a large copy reaches 5.2).  A workgroup a tile of 64 slots of one key head's keys or values, a thread 8
-// channels of four slots in a row: rows come in and go out whole (a thread a row: 692 us for both).  Four slots of a value channel are one word of its 64 places (slot 16 t + 4 g
-// + i at 16 g + 4 t + i), so value tiles change between rows of channels and rows of places by words, through LDS.
+// channels of four slots in a row: rows come in and go out whole (a thread a row: 692 us for both).  Four slots of a
+// value channel are one word of its 64 places (slot 16 t + 4 g + i at 16 g + 4 t + i), so value tiles change between
+// rows of channels and rows of places by words, through LDS.
 constexpr int kPlaceWords = 17;  // from channel to channel there: 16 and a turn of the banks
 
 struct Unit {
