@@ -71,10 +71,9 @@ struct Query<float> {
   static constexpr int kTerms = 3;
 };
 
-// A weight times its value's scale is one float16 operand of the second product for bfloat16 results (2^-12 of
-// every weight, where the result keeps 2^-9), and for the others two, its rounded value and the rest (2^-23).
-template <class T>
-constexpr int kWeightTerms = std::is_same<T, bf16>::value ? 1 : 2;
+// A weight times its value's scale is two float16 operands of the second product, its rounded value and the rest
+// (2^-23), whatever the result's type: one rounds every weight by 2^-12, which shows in a bfloat16 result's last place.
+constexpr int kWeightTerms = 2;
 
 // Values' scales are taken relative to a power of two at or above the largest so far, and a row's weights to a
 // logit that a tile leaves alone while 16 slots' weights add up to kMostWeight at most (the largest is only looked for
@@ -148,7 +147,7 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
   using Q = Query<T>;
   using E = typename Q::E;
   using Row = Rows<T, DP, R>;
-  constexpr int KF = Row::KF, CT = Row::CT, WT = kWeightTerms<T>;
+  constexpr int KF = Row::KF, CT = Row::CT, WT = kWeightTerms;
   __shared__ __attribute__((aligned(16))) f32x4 exchange[2][R * CT][64];
   __shared__ float exchange_ml[2][2 * R][64];
   __shared__ __attribute__((aligned(16))) float slot_scales[4][128];
@@ -392,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
           float left = e[t][i] * by[i];
           // one value for all operands: a product that is rounded to float16 at once may be another than the one that
           // it is then taken from
-          if constexpr (WT > 1) asm("" : "+v"(left));
+          asm("" : "+v"(left));
 #pragma unroll
           for (int term = 0; term < WT; ++term) {
             const f16 part = from_float<f16>(left);
