@@ -50,6 +50,23 @@ __device__ __forceinline__ Frag<E> codes_to(uint32_t lo, uint32_t hi) {
   return f;
 }
 
+// Eight values as bfloat16 operands that add up to them: cut, not rounded, the next bits eight at a time.
+__device__ __forceinline__ void cut_in_three(f32x4 lo, f32x4 hi, Frag<bf16> (&q)[3]) {
+  float left[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) left[i] = lo[i], left[4 + i] = hi[i];
+#pragma unroll
+  for (int term = 0; term < 3; ++term) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r[i] = __builtin_amdgcn_perm(__float_as_uint(left[2 * i + 1]), __float_as_uint(left[2 * i]), 0x07060302);
+    __builtin_memcpy(&q[term], &r, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) left[i] -= __uint_as_float(__float_as_uint(left[i]) & 0xffff0000u);
+  }
+}
+
 // The four lanes that hold a row (l, l ^ 16, l ^ 32, l ^ 48) agree.
 template <class F>
 __device__ __forceinline__ float rows_reduce(float v, F op) {
@@ -71,16 +88,17 @@ struct Query<float> {
   static constexpr int kTerms = 3;
 };
 
-// A weight times its value's scale is two float16 operands of the second product, its rounded value and the rest
-// (2^-23), whatever the result's type: one rounds every weight by 2^-12, which shows in a bfloat16 result's last place.
-constexpr int kWeightTerms = 2;
+// A weight times its value's scale is three bfloat16 operands of the second product, eight bits each, that add up to
+// it exactly and reach as far as float32 does: no slot's value, seen or not, changes how exact another's is.  (Two float16
+// operands, 2^-23 of a power of two that all slots share, lose values 2^-24 as large as another slot's.)
+constexpr int kWeightTerms = 3;
 
-// Values' scales are taken relative to a power of two at or above the largest so far, and a row's weights to a
-// logit that a tile leaves alone while 16 slots' weights add up to kMostWeight at most (the largest is only looked for
-// when they do not).  2^kRoom puts their products in float16's range: they pass no kMostWeight 2^kRoom = 2^15,
-// and are normal down to 2^(-14 - kRoom).
+// A row's weights are relative to a logit that a tile leaves alone while 16 slots' weights add up to kMostWeight at
+// most (the largest is only looked for when they do not).  Scales are multiplied by kDown: 2^32 slots' weights (2 each at
+// most, by the sixteen) times values at float32's end stay below it, and of the smallest scale that is held, 2^-67, the last
+// operand's bits are above 2^-126.
 constexpr float kMostWeight = 32.f;
-constexpr int kRoom = 10;
+constexpr float kDown = 0x1p-34f, kUp = 0x1p34f;
 
 // Beyond this a logit's last place is more than the weights' own errors: there logits are rounded before the
 // reference is taken off, so that equal ones stay equal (one instruction more a logit).
@@ -116,12 +134,6 @@ __device__ __forceinline__ int unit_of_block(int block, int blocks) {
   if (block >= blocks / (kXcds * kTogether) * (kXcds * kTogether)) return block;
   const int xcd = block % kXcds, at = block / kXcds;
   return (at / kTogether * kXcds + xcd) * kTogether + at % kTogether;
-}
-
-// op over all 64 lanes.
-template <class F>
-__device__ __forceinline__ float wave_reduce(float v, F op) {
-  return rows_reduce(lanes_reduce<16>(v, op), op);
 }
 
 // First dimension of the eight that fragment s takes in lane group g: 16 bytes a lane in whole 64s, 8 in what is left.
@@ -250,7 +262,6 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
   };
 
   bool far = false;     // some row's reference is further from 0 than kFar
-  int exponent = -70;  // of the values' power of two; held scales other than 0 are above it
   const auto larger = [](float u, float v) { return fmaxf(u, v); };
   int j = j0 + wave;
   if (j < j1) {
@@ -262,19 +273,9 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
     const bool shown = (!mask || mark) && 64 * j + lane < most;
     const uint64_t seen = __ballot(shown);
     const bool whole = seen == ~0ull && 64 * (j + 1) <= least;
-    const float mine = shown ? value_scale : 0.f;
-    if (__any(fabsf(mine) > __builtin_amdgcn_ldexpf(1.f, exponent))) {
-      const int next = __builtin_amdgcn_frexp_expf(wave_reduce(fabsf(mine), larger));
-      const float back = __builtin_amdgcn_ldexpf(1.f, exponent - next);
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) w.o[r][c] *= back;
-      exponent = __builtin_amdgcn_readfirstlane(next);
-    }
     wave_sync();
     scales[lane] = key_scale * h.c2;
-    scales[64 + lane] = __builtin_amdgcn_ldexpf(mine, kRoom - exponent);
+    scales[64 + lane] = value_scale * kDown;
     wave_sync();
     f32x4 x[R][4];  // logits in units of log 2, relative to the row's reference
 #pragma unroll
@@ -342,18 +343,17 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
           for (int i = 0; i < 4; ++i) x[r][t][i] = bits & (1u << i) ? x[r][t][i] : -INFINITY;
         }
     }
-    Frag<f16> p[R][WT][2];
+    f32x4 e[R][4];  // weights, then times their values' scales
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      f32x4 e[4];
       const auto weights = [&] {
         f32x4 sum{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            e[t][i] = __builtin_amdgcn_exp2f(x[r][t][i]);
-            sum[i] += e[t][i];
+            e[r][t][i] = __builtin_amdgcn_exp2f(x[r][t][i]);
+            sum[i] += e[r][t][i];
           }
         return (sum[0] + sum[1]) + (sum[2] + sum[3]);
       };
@@ -384,22 +384,7 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
       }
       w.l[r] += sum;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const f32x4 by = *(const f32x4*)__builtin_assume_aligned(scales + 64 + 16 * t + 4 * g, 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float left = e[t][i] * by[i];
-          // one value for all operands: a product that is rounded to float16 at once may be another than the one that
-          // it is then taken from
-          asm("" : "+v"(left));
-#pragma unroll
-          for (int term = 0; term < WT; ++term) {
-            const f16 part = from_float<f16>(left);
-            p[r][term][t / 2][t % 2 * 4 + i] = part;
-            left -= to_float(part);
-          }
-        }
-      }
+      for (int t = 0; t < 4; ++t) e[r][t] *= *(const f32x4*)__builtin_assume_aligned(scales + 64 + 16 * t + 4 * g, 16);
     }
     if (!whole) {  // a weight of 0 keeps out no value that is not a number
 #pragma unroll
@@ -408,23 +393,24 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
         for (int t = 0; t < 4; ++t) {
           const uint32_t bits = row_sees(r, t);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int term = 0; term < WT; ++term)
-              p[r][term][t / 2][t % 2 * 4 + i] = bits & (1u << i) ? p[r][term][t / 2][t % 2 * 4 + i] : (f16)0.f;
+          for (int i = 0; i < 4; ++i) e[r][t][i] = bits & (1u << i) ? e[r][t][i] : 0.f;
         }
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
+    for (int u = 0; u < 2; ++u) {
+      Frag<bf16> p[R][WT];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const Frag<f16> v = codes_to<f16>(values[c][2 * u], values[c][2 * u + 1]);
+      for (int r = 0; r < R; ++r) cut_in_three(e[r][2 * u], e[r][2 * u + 1], p[r]);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const Frag<bf16> v = codes_to<bf16>(values[c][2 * u], values[c][2 * u + 1]);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int term = 0; term < WT; ++term) w.o[r][c] = mfma(v, p[r][term][u], w.o[r][c]);
+          for (int term = 0; term < WT; ++term) w.o[r][c] = mfma(v, p[r][term], w.o[r][c]);
       }
+    }
     __builtin_amdgcn_sched_barrier(0);
     load_values(min(j + 4, j1 - 1));
   }
@@ -438,7 +424,7 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w.o[r][c][i] = __builtin_amdgcn_ldexpf(w.o[r][c][i] * whole, exponent - kRoom);
+      for (int i = 0; i < 4; ++i) w.o[r][c][i] = w.o[r][c][i] * whole * kUp;
   }
 
   // waves 2 and 3 into 0 and 1, then 1 into 0; lanes hold the same places
