@@ -195,6 +195,9 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float left = to_float(x.v[e]) * h.query;
+        // an infinite element makes its row NaN whatever the signs of its products: logits that are all -inf would
+        // look like slots that are not seen
+        if (!(fabsf(left) < INFINITY)) left = NAN;
         if constexpr (Q::kTerms == 1) {
           w.q[r][0][s][e] = from_float<E>(left);
         } else {

@@ -129,3 +129,22 @@ def test_values_of_one_size(device, dtype, power):
     else:
         off = 4 * U[dtype] * want.double().abs() + 2.0**-17
         assert bool(((got.double() * 2.0**-power - want.double()).abs() <= off).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 70, 5000])
+@pytest.mark.parametrize("queries", [1, 40])
+def test_infinite_queries(device, queries, n, dtype):
+    """An infinite element makes its row NaN, as the softmax of infinite logits is, also where all of them are -inf."""
+    k, v = (torch.randn(1, n, 2, 32, generator=_gen(i)).cuda() for i in (11, 12))
+    held = tokens.hold_tokens(tokens.held_tokens(1, n, 2, 32), k.abs() + 0.5, v)
+    q = torch.randn(1, queries, 4, 32, generator=_gen(13)).to(dtype).cuda()
+    want = tokens.held_attention(q, held, n)
+    for sign in (-1, 1):
+        odd = q.clone()
+        odd[0, -1, 3, 9] = sign * float("inf")
+        got = tokens.held_attention(odd, held, n)
+        assert torch.isnan(got[0, -1, 3]).all()
+        got[0, -1, 3] = want[0, -1, 3]
+        assert torch.equal(got, want)
+        assert not tokens.held_attention(odd, held, 0).any()
