@@ -120,7 +120,7 @@ __device__ __forceinline__ void split(const Vec<T, 8>& x, Frag<typename Operand<
         // cut, not rounded: the next bits, eight at a time
         const float part = __uint_as_float(__float_as_uint(left) & 0xffff0000u);
         q[term][e] = from_float<bf16>(part);
-        left -= part;
+        left = term == 0 && fabsf(left) == INFINITY ? 0.f : left - part;  // of infinity nothing is left, not NaN
       }
     }
   }
