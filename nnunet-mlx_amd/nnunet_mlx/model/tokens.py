@@ -8,8 +8,9 @@ three in ``sparse_attention``) and the norms around the block with its gate and 
 values in 8 bits (``held_tokens``, ``hold_tokens``, ``read_held``), the attention that reads them
 so (``held_attention``) and products of few rows with 4-bit weights (``pack_weight``,
 ``unpack_weight``, ``packed_linear``).  Everything runs in libnnunet_hip.so on the current stream of the tensors'
-device, forward only (a gradient asked of a result raises ``ContractError``; a selection has
-none); float32, float16 and bfloat16 tensors with a contiguous last axis and any other strides.
+device, forward only (a gradient asked of a result raises ``ContractError``, and so does writing
+in place what should keep one; a selection has none); float32, float16 and bfloat16 tensors with a
+contiguous last axis and any other strides.
 No reference counterpart.
 """
 
@@ -700,6 +701,7 @@ def hold_tokens(held: HeldTokens, k: torch.Tensor, v: torch.Tensor, *, start: to
     Each row is held as whole numbers -127 to 127 times its largest magnitude / 127; a row with an
     element that is not finite is held as NaN, one below 2^-60 as zero.  Slots that no token is
     written to stay as they were; where ``start`` is a tensor, tokens past the slots are left out.
+    Codes have no gradient: keys and values that ask for one are refused unless gradients are off.
     Returns ``held``."""
     starts, at = (start, 0) if isinstance(start, torch.Tensor) else (None, _one_start(start))
     if not isinstance(lengths, (torch.Tensor, type(None))):
@@ -707,10 +709,13 @@ def hold_tokens(held: HeldTokens, k: torch.Tensor, v: torch.Tensor, *, start: to
     key = ("hold", _signature(*held, k, v, starts, lengths))
     known = _checked.get(key)
     if known is None:
-        known = _remember(key, _hold_config(held, k, v, starts, lengths))
-    config, most = known
+        known = _remember(key, (*_hold_config(held, k, v, starts, lengths),
+                                _gradients(k, v, held.k_scales, held.v_scales)))
+    config, most, gradients = known
     if at > most:
         raise ContractError(f"tokens from slot {at} on pass the slots, the last place for them is {most}")
+    if gradients:
+        _without_gradient("hold_tokens", (), True)
     if config:
         _launch(k.device, "nnx_hold_tokens", _placed(config, at) if at else config, k.data_ptr(), v.data_ptr(),
                 _address(starts), _address(lengths), *_addresses(held))
@@ -751,12 +756,13 @@ def read_held(held: HeldTokens, dtype: torch.dtype, *, first: int = 0, count: in
     key = ("read", _signature(*held, yk, yv), dtype, count)
     known = _checked.get(key)
     if known is None:
-        known = _remember(key, (*_read_config(held, dtype, count, out), _gradients(yk, yv)))
+        known = _remember(key, (*_read_config(held, dtype, count, out),
+                                _gradients(held.k_scales, held.v_scales, yk, yv)))
     config, shape, gradients = known
-    if gradients:
-        _without_gradient("read_held", (), True)
     if out is None:
         yk, yv = held.k_codes.new_empty(shape, dtype=dtype), held.k_codes.new_empty(shape, dtype=dtype)
+    if gradients:
+        yk, yv = _without_gradient("read_held", (yk, yv), out is not None, held.k_scales, held.v_scales)
     if config:
         _launch(yk.device, "nnx_read_held", _placed(config, first) if first else config, *_addresses(held),
                 yk.data_ptr(), yv.data_ptr())
@@ -804,7 +810,7 @@ def held_attention(q: torch.Tensor, held: HeldTokens, lengths: torch.Tensor | in
     known = _checked.get(key)
     if known is None:
         known = _remember(key, (*_held_attention_config(q, held, counts, scale, causal, starts, key_mask, out),
-                                _gradients(q, out)))
+                                _gradients(q, held.k_scales, held.v_scales, out)))
     config, size, slots, gradients = known
     if keys is not None and not 0 <= keys <= slots:
         raise ContractError(f"lengths must be 0 to the {slots} slots, got {keys}")
@@ -813,7 +819,7 @@ def held_attention(q: torch.Tensor, held: HeldTokens, lengths: torch.Tensor | in
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     results = (out,)
     if gradients:
-        results = _without_gradient("held_attention", results, given, q)
+        results = _without_gradient("held_attention", results, given, q, held.k_scales, held.v_scales)
     if config and keys != 0:
         if keys is not None:
             config = _placed(config, at, min(keys, config.keys))
@@ -910,6 +916,8 @@ def pack_weight(w: torch.Tensor, group: int = 64) -> PackedWeight:
     config = _packed_config(w.dtype, outputs, inputs, group, x_stride=w.stride(0))
     codes = torch.empty(shapes[0], dtype=torch.uint8, device=w.device)
     scales = torch.empty(shapes[1], dtype=torch.float32, device=w.device)
+    if w.requires_grad:
+        codes, scales = _without_gradient("pack_weight", (codes, scales), False, w)
     _launch(w.device, "nnx_pack_weight", config, w.data_ptr(), codes.data_ptr(), scales.data_ptr())
     return PackedWeight(codes, scales, outputs, inputs, group)
 
@@ -921,6 +929,8 @@ def unpack_weight(weight: PackedWeight, dtype: torch.dtype) -> torch.Tensor:
     _check_packed("weight", weight, weight.codes.device)
     config = _packed_config(dtype, weight.outputs, weight.inputs, weight.group, x_stride=weight.inputs)
     w = torch.empty((weight.outputs, weight.inputs), dtype=dtype, device=weight.codes.device)
+    if weight.scales.requires_grad:
+        w, = _without_gradient("unpack_weight", (w,), False, weight.scales)
     _launch(w.device, "nnx_unpack_weight", config, weight.codes.data_ptr(), weight.scales.data_ptr(), w.data_ptr())
     return w
 
@@ -940,12 +950,13 @@ def packed_linear(x: torch.Tensor, weight: PackedWeight, *, bias: torch.Tensor |
     key = ("linear", _signature(x, codes, scales, bias, gate_codes, gate_scales), *sizes, *gate_sizes, gate_activation)
     known = _checked.get(key)
     if known is None:
-        known = _remember(key, (*_linear_config(x, weight, bias, gate, gate_activation), _gradients(x, bias)))
+        known = _remember(key, (*_linear_config(x, weight, bias, gate, gate_activation),
+                                _gradients(x, bias, scales, gate_scales)))
     config, shape, gradients = known
     y = x.new_empty(shape)
     results = (y,)
     if gradients:
-        results = _without_gradient("packed_linear", results, False, x, bias)
+        results = _without_gradient("packed_linear", results, False, x, bias, scales, gate_scales)
     if config:
         _launch(x.device, "nnx_packed_linear", config, x.data_ptr(), codes.data_ptr(), scales.data_ptr(),
                 _address(bias), _address(gate_codes), _address(gate_scales), y.data_ptr())
