@@ -654,7 +654,7 @@ typedef struct nnx_held_config {
   int kv_heads;
   int head_dim;  /* a multiple of 16, 16..128 */
   int causal;    /* attention: a query sees the slots up to its position */
-  float scale;   /* attention: of the logits */
+  float scale;   /* attention: of the logits, finite also times log2 e */
   int64_t start; /* the first token's slot or the first query's position */
   int64_t strides[2][3]; /* (batch, token, head) of k and v, or of q and out */
   int64_t mask_stride;

@@ -300,6 +300,9 @@ __global__ __launch_bounds__(256) void join_few_kernel(HeldAttention h, int rows
   store_vec(out, Vec<T, 4>{from_float<T>(o.x), from_float<T>(o.y), from_float<T>(o.z), from_float<T>(o.w)});
 }
 
+// Logits are in units of log 2.
+float in_octaves(float scale) { return scale * 1.4426950408889634f; }
+
 void check_config(const nnx_held_config& c, const char* name, bool attention) {
   const std::string n(name);
   require(known_type(c.type), n + ": unknown type");
@@ -315,7 +318,7 @@ void check_config(const nnx_held_config& c, const char* name, bool attention) {
   require(c.heads >= 1 && c.heads <= 65536 && c.heads % c.kv_heads == 0,
           n + ": heads must be a multiple of the key heads, up to 65536");
   require((double)c.batch * c.tokens * c.heads < 2147483648.0, n + ": fewer than 2^31 queries times heads");
-  require(std::isfinite(c.scale), n + ": the scale must be finite");
+  require(std::isfinite(in_octaves(c.scale)), n + ": the scale must be finite, and so must it be times log2 e");
 }
 
 void check_held(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
@@ -425,10 +428,10 @@ void held_attention(const nnx_held_config& c, const void* q, const int8_t* k_cod
   check_held(k_codes, k_scales, v_codes, v_scales, "held attention");
   require(p.bytes == 0 || (ws && ws_bytes >= p.bytes && reinterpret_cast<uintptr_t>(ws) % 16 == 0),
           "held attention: the workspace is too small or not 16-byte aligned");
-  // The keys' scales are multiplied by at most 64, which none of them overflows by, and the queries by the
-  // rest: their products with codes are finite below 2^122 and so are logits up to the type's end.  A float16
-  // query is taken as it is.
-  const float factor = c.scale * 1.4426950408889634f;
+  // Of factors up to 2^26 the keys' scales are multiplied by 64 at most, which none of them overflows by, and the queries
+  // by the rest, 2^20 at most: their products with codes are finite below 2^122 and so are logits up to the type's
+  // end.  A float16 query is taken as it is and its keys' scales by the whole factor, as by what larger ones leave.
+  const float factor = in_octaves(c.scale);
   const float query = c.type == NNX_TYPE_F16 || factor == 0.f
                           ? 1.f : std::exp2(std::min(20.f, std::max(-16.f, std::ceil(std::log2(std::fabs(factor) / 64.f)))));
   HeldAttention h{make_args(c, start, lengths, mask), q, k_codes, v_codes, k_scales, v_scales, out, (float*)ws,
