@@ -36,8 +36,8 @@ struct HeldAttention {
 
 // 16 rows a wave or 32: two share what a code's conversion costs, where a wave's registers hold them beside two
 // waves a SIMD.
-constexpr bool held_pairs(int type, int dim) { return type != NNX_TYPE_F32 && dim <= 96; }
-inline int held_rows(int type, int dim, int rows) { return rows > 16 && held_pairs(type, dim) ? 2 : 1; }
+constexpr bool held_pairs(bool f32, int dim) { return !f32 && dim <= 96; }
+inline int held_rows(int type, int dim, int rows) { return rows > 16 && held_pairs(type == NNX_TYPE_F32, dim) ? 2 : 1; }
 
 void held_units_f32(const HeldAttention& h, const HeldPlan& p, hipStream_t st);
 void held_units_f16(const HeldAttention& h, const HeldPlan& p, hipStream_t st);

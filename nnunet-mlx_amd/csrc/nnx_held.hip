@@ -4,13 +4,12 @@
 #include <cmath>
 
 #include "nnx_held.h"
+#include "nnx_operands.h"
 
 namespace nnx {
 
 namespace {
 
-constexpr float kTiny = 8.673617379884035e-19f;  // 2^-60
-constexpr float kMost = 3.4028233e38f;           // 127 * (kMost / 127) is finite
 constexpr int kMostSplits = 512, kUnits = 256;  // a workgroup a CU
 
 HeldArgs make_args(const nnx_held_config& c, const int32_t* start, const int32_t* lengths, const uint8_t* mask) {
@@ -94,10 +93,10 @@ __global__ __launch_bounds__(256, 4) void hold_kernel(HeldArgs a, const T* k, co
     for (int r = threadIdx.x; r < 64; r += blockDim.x) {
       float top = 0.f;
       for (int n = 0; n < chunks; ++n) top = fmaxf(top, tops[r * kPlaceWords + n]);
-      const bool odd = !(top < INFINITY), zero = odd || top < kTiny;
+      const bool odd = !(top < INFINITY), zero = odd || top < kLeastTop;
       ups[r] = zero ? 0.f : 127.f / top;  // codes of 0 where it is 0
       if (r >= r0 && r < r1)
-        (w.which ? v_scales : k_scales)[item * a.slots + slot0 + r] = odd ? NAN : zero ? 0.f : fminf(top, kMost) / 127.f;
+        (w.which ? v_scales : k_scales)[item * a.slots + slot0 + r] = odd ? NAN : zero ? 0.f : fminf(top, kMostTop) / 127.f;
     }
     __syncthreads();
     int8_t* codes = (w.which ? v_codes : k_codes) + (item * a.slots + slot0) * a.dim;

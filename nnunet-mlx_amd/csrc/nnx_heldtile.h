@@ -4,23 +4,12 @@
 #include <type_traits>
 
 #include "nnx_held.h"
+#include "nnx_operands.h"
 
 namespace nnx {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-template <class T>
-using Frag = T __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ f32x4 mfma(Frag<f16> a, Frag<f16> b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mfma(Frag<bf16> a, Frag<bf16> b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
 
 // Eight codes as E, exactly.  float16: a code's byte under 0x64 is 1024 + (code + 128), less 1152 in pairs: 5
 // instructions for 4 codes; bfloat16 takes 6, through float32.
@@ -50,23 +39,6 @@ __device__ __forceinline__ Frag<E> codes_to(uint32_t lo, uint32_t hi) {
   return f;
 }
 
-// Eight values as bfloat16 operands that add up to them: cut, not rounded, the next bits eight at a time.
-__device__ __forceinline__ void cut_in_three(f32x4 lo, f32x4 hi, Frag<bf16> (&q)[3]) {
-  float left[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) left[i] = lo[i], left[4 + i] = hi[i];
-#pragma unroll
-  for (int term = 0; term < 3; ++term) {
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r[i] = __builtin_amdgcn_perm(__float_as_uint(left[2 * i + 1]), __float_as_uint(left[2 * i]), 0x07060302);
-    __builtin_memcpy(&q[term], &r, 16);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) left[i] -= __uint_as_float(__float_as_uint(left[i]) & 0xffff0000u);
-  }
-}
-
 // The four lanes that hold a row (l, l ^ 16, l ^ 32, l ^ 48) agree.
 template <class F>
 __device__ __forceinline__ float rows_reduce(float v, F op) {
@@ -76,22 +48,9 @@ __device__ __forceinline__ float rows_reduce(float v, F op) {
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// What a query's element is multiplied in: 16-bit types as they are, float32 in bfloat16 operands that add up to it.
-template <class T>
-struct Query {
-  using E = T;
-  static constexpr int kTerms = 1;
-};
-template <>
-struct Query<float> {
-  using E = bf16;
-  static constexpr int kTerms = 3;
-};
-
 // A weight times its value's scale is three bfloat16 operands of the second product, eight bits each, that add up to
 // it exactly and reach as far as float32 does: no slot's value, seen or not, changes how exact another's is.  (Two float16
 // operands, 2^-23 of a power of two that all slots share, lose values 2^-24 as large as another slot's.)
-constexpr int kWeightTerms = 3;
 
 // A row's weights are relative to a logit that a tile leaves alone while 16 slots' weights add up to kMostWeight at
 // most (the largest is only looked for when they do not).  Scales are multiplied by kDown: 2^32 slots' weights (2 each at
@@ -109,8 +68,8 @@ constexpr float kFar = 0x1p16f;
 // stand, and of the result channels 16 c + 4 g + i.
 template <class T, int DP, int R>
 struct Rows {
-  static constexpr int KF = DP / 32, CT = DP / 16, QT = Query<T>::kTerms;
-  Frag<typename Query<T>::E> q[R][QT][KF];
+  static constexpr int KF = DP / 32, CT = DP / 16, QT = Operand<T>::kTerms;
+  Frag<typename Operand<T>::E> q[R][QT][KF];
   f32x4 o[R][CT];
   // the logit that weights are relative to, how much the weights of 16 slots may add up to before it moves (-1:
   // nothing seen yet), and the sum of the weights of the lane's slots
@@ -156,10 +115,10 @@ __device__ __forceinline__ int dims_at(int s, int g) {
 // barrier a tile, were slower (355 against 349).
 template <class T, int DP, int R>
 __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
-  using Q = Query<T>;
+  using Q = Operand<T>;
   using E = typename Q::E;
   using Row = Rows<T, DP, R>;
-  constexpr int KF = Row::KF, CT = Row::CT, WT = kWeightTerms;
+  constexpr int KF = Row::KF, CT = Row::CT;
   __shared__ __attribute__((aligned(16))) f32x4 exchange[2][R * CT][64];
   __shared__ float exchange_ml[2][2 * R][64];
   __shared__ __attribute__((aligned(16))) float slot_scales[4][128];
@@ -192,23 +151,22 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
       const int d = dims_at<DP>(s, g);
       Vec<T, 8> x{};
       if (live && d < a.dim) x = load_vec<8>(q + d);
+      float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float left = to_float(x.v[e]) * h.query;
+        y[e] = to_float(x.v[e]) * h.query;
         // an infinite element makes its row NaN whatever the signs of its products: logits that are all -inf would
         // look like slots that are not seen
-        if (!(fabsf(left) < INFINITY)) left = NAN;
-        if constexpr (Q::kTerms == 1) {
-          w.q[r][0][s][e] = from_float<E>(left);
-        } else {
+        if (!(fabsf(y[e]) < INFINITY)) y[e] = NAN;
+      }
+      if constexpr (Q::kTerms == 1) {
 #pragma unroll
-          for (int term = 0; term < Q::kTerms; ++term) {
-            // cut, not rounded: the next bits, eight at a time
-            const float part = __uint_as_float(__float_as_uint(left) & 0xffff0000u);
-            w.q[r][term][s][e] = from_float<E>(part);
-            left -= part;
-          }
-        }
+        for (int e = 0; e < 8; ++e) w.q[r][0][s][e] = from_float<E>(y[e]);
+      } else {
+        Frag<bf16> parts[3];
+        cut_in_three<false>(y, parts);
+#pragma unroll
+        for (int term = 0; term < 3; ++term) w.q[r][term][s] = parts[term];
       }
     }
 #pragma unroll
@@ -402,16 +360,21 @@ __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      Frag<bf16> p[R][WT];
+      Frag<bf16> p[R][3];
 #pragma unroll
-      for (int r = 0; r < R; ++r) cut_in_three(e[r][2 * u], e[r][2 * u + 1], p[r]);
+      for (int r = 0; r < R; ++r) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = e[r][2 * u][i], y[4 + i] = e[r][2 * u + 1][i];
+        cut_in_three<false>(y, p[r]);
+      }
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         const Frag<bf16> v = codes_to<bf16>(values[c][2 * u], values[c][2 * u + 1]);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int term = 0; term < WT; ++term) w.o[r][c] = mfma(v, p[r][term], w.o[r][c]);
+          for (int term = 0; term < 3; ++term) w.o[r][c] = mfma(v, p[r][term], w.o[r][c]);
       }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -496,7 +459,7 @@ void held_units(const HeldAttention& h, const HeldPlan& p, hipStream_t st) {
   using std::integral_constant;
   auto rows = [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    if constexpr (!std::is_same<T, float>::value && DP <= 96) {
+    if constexpr (held_pairs(std::is_same<T, float>::value, DP)) {
       if (p.r == 2) return held_launch<T, DP, 2>(h, p, st);
     }
     held_launch<T, DP, 1>(h, p, st);

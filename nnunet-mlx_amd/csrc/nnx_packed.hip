@@ -3,14 +3,11 @@
 #include <cmath>
 #include <type_traits>
 
-#include "nnx_elements.h"
+#include "nnx_operands.h"
 
 namespace nnx {
 
 namespace {
-
-constexpr float kTiny = 8.673617379884035e-19f;  // 2^-60
-constexpr float kMost = 3.4028233e38f;           // 6 * (kMost / 6) is finite
 
 struct PackedArgs {
   int inputs, outputs, group, blocks, act;
@@ -52,7 +49,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackedArgs a, const T* w, uin
       top = fmaxf(top, e);
       odd |= !(e < INFINITY);
     }
-    const bool zero = odd || top < kTiny;
+    const bool zero = odd || top < kLeastTop;
     const float up = zero ? 0.f : 6.f / top;
     auto code_of = [&](int i) {
       if (zero || i >= i1) return 0;
@@ -61,7 +58,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackedArgs a, const T* w, uin
       return e | (e && x < 0.f ? 8 : 0);
     };
     for (int i = i0; i < i0 + a.group; i += 2) codes[code_at(a, o, i)] = (uint8_t)(code_of(i) | code_of(i + 1) << 4);
-    scales[scale_at(a, o, g)] = odd ? NAN : zero ? 0.f : fminf(top, kMost) / 6.f;
+    scales[scale_at(a, o, g)] = odd ? NAN : zero ? 0.f : fminf(top, kMostTop) / 6.f;
   }
 }
 
@@ -83,46 +80,14 @@ __device__ __forceinline__ float open_gate(float g, int act) {
   return act == NNX_GATE_SIGMOID ? s : g * s;
 }
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-template <class T>
-using Frag = T __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ f32x4 mfma(Frag<f16> a, Frag<f16> b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mfma(Frag<bf16> a, Frag<bf16> b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-// What x is multiplied in: 16-bit types as they are, float32 in three bfloat16 operands that add up to it.
-template <class T>
-struct Operand {
-  using E = T;
-  static constexpr int kTerms = 1;
-};
-template <>
-struct Operand<float> {
-  using E = bf16;
-  static constexpr int kTerms = 3;
-};
-
 template <class T>
 __device__ __forceinline__ void split(const Vec<T, 8>& x, Frag<typename Operand<T>::E> (&q)[Operand<T>::kTerms]) {
   if constexpr (sizeof(T) == 2) {
     __builtin_memcpy(&q[0], &x, 16);
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float left = x.v[e];
-#pragma unroll
-      for (int term = 0; term < 3; ++term) {
-        // cut, not rounded: the next bits, eight at a time
-        const float part = __uint_as_float(__float_as_uint(left) & 0xffff0000u);
-        q[term][e] = from_float<bf16>(part);
-        left = term == 0 && fabsf(left) == INFINITY ? 0.f : left - part;  // of infinity nothing is left, not NaN
-      }
-    }
+    float left[8];
+    __builtin_memcpy(left, &x, 32);
+    cut_in_three<true>(left, q);
   }
 }
 
