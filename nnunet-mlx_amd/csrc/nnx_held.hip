@@ -23,8 +23,8 @@ HeldArgs make_args(const nnx_held_config& c, const int32_t* start, const int32_t
   return a;
 }
 
-// Bound by memory: 32768 tokens of 5 heads of 64 in bfloat16 are written in 16 us (42 MB in, 22 out) and read back in
-// 11 (5.8 TB/s; a large copy reaches 5.2).  A workgroup a tile of 64 slots of one key head's keys or values, a thread 8
+// Bound by memory: 32768 tokens of 5 heads of 64 in bfloat16 are written in 18 us (42 MB in, 22 out) and read back in
+// 13 (5.1 TB/s; a large copy reaches 5.2), both in 29 back to back.  A workgroup a tile of 64 slots of one key head's keys or values, a thread 8
 // channels of four slots in a row: rows come in and go out whole (a thread a row: 692 us for both).  Four slots of a
 // value channel are one word of its 64 places (slot 16 t + 4 g + i at 16 g + 4 t + i), so value tiles change between
 // rows of channels and rows of places by words, through LDS.
@@ -381,15 +381,15 @@ HeldPlan make_plan(const nnx_held_config& c) {
   p.units = (int64_t)c.batch * c.kv_heads * p.tiles;
   p.splits = 1;
   if (p.units < kUnits) {
-    // Few units: parts of at least 4 tiles of 64 slots, a wave each, up to two workgroups a CU.  (4 queries of 3 items
-    // over up to 131072 slots 50 us, with four workgroups a CU 59.)  Not where one workgroup is done before another
-    // launch would begin: one query of 5 heads of 64 over 2048 slots takes 12.4 us in one launch and 15.3 in two, over
-    // 3000 15.8 and 15.3 (heads of 128: 1536 14.3 and 15.2, 2048 17.0 and 15.6).
+    // Few units: parts of at least 4 tiles of 64 slots, a wave each, up to two workgroups a CU.  (One query of 32 heads
+    // over 131072 slots 38.6 us, with four workgroups a CU 47.5.)  Not where one workgroup is done before another
+    // launch would begin: one query of 5 heads of 64 over 2048 slots takes 13.8 us in one launch and 15.4 in two, over
+    // 3000 18.7 and 15.3 (heads of 128: 1536 16.8 and 15.7, 2048 19.9 and 15.8).
     if ((int64_t)c.keys * c.head_dim > 2048 * 64)
       p.splits = (int)std::max<int64_t>(1, std::min(kMostSplits / p.units, ceil_div(c.keys, 256)));
   } else {
     // Many: parts that even out what the CUs get, in tiles a wave and with what a workgroup (6) and the join (8) cost.
-    // 640 units over 32768 slots: 380, 328, 357 and 350 us in 1 to 4 parts; 1280 units over 4096: 124 in 1, 143 in 2.
+    // 640 units over 32768 slots: 550, 468, 505 and 487 us in 1 to 4 parts; 1280 units over 4096: 135 in 1, 155 in 2.
     int64_t least = INT64_MAX;
     for (int s = 1; s <= 4; ++s) {
       const int64_t cost = ceil_div(p.units * s, kUnits) * (ceil_div(c.keys, 256 * s) + 6) + (s > 1 ? 8 : 0);

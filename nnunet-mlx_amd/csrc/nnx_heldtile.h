@@ -105,14 +105,14 @@ __device__ __forceinline__ int dims_at(int s, int g) {
 // on its own with a running softmax, and join their results in the end; a tile's codes go from memory to the lanes that
 // multiply them, the next tile's are on their way meanwhile.
 //
-// Few rows are bound by memory: one query of 32 heads over 131072 slots of 4 heads of 128, 138 MB, takes 37 us with the
-// join (3.7 TB/s), 4 queries of 16 heads, twice 16 rows a key head that read the same slots through the L2, 45 us for 156 MB.
-// Many are bound by vector instructions, of which 64 slots by 32 rows of 64 take 460 (conversions of codes 176, logits
-// to weights 112, of them 32 exponentials at a quarter of the rate, the rest addresses, scales and sums): 4096 queries of
-// 5 heads over 32768 slots take 322 us and the join 5, 530 TFLOP/s, the vector units busy for 80% and the matrix units
-// for 20% of it.  32 rows a wave share conversions (372 us with 16 rows 403 at the time); 64 rows leave one wave a SIMD
-// (785), three waves a SIMD spill (443).  Operands converted once for four waves' rows and passed through LDS, with a
-// barrier a tile, were slower (355 against 349).
+// Few rows are bound by memory: one query of 32 heads over 131072 slots of 4 heads of 128, 138 MB, takes 39 us with the
+// join (3.6 TB/s), 4 queries of 16 heads, twice 16 rows a key head that read the same slots through the L2, 53 us for 156 MB.
+// Many are bound by vector instructions, of which 64 slots by 32 rows of 64 take 645 (conversions of codes 192, weights
+// cut into operands 176, logits to weights 128, of them 32 exponentials at a quarter of the rate, the rest addresses, scales
+// and sums) beside 64 matrix instructions: 4096 queries of 5 heads over 32768 slots take 468 us with the join, 370 TFLOP/s,
+// the vector units busy for 85% and the matrix units for 29% of it.  32 rows a wave share conversions (16 rows: 558).
+// With one operand a weight, 372 us then: 64 rows leave one wave a SIMD (785), three waves a SIMD spill (443); operands
+// converted once for four waves' rows and passed through LDS, with a barrier a tile, were slower (355 against 349).
 template <class T, int DP, int R>
 __global__ __launch_bounds__(256, 2) void held_kernel(HeldAttention h) {
   using Q = Operand<T>;

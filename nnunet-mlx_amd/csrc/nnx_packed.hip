@@ -92,6 +92,7 @@ __device__ __forceinline__ void split(const Vec<T, 8>& x, Frag<typename Operand<
 }
 
 // Products are formed 2^-10 times as large, by what a code stands for: 128 of them add up to no more than the largest of x.
+// (Of x below 2^-110 last places fall below float32's least value on the way.)
 constexpr float kDown = 0x1p-10f, kUp = 0x1p10f;
 
 // Eight codes as E, exactly.
@@ -159,10 +160,11 @@ __device__ __forceinline__ Vec<T, 8> load_row(const T* row, int at, int end) {
 // A workgroup 16 outputs of 16 R rows, its eight waves blocks of 128 inputs in turn, without a word to each other
 // until their sums are added up.  Weights are the matrix instruction's rows, x its columns: a lane's 16 bytes of
 // codes are its operands of four instructions, and its results four neighbouring outputs of one row, which a
-// group's scales multiply as they stand.  Bound by memory: one row by two matrices of 16384 x 4096 in 13 us (71 MB,
-// 5.4 TB/s), by 4096 x 16384 in less than the call from Python takes (10 us).  More than 16 rows are read in
-// pieces of 256 bytes and more and turned in LDS (64 rows by 4096 x 4096 11 us; straight into the operands, 64 bytes of
-// 16 rows an access, 18 us); 128 rows take 19 us, bound by the L2, from which every workgroup reads its rows (268 MB).
+// group's scales multiply as they stand.  Bound by memory: one row by two matrices of 16384 x 4096 in 13.5 us (71 MB,
+// 5.3 TB/s, part of it from the last-level cache), by one of them in 9.7, as long as the call from Python takes.  More than
+// 16 rows are read in pieces of 256 bytes and more and turned in LDS (64 rows by 4096 x 4096 11.4 us; straight into the
+// operands, 64 bytes of 16 rows an access, 18 us); 128 rows take 19 us, bound by the L2, from which every workgroup reads
+// its rows (268 MB).
 constexpr int kFewWaves = 8;
 
 template <class T, int G32, int MATRICES, int R>
@@ -314,7 +316,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_kernel(LinearArgs h, in
 // once; its weights are the waves' own, as above.  Chunk c (8 inputs) of row r lies at place c * 64 + (r ^ c), so that
 // neither the rows' chunks on their way in nor the chunks' rows on their way out meet in a bank.  What bounds it is the
 // way of a block from memory, so two are on theirs while one is multiplied: 4096 rows by 320 x 1280 in float16 14 us
-// (with 32 rows a workgroup, and four workgroups a CU, 13.8), 512 rows by 4096 x 4096 32 us, 540 TFLOP/s (39).
+// (with 32 rows a workgroup, and four workgroups a CU, 13.8), 512 rows by 4096 x 4096 32 us, 530 TFLOP/s (39).
 template <class T, int G32, int MATRICES>
 __global__ __launch_bounds__(256, 2) void linear_many_kernel(LinearArgs h, int row_tiles, int64_t units) {
   using E = typename Operand<T>::E;
@@ -456,8 +458,9 @@ __global__ __launch_bounds__(256, 2) void linear_many_kernel(LinearArgs h, int r
 
 // Pieces of 64 rows by 64 outputs, half as many as CUs: with more of them waves that take a piece each are faster, with
 // fewer or as many waves that share the inputs of smaller pieces (us, shared and a piece each, bfloat16): 128 pieces of
-// 4096 inputs 19.3 and 24.0; 160 of 1280 inputs 13.4 and 10.8, 165 of 960 with a gate 22.9 and 14.5, 256 of 4096 inputs
-// 35.1 and 24.4.
+// 4096 inputs 18.8 and 23.7; 160 of 1280 inputs 13.3 and 10.7, 165 of 960 with a gate 22.0 and 13.8, 256 of 4096 inputs
+// 35.3 and 24.3.  Float32 alike: 96 pieces of 1280 inputs 17.6 and 20.7, 128 of 4096 52.2 and 54.7; 160 of 1280 28.4 and 21.0,
+// 256 of 4096 146 and 55.5.
 constexpr int kManyUnits = 128;
 
 template <class T, int G32, int MATRICES>
